@@ -16,6 +16,8 @@ MATH_FASTMATH = 0
 MATH_IEEE = 1
 FLAG_NEAR_MOMENTS = 1
 FLAG_NEAR_TENSOR_CORES = 2
+TYPE_BF16, TYPE_F16 = 1, 2
+MAX_WIDTH = 128
 
 # array ids of f3m_plan_copy_array
 ARR_SORTED_INDEX, ARR_BOX_OFFSETS, ARR_BOX_CENTERS = 0, 1, 2
@@ -44,6 +46,15 @@ class PlanStats(C.Structure):
     _fields_ = [("levels", C.c_int32), ("shared_tree", C.c_int32), ("direct_pairs", C.c_int64),
                 ("node_pairs", C.c_int64), ("far_box_pairs", C.c_int64), ("near_box_pairs", C.c_int64),
                 ("edge0", C.c_float), ("build_ms", C.c_float)]
+
+
+class Rows(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("token_stride", C.c_int64), ("head_stride", C.c_int64)]
+
+
+class Seqs(C.Structure):
+    _fields_ = [("table", C.c_void_p), ("tokens", C.c_int64), ("sequences", C.c_int32), ("tiles", C.c_int32), ("longest", C.c_int32),
+                ("table_words", C.c_int32)]
 
 
 _P = C.c_void_p
@@ -97,6 +108,19 @@ SIGNATURES = {
     "f3m_plan_last_work": (C.c_int, [_P, C.POINTER(_I64)]),
     "f3m_plan_last_pairs_by_form": (C.c_int, [_P, C.POINTER(_I64)]),
     "f3m_launch_count": (C.c_longlong, []),
+    "f3m_seqs_layout": (C.c_int, [_P, _I32, C.POINTER(Seqs), _P]),
+    "f3m_window_attention": (C.c_int, [C.POINTER(Seqs), _I32, _I32, _I32, _I32, _I32, _I32, _F32, Rows, Rows, Rows, Rows, _P, _P]),
+    "f3m_window_attention_grad_workspace_bytes": (C.c_size_t, [C.POINTER(Seqs), _I32]),
+    "f3m_window_attention_grad": (C.c_int, [C.POINTER(Seqs), _I32, _I32, _I32, _I32, _I32, _I32, _F32, Rows, Rows, Rows, Rows, _P, Rows,
+                                            Rows, Rows, Rows, _P, C.c_size_t, _P]),
+    "f3m_window_attention_step_workspace_bytes": (C.c_size_t, [_I32, _I32, _I32, _I32, _I64, _I32, _I32]),
+    "f3m_window_attention_step": (C.c_int, [_I32, _I32, _I32, _I32, _I32, _I64, _I32, _I32, _F32, Rows, Rows, _I64, Rows, _I64, _P, Rows,
+                                            _P, C.c_size_t, _P]),
+    "f3m_decay_attention_workspace_bytes": (C.c_size_t, [C.POINTER(Seqs), _I32, _I32, _I32]),
+    "f3m_decay_attention": (C.c_int, [C.POINTER(Seqs), _I32, _I32, _I32, _I32, _P, _F32, Rows, Rows, Rows, _P, Rows, _P, _P, C.c_size_t, _P]),
+    "f3m_decay_attention_grad": (C.c_int, [C.POINTER(Seqs), _I32, _I32, _I32, _I32, _P, _F32, Rows, Rows, Rows, _P, Rows, _P, Rows, Rows,
+                                           Rows, _P, _P, C.c_size_t, _P]),
+    "f3m_decay_attention_step": (C.c_int, [_I32, _I32, _I32, _I32, _I32, _P, _F32, Rows, Rows, Rows, _P, Rows, _P]),
 }
 
 _lib = None

@@ -1,0 +1,96 @@
+// What the kernel products over sequences share: arguments, 16-bit types, the table of tiles.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include "common.cuh"
+
+namespace f3m {
+
+constexpr int SEQ_TILE = F3M_SEQ_TILE;
+
+// The table of a packed batch, as int4: three orders of the tiles {first row of the sequence, its length, first token of the tile, sequence}
+// -- by place, by the tokens before the tile (the rows of late tiles see the most keys) and by the tokens from it on (the keys of early
+// tiles are seen most), the heaviest first in both -- and behind them the sequences {first row, length, first tile, tiles}.
+__host__ __device__ __forceinline__ size_t seq_by_place(const f3m_seqs &, int i) { return (size_t)i; }
+__host__ __device__ __forceinline__ size_t seq_by_past(const f3m_seqs &s, int i) { return (size_t)s.tiles + i; }
+__host__ __device__ __forceinline__ size_t seq_by_future(const f3m_seqs &s, int i) { return 2 * (size_t)s.tiles + i; }
+__host__ __device__ __forceinline__ size_t seq_of(const f3m_seqs &s, int i) { return 3 * (size_t)s.tiles + i; }
+
+template <typename T> struct Half;
+template <> struct Half<__nv_bfloat16> {
+    static constexpr int type = F3M_TYPE_BF16;
+    static __device__ __forceinline__ float2 unpack(uint32_t v) { return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u)); }
+    static __device__ __forceinline__ uint32_t pack(float lo, float hi) {   // round to nearest even
+        uint32_t r;
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+        return r;
+    }
+};
+template <> struct Half<__half> {
+    static constexpr int type = F3M_TYPE_F16;
+    static __device__ __forceinline__ float2 unpack(uint32_t v) {
+        const __half2 h = *reinterpret_cast<const __half2 *>(&v);
+        return __half22float2(h);
+    }
+    static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+        uint32_t r;
+        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+        return r;
+    }
+};
+
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+struct WindowArgs {
+    f3m_seqs s;
+    int heads, kv_heads, width, window, sinks;
+    float scale;
+    f3m_rows q, k, v, out;
+    float *lse;
+    f3m_rows dout, dq, dk, dv;   // gradients only
+    float *delta;                // (heads, tokens): rows of dout . out
+};
+void window_forward(int type, const WindowArgs &a, cudaStream_t s);
+void window_backward(int type, const WindowArgs &a, cudaStream_t s);
+
+struct StepArgs {
+    int n, heads, kv_heads, width, window, sinks;
+    int64_t capacity;
+    float scale;
+    f3m_rows q, k, v, out;
+    int64_t k_seq, v_seq;
+    const int *lengths;
+    int parts;      // splits of the keys
+    float *part;    // their sums
+};
+int window_step_parts(int n, int heads, int kv_heads, int64_t capacity, int window, int sinks);
+size_t window_step_part_floats(int n, int heads, int width, int parts);
+void window_step(int type, const StepArgs &a, cudaStream_t s);
+
+// out_i = use * sum_(j before or at i) decay^|i-j| upd (a_i.b_j) c_j + use * decay^(steps to i) a_i S, S (width of b, width of c).
+// `reversed`: sequences run from their last token to their first; the state that enters does so undecayed, the one that
+// leaves has been decayed once more (the adjoint of the recurrence).  `transposed`: states lie in memory as (width of c, width of b).
+struct DecayArgs {
+    f3m_seqs s;
+    int heads, width_b, width_c;
+    const float *log_decay;
+    float use, upd;
+    bool reversed, transposed;
+    f3m_rows a, b, c, out;
+    const float *state_in;
+    float *state_out;
+    void *ws;
+};
+size_t decay_workspace(const f3m_seqs &s, int heads, int width_b, int width_c);
+void decay_product(int type, const DecayArgs &a, cudaStream_t s);
+void decay_step(int type, int n, int heads, int width_k, int width_v, const float *log_decay, float scale, const f3m_rows &q, const f3m_rows &k,
+                const f3m_rows &v, float *state, const f3m_rows &out, cudaStream_t s);
+
+// log2 of a head's decay: at most 0; -256 makes every power but the zeroth 0 in FP32 and keeps 0 * log a number
+__device__ __forceinline__ float log2_decay(float log_decay) { return fmaxf(fminf(log_decay * 1.4426950408889634f, 0.f), -256.f); }
+
+}  // namespace f3m

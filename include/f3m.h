@@ -286,6 +286,87 @@ int f3m_rbf_dense_grad_f32(const float *X, int64_t N, const float *Y, int64_t M,
 int f3m_rbf_dense_f32_static(const float *X, int64_t N, const float *Y, int64_t M, const float *b, int32_t R,
                              int32_t d, float ls, float *out, void *stream);
 
+/* -------- kernel products over sequences ------------------------------------------------------------ */
+
+/* Products whose points are the tokens of sequences (no counterpart in the reference, whose kernel matrices are those of point
+ * sets in space).  Both are the two products above on a line of positions:
+ *
+ *   window attention  every pair is summed, as in f3m_rbf_dense_f32.  Query i of a sequence sees key j if j <= i and
+ *                     (i - j < window or j < sinks); o_i = sum_j w_ij v_j / sum_j w_ij with w_ij = exp(scale q_i.k_j) over the
+ *                     keys seen.  (With keys of one length this is the Gaussian kernel, rows normalised.)
+ *   decay attention   near pairs one by one, far ones through moments, as in f3m_kmvm_f32, but exact: the kernel
+ *                     decay^(i-j) scale q_i.k_j (j <= i) is of low rank up to a factor that is a product.  It is the recurrence
+ *                     S_t = decay S_(t-1) + k_t v_t^T,  o_t = scale q_t S_t,  S (width_k, width_v) per sequence and head.
+ *
+ * Sequences are packed: row t of an array is token t of all sequences laid end to end.  Data are 16-bit floats of one type
+ * (F3M_TYPE_*), sums and states float32.  Columns are contiguous; token and head strides are in elements, multiples of 8, and
+ * data start on 16 bytes.  Widths are multiples of 8 up to F3M_MAX_WIDTH.  Inputs have to be finite: what is not finite in a
+ * token may reach every row of the 128-token tiles that see the token's tile (never another sequence).
+ *
+ * These entry points only enqueue work: they neither wait for the stream nor allocate, so they may be captured into a graph, and calls
+ * on several streams or host threads need no order among them.  Temporaries lie in the caller's workspace (f3m_*_workspace_bytes; 16-byte
+ * aligned), which a call owns until its work has ended.  A repeated call gives the same bits. */
+#define F3M_TYPE_BF16 1
+#define F3M_TYPE_F16 2
+#define F3M_MAX_WIDTH 128
+#define F3M_SEQ_TILE 128        /* tokens per tile of a sequence */
+#define F3M_SEQ_MAX_TOKENS 0x7fffff00   /* of all sequences together */
+
+typedef struct f3m_rows {       /* (tokens, heads, width): element (t, h, c) is data[t * token_stride + h * head_stride + c] */
+    void *data;
+    int64_t token_stride, head_stride;
+} f3m_rows;
+
+/* Where the sequences of a packed batch lie.  f3m_seqs_layout fills the counts from the lengths (HOST array, each >= 0) and, if
+ * table is not NULL, the table (HOST array of table_words ints); the caller puts a copy of it on the device and sets
+ * `table` to that before other calls.  Any number of calls may use it. */
+typedef struct f3m_seqs {
+    const int32_t *table;       /* device */
+    int64_t tokens;             /* sum of the lengths: rows of every array */
+    int32_t sequences, tiles, longest;
+    int32_t table_words;
+} f3m_seqs;
+int f3m_seqs_layout(const int32_t *lengths, int32_t n, f3m_seqs *seqs, int32_t *table);
+
+/* out (tokens, heads, width), lse (heads, tokens) float32: log of the row sums sum_j w_ij.  heads is a multiple of kv_heads; query head h
+ * reads key head h / (heads / kv_heads).  window >= 1, sinks >= 0. */
+int f3m_window_attention(const f3m_seqs *seqs, int32_t type, int32_t heads, int32_t kv_heads, int32_t width, int32_t window,
+                         int32_t sinks, float scale, f3m_rows q, f3m_rows k, f3m_rows v, f3m_rows out, float *lse, void *stream);
+/* Gradients of sum(out * dout) by q, k and v, from out and lse of the call above.  dk and dv are sums over the query heads that share
+ * them. */
+size_t f3m_window_attention_grad_workspace_bytes(const f3m_seqs *seqs, int32_t heads);
+int f3m_window_attention_grad(const f3m_seqs *seqs, int32_t type, int32_t heads, int32_t kv_heads, int32_t width, int32_t window,
+                              int32_t sinks, float scale, f3m_rows q, f3m_rows k, f3m_rows v, f3m_rows out, const float *lse,
+                              f3m_rows dout, f3m_rows dq, f3m_rows dk, f3m_rows dv, void *workspace, size_t workspace_bytes,
+                              void *stream);
+/* One new token for each of n sequences against its cache: q, out (n, heads, width); k_cache, v_cache (n, capacity, kv_heads, width),
+ * element (b, t, h, c) at data[b * seq_stride + t * token_stride + h * head_stride + c].  lengths (DEVICE, n): tokens in
+ * the cache, the new one, at length - 1, among them; values outside 0..capacity are taken as the nearest of these.  Length 0: a row of zeros. */
+size_t f3m_window_attention_step_workspace_bytes(int32_t n, int32_t heads, int32_t kv_heads, int32_t width, int64_t capacity,
+                                                 int32_t window, int32_t sinks);
+int f3m_window_attention_step(int32_t n, int32_t type, int32_t heads, int32_t kv_heads, int32_t width, int64_t capacity,
+                              int32_t window, int32_t sinks, float scale, f3m_rows q, f3m_rows k_cache, int64_t k_seq_stride,
+                              f3m_rows v_cache, int64_t v_seq_stride, const int32_t *lengths, f3m_rows out, void *workspace,
+                              size_t workspace_bytes, void *stream);
+
+/* log_decay (DEVICE, heads) float32: log of each head's decay, at most 0 (larger values are taken as 0, -inf is no memory at all).
+ * q, k (tokens, heads, width_k), v, out (tokens, heads, width_v).  state_in, state_out (sequences, heads, width_k, width_v)
+ * float32, dense, 16-byte aligned: the state before the first token (NULL: zeros) and behind the last one (NULL: not wanted; another
+ * array than state_in). */
+size_t f3m_decay_attention_workspace_bytes(const f3m_seqs *seqs, int32_t heads, int32_t width_k, int32_t width_v);
+int f3m_decay_attention(const f3m_seqs *seqs, int32_t type, int32_t heads, int32_t width_k, int32_t width_v, const float *log_decay,
+                        float scale, f3m_rows q, f3m_rows k, f3m_rows v, const float *state_in, f3m_rows out, float *state_out,
+                        void *workspace, size_t workspace_bytes, void *stream);
+/* Gradients of sum(out * dout) + sum(state_out * dstate_out) by q, k, v and state_in (dstate_out NULL: zeros; dstate_in NULL: not
+ * wanted).  The decay is a constant. */
+int f3m_decay_attention_grad(const f3m_seqs *seqs, int32_t type, int32_t heads, int32_t width_k, int32_t width_v,
+                             const float *log_decay, float scale, f3m_rows q, f3m_rows k, f3m_rows v, const float *state_in,
+                             f3m_rows dout, const float *dstate_out, f3m_rows dq, f3m_rows dk, f3m_rows dv, float *dstate_in,
+                             void *workspace, size_t workspace_bytes, void *stream);
+/* One new token for each of n sequences: state (n, heads, width_k, width_v) float32 is updated in place. */
+int f3m_decay_attention_step(int32_t n, int32_t type, int32_t heads, int32_t width_k, int32_t width_v, const float *log_decay,
+                             float scale, f3m_rows q, f3m_rows k, f3m_rows v, float *state, f3m_rows out, void *stream);
+
 /* -------- measurement helpers -------------------------------------------------------------- */
 
 /* Measures the SM's exponential (MUFU.EX2) and FP32 FMA issue peaks with two register-only

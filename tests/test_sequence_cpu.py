@@ -1,0 +1,101 @@
+"""What the kernel products over sequences check before they touch a GPU: the table of tiles, arguments of the C entries."""
+import ctypes as C
+
+import numpy as np
+import pytest
+import torch
+
+from f3m_b200 import _lib, sequence
+from f3m_b200._lib import Rows, Seqs
+
+
+def layout(lengths):
+    L, s = _lib.lib(), Seqs()
+    host = np.array(lengths, dtype=np.int32)
+    assert L.f3m_seqs_layout(host.ctypes.data, len(lengths), C.byref(s), None) == 0
+    table = np.full(s.table_words, -1, dtype=np.int32)
+    assert L.f3m_seqs_layout(host.ctypes.data, len(lengths), C.byref(s), table.ctypes.data) == 0
+    return s, table.reshape(-1, 4)
+
+
+@pytest.mark.parametrize("lengths", [[1], [0], [128, 129, 0, 1, 5000], [7] * 40])
+def test_layout(lengths):
+    s, t = layout(lengths)
+    assert (s.tokens, s.sequences, s.longest) == (sum(lengths), len(lengths), max(lengths))
+    first = np.cumsum(lengths) - lengths
+    tiles = [(first[i], n, a, i) for i, n in enumerate(lengths) for a in range(0, n, 128)]
+    assert s.tiles == len(tiles) and len(t) == 3 * len(tiles) + len(lengths)
+    by = [t[k * s.tiles:(k + 1) * s.tiles] for k in range(3)]
+    assert by[0].tolist() == [list(map(int, x)) for x in tiles]
+    for b in by[1:]:
+        assert sorted(b.tolist()) == sorted(by[0].tolist())
+    assert (np.diff(by[1][:, 2]) <= 0).all() and (np.diff(by[2][:, 1] - by[2][:, 2]) <= 0).all()
+    at = 0
+    for i, row in enumerate(t[3 * s.tiles:].tolist()):
+        n = -(-lengths[i] // 128)
+        assert row == [first[i], lengths[i], at, n]
+        at += n
+
+
+def test_layout_refusals():
+    L, s = _lib.lib(), Seqs()
+    for bad in ([-1], [2 ** 31 - 1, 2 ** 31 - 1]):
+        host = np.array(bad, dtype=np.int32)
+        assert L.f3m_seqs_layout(host.ctypes.data, len(bad), C.byref(s), None) in (1, 4)
+        assert L.f3m_last_error()
+    for bad in ([1.5], [[1, 2]], [-1], [2 ** 31]):
+        with pytest.raises(ValueError):
+            sequence.SequencePlan(bad)
+    with pytest.raises(ValueError):
+        sequence.SequencePlan([1], device="cpu")
+
+
+def test_argument_checks_of_the_entries():
+    """Every call here is refused before anything is launched: the pointers are never followed."""
+    L = _lib.lib()
+    s, t = layout([100, 30])
+    buf = np.zeros(64, dtype=np.uint8)
+    base = buf.ctypes.data + (-buf.ctypes.data) % 16
+    s.table = base
+    ok = Rows(base, 128, 64)        # 130 tokens, 2 heads, width 64
+
+    def window(q=ok, k=ok, v=ok, out=ok, type=1, heads=2, kv=2, width=64, window=4, sinks=0, scale=0.1, lse=base, seqs=s):
+        return L.f3m_window_attention(C.byref(seqs), type, heads, kv, width, window, sinks, scale, q, k, v, out, lse, None)
+
+    none = Rows(None, 128, 64)
+    assert window(type=3) == 5 and window(width=60) == 5 and window(width=136) == 5 and window(width=0) == 5
+    assert window(heads=3) == 1 and window(kv=0) == 1 and window(heads=0, kv=1) == 1
+    assert window(window=0) == 1 and window(sinks=-1) == 1 and window(scale=float("inf")) == 1
+    assert window(q=none) == 1 and window(out=none) == 1 and window(lse=None) == 1
+    assert window(q=Rows(base + 2, 128, 64)) == 1 and window(k=Rows(base, 132, 64)) == 1 and window(v=Rows(base, 128, -64)) == 1
+    assert window(out=Rows(base, 64, 64)) == 1 and b"overlap" in L.f3m_last_error()
+    assert window(out=Rows(base, 128, 0)) == 1
+    bad = Seqs(None, 130, 2, 3, 100, 0)
+    assert window(seqs=bad) == 1
+
+    def grad(ws=base, have=1 << 20, dk=ok):
+        return L.f3m_window_attention_grad(C.byref(s), 1, 2, 2, 64, 4, 0, 0.1, ok, ok, ok, ok, base, ok, ok, dk, ok, ws, have, None)
+
+    need = L.f3m_window_attention_grad_workspace_bytes(C.byref(s), 2)
+    assert need > 0 and grad(have=need - 1) == 7 and grad(ws=None) == 1 and grad(ws=base + 4) == 1 and grad(dk=Rows(base, 8, 64)) == 1
+
+    def step(n=2, cap=100, lens=base, ws=base, have=1 << 40, k=ok, seq=12800):
+        return L.f3m_window_attention_step(n, 1, 2, 2, 64, cap, 50, 0, 0.1, ok, k, seq, ok, seq, lens, ok, ws, have, None)
+
+    assert step(n=-1) == 1 and step(cap=-1) == 1 and step(cap=1 << 31) == 1 and step(lens=None) == 1 and step(k=none) == 1 and step(seq=4) == 1
+
+    def decay(q=ok, state_in=None, state_out=None, ld=base, wk=64, ws=base, have=1 << 40):
+        return L.f3m_decay_attention(C.byref(s), 1, 2, wk, 64, ld, 0.1, q, ok, ok, state_in, ok, state_out, ws, have, None)
+
+    assert decay(q=none) == 1 and decay(ld=None) == 1 and decay(wk=12) == 5 and decay(state_in=base + 4) == 1
+    assert decay(state_in=base, state_out=base) == 1 and b"same array" in L.f3m_last_error()
+    assert L.f3m_decay_attention_step(2, 1, 2, 64, 64, base, 0.1, ok, ok, ok, None, ok, None) == 1
+    assert L.f3m_decay_attention_step(2, 1, 2, 64, 64, base, float("nan"), ok, ok, ok, base, ok, None) == 1
+
+
+def test_cpu_tensors_are_refused():
+    x = torch.zeros(4, 2, 64, dtype=torch.bfloat16)
+    with pytest.raises(ValueError):
+        sequence.window_attention_step(x, x[:, None], x[:, None], torch.ones(4, dtype=torch.int32), 4)
+    with pytest.raises(ValueError):
+        sequence.decay_attention_step(x, x, x, torch.zeros(2), torch.zeros(4, 2, 64, 64))
