@@ -3,47 +3,437 @@
 
 namespace f3m {
 
-// A CTA per (sequence, head) walks the tokens; thread c holds column c of the state.
-template <typename T>
-__global__ void __launch_bounds__(128) decay_walk(DecayArgs a) {
-    __shared__ float as[F3M_MAX_WIDTH], bs[F3M_MAX_WIDTH];
-    const int4 e = reinterpret_cast<const int4 *>(a.s.table)[seq_of(a.s, blockIdx.x)];
-    const int h = blockIdx.y, c = threadIdx.x, wb = a.width_b, wc = a.width_c;
-    const float decay = exp2f(log2_decay(a.log_decay[h]));
-    const int64_t base = ((int64_t)blockIdx.x * a.heads + h) * wb * wc;
-    float S[F3M_MAX_WIDTH];
-#pragma unroll
-    for (int d = 0; d < F3M_MAX_WIDTH; d++) S[d] = a.state_in && c < wc && d < wb ? a.state_in[base + (a.transposed ? (int64_t)c * wb + d : (int64_t)d * wc + c)] : 0.f;
-    for (int n = 0; n < e.y; n++) {
-        const int64_t t = e.x + (a.reversed ? e.y - 1 - n : n);
-        __syncthreads();
-        if (c < wb) {
-            as[c] = (float)(reinterpret_cast<const T *>(a.a.data)[t * a.a.token_stride + h * a.a.head_stride + c]);
-            bs[c] = (float)(reinterpret_cast<const T *>(a.b.data)[t * a.b.token_stride + h * a.b.head_stride + c]);
-        }
-        __syncthreads();
-        const float cv = c < wc ? a.upd * (float)(reinterpret_cast<const T *>(a.c.data)[t * a.c.token_stride + h * a.c.head_stride + c]) : 0.f;
-        float o = 0.f;
-#pragma unroll
-        for (int d = 0; d < F3M_MAX_WIDTH; d++)
-            if (d < wb) {
-                S[d] = (a.reversed && n == 0 ? S[d] : decay * S[d]) + bs[d] * cv;
-                o = fmaf(as[d], S[d], o);
-            }
-        if (c < wc) reinterpret_cast<T *>(a.out.data)[t * a.out.token_stride + h * a.out.head_stride + c] = (T)(a.use * o);
-    }
-    if (a.state_out && c < wc)
-#pragma unroll
-        for (int d = 0; d < F3M_MAX_WIDTH; d++)
-            if (d < wb) a.state_out[base + (a.transposed ? (int64_t)c * wb + d : (int64_t)d * wc + c)] = a.reversed && e.y ? decay * S[d] : S[d];
+// A head's sequences, laid end to end in tiles of 128 tokens, are cut into ranges of equally many tiles; a CTA takes one range and carries the
+// state S (width of b x width of c, FP32, in tensor memory) through it.  For a tile of m tokens, with L the triangle of powers of the decay:
+//
+//     O = use * ( upd * (L o A B^T) C + diag(decay^steps) A S )        near pairs one by one, far ones through the state
+//     S = decay^m S + (diag(upd * decay^left) B)^T C                   the state moves on by a tile
+//
+// All five products run on the tensor cores: A B^T and A S as soon as a tile has landed, then, while warps 0-3 turn A B^T into the weights
+// (rounded to 16 bits, written over it in tensor memory), warps 4-7 split the scaled rows of B into a head and a tail of 16 bits each, in place
+// and over A: the state is returned in FP32, and one rounding of its operand would leave it 2^-9 off; head and tail together lose 2^-17.
+// As an operand of A S the state is rounded to 16 bits, like the weights.
+//
+// A range that does not begin with a sequence needs the state that the ranges before it leave: decay_tiles<true> computes what each range
+// adds to the state (B and C only), decay_join runs over the ranges, and decay_tiles<false> starts from that.  B and C are then read
+// twice, which is the price of using all SMs when there are fewer heads than SMs.
+constexpr int DK_THREADS = 320, DK_BLOCK = SEQ_TILE * 128;   // bytes of a block of 64 columns
+constexpr int DK_TILES = 14;                                 // blocks of 64 columns in shared memory: the tiles of all stages and the state
+
+struct DecayKernel {
+    DecayArgs a;
+    CUtensorMap ma, mb, mc;
+    int ranges, per_range;      // per_range tiles each
+    float *carry;               // (ranges, heads, width of b, width of c): the state behind each range
+    int *err;
+};
+
+__device__ __forceinline__ int4 tile_at(const DecayArgs &a, int place) {
+    return reinterpret_cast<const int4 *>(a.s.table)[seq_by_place(a.s, a.reversed ? a.s.tiles - 1 - place : place)];
+}
+__device__ __forceinline__ bool tile_begins(const DecayArgs &a, const int4 &e) { return a.reversed ? e.z + SEQ_TILE >= e.y : e.z == 0; }
+__device__ __forceinline__ bool tile_ends(const DecayArgs &a, const int4 &e) { return a.reversed ? e.z == 0 : e.z + SEQ_TILE >= e.y; }
+__device__ __forceinline__ int tile_rows(const int4 &e) { return min(SEQ_TILE, e.y - e.z); }
+// tiles of e's sequence before e, in the order of the walk
+__device__ __forceinline__ int tiles_before(const DecayArgs &a, const int4 &e) {
+    const int i = e.z / SEQ_TILE, n = (e.y + SEQ_TILE - 1) / SEQ_TILE;
+    return a.reversed ? n - 1 - i : i;
 }
 
-size_t decay_workspace(const f3m_seqs &, int, int, int) { return 0; }
-void decay_product(int type, const DecayArgs &a, cudaStream_t s) {
-    if (type == F3M_TYPE_BF16) decay_walk<__nv_bfloat16><<<dim3(a.s.sequences, a.heads), 128, 0, s>>>(a);
-    else decay_walk<__half><<<dim3(a.s.sequences, a.heads), 128, 0, s>>>(a);
+template <typename T, bool STATES>
+__global__ void __launch_bounds__(DK_THREADS, 1) decay_tiles(const __grid_constant__ DecayKernel p) {
+    extern __shared__ unsigned char raw[];
+    __shared__ __align__(8) uint64_t bars[2 * 4 + 6];
+    __shared__ uint32_t tmem_s;
+    __shared__ int gave_up_s;
+    __shared__ __align__(16) float pw[32], pr[32];   // decay^n, decay^(31 - n)
+    const DecayArgs &a = p.a;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, h = blockIdx.y;
+    const int nb = (a.width_b + 63) / 64, nc = (a.width_c + 63) / 64;
+    const int stage_blocks = 2 * nb + nc, stages = min(4, (DK_TILES - nc) / stage_blocks);
+    const uint32_t smem = (tc::smem_u32(raw) + 1023) & ~1023u, state_s = smem + stages * stage_blocks * DK_BLOCK;
+    const float l2 = log2_decay(a.log_decay[h]);
+
+    int first = blockIdx.x * p.per_range;
+    const int last = min(a.s.tiles, first + p.per_range);
+    if (STATES) {   // only the sequence that runs on into the next range
+        const int4 e = tile_at(a, last - 1);
+        first = tile_ends(a, e) ? last : max(first, last - 1 - tiles_before(a, e));
+        if (first >= last) return;
+    }
+    const int tiles = last - first;
+
+    if (warp == 8) tc::tmem_alloc(tc::smem_u32(&tmem_s), 512);
+    if (tid == 0) {
+        for (int i = 0; i < 8; i++) tc::mbar_init(tc::smem_u32(&bars[i]), 1);          // landed, free again (by stage)
+        tc::mbar_init(tc::smem_u32(&bars[8]), 1);                                      // A B^T and A S done
+        tc::mbar_init(tc::smem_u32(&bars[9]), 128);                                    // weights written
+        tc::mbar_init(tc::smem_u32(&bars[10]), 128);                                   // B split
+        tc::mbar_init(tc::smem_u32(&bars[11]), 128);                                   // state ready as operand and in tensor memory
+        tc::mbar_init(tc::smem_u32(&bars[12]), 1);                                     // outputs and state done
+        tc::mbar_init(tc::smem_u32(&bars[13]), 128);                                   // outputs read
+        tc::fence_mbar_init();
+        gave_up_s = 0;
+    }
+    if (tid < 32) {
+        pw[tid] = exp2f(l2 * tid);
+        pr[tid] = exp2f(l2 * (31 - tid));
+    }
+    tc::fence_before_sync();
+    __syncthreads();
+    tc::fence_after_sync();
+    const Waits wait{&gave_up_s, p.err};
+    const uint32_t tmem = tmem_s, t_score = tmem, t_inter = tmem + 128, t_intra = tmem + 256, t_state = tmem + 384;
+    const uint32_t b_full = tc::smem_u32(&bars[0]), b_free = tc::smem_u32(&bars[4]), b_score = tc::smem_u32(&bars[8]), b_weights = tc::smem_u32(&bars[9]),
+                   b_split = tc::smem_u32(&bars[10]), b_state = tc::smem_u32(&bars[11]), b_done = tc::smem_u32(&bars[12]), b_read = tc::smem_u32(&bars[13]);
+    auto a_tile = [&](int s) { return smem + s * stage_blocks * DK_BLOCK; };
+    auto b_tile = [&](int s) { return a_tile(s) + nb * DK_BLOCK; };
+    auto c_tile = [&](int s) { return a_tile(s) + 2 * nb * DK_BLOCK; };
+
+    auto all_wait = [&](uint32_t bar, uint32_t parity) {   // a whole warp, which stays together for the instructions that need that
+        wait(bar, parity);
+        __syncwarp();
+    };
+    if (warp == 8) {
+        // ---- copies ----
+        if (lane == 0) {
+            int n = 0;
+            for (; n < tiles && !gave_up_s; n++) {
+                const int s = n % stages;
+                if (n >= stages) wait(b_free + 8 * s, (n / stages - 1) & 1);
+                if (gave_up_s) break;
+                const int4 e = tile_at(a, first + n);
+                tc::mbar_expect_tx(b_full + 8 * s, (STATES ? nb + nc : stage_blocks) * DK_BLOCK);
+                for (int k = 0; k < nb; k++) {
+                    if (!STATES) tc::tma_rows(a_tile(s) + k * DK_BLOCK, &p.ma, 64 * k, h, e.x + e.z, b_full + 8 * s);
+                    tc::tma_rows(b_tile(s) + k * DK_BLOCK, &p.mb, 64 * k, h, e.x + e.z, b_full + 8 * s);
+                }
+                for (int k = 0; k < nc; k++) tc::tma_rows(c_tile(s) + k * DK_BLOCK, &p.mc, 64 * k, h, e.x + e.z, b_full + 8 * s);
+            }
+            for (int s = 0; s < stages; s++)   // the last copy into each stage
+                if (n > s) wait.drain(b_full + 8 * s, ((n - 1 - s) / stages) & 1);
+        }
+    } else if (warp == 9) {
+        // ---- products ----
+        if (lane == 0) {
+            constexpr bool bf = Half<T>::type == F3M_TYPE_BF16;
+            const uint32_t i_score = tc::idesc_f16(bf, 128, 128, false, false), i_rows = tc::idesc_f16(bf, 128, 64 * nc, false, true),
+                           i_state = tc::idesc_f16(bf, 128, 64 * nc, true, true);
+            for (int n = 0; n < tiles; n++) {
+                const int s = n % stages;
+                wait(b_full + 8 * s, (n / stages) & 1);
+                tc::fence_after_sync();
+                if (!STATES) {
+                    for (int k = 0; k < 4 * nb; k++)
+                        tc::mma_f16(t_score, tc::desc_k(a_tile(s) + (k >> 2) * DK_BLOCK + (k & 3) * 32), tc::desc_k(b_tile(s) + (k >> 2) * DK_BLOCK + (k & 3) * 32), i_score, k > 0);
+                    if (n) wait(b_read, (n - 1) & 1);
+                }
+                wait(b_state, n & 1);
+                tc::fence_after_sync();
+                if (!STATES) {
+                    for (int k = 0; k < 4 * nb; k++)
+                        tc::mma_f16(t_inter, tc::desc_k(a_tile(s) + (k >> 2) * DK_BLOCK + (k & 3) * 32), tc::desc_mn(state_s + k * 2048, DK_BLOCK), i_rows, k > 0);
+                    tc::mma_commit(b_score);
+                    wait(b_split, n & 1);      // also clears the rows of C that belong to another sequence
+                    wait(b_weights, n & 1);
+                    tc::fence_after_sync();
+                    for (int k = 0; k < 8; k++) tc::mma_f16_ta(t_intra, t_score + 8 * k, tc::desc_mn(c_tile(s) + k * 2048, DK_BLOCK), i_rows, k > 0);
+                } else {
+                    wait(b_split, n & 1);
+                    tc::fence_after_sync();
+                }
+                for (int half = 0; half < 2; half++)
+                    for (int k = 0; k < 8; k++)
+                        tc::mma_f16(t_state, tc::desc_mn((half ? a_tile(s) : b_tile(s)) + k * 2048, DK_BLOCK), tc::desc_mn(c_tile(s) + k * 2048, DK_BLOCK), i_state, 1);
+                tc::mma_commit(b_free + 8 * s);
+                tc::mma_commit(b_done);
+            }
+        }
+    } else if (warp < 4 && !STATES) {
+        // ---- weights and outputs: thread i has row i ----
+        const int i = tid;
+        const uint32_t lanes = (uint32_t)(32 * warp) << 16;
+        for (int n = 0; n < tiles; n++) {
+            const int4 e = tile_at(a, first + n);
+            const int m = tile_rows(e);
+            all_wait(b_score, n & 1);
+            tc::fence_after_sync();
+            const float coef = a.use * a.upd;
+#pragma unroll
+            for (int cb = 0; cb < 4; cb++) {
+                uint32_t w[16];
+                const bool near = a.reversed ? cb >= warp : cb <= warp;   // warp-uniform
+                if (near) {
+                    uint32_t r[32];
+                    tc::tmem_ld32(t_score + lanes + 32 * cb, r);
+                    tc::tmem_ld_wait(r);
+                    if (cb == warp) {
+#pragma unroll
+                        for (int c = 0; c < 32; c += 2) {
+                            float x[2];
+#pragma unroll
+                            for (int q = 0; q < 2; q++) {
+                                const int apart = a.reversed ? c + q - lane : lane - c - q;
+                                x[q] = apart >= 0 && 32 * cb + c + q < m ? __uint_as_float(r[c + q]) * (coef * pw[max(apart, 0)]) : 0.f;
+                            }
+                            w[c / 2] = Half<T>::pack(x[0], x[1]);
+                        }
+                    } else {
+                        const float f = coef * exp2f(l2 * (a.reversed ? 32 * cb - i : i - 32 * cb - 31));
+                        const float *tab = a.reversed ? pw : pr;
+#pragma unroll
+                        for (int c = 0; c < 32; c += 2) {
+                            const float2 t = *reinterpret_cast<const float2 *>(tab + c);
+                            const float x0 = __uint_as_float(r[c]) * (f * t.x), x1 = __uint_as_float(r[c + 1]) * (f * t.y);
+                            w[c / 2] = Half<T>::pack(32 * cb + c < m ? x0 : 0.f, 32 * cb + c + 1 < m ? x1 : 0.f);
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 16; c++) w[c] = 0u;
+                }
+                // columns 16 cb .. of the weights lie over scores that this warp has read
+                tc::tmem_st16(t_score + lanes + 16 * cb, w);
+            }
+            tc::tmem_st_wait();
+            tc::fence_before_sync();
+            tc::mbar_arrive(b_weights);
+
+            all_wait(b_done, n & 1);
+            tc::fence_after_sync();
+            const float f = a.use * exp2f(l2 * (a.reversed ? m - 1 - i : i + 1));
+            T *out = reinterpret_cast<T *>(a.out.data) + (int64_t)(e.x + e.z + i) * a.out.token_stride + (int64_t)h * a.out.head_stride;
+#pragma unroll
+            for (int cb = 0; cb < 4; cb++) {
+                if (cb >= 2 * nc) break;
+                uint32_t x[32], y[32];
+                tc::tmem_ld32(t_inter + lanes + 32 * cb, x);
+                tc::tmem_ld32(t_intra + lanes + 32 * cb, y);
+                tc::tmem_ld_wait(x);
+                tc::tmem_ld_wait(y);
+                if (cb == 2 * nc - 1) {
+                    tc::fence_before_sync();
+                    tc::mbar_arrive(b_read);
+                }
+#pragma unroll
+                for (int c = 0; c < 32; c += 8) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int q = 0; q < 4; q++)
+                        w[q] = Half<T>::pack(fmaf(f, __uint_as_float(x[c + 2 * q]), __uint_as_float(y[c + 2 * q])),
+                                             fmaf(f, __uint_as_float(x[c + 2 * q + 1]), __uint_as_float(y[c + 2 * q + 1])));
+                    if (i < m && 32 * cb + c < a.width_c) *reinterpret_cast<uint4 *>(out + 32 * cb + c) = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+                __syncwarp();
+            }
+        }
+    } else if (warp >= 4 && warp < 8) {
+        // ---- operands: thread j has row j of B and C, and row j of the state ----
+        const int j = tid - 128;
+        const uint32_t lanes = (uint32_t)(32 * (warp - 4)) << 16;
+        const int64_t plane = (int64_t)a.width_b * a.width_c;
+        // the state before tile n: from tensor memory, or where a sequence or the range begins
+        auto state_before = [&](int n) {
+            const int4 e = tile_at(a, first + n);
+            const bool begins = tile_begins(a, e);
+            const float scale = exp2f(l2 * tile_rows(e));
+            const float *src = nullptr;
+            bool turned = false;
+            if (begins) {
+                if (a.state_in) { src = a.state_in + ((int64_t)e.w * a.heads + h) * plane; turned = a.transposed; }
+            } else if (n == 0 && !STATES) {
+                src = p.carry + ((int64_t)(blockIdx.x - 1) * a.heads + h) * plane;
+            }
+            const bool fresh = begins || n == 0;
+#pragma unroll
+            for (int cb = 0; cb < 4; cb++) {
+                if (cb >= 2 * nc) break;
+                uint32_t r[32];
+                if (!fresh) {
+                    tc::tmem_ld32(t_state + lanes + 32 * cb, r);
+                    tc::tmem_ld_wait(r);
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 32; c++) r[c] = 0u;
+                    if (src && j < a.width_b) {
+                        if (turned) {
+#pragma unroll
+                            for (int c = 0; c < 32; c++)
+                                if (32 * cb + c < a.width_c) r[c] = __float_as_uint(src[(int64_t)(32 * cb + c) * a.width_b + j]);
+                        } else {
+#pragma unroll
+                            for (int c = 0; c < 32; c += 4)
+                                if (32 * cb + c < a.width_c) {
+                                    const uint4 v = *reinterpret_cast<const uint4 *>(src + (int64_t)j * a.width_c + 32 * cb + c);
+                                    r[c] = v.x; r[c + 1] = v.y; r[c + 2] = v.z; r[c + 3] = v.w;
+                                }
+                        }
+                    }
+                }
+                if (!STATES) {
+                    const uint32_t row = state_s + (cb >> 1) * DK_BLOCK;
+#pragma unroll
+                    for (int c = 0; c < 32; c += 8) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int q = 0; q < 4; q++) w[q] = Half<T>::pack(__uint_as_float(r[c + 2 * q]), __uint_as_float(r[c + 2 * q + 1]));
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row + tc::swz(j, 4 * (cb & 1) + c / 8)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+                    }
+                }
+#pragma unroll
+                for (int c = 0; c < 32; c++) r[c] = __float_as_uint(scale * __uint_as_float(r[c]));
+                __syncwarp();
+                tc::tmem_st32(t_state + lanes + 32 * cb, r);
+            }
+            tc::tmem_st_wait();
+            tc::fence_async_smem();
+            tc::fence_before_sync();
+            tc::mbar_arrive(b_state);
+        };
+        auto state_to = [&](float *dst, bool turned) {
+            if (32 * (warp - 4) >= a.width_b) return;   // the whole warp
+#pragma unroll
+            for (int cb = 0; cb < 4; cb++) {
+                if (cb >= 2 * nc) break;
+                uint32_t r[32];
+                tc::tmem_ld32(t_state + lanes + 32 * cb, r);
+                tc::tmem_ld_wait(r);
+                const bool in = j < a.width_b;
+                if (turned) {
+#pragma unroll
+                    for (int c = 0; c < 32; c++)
+                        if (in && 32 * cb + c < a.width_c) dst[(int64_t)(32 * cb + c) * a.width_b + j] = __uint_as_float(r[c]);
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 32; c += 4)
+                        if (in && 32 * cb + c < a.width_c) *reinterpret_cast<uint4 *>(dst + (int64_t)j * a.width_c + 32 * cb + c) = make_uint4(r[c], r[c + 1], r[c + 2], r[c + 3]);
+                }
+                __syncwarp();
+            }
+        };
+        state_before(0);
+        for (int n = 0; n < tiles; n++) {
+            const int4 e = tile_at(a, first + n);
+            const int m = tile_rows(e), s = n % stages;
+            all_wait(b_full + 8 * s, (n / stages) & 1);
+            if (!STATES) all_wait(b_score, n & 1);   // A and B have been read
+            const float f = a.upd * exp2f(l2 * (a.reversed ? j + 1 : m - 1 - j));
+            for (int k = 0; k < nb; k++) {
+                const uint32_t head = b_tile(s) + k * DK_BLOCK, tail = a_tile(s) + k * DK_BLOCK;
+#pragma unroll
+                for (int c = 0; c < 8; c++) {
+                    uint32_t v[4], w[4];
+                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(head + tc::swz(j, c)) : "memory");
+#pragma unroll
+                    for (int q = 0; q < 4; q++) {
+                        float2 x = Half<T>::unpack(v[q]);
+                        x.x *= f; x.y *= f;
+                        v[q] = j < m ? Half<T>::pack(x.x, x.y) : 0u;
+                        const float2 y = Half<T>::unpack(v[q]);
+                        w[q] = j < m ? Half<T>::pack(x.x - y.x, x.y - y.y) : 0u;
+                    }
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(head + tc::swz(j, c)), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(tail + tc::swz(j, c)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+                }
+            }
+            if (j >= m)   // tokens of the next sequence: nothing of theirs may meet a weight, not even a weight of zero
+                for (int k = 0; k < nc; k++)
+#pragma unroll
+                    for (int c = 0; c < 8; c++)
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(c_tile(s) + k * DK_BLOCK + tc::swz(j, c)), "r"(0) : "memory");
+            tc::fence_async_smem();
+            tc::mbar_arrive(b_split);
+            all_wait(b_done, n & 1);
+            tc::fence_after_sync();
+            if (!STATES && a.state_out && tile_ends(a, e)) state_to(a.state_out + ((int64_t)e.w * a.heads + h) * plane, a.transposed);
+            if (n + 1 < tiles) state_before(n + 1);
+        }
+        if (STATES) state_to(p.carry + ((int64_t)blockIdx.x * a.heads + h) * plane, false);
+    }
+    __syncwarp();
+    tc::fence_before_sync();
+    __syncthreads();
+    if (warp == 8) tc::tmem_dealloc(tmem, 512);
+}
+
+// Runs over the ranges of a head: where range r is a stretch of one sequence that began before it, the state behind it is what it adds
+// plus the state behind range r - 1, decayed over its tokens.
+__global__ void __launch_bounds__(256) decay_join(const __grid_constant__ DecayKernel p) {
+    const DecayArgs &a = p.a;
+    const int h = blockIdx.y, plane = a.width_b * a.width_c, at = 4 * (blockIdx.x * 256 + threadIdx.x);
+    const float l2 = log2_decay(a.log_decay[h]);
+    float4 before = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int r = 0; r + 1 < p.ranges; r++) {
+        const int last = (r + 1) * p.per_range;
+        const int4 e = tile_at(a, last - 1), b = tile_at(a, r * p.per_range);
+        if (tile_ends(a, e) || at >= plane) continue;
+        float4 *mine = reinterpret_cast<float4 *>(p.carry + ((int64_t)r * a.heads + h) * plane + at);
+        float4 x = *mine;
+        if (e.w == b.w && !tile_begins(a, b)) {
+            const float f = exp2f(l2 * (a.reversed ? min(b.y, b.z + SEQ_TILE) - e.z : e.z + tile_rows(e) - b.z));
+            x.x = fmaf(f, before.x, x.x); x.y = fmaf(f, before.y, x.y); x.z = fmaf(f, before.z, x.z); x.w = fmaf(f, before.w, x.w);
+            *mine = x;
+        }
+        before = x;
+    }
+}
+
+// Sequences without tokens hand their state on.
+__global__ void __launch_bounds__(256) decay_empty(DecayArgs a) {
+    const int4 e = reinterpret_cast<const int4 *>(a.s.table)[seq_of(a.s, blockIdx.x)];
+    if (e.y) return;
+    const int64_t plane = (int64_t)a.width_b * a.width_c * a.heads;
+    for (int64_t i = threadIdx.x; i < plane; i += 256) a.state_out[blockIdx.x * plane + i] = a.state_in ? a.state_in[blockIdx.x * plane + i] : 0.f;
+}
+
+// How many ranges a head's tiles are cut into.  One CTA of decay_tiles fills an SM.  With one range the SMs without a head idle; with more, B
+// and C are read twice, half as much again: the number that gives the least of (bytes read) / (share of the SMs busy), up to three waves.
+static int decay_ranges(const f3m_seqs &s, int heads) {
+    int best = 1;
+    float least = 0.f;
+    for (int r = 1; r <= s.tiles && (r == 1 || (int64_t)heads * r <= 3 * NUM_SMS_HINT); r++) {
+        const int64_t ctas = (int64_t)heads * r, waves = (ctas + NUM_SMS_HINT - 1) / NUM_SMS_HINT;
+        const int per = (s.tiles + r - 1) / r;
+        const float cost = (r == 1 ? 1.f : 1.5f) * (float)(waves * per);
+        if (r == 1 || cost < least) { least = cost; best = r; }
+    }
+    return best;
+}
+size_t decay_workspace(const f3m_seqs &s, int heads, int width_b, int width_c) {
+    const int r = decay_ranges(s, heads);
+    return r == 1 ? 0 : (size_t)r * heads * width_b * width_c * sizeof(float);
+}
+
+template <typename T>
+static void decay_product_t(const DecayArgs &a, cudaStream_t s) {
+    if (a.state_out) {
+        decay_empty<<<a.s.sequences, 256, 0, s>>>(a);
+        F3M_LAUNCH_CHECK();
+    }
+    if (a.s.tiles == 0) return;
+    DecayKernel p;
+    p.a = a;
+    p.ma = seq_tensor_map(Half<T>::type, a.a, a.s.tokens, a.heads, a.width_b);
+    p.mb = seq_tensor_map(Half<T>::type, a.b, a.s.tokens, a.heads, a.width_b);
+    p.mc = seq_tensor_map(Half<T>::type, a.c, a.s.tokens, a.heads, a.width_c);
+    p.ranges = decay_ranges(a.s, a.heads);
+    p.per_range = (a.s.tiles + p.ranges - 1) / p.ranges;
+    p.ranges = (a.s.tiles + p.per_range - 1) / p.per_range;
+    p.carry = (float *)a.ws;
+    p.err = seq_error_word();
+    constexpr int bytes = DK_TILES * DK_BLOCK + 1024;
+    if (p.ranges > 1) {
+        F3M_CUDA(cudaFuncSetAttribute(decay_tiles<T, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+        decay_tiles<T, true><<<dim3(p.ranges - 1, a.heads), DK_THREADS, bytes, s>>>(p);
+        F3M_LAUNCH_CHECK();
+        decay_join<<<dim3((a.width_b * a.width_c / 4 + 255) / 256, a.heads), 256, 0, s>>>(p);
+        F3M_LAUNCH_CHECK();
+    }
+    F3M_CUDA(cudaFuncSetAttribute(decay_tiles<T, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    decay_tiles<T, false><<<dim3(p.ranges, a.heads), DK_THREADS, bytes, s>>>(p);
     F3M_LAUNCH_CHECK();
 }
+void decay_product(int type, const DecayArgs &a, cudaStream_t s) { type == F3M_TYPE_BF16 ? decay_product_t<__nv_bfloat16>(a, s) : decay_product_t<__half>(a, s); }
 
 // A CTA per (sequence, head): 32 threads across the columns, four each, 8 rows of threads down the state.  The state is read and written
 // once, 16 bytes a thread, and that is all the time there is.

@@ -14,6 +14,7 @@
 #include <algorithm>
 #include "common.cuh"
 #include "packed.cuh"
+#include "tc.cuh"
 
 namespace f3m {
 

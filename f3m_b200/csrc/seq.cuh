@@ -3,6 +3,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include "common.cuh"
+#include "tc.cuh"
 
 namespace f3m {
 
@@ -89,6 +90,37 @@ size_t decay_workspace(const f3m_seqs &s, int heads, int width_b, int width_c);
 void decay_product(int type, const DecayArgs &a, cudaStream_t s);
 void decay_step(int type, int n, int heads, int width_k, int width_v, const float *log_decay, float scale, const f3m_rows &q, const f3m_rows &k,
                 const f3m_rows &v, float *state, const f3m_rows &out, cudaStream_t s);
+
+// A tensor map of (tokens, heads, width) rows whose boxes are 64 columns x 1 head x 128 tokens, swizzled
+CUtensorMap seq_tensor_map(int type, const f3m_rows &r, int64_t tokens, int heads, int width);
+// The word in mapped host memory where a kernel notes that a wait of its ran out; the next call reports it
+int *seq_error_word();
+void seq_check_error();
+
+// Waits of a kernel's roles on one another.  None is longer than about two seconds: what expires raises `gave_up`, after which every wait of
+// the block returns at once and the block runs to its end on whatever it finds, inside its buffers.
+struct Waits {
+    volatile int *gave_up;
+    int *err;
+    __device__ __forceinline__ void operator()(uint32_t bar, uint32_t parity) const {
+        if (tc::mbar_try_wait(bar, parity)) return;
+        const long long t0 = clock64();
+        while (!tc::mbar_try_wait(bar, parity)) {
+            if (*gave_up) return;
+            if (clock64() - t0 > 4000000000ll) {
+                *gave_up = 1;
+                *(volatile int *)err = 1;
+                __threadfence_system();
+                return;
+            }
+        }
+    }
+    // also when the block has given up: copies in flight are waited for before it ends
+    __device__ __forceinline__ void drain(uint32_t bar, uint32_t parity) const {
+        const long long t0 = clock64();
+        while (!tc::mbar_try_wait(bar, parity) && clock64() - t0 < 4000000000ll) {}
+    }
+};
 
 // log2 of a head's decay: at most 0; -256 makes every power but the zeroth 0 in FP32 and keeps 0 * log a number
 __device__ __forceinline__ float log2_decay(float log_decay) { return fmaxf(fminf(log_decay * 1.4426950408889634f, 0.f), -256.f); }

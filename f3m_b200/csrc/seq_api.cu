@@ -4,6 +4,51 @@
 #include <numeric>
 #include "seq.cuh"
 
+namespace f3m {
+
+int *seq_error_word() {
+    static int *word = [] {   // once per process, possibly while a stream is being captured
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        int *p = nullptr;
+        const cudaError_t e = cudaHostAlloc((void **)&p, 64, cudaHostAllocMapped | cudaHostAllocPortable);
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        F3M_REQUIRE(e == cudaSuccess, F3M_ERR_CUDA, "cudaHostAlloc failed: %s", cudaGetErrorString(e));
+        *p = 0;
+        return p;
+    }();
+    return word;
+}
+void seq_check_error() {
+    volatile int *w = seq_error_word();
+    if (*w) {
+        *w = 0;
+        F3M_REQUIRE(false, F3M_ERR_INTERNAL, "a kernel of an earlier call on sequences gave up waiting: that call's outputs are not valid");
+    }
+}
+
+CUtensorMap seq_tensor_map(int type, const f3m_rows &r, int64_t tokens, int heads, int width) {
+    typedef CUresult (*Encode)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
+                               const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static Encode encode = [] {
+        void *f = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        F3M_CUDA(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &found));
+        F3M_REQUIRE(f && found == cudaDriverEntryPointSuccess, F3M_ERR_CUDA, "the driver has no cuTensorMapEncodeTiled");
+        return (Encode)f;
+    }();
+    CUtensorMap m;
+    const cuuint64_t dims[3] = {(cuuint64_t)width, (cuuint64_t)heads, (cuuint64_t)tokens}, strides[2] = {2ull * r.head_stride, 2ull * r.token_stride};
+    const cuuint32_t box[3] = {64, 1, SEQ_TILE}, step[3] = {1, 1, 1};
+    const CUresult e = encode(&m, type == F3M_TYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, r.data, dims, strides, box, step,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    F3M_REQUIRE(e == CUDA_SUCCESS, F3M_ERR_ARG, "no tensor map for %lld tokens, %d heads, width %d, strides %lld, %lld (driver error %d)", (long long)tokens, heads,
+                width, (long long)r.token_stride, (long long)r.head_stride, (int)e);
+    return m;
+}
+
+}  // namespace f3m
+
 using namespace f3m;
 
 namespace {
@@ -122,6 +167,7 @@ int f3m_window_attention(const f3m_seqs *seqs, int32_t type, int32_t heads, int3
         check_out(out, n, heads, width, "out");
         F3M_REQUIRE(n == 0 || lse, F3M_ERR_ARG, "lse: null pointer");
         if (n == 0) return;
+        seq_check_error();
         WindowArgs a{*seqs, heads, kv_heads, width, window, sinks, scale, q, k, v, out, lse};
         window_forward(type, a, (cudaStream_t)stream);
     });
@@ -143,6 +189,7 @@ int f3m_window_attention_grad(const f3m_seqs *seqs, int32_t type, int32_t heads,
         F3M_REQUIRE(n == 0 || lse, F3M_ERR_ARG, "lse: null pointer");
         check_workspace(workspace, workspace_bytes, grad_workspace(*seqs, heads));
         if (n == 0) return;
+        seq_check_error();
         WindowArgs a{*seqs, heads, kv_heads, width, window, sinks, scale, q, k, v, out, const_cast<float *>(lse), dout, dq, dk, dv, (float *)workspace};
         window_backward(type, a, (cudaStream_t)stream);
     });
@@ -198,6 +245,7 @@ int f3m_decay_attention(const f3m_seqs *seqs, int32_t type, int32_t heads, int32
         F3M_REQUIRE(!state_in || state_in != state_out, F3M_ERR_ARG, "state_in and state_out are the same array");
         check_workspace(workspace, workspace_bytes, decay_workspace(*seqs, heads, width_k, width_v));
         if (seqs->sequences == 0) return;
+        seq_check_error();
         decay_product(type, DecayArgs{*seqs, heads, width_k, width_v, log_decay, scale, 1.f, false, false, q, k, v, out, state_in, state_out, workspace}, (cudaStream_t)stream);
     });
 }
@@ -215,6 +263,7 @@ int f3m_decay_attention_grad(const f3m_seqs *seqs, int32_t type, int32_t heads, 
         F3M_REQUIRE(!dstate_out || dstate_out != dstate_in, F3M_ERR_ARG, "dstate_out and dstate_in are the same array");
         check_workspace(workspace, workspace_bytes, decay_workspace(*seqs, heads, width_k, width_v));
         if (seqs->sequences == 0) return;
+        seq_check_error();
         // dq_i = scale sum_(j <= i) decay^(i-j) (dout_i.v_j) k_j + scale decay^(i+1) S dout_i: the product itself with (dout, v, k), state
         // transposed.  dk and dv come from the adjoint recurrence D_t = scale q_t dout_t^T + decay D_(t+1), dk_t = D_t v_t, dv_t = D_t^T k_t:
         // the product from the end with (v, dout, q) and (k, q, dout).
