@@ -9,10 +9,14 @@ namespace f3m {
 //     O = use * ( upd * (L o A B^T) C + diag(decay^steps) A S )        near pairs one by one, far ones through the state
 //     S = decay^m S + (diag(upd * decay^left) B)^T C                   the state moves on by a tile
 //
-// All five products run on the tensor cores: A B^T and A S as soon as a tile has landed, then, while warps 0-3 turn A B^T into the weights
-// (rounded to 16 bits, written over it in tensor memory), warps 4-7 split the scaled rows of B into a head and a tail of 16 bits each, in place
-// and over A: the state is returned in FP32, and one rounding of its operand would leave it 2^-9 off; head and tail together lose 2^-17.
-// As an operand of A S the state is rounded to 16 bits, like the weights.
+// All products run on the tensor cores.  While warps 0-3 turn A B^T into the weights (rounded to 16 bits, written over it in tensor memory),
+// warps 4-7 split the scaled rows of B into a sum of 16-bit parts, in place, over A, and over the state's operand: the state is kept and returned
+// in FP32, and one rounding of what is added to it would leave it 2^-9 off in bf16.  Two parts lose 2^-17 (bf16) or 2^-23 (fp16); a state that is
+// returned takes a third in bf16, one that only serves the tiles behind it does not.  As an operand of A S the state is rounded to 16
+// bits, like the weights.
+//
+// What bounds it: tile by tile, the state's way round -- parts written, their products, the state read, rounded and scaled, A S, parts of the next
+// tile.  A B^T, the weights, their product and the outputs run beside it, and so do the copies of the next tile.
 //
 // A range that does not begin with a sequence needs the state that the ranges before it leave: decay_tiles<true> computes what each range
 // adds to the state (B and C only), decay_join runs over the ranges, and decay_tiles<false> starts from that.  B and C are then read
@@ -24,6 +28,7 @@ struct DecayKernel {
     DecayArgs a;
     CUtensorMap ma, mb, mc;
     int ranges, per_range;      // per_range tiles each
+    int parts;                  // of a row of B, 2 or 3
     float *carry;               // (ranges, heads, width of b, width of c): the state behind each range
     int *err;
 };
@@ -40,17 +45,21 @@ __device__ __forceinline__ int tiles_before(const DecayArgs &a, const int4 &e) {
     return a.reversed ? n - 1 - i : i;
 }
 
+__device__ __forceinline__ void sts16(uint32_t at, const uint32_t (&w)[4]) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+}
+
 template <typename T, bool STATES>
 __global__ void __launch_bounds__(DK_THREADS, 1) decay_tiles(const __grid_constant__ DecayKernel p) {
     extern __shared__ unsigned char raw[];
-    __shared__ __align__(8) uint64_t bars[2 * 4 + 6];
+    __shared__ __align__(8) uint64_t bars[2 * 4 + 8];
     __shared__ uint32_t tmem_s;
     __shared__ int gave_up_s;
     __shared__ __align__(16) float pw[32], pr[32];   // decay^n, decay^(31 - n)
     const DecayArgs &a = p.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, h = blockIdx.y;
     const int nb = (a.width_b + 63) / 64, nc = (a.width_c + 63) / 64;
-    const int stage_blocks = 2 * nb + nc, stages = min(4, (DK_TILES - nc) / stage_blocks);
+    const int stage_blocks = 2 * nb + nc, stages = min(4, (DK_TILES - max(nb, nc)) / stage_blocks);
     const uint32_t smem = (tc::smem_u32(raw) + 1023) & ~1023u, state_s = smem + stages * stage_blocks * DK_BLOCK;
     const float l2 = log2_decay(a.log_decay[h]);
 
@@ -66,12 +75,14 @@ __global__ void __launch_bounds__(DK_THREADS, 1) decay_tiles(const __grid_consta
     if (warp == 8) tc::tmem_alloc(tc::smem_u32(&tmem_s), 512);
     if (tid == 0) {
         for (int i = 0; i < 8; i++) tc::mbar_init(tc::smem_u32(&bars[i]), 1);          // landed, free again (by stage)
-        tc::mbar_init(tc::smem_u32(&bars[8]), 1);                                      // A B^T and A S done
-        tc::mbar_init(tc::smem_u32(&bars[9]), 128);                                    // weights written
-        tc::mbar_init(tc::smem_u32(&bars[10]), 128);                                   // B split
-        tc::mbar_init(tc::smem_u32(&bars[11]), 128);                                   // state ready as operand and in tensor memory
-        tc::mbar_init(tc::smem_u32(&bars[12]), 1);                                     // outputs and state done
-        tc::mbar_init(tc::smem_u32(&bars[13]), 128);                                   // outputs read
+        tc::mbar_init(tc::smem_u32(&bars[8]), 1);                                      // A B^T done
+        tc::mbar_init(tc::smem_u32(&bars[9]), 1);                                      // A S done
+        tc::mbar_init(tc::smem_u32(&bars[10]), 1);                                     // state done
+        tc::mbar_init(tc::smem_u32(&bars[11]), 1);                                     // outputs done
+        tc::mbar_init(tc::smem_u32(&bars[12]), 128);                                   // weights written
+        tc::mbar_init(tc::smem_u32(&bars[13]), 128);                                   // B split
+        tc::mbar_init(tc::smem_u32(&bars[14]), 128);                                   // state ready as operand and in tensor memory
+        tc::mbar_init(tc::smem_u32(&bars[15]), 128);                                   // outputs read
         tc::fence_mbar_init();
         gave_up_s = 0;
     }
@@ -84,8 +95,9 @@ __global__ void __launch_bounds__(DK_THREADS, 1) decay_tiles(const __grid_consta
     tc::fence_after_sync();
     const Waits wait{&gave_up_s, p.err};
     const uint32_t tmem = tmem_s, t_score = tmem, t_inter = tmem + 128, t_intra = tmem + 256, t_state = tmem + 384;
-    const uint32_t b_full = tc::smem_u32(&bars[0]), b_free = tc::smem_u32(&bars[4]), b_score = tc::smem_u32(&bars[8]), b_weights = tc::smem_u32(&bars[9]),
-                   b_split = tc::smem_u32(&bars[10]), b_state = tc::smem_u32(&bars[11]), b_done = tc::smem_u32(&bars[12]), b_read = tc::smem_u32(&bars[13]);
+    const uint32_t b_full = tc::smem_u32(&bars[0]), b_free = tc::smem_u32(&bars[4]), b_score = tc::smem_u32(&bars[8]), b_inter = tc::smem_u32(&bars[9]),
+                   b_moved = tc::smem_u32(&bars[10]), b_done = tc::smem_u32(&bars[11]), b_weights = tc::smem_u32(&bars[12]), b_split = tc::smem_u32(&bars[13]),
+                   b_state = tc::smem_u32(&bars[14]), b_read = tc::smem_u32(&bars[15]);
     auto a_tile = [&](int s) { return smem + s * stage_blocks * DK_BLOCK; };
     auto b_tile = [&](int s) { return a_tile(s) + nb * DK_BLOCK; };
     auto c_tile = [&](int s) { return a_tile(s) + 2 * nb * DK_BLOCK; };
@@ -126,27 +138,30 @@ __global__ void __launch_bounds__(DK_THREADS, 1) decay_tiles(const __grid_consta
                 if (!STATES) {
                     for (int k = 0; k < 4 * nb; k++)
                         tc::mma_f16(t_score, tc::desc_k(a_tile(s) + (k >> 2) * DK_BLOCK + (k & 3) * 32), tc::desc_k(b_tile(s) + (k >> 2) * DK_BLOCK + (k & 3) * 32), i_score, k > 0);
+                    tc::mma_commit(b_score);
                     if (n) wait(b_read, (n - 1) & 1);
-                }
-                wait(b_state, n & 1);
-                tc::fence_after_sync();
-                if (!STATES) {
+                    wait(b_state, n & 1);
+                    tc::fence_after_sync();
                     for (int k = 0; k < 4 * nb; k++)
                         tc::mma_f16(t_inter, tc::desc_k(a_tile(s) + (k >> 2) * DK_BLOCK + (k & 3) * 32), tc::desc_mn(state_s + k * 2048, DK_BLOCK), i_rows, k > 0);
-                    tc::mma_commit(b_score);
-                    wait(b_split, n & 1);      // also clears the rows of C that belong to another sequence
+                    tc::mma_commit(b_inter);
+                } else {
+                    wait(b_state, n & 1);
+                }
+                wait(b_split, n & 1);   // also clears the rows of C that belong to another sequence
+                tc::fence_after_sync();
+                for (int part = 0; part < p.parts; part++) {
+                    const uint32_t rows = part == 0 ? b_tile(s) : part == 1 ? a_tile(s) : state_s;
+                    for (int k = 0; k < 8; k++) tc::mma_f16(t_state, tc::desc_mn(rows + k * 2048, DK_BLOCK), tc::desc_mn(c_tile(s) + k * 2048, DK_BLOCK), i_state, 1);
+                }
+                tc::mma_commit(b_moved);
+                if (!STATES) {
                     wait(b_weights, n & 1);
                     tc::fence_after_sync();
                     for (int k = 0; k < 8; k++) tc::mma_f16_ta(t_intra, t_score + 8 * k, tc::desc_mn(c_tile(s) + k * 2048, DK_BLOCK), i_rows, k > 0);
-                } else {
-                    wait(b_split, n & 1);
-                    tc::fence_after_sync();
+                    tc::mma_commit(b_done);
                 }
-                for (int half = 0; half < 2; half++)
-                    for (int k = 0; k < 8; k++)
-                        tc::mma_f16(t_state, tc::desc_mn((half ? a_tile(s) : b_tile(s)) + k * 2048, DK_BLOCK), tc::desc_mn(c_tile(s) + k * 2048, DK_BLOCK), i_state, 1);
                 tc::mma_commit(b_free + 8 * s);
-                tc::mma_commit(b_done);
             }
         }
     } else if (warp < 4 && !STATES) {
@@ -159,7 +174,7 @@ __global__ void __launch_bounds__(DK_THREADS, 1) decay_tiles(const __grid_consta
             all_wait(b_score, n & 1);
             tc::fence_after_sync();
             const float coef = a.use * a.upd;
-#pragma unroll
+#pragma unroll 1
             for (int cb = 0; cb < 4; cb++) {
                 uint32_t w[16];
                 const bool near = a.reversed ? cb >= warp : cb <= warp;   // warp-uniform
@@ -203,9 +218,8 @@ __global__ void __launch_bounds__(DK_THREADS, 1) decay_tiles(const __grid_consta
             tc::fence_after_sync();
             const float f = a.use * exp2f(l2 * (a.reversed ? m - 1 - i : i + 1));
             T *out = reinterpret_cast<T *>(a.out.data) + (int64_t)(e.x + e.z + i) * a.out.token_stride + (int64_t)h * a.out.head_stride;
-#pragma unroll
-            for (int cb = 0; cb < 4; cb++) {
-                if (cb >= 2 * nc) break;
+#pragma unroll 1
+            for (int cb = 0; cb < 2 * nc; cb++) {
                 uint32_t x[32], y[32];
                 tc::tmem_ld32(t_inter + lanes + 32 * cb, x);
                 tc::tmem_ld32(t_intra + lanes + 32 * cb, y);
@@ -245,9 +259,8 @@ __global__ void __launch_bounds__(DK_THREADS, 1) decay_tiles(const __grid_consta
                 src = p.carry + ((int64_t)(blockIdx.x - 1) * a.heads + h) * plane;
             }
             const bool fresh = begins || n == 0;
-#pragma unroll
-            for (int cb = 0; cb < 4; cb++) {
-                if (cb >= 2 * nc) break;
+#pragma unroll 1
+            for (int cb = 0; cb < 2 * nc; cb++) {
                 uint32_t r[32];
                 if (!fresh) {
                     tc::tmem_ld32(t_state + lanes + 32 * cb, r);
@@ -277,7 +290,7 @@ __global__ void __launch_bounds__(DK_THREADS, 1) decay_tiles(const __grid_consta
                         uint32_t w[4];
 #pragma unroll
                         for (int q = 0; q < 4; q++) w[q] = Half<T>::pack(__uint_as_float(r[c + 2 * q]), __uint_as_float(r[c + 2 * q + 1]));
-                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row + tc::swz(j, 4 * (cb & 1) + c / 8)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+                        sts16(row + tc::swz(j, 4 * (cb & 1) + c / 8), w);
                     }
                 }
 #pragma unroll
@@ -292,9 +305,8 @@ __global__ void __launch_bounds__(DK_THREADS, 1) decay_tiles(const __grid_consta
         };
         auto state_to = [&](float *dst, bool turned) {
             if (32 * (warp - 4) >= a.width_b) return;   // the whole warp
-#pragma unroll
-            for (int cb = 0; cb < 4; cb++) {
-                if (cb >= 2 * nc) break;
+#pragma unroll 1
+            for (int cb = 0; cb < 2 * nc; cb++) {
                 uint32_t r[32];
                 tc::tmem_ld32(t_state + lanes + 32 * cb, r);
                 tc::tmem_ld_wait(r);
@@ -311,44 +323,51 @@ __global__ void __launch_bounds__(DK_THREADS, 1) decay_tiles(const __grid_consta
                 __syncwarp();
             }
         };
-        state_before(0);
         for (int n = 0; n < tiles; n++) {
+            state_before(n);
             const int4 e = tile_at(a, first + n);
             const int m = tile_rows(e), s = n % stages;
             all_wait(b_full + 8 * s, (n / stages) & 1);
-            if (!STATES) all_wait(b_score, n & 1);   // A and B have been read
+            if (!STATES) all_wait(b_inter, n & 1);   // A, B and the state's operand have been read
             const float f = a.upd * exp2f(l2 * (a.reversed ? j + 1 : m - 1 - j));
+#pragma unroll 1
             for (int k = 0; k < nb; k++) {
-                const uint32_t head = b_tile(s) + k * DK_BLOCK, tail = a_tile(s) + k * DK_BLOCK;
-#pragma unroll
+                const uint32_t head = b_tile(s) + k * DK_BLOCK, tail = a_tile(s) + k * DK_BLOCK, rest = state_s + k * DK_BLOCK;
+#pragma unroll 4
                 for (int c = 0; c < 8; c++) {
-                    uint32_t v[4], w[4];
+                    uint32_t v[4], w[4], z[4];
                     asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(head + tc::swz(j, c)) : "memory");
 #pragma unroll
                     for (int q = 0; q < 4; q++) {
                         float2 x = Half<T>::unpack(v[q]);
-                        x.x *= f; x.y *= f;
-                        v[q] = j < m ? Half<T>::pack(x.x, x.y) : 0u;
-                        const float2 y = Half<T>::unpack(v[q]);
-                        w[q] = j < m ? Half<T>::pack(x.x - y.x, x.y - y.y) : 0u;
+                        x.x = j < m ? x.x * f : 0.f;
+                        x.y = j < m ? x.y * f : 0.f;
+                        v[q] = Half<T>::pack(x.x, x.y);
+                        float2 y = Half<T>::unpack(v[q]);
+                        x.x -= y.x; x.y -= y.y;
+                        w[q] = Half<T>::pack(x.x, x.y);
+                        y = Half<T>::unpack(w[q]);
+                        z[q] = Half<T>::pack(x.x - y.x, x.y - y.y);
                     }
-                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(head + tc::swz(j, c)), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
-                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(tail + tc::swz(j, c)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+                    sts16(head + tc::swz(j, c), v);
+                    sts16(tail + tc::swz(j, c), w);
+                    if (p.parts == 3) sts16(rest + tc::swz(j, c), z);
                 }
             }
-            if (j >= m)   // tokens of the next sequence: nothing of theirs may meet a weight, not even a weight of zero
+            if (j >= m) {   // tokens of the next sequence: nothing of theirs may meet a weight, not even a weight of zero
+                const uint32_t zero[4] = {0u, 0u, 0u, 0u};
                 for (int k = 0; k < nc; k++)
-#pragma unroll
-                    for (int c = 0; c < 8; c++)
-                        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(c_tile(s) + k * DK_BLOCK + tc::swz(j, c)), "r"(0) : "memory");
+                    for (int c = 0; c < 8; c++) sts16(c_tile(s) + k * DK_BLOCK + tc::swz(j, c), zero);
+            }
             tc::fence_async_smem();
             tc::mbar_arrive(b_split);
-            all_wait(b_done, n & 1);
+            all_wait(b_moved, n & 1);
             tc::fence_after_sync();
-            if (!STATES && a.state_out && tile_ends(a, e)) state_to(a.state_out + ((int64_t)e.w * a.heads + h) * plane, a.transposed);
-            if (n + 1 < tiles) state_before(n + 1);
+            float *dst = nullptr;
+            if (STATES) dst = n + 1 == tiles ? p.carry + ((int64_t)blockIdx.x * a.heads + h) * plane : nullptr;
+            else if (a.state_out && tile_ends(a, e)) dst = a.state_out + ((int64_t)e.w * a.heads + h) * plane;
+            if (dst) state_to(dst, !STATES && a.transposed);
         }
-        if (STATES) state_to(p.carry + ((int64_t)blockIdx.x * a.heads + h) * plane, false);
     }
     __syncwarp();
     tc::fence_before_sync();
@@ -419,6 +438,7 @@ static void decay_product_t(const DecayArgs &a, cudaStream_t s) {
     p.ranges = decay_ranges(a.s, a.heads);
     p.per_range = (a.s.tiles + p.ranges - 1) / p.ranges;
     p.ranges = (a.s.tiles + p.per_range - 1) / p.per_range;
+    p.parts = Half<T>::type == F3M_TYPE_BF16 && a.state_out ? 3 : 2;
     p.carry = (float *)a.ws;
     p.err = seq_error_word();
     constexpr int bytes = DK_TILES * DK_BLOCK + 1024;
