@@ -1,7 +1,14 @@
 // Linear attention with a decay for each head: the recurrence over packed sequences, and one new token.
+#include "packed.cuh"
 #include "seq.cuh"
 
 namespace f3m {
+
+__device__ __forceinline__ float2 unpack2(f32x2 v) {
+    float2 r;
+    unpack2(v, r.x, r.y);
+    return r;
+}
 
 // A head's sequences, laid end to end in tiles of 128 tokens, are cut into ranges of equally many tiles; a CTA takes one range and carries the
 // state S (width of b x width of c, FP32, in tensor memory) through it.  For a tile of m tokens, with L the triangle of powers of the decay:
@@ -10,7 +17,7 @@ namespace f3m {
 //     S = decay^m S + (diag(upd * decay^left) B)^T C                   the state moves on by a tile
 //
 // All products run on the tensor cores.  While warps 0-3 turn A B^T into the weights (rounded to 16 bits, written over it in tensor memory),
-// warps 4-7 split the scaled rows of B into a sum of 16-bit parts, in place, over A, and over the state's operand: the state is kept and returned
+// warps 4-11 split the scaled rows of B into a sum of 16-bit parts, in place, over A, and over the state's operand: the state is kept and returned
 // in FP32, and one rounding of what is added to it would leave it 2^-9 off in bf16.  Two parts lose 2^-17 (bf16) or 2^-23 (fp16); a state that is
 // returned takes a third in bf16, one that only serves the tiles behind it does not.  As an operand of A S the state is rounded to 16
 // bits, like the weights.
@@ -18,17 +25,18 @@ namespace f3m {
 // What bounds it: tile by tile, the state's way round -- parts written, their products, the state read, rounded and scaled, A S, parts of the next
 // tile.  A B^T, the weights, their product and the outputs run beside it, and so do the copies of the next tile.
 //
-// A range that does not begin with a sequence needs the state that the ranges before it leave: decay_tiles<true> computes what each range
-// adds to the state (B and C only), decay_join runs over the ranges, and decay_tiles<false> starts from that.  B and C are then read
+// A range that does not begin with a sequence needs the state that the ranges before it leave: decay_states computes what each range
+// adds to the state (B and C only), decay_join runs over the ranges, and decay_tiles starts from that.  B and C are then read
 // twice, which is the price of using all SMs when there are fewer heads than SMs.
-constexpr int DK_THREADS = 320, DK_BLOCK = SEQ_TILE * 128;   // bytes of a block of 64 columns
+constexpr int DK_COPY = 12, DK_PRODUCTS = 13, DK_THREADS = 32 * 14;   // warps: 0-3 weights and outputs, 4-11 operands, copies, products
+constexpr int DS_THREADS = 32 * 10;                                   // decay_states: 0-7 operands, copies, products
+constexpr int DK_BLOCK = SEQ_TILE * 128;                     // bytes of a block of 64 columns
 constexpr int DK_TILES = 14;                                 // blocks of 64 columns in shared memory: the tiles of all stages and the state
 
 struct DecayKernel {
     DecayArgs a;
-    CUtensorMap ma, mb, mc;
+    CUtensorMap ma, mb, mc, mo;
     int ranges, per_range;      // per_range tiles each
-    int parts;                  // of a row of B, 2 or 3
     float *carry;               // (ranges, heads, width of b, width of c): the state behind each range
     int *err;
 };
@@ -45,11 +53,59 @@ __device__ __forceinline__ int tiles_before(const DecayArgs &a, const int4 &e) {
     return a.reversed ? n - 1 - i : i;
 }
 
+// 32 columns of row j of a state, from column c0 on
+__device__ __forceinline__ void state_row(const uint32_t (&r)[32], float *dst, bool transposed, int wb, int wc, int j, int c0) {
+    if (transposed) {
+#pragma unroll
+        for (int c = 0; c < 32; c++)
+            if (j < wb && c0 + c < wc) dst[(int64_t)(c0 + c) * wb + j] = __uint_as_float(r[c]);
+    } else {
+#pragma unroll
+        for (int c = 0; c < 32; c += 4)
+            if (j < wb && c0 + c < wc) *reinterpret_cast<uint4 *>(dst + (int64_t)j * wc + c0 + c) = make_uint4(r[c], r[c + 1], r[c + 2], r[c + 3]);
+    }
+}
 __device__ __forceinline__ void sts16(uint32_t at, const uint32_t (&w)[4]) {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
 }
 
-template <typename T, bool STATES>
+// Row j of a tile of B, times f, as a sum of 16-bit parts: 16-byte chunks [c0, c1) of its blocks; the first part stays in place.  j >= rows: zeros.
+template <typename T, int PARTS>
+__device__ __forceinline__ void split_rows(uint32_t head, uint32_t tail, uint32_t rest, int j, bool in, f32x2 f, int c0, int c1) {
+    const f32x2 minus = pack2(-1.f, -1.f);
+#pragma unroll 2
+    for (int i = c0; i < c1; i++) {
+        const uint32_t at = (i >> 3) * DK_BLOCK + tc::swz(j, i & 7);
+        uint32_t v[4], w[4], z[4];
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(head + at) : "memory");
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            const float2 u = Half<T>::unpack(in ? v[q] : 0u);
+            f32x2 x = mul2(pack2(u.x, u.y), f);
+            float2 y = unpack2(x);
+            v[q] = Half<T>::pack(y.x, y.y);
+            y = Half<T>::unpack(v[q]);
+            x = fma2(pack2(y.x, y.y), minus, x);
+            y = unpack2(x);
+            w[q] = Half<T>::pack(y.x, y.y);
+            if (PARTS == 3) {
+                y = Half<T>::unpack(w[q]);
+                y = unpack2(fma2(pack2(y.x, y.y), minus, x));
+                z[q] = Half<T>::pack(y.x, y.y);
+            }
+        }
+        sts16(head + at, v);
+        sts16(tail + at, w);
+        if (PARTS == 3) sts16(rest + at, z);
+    }
+}
+// Chunks [c0, c1) of row j of a tile become zero: tokens of the next sequence meet no weight, not even a weight of zero
+__device__ __forceinline__ void clear_row(uint32_t tile, int j, int c0, int c1) {
+    const uint32_t zero[4] = {0u, 0u, 0u, 0u};
+    for (int i = c0; i < c1; i++) sts16(tile + (i >> 3) * DK_BLOCK + tc::swz(j, i & 7), zero);
+}
+
+template <typename T, int PARTS>
 __global__ void __launch_bounds__(DK_THREADS, 1) decay_tiles(const __grid_constant__ DecayKernel p) {
     extern __shared__ unsigned char raw[];
     __shared__ __align__(8) uint64_t bars[2 * 4 + 8];
@@ -62,26 +118,21 @@ __global__ void __launch_bounds__(DK_THREADS, 1) decay_tiles(const __grid_consta
     const int stage_blocks = 2 * nb + nc, stages = min(4, (DK_TILES - max(nb, nc)) / stage_blocks);
     const uint32_t smem = (tc::smem_u32(raw) + 1023) & ~1023u, state_s = smem + stages * stage_blocks * DK_BLOCK;
     const float l2 = log2_decay(a.log_decay[h]);
+    const int first = blockIdx.x * p.per_range, tiles = min(a.s.tiles, first + p.per_range) - first;
 
-    int first = blockIdx.x * p.per_range;
-    const int last = min(a.s.tiles, first + p.per_range);
-    if (STATES) {   // only the sequence that runs on into the next range
-        const int4 e = tile_at(a, last - 1);
-        first = tile_ends(a, e) ? last : max(first, last - 1 - tiles_before(a, e));
-        if (first >= last) return;
-    }
-    const int tiles = last - first;
-
-    if (warp == 8) tc::tmem_alloc(tc::smem_u32(&tmem_s), 512);
+    if (warp == DK_COPY) tc::tmem_alloc(tc::smem_u32(&tmem_s), 512);
     if (tid == 0) {
-        for (int i = 0; i < 8; i++) tc::mbar_init(tc::smem_u32(&bars[i]), 1);          // landed, free again (by stage)
+        for (int i = 0; i < 4; i++) {
+            tc::mbar_init(tc::smem_u32(&bars[i]), 1);                                  // landed (by stage)
+            tc::mbar_init(tc::smem_u32(&bars[4 + i]), 2);                              // free again: products done, outputs on their way
+        }
         tc::mbar_init(tc::smem_u32(&bars[8]), 1);                                      // A B^T done
         tc::mbar_init(tc::smem_u32(&bars[9]), 1);                                      // A S done
         tc::mbar_init(tc::smem_u32(&bars[10]), 1);                                     // state done
         tc::mbar_init(tc::smem_u32(&bars[11]), 1);                                     // outputs done
         tc::mbar_init(tc::smem_u32(&bars[12]), 128);                                   // weights written
-        tc::mbar_init(tc::smem_u32(&bars[13]), 128);                                   // B split
-        tc::mbar_init(tc::smem_u32(&bars[14]), 128);                                   // state ready as operand and in tensor memory
+        tc::mbar_init(tc::smem_u32(&bars[13]), 256);                                   // B split
+        tc::mbar_init(tc::smem_u32(&bars[14]), 256);                                   // state ready as operand and in tensor memory
         tc::mbar_init(tc::smem_u32(&bars[15]), 128);                                   // outputs read
         tc::fence_mbar_init();
         gave_up_s = 0;
@@ -101,23 +152,23 @@ __global__ void __launch_bounds__(DK_THREADS, 1) decay_tiles(const __grid_consta
     auto a_tile = [&](int s) { return smem + s * stage_blocks * DK_BLOCK; };
     auto b_tile = [&](int s) { return a_tile(s) + nb * DK_BLOCK; };
     auto c_tile = [&](int s) { return a_tile(s) + 2 * nb * DK_BLOCK; };
-
     auto all_wait = [&](uint32_t bar, uint32_t parity) {   // a whole warp, which stays together for the instructions that need that
         wait(bar, parity);
         __syncwarp();
     };
-    if (warp == 8) {
+
+    if (warp == DK_COPY) {
         // ---- copies ----
         if (lane == 0) {
             int n = 0;
             for (; n < tiles && !gave_up_s; n++) {
                 const int s = n % stages;
+                const int4 e = tile_at(a, first + n);
                 if (n >= stages) wait(b_free + 8 * s, (n / stages - 1) & 1);
                 if (gave_up_s) break;
-                const int4 e = tile_at(a, first + n);
-                tc::mbar_expect_tx(b_full + 8 * s, (STATES ? nb + nc : stage_blocks) * DK_BLOCK);
+                tc::mbar_expect_tx(b_full + 8 * s, stage_blocks * DK_BLOCK);
                 for (int k = 0; k < nb; k++) {
-                    if (!STATES) tc::tma_rows(a_tile(s) + k * DK_BLOCK, &p.ma, 64 * k, h, e.x + e.z, b_full + 8 * s);
+                    tc::tma_rows(a_tile(s) + k * DK_BLOCK, &p.ma, 64 * k, h, e.x + e.z, b_full + 8 * s);
                     tc::tma_rows(b_tile(s) + k * DK_BLOCK, &p.mb, 64 * k, h, e.x + e.z, b_full + 8 * s);
                 }
                 for (int k = 0; k < nc; k++) tc::tma_rows(c_tile(s) + k * DK_BLOCK, &p.mc, 64 * k, h, e.x + e.z, b_full + 8 * s);
@@ -125,7 +176,7 @@ __global__ void __launch_bounds__(DK_THREADS, 1) decay_tiles(const __grid_consta
             for (int s = 0; s < stages; s++)   // the last copy into each stage
                 if (n > s) wait.drain(b_full + 8 * s, ((n - 1 - s) / stages) & 1);
         }
-    } else if (warp == 9) {
+    } else if (warp == DK_PRODUCTS) {
         // ---- products ----
         if (lane == 0) {
             constexpr bool bf = Half<T>::type == F3M_TYPE_BF16;
@@ -135,45 +186,39 @@ __global__ void __launch_bounds__(DK_THREADS, 1) decay_tiles(const __grid_consta
                 const int s = n % stages;
                 wait(b_full + 8 * s, (n / stages) & 1);
                 tc::fence_after_sync();
-                if (!STATES) {
-                    for (int k = 0; k < 4 * nb; k++)
-                        tc::mma_f16(t_score, tc::desc_k(a_tile(s) + (k >> 2) * DK_BLOCK + (k & 3) * 32), tc::desc_k(b_tile(s) + (k >> 2) * DK_BLOCK + (k & 3) * 32), i_score, k > 0);
-                    tc::mma_commit(b_score);
-                    if (n) wait(b_read, (n - 1) & 1);
-                    wait(b_state, n & 1);
-                    tc::fence_after_sync();
-                    for (int k = 0; k < 4 * nb; k++)
-                        tc::mma_f16(t_inter, tc::desc_k(a_tile(s) + (k >> 2) * DK_BLOCK + (k & 3) * 32), tc::desc_mn(state_s + k * 2048, DK_BLOCK), i_rows, k > 0);
-                    tc::mma_commit(b_inter);
-                } else {
-                    wait(b_state, n & 1);
-                }
+                for (int k = 0; k < 4 * nb; k++)
+                    tc::mma_f16(t_score, tc::desc_k(a_tile(s) + (k >> 2) * DK_BLOCK + (k & 3) * 32), tc::desc_k(b_tile(s) + (k >> 2) * DK_BLOCK + (k & 3) * 32), i_score, k > 0);
+                tc::mma_commit(b_score);
+                if (n) wait(b_read, (n - 1) & 1);
+                wait(b_state, n & 1);
+                tc::fence_after_sync();
+                for (int k = 0; k < 4 * nb; k++)
+                    tc::mma_f16(t_inter, tc::desc_k(a_tile(s) + (k >> 2) * DK_BLOCK + (k & 3) * 32), tc::desc_mn(state_s + k * 2048, DK_BLOCK), i_rows, k > 0);
+                tc::mma_commit(b_inter);
                 wait(b_split, n & 1);   // also clears the rows of C that belong to another sequence
                 tc::fence_after_sync();
-                for (int part = 0; part < p.parts; part++) {
+                for (int part = 0; part < PARTS; part++) {
                     const uint32_t rows = part == 0 ? b_tile(s) : part == 1 ? a_tile(s) : state_s;
                     for (int k = 0; k < 8; k++) tc::mma_f16(t_state, tc::desc_mn(rows + k * 2048, DK_BLOCK), tc::desc_mn(c_tile(s) + k * 2048, DK_BLOCK), i_state, 1);
                 }
                 tc::mma_commit(b_moved);
-                if (!STATES) {
-                    wait(b_weights, n & 1);
-                    tc::fence_after_sync();
-                    for (int k = 0; k < 8; k++) tc::mma_f16_ta(t_intra, t_score + 8 * k, tc::desc_mn(c_tile(s) + k * 2048, DK_BLOCK), i_rows, k > 0);
-                    tc::mma_commit(b_done);
-                }
+                wait(b_weights, n & 1);
+                tc::fence_after_sync();
+                for (int k = 0; k < 8; k++) tc::mma_f16_ta(t_intra, t_score + 8 * k, tc::desc_mn(c_tile(s) + k * 2048, DK_BLOCK), i_rows, k > 0);
+                tc::mma_commit(b_done);
                 tc::mma_commit(b_free + 8 * s);
             }
         }
-    } else if (warp < 4 && !STATES) {
+    } else if (warp < 4) {
         // ---- weights and outputs: thread i has row i ----
         const int i = tid;
         const uint32_t lanes = (uint32_t)(32 * warp) << 16;
+        const float coef = a.use * a.upd;
         for (int n = 0; n < tiles; n++) {
             const int4 e = tile_at(a, first + n);
-            const int m = tile_rows(e);
+            const int m = tile_rows(e), s = n % stages;
             all_wait(b_score, n & 1);
             tc::fence_after_sync();
-            const float coef = a.use * a.upd;
 #pragma unroll 1
             for (int cb = 0; cb < 4; cb++) {
                 uint32_t w[16];
@@ -216,8 +261,8 @@ __global__ void __launch_bounds__(DK_THREADS, 1) decay_tiles(const __grid_consta
 
             all_wait(b_done, n & 1);
             tc::fence_after_sync();
+            // the outputs go over C, which has been read, and leave from there
             const float f = a.use * exp2f(l2 * (a.reversed ? m - 1 - i : i + 1));
-            T *out = reinterpret_cast<T *>(a.out.data) + (int64_t)(e.x + e.z + i) * a.out.token_stride + (int64_t)h * a.out.head_stride;
 #pragma unroll 1
             for (int cb = 0; cb < 2 * nc; cb++) {
                 uint32_t x[32], y[32];
@@ -225,10 +270,6 @@ __global__ void __launch_bounds__(DK_THREADS, 1) decay_tiles(const __grid_consta
                 tc::tmem_ld32(t_intra + lanes + 32 * cb, y);
                 tc::tmem_ld_wait(x);
                 tc::tmem_ld_wait(y);
-                if (cb == 2 * nc - 1) {
-                    tc::fence_before_sync();
-                    tc::mbar_arrive(b_read);
-                }
 #pragma unroll
                 for (int c = 0; c < 32; c += 8) {
                     uint32_t w[4];
@@ -236,31 +277,36 @@ __global__ void __launch_bounds__(DK_THREADS, 1) decay_tiles(const __grid_consta
                     for (int q = 0; q < 4; q++)
                         w[q] = Half<T>::pack(fmaf(f, __uint_as_float(x[c + 2 * q]), __uint_as_float(y[c + 2 * q])),
                                              fmaf(f, __uint_as_float(x[c + 2 * q + 1]), __uint_as_float(y[c + 2 * q + 1])));
-                    if (i < m && 32 * cb + c < a.width_c) *reinterpret_cast<uint4 *>(out + 32 * cb + c) = make_uint4(w[0], w[1], w[2], w[3]);
+                    sts16(c_tile(s) + (cb >> 1) * DK_BLOCK + tc::swz(i, 4 * (cb & 1) + c / 8), w);
                 }
-                __syncwarp();
             }
+            tc::fence_before_sync();
+            tc::mbar_arrive(b_read);
+            store_rows<128>(p.mo, a.out, c_tile(s), h, e.x + e.z, m, nc, a.width_c, i, 1);
+            if (i == 0) tc::mbar_arrive(b_free + 8 * s);
         }
-    } else if (warp >= 4 && warp < 8) {
-        // ---- operands: thread j has row j of B and C, and row j of the state ----
-        const int j = tid - 128;
-        const uint32_t lanes = (uint32_t)(32 * (warp - 4)) << 16;
+        if (i == 0) tc::tma_store_wait_all();
+    } else if (warp < DK_COPY) {
+        // ---- operands: threads j and j + 128 have row j of B and C, and row j of the state, half each ----
+        const int j = tid & 127, half = (tid - 128) >> 7;
+        const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
         const int64_t plane = (int64_t)a.width_b * a.width_c;
-        // the state before tile n: from tensor memory, or where a sequence or the range begins
-        auto state_before = [&](int n) {
-            const int4 e = tile_at(a, first + n);
-            const bool begins = tile_begins(a, e);
-            const float scale = exp2f(l2 * tile_rows(e));
+        int4 e = tile_at(a, first);
+        for (int n = 0; n < tiles; n++) {
+            const int m = tile_rows(e), s = n % stages;
+            const int4 ahead = n + 1 < tiles ? tile_at(a, first + n + 1) : e;
+            // the state before the tile: from tensor memory, or where a sequence or the range begins
+            const bool begins = tile_begins(a, e), fresh = begins || n == 0;
+            const float scale = exp2f(l2 * m);
             const float *src = nullptr;
-            bool turned = false;
             if (begins) {
-                if (a.state_in) { src = a.state_in + ((int64_t)e.w * a.heads + h) * plane; turned = a.transposed; }
-            } else if (n == 0 && !STATES) {
+                if (a.state_in) src = a.state_in + ((int64_t)e.w * a.heads + h) * plane;
+            } else if (n == 0) {
                 src = p.carry + ((int64_t)(blockIdx.x - 1) * a.heads + h) * plane;
             }
-            const bool fresh = begins || n == 0;
+            const bool turned = begins && a.transposed;
 #pragma unroll 1
-            for (int cb = 0; cb < 2 * nc; cb++) {
+            for (int cb = half * nc; cb < (half + 1) * nc; cb++) {
                 uint32_t r[32];
                 if (!fresh) {
                     tc::tmem_ld32(t_state + lanes + 32 * cb, r);
@@ -283,15 +329,13 @@ __global__ void __launch_bounds__(DK_THREADS, 1) decay_tiles(const __grid_consta
                         }
                     }
                 }
-                if (!STATES) {
-                    const uint32_t row = state_s + (cb >> 1) * DK_BLOCK;
+                const uint32_t row = state_s + (cb >> 1) * DK_BLOCK;
 #pragma unroll
-                    for (int c = 0; c < 32; c += 8) {
-                        uint32_t w[4];
+                for (int c = 0; c < 32; c += 8) {
+                    uint32_t w[4];
 #pragma unroll
-                        for (int q = 0; q < 4; q++) w[q] = Half<T>::pack(__uint_as_float(r[c + 2 * q]), __uint_as_float(r[c + 2 * q + 1]));
-                        sts16(row + tc::swz(j, 4 * (cb & 1) + c / 8), w);
-                    }
+                    for (int q = 0; q < 4; q++) w[q] = Half<T>::pack(__uint_as_float(r[c + 2 * q]), __uint_as_float(r[c + 2 * q + 1]));
+                    sts16(row + tc::swz(j, 4 * (cb & 1) + c / 8), w);
                 }
 #pragma unroll
                 for (int c = 0; c < 32; c++) r[c] = __float_as_uint(scale * __uint_as_float(r[c]));
@@ -302,77 +346,151 @@ __global__ void __launch_bounds__(DK_THREADS, 1) decay_tiles(const __grid_consta
             tc::fence_async_smem();
             tc::fence_before_sync();
             tc::mbar_arrive(b_state);
-        };
-        auto state_to = [&](float *dst, bool turned) {
-            if (32 * (warp - 4) >= a.width_b) return;   // the whole warp
-#pragma unroll 1
-            for (int cb = 0; cb < 2 * nc; cb++) {
-                uint32_t r[32];
-                tc::tmem_ld32(t_state + lanes + 32 * cb, r);
-                tc::tmem_ld_wait(r);
-                const bool in = j < a.width_b;
-                if (turned) {
-#pragma unroll
-                    for (int c = 0; c < 32; c++)
-                        if (in && 32 * cb + c < a.width_c) dst[(int64_t)(32 * cb + c) * a.width_b + j] = __uint_as_float(r[c]);
-                } else {
-#pragma unroll
-                    for (int c = 0; c < 32; c += 4)
-                        if (in && 32 * cb + c < a.width_c) *reinterpret_cast<uint4 *>(dst + (int64_t)j * a.width_c + 32 * cb + c) = make_uint4(r[c], r[c + 1], r[c + 2], r[c + 3]);
-                }
-                __syncwarp();
-            }
-        };
-        for (int n = 0; n < tiles; n++) {
-            state_before(n);
-            const int4 e = tile_at(a, first + n);
-            const int m = tile_rows(e), s = n % stages;
+
             all_wait(b_full + 8 * s, (n / stages) & 1);
-            if (!STATES) all_wait(b_inter, n & 1);   // A, B and the state's operand have been read
-            const float f = a.upd * exp2f(l2 * (a.reversed ? j + 1 : m - 1 - j));
-#pragma unroll 1
-            for (int k = 0; k < nb; k++) {
-                const uint32_t head = b_tile(s) + k * DK_BLOCK, tail = a_tile(s) + k * DK_BLOCK, rest = state_s + k * DK_BLOCK;
-#pragma unroll 4
-                for (int c = 0; c < 8; c++) {
-                    uint32_t v[4], w[4], z[4];
-                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(head + tc::swz(j, c)) : "memory");
-#pragma unroll
-                    for (int q = 0; q < 4; q++) {
-                        float2 x = Half<T>::unpack(v[q]);
-                        x.x = j < m ? x.x * f : 0.f;
-                        x.y = j < m ? x.y * f : 0.f;
-                        v[q] = Half<T>::pack(x.x, x.y);
-                        float2 y = Half<T>::unpack(v[q]);
-                        x.x -= y.x; x.y -= y.y;
-                        w[q] = Half<T>::pack(x.x, x.y);
-                        y = Half<T>::unpack(w[q]);
-                        z[q] = Half<T>::pack(x.x - y.x, x.y - y.y);
-                    }
-                    sts16(head + tc::swz(j, c), v);
-                    sts16(tail + tc::swz(j, c), w);
-                    if (p.parts == 3) sts16(rest + tc::swz(j, c), z);
-                }
-            }
-            if (j >= m) {   // tokens of the next sequence: nothing of theirs may meet a weight, not even a weight of zero
-                const uint32_t zero[4] = {0u, 0u, 0u, 0u};
-                for (int k = 0; k < nc; k++)
-                    for (int c = 0; c < 8; c++) sts16(c_tile(s) + k * DK_BLOCK + tc::swz(j, c), zero);
-            }
+            all_wait(b_inter, n & 1);   // A, B and the state's operand have been read
+            const float f = a.upd * exp2f(l2 * (a.reversed ? j + 1 : max(m - 1 - j, 0)));   // rows behind the sequence: a number, to be times 0
+            split_rows<T, PARTS>(b_tile(s), a_tile(s), state_s, j, j < m, pack2(f, f), 4 * nb * half, 4 * nb * (half + 1));
+            if (j >= m) clear_row(c_tile(s), j, 4 * nc * half, 4 * nc * (half + 1));
             tc::fence_async_smem();
             tc::mbar_arrive(b_split);
             all_wait(b_moved, n & 1);
             tc::fence_after_sync();
-            float *dst = nullptr;
-            if (STATES) dst = n + 1 == tiles ? p.carry + ((int64_t)blockIdx.x * a.heads + h) * plane : nullptr;
-            else if (a.state_out && tile_ends(a, e)) dst = a.state_out + ((int64_t)e.w * a.heads + h) * plane;
-            if (dst) state_to(dst, !STATES && a.transposed);
+            if (a.state_out && tile_ends(a, e) && 32 * (warp & 3) < a.width_b) {   // whole warps
+                float *dst = a.state_out + ((int64_t)e.w * a.heads + h) * plane;
+#pragma unroll 1
+                for (int cb = half * nc; cb < (half + 1) * nc; cb++) {
+                    uint32_t r[32];
+                    tc::tmem_ld32(t_state + lanes + 32 * cb, r);
+                    tc::tmem_ld_wait(r);
+                    state_row(r, dst, a.transposed, a.width_b, a.width_c, j, 32 * cb);
+                    __syncwarp();
+                }
+            }
+            e = ahead;
         }
     }
     __syncwarp();
     tc::fence_before_sync();
     __syncthreads();
-    if (warp == 8) tc::tmem_dealloc(tmem, 512);
+    if (warp == DK_COPY) tc::tmem_dealloc(tmem, 512);
+}
+
+// What the range adds to the state of the sequence that runs on into the next range, from zero or from where the sequence begins.  The rows
+// of B are scaled to the end of the range at once, so that the state gathers in tensor memory without being touched between tiles: splitting a
+// tile runs beside the products of the one before.
+template <typename T, int PARTS>
+__global__ void __launch_bounds__(DS_THREADS, 1) decay_states(const __grid_constant__ DecayKernel p) {
+    extern __shared__ unsigned char raw[];
+    __shared__ __align__(8) uint64_t bars[2 * 4 + 3];
+    __shared__ uint32_t tmem_s;
+    __shared__ int gave_up_s;
+    const DecayArgs &a = p.a;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, h = blockIdx.y;
+    const int nb = (a.width_b + 63) / 64, nc = (a.width_c + 63) / 64, stage_blocks = nb + nc, parts_blocks = (PARTS - 1) * nb;
+    // a product reads 128 columns of B, with one block of them the block behind it too: what it finds there goes to rows of the state that are not used
+    const int stages = min(4, (DK_TILES - parts_blocks - (nb == 1)) / stage_blocks);
+    const uint32_t smem = (tc::smem_u32(raw) + 1023) & ~1023u, parts_s = smem + stages * stage_blocks * DK_BLOCK;
+    const float l2 = log2_decay(a.log_decay[h]);
+    const int last = min(a.s.tiles, (int)(blockIdx.x + 1) * p.per_range);
+    const int4 end = tile_at(a, last - 1);
+    if (tile_ends(a, end)) return;
+    const int first = max((int)blockIdx.x * p.per_range, last - 1 - tiles_before(a, end)), tiles = last - first;
+    // token behind the range, as its place in the sequence
+    const int stop = a.reversed ? end.z : end.z + SEQ_TILE;
+
+    if (warp == 8) tc::tmem_alloc(tc::smem_u32(&tmem_s), 128);
+    if (tid == 0) {
+        for (int i = 0; i < 8; i++) tc::mbar_init(tc::smem_u32(&bars[i]), 1);   // landed, free again (by stage)
+        tc::mbar_init(tc::smem_u32(&bars[8]), 256);                             // B split
+        tc::mbar_init(tc::smem_u32(&bars[9]), 1);                               // tail and rest have been read
+        tc::mbar_init(tc::smem_u32(&bars[10]), 1);                              // all done
+        tc::fence_mbar_init();
+        gave_up_s = 0;
+    }
+    tc::fence_before_sync();
+    __syncthreads();
+    tc::fence_after_sync();
+    const Waits wait{&gave_up_s, p.err};
+    const uint32_t t_state = tmem_s;
+    const uint32_t b_full = tc::smem_u32(&bars[0]), b_free = tc::smem_u32(&bars[4]), b_split = tc::smem_u32(&bars[8]), b_tails = tc::smem_u32(&bars[9]),
+                   b_done = tc::smem_u32(&bars[10]);
+    auto b_tile = [&](int s) { return smem + s * stage_blocks * DK_BLOCK; };
+    auto c_tile = [&](int s) { return b_tile(s) + nb * DK_BLOCK; };
+    if (warp == 8) {
+        if (lane == 0) {
+            int n = 0;
+            for (; n < tiles && !gave_up_s; n++) {
+                const int s = n % stages;
+                const int4 e = tile_at(a, first + n);
+                if (n >= stages) wait(b_free + 8 * s, (n / stages - 1) & 1);
+                if (gave_up_s) break;
+                tc::mbar_expect_tx(b_full + 8 * s, stage_blocks * DK_BLOCK);
+                for (int k = 0; k < nb; k++) tc::tma_rows(b_tile(s) + k * DK_BLOCK, &p.mb, 64 * k, h, e.x + e.z, b_full + 8 * s);
+                for (int k = 0; k < nc; k++) tc::tma_rows(c_tile(s) + k * DK_BLOCK, &p.mc, 64 * k, h, e.x + e.z, b_full + 8 * s);
+            }
+            for (int s = 0; s < stages; s++)
+                if (n > s) wait.drain(b_full + 8 * s, ((n - 1 - s) / stages) & 1);
+        }
+    } else if (warp == 9) {
+        if (lane == 0) {
+            const uint32_t i_state = tc::idesc_f16(Half<T>::type == F3M_TYPE_BF16, 128, 64 * nc, true, true);
+            for (int n = 0; n < tiles; n++) {
+                const int s = n % stages;
+                wait(b_full + 8 * s, (n / stages) & 1);
+                wait(b_split, n & 1);
+                tc::fence_after_sync();
+                for (int part = PARTS - 1; part >= 0; part--) {
+                    const uint32_t rows = part == 0 ? b_tile(s) : parts_s + (part - 1) * nb * DK_BLOCK;
+                    for (int k = 0; k < 8; k++)
+                        tc::mma_f16(t_state, tc::desc_mn(rows + k * 2048, DK_BLOCK), tc::desc_mn(c_tile(s) + k * 2048, DK_BLOCK), i_state, n > 0 || part < PARTS - 1 || k > 0);
+                    if (part == 1) tc::mma_commit(b_tails);
+                }
+                tc::mma_commit(b_free + 8 * s);
+            }
+            tc::mma_commit(b_done);
+        }
+    } else {
+        const int j = tid & 127, half = tid >> 7;
+        for (int n = 0; n < tiles; n++) {
+            const int4 e = tile_at(a, first + n);
+            const int m = tile_rows(e), s = n % stages;
+            const float f = a.upd * exp2f(l2 * (a.reversed ? e.z + j + 1 - stop : stop - 1 - e.z - j));
+            wait(b_full + 8 * s, (n / stages) & 1);
+            if (n) wait(b_tails, (n - 1) & 1);
+            split_rows<T, PARTS>(b_tile(s), parts_s, parts_s + nb * DK_BLOCK, j, j < m, pack2(f, f), 4 * nb * half, 4 * nb * (half + 1));
+            if (j >= m) clear_row(c_tile(s), j, 4 * nc * half, 4 * nc * (half + 1));
+            tc::fence_async_smem();
+            tc::mbar_arrive(b_split);
+        }
+        wait(b_done, 0);
+        __syncwarp();
+        tc::fence_after_sync();
+        if (32 * (warp & 3) < a.width_b) {
+            const int64_t plane = (int64_t)a.width_b * a.width_c;
+            const int4 b = tile_at(a, first);
+            const float *src = tile_begins(a, b) && a.state_in ? a.state_in + ((int64_t)b.w * a.heads + h) * plane : nullptr;
+            const float f = exp2f(l2 * (a.reversed ? min(b.y, b.z + SEQ_TILE) - stop : stop - b.z));
+            float *dst = p.carry + ((int64_t)blockIdx.x * a.heads + h) * plane;
+#pragma unroll 1
+            for (int cb = half * nc; cb < (half + 1) * nc; cb++) {
+                uint32_t r[32];
+                tc::tmem_ld32(t_state + ((uint32_t)(32 * (warp & 3)) << 16) + 32 * cb, r);
+                tc::tmem_ld_wait(r);
+                if (src && j < a.width_b)
+#pragma unroll
+                    for (int c = 0; c < 32; c++)
+                        if (32 * cb + c < a.width_c)
+                            r[c] = __float_as_uint(fmaf(f, src[a.transposed ? (int64_t)(32 * cb + c) * a.width_b + j : (int64_t)j * a.width_c + 32 * cb + c], __uint_as_float(r[c])));
+                state_row(r, dst, false, a.width_b, a.width_c, j, 32 * cb);
+                __syncwarp();
+            }
+        }
+    }
+    __syncwarp();
+    tc::fence_before_sync();
+    __syncthreads();
+    if (warp == 8) tc::tmem_dealloc(t_state, 128);
 }
 
 // Runs over the ranges of a head: where range r is a stretch of one sequence that began before it, the state behind it is what it adds
@@ -423,6 +541,21 @@ size_t decay_workspace(const f3m_seqs &s, int heads, int width_b, int width_c) {
     return r == 1 ? 0 : (size_t)r * heads * width_b * width_c * sizeof(float);
 }
 
+template <typename T, int PARTS>
+static void launch_parts(const DecayKernel &p, cudaStream_t s) {
+    constexpr int bytes = DK_TILES * DK_BLOCK + 1024;
+    if (p.ranges > 1) {
+        F3M_CUDA(cudaFuncSetAttribute(decay_states<T, PARTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+        decay_states<T, PARTS><<<dim3(p.ranges - 1, p.a.heads), DS_THREADS, bytes, s>>>(p);
+        F3M_LAUNCH_CHECK();
+        decay_join<<<dim3((p.a.width_b * p.a.width_c / 4 + 255) / 256, p.a.heads), 256, 0, s>>>(p);
+        F3M_LAUNCH_CHECK();
+    }
+    F3M_CUDA(cudaFuncSetAttribute(decay_tiles<T, PARTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    decay_tiles<T, PARTS><<<dim3(p.ranges, p.a.heads), DK_THREADS, bytes, s>>>(p);
+    F3M_LAUNCH_CHECK();
+}
+
 template <typename T>
 static void decay_product_t(const DecayArgs &a, cudaStream_t s) {
     if (a.state_out) {
@@ -438,20 +571,14 @@ static void decay_product_t(const DecayArgs &a, cudaStream_t s) {
     p.ranges = decay_ranges(a.s, a.heads);
     p.per_range = (a.s.tiles + p.ranges - 1) / p.ranges;
     p.ranges = (a.s.tiles + p.per_range - 1) / p.per_range;
-    p.parts = Half<T>::type == F3M_TYPE_BF16 && a.state_out ? 3 : 2;
+    p.mo = seq_tensor_map(Half<T>::type, a.out, a.s.tokens, a.heads, a.width_c);
     p.carry = (float *)a.ws;
     p.err = seq_error_word();
-    constexpr int bytes = DK_TILES * DK_BLOCK + 1024;
-    if (p.ranges > 1) {
-        F3M_CUDA(cudaFuncSetAttribute(decay_tiles<T, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-        decay_tiles<T, true><<<dim3(p.ranges - 1, a.heads), DK_THREADS, bytes, s>>>(p);
-        F3M_LAUNCH_CHECK();
-        decay_join<<<dim3((a.width_b * a.width_c / 4 + 255) / 256, a.heads), 256, 0, s>>>(p);
-        F3M_LAUNCH_CHECK();
+    // a state that is returned in FP32 takes three parts of bf16
+    if constexpr (Half<T>::type == F3M_TYPE_BF16) {
+        if (a.state_out) return launch_parts<T, 3>(p, s);
     }
-    F3M_CUDA(cudaFuncSetAttribute(decay_tiles<T, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-    decay_tiles<T, false><<<dim3(p.ranges, a.heads), DK_THREADS, bytes, s>>>(p);
-    F3M_LAUNCH_CHECK();
+    launch_parts<T, 2>(p, s);
 }
 void decay_product(int type, const DecayArgs &a, cudaStream_t s) { type == F3M_TYPE_BF16 ? decay_product_t<__nv_bfloat16>(a, s) : decay_product_t<__half>(a, s); }
 

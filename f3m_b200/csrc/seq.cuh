@@ -122,6 +122,33 @@ struct Waits {
     }
 };
 
+// Rows 0 .. m of a swizzled tile in shared memory to tokens token .. token + m, by THREADS threads (t) that have each written rows of it;
+// on return thread 0 knows that the tile has been read.  A whole tile leaves as bulk copies; one that ends inside would write over the
+// next sequence's rows, so its rows are written one by one.
+template <int THREADS>
+__device__ __forceinline__ void store_rows(const CUtensorMap &map, const f3m_rows &out, uint32_t tile, int head, int token, int m, int blocks, int width,
+                                           int t, int barrier) {
+    if (m == SEQ_TILE) {
+        tc::fence_async_smem();
+        tc::bar_sync(barrier, THREADS);
+        if (t == 0) {
+            for (int k = 0; k < blocks; k++) tc::tma_store_rows(&map, tile + k * SEQ_TILE * 128, 64 * k, head, token);
+            tc::tma_store_commit();
+            tc::tma_store_wait_read();
+        }
+    } else {
+        tc::bar_sync(barrier, THREADS);
+        for (int i = t; i < m * 8 * blocks; i += THREADS) {   // 16-byte chunks; consecutive threads along a row
+            const int r = i / (8 * blocks), c = i % (8 * blocks);
+            uint32_t v[4];
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(tile + (c >> 3) * SEQ_TILE * 128 + tc::swz(r, c & 7)) : "memory");
+            if (8 * c < width)
+                *reinterpret_cast<uint4 *>(reinterpret_cast<uint16_t *>(out.data) + (int64_t)(token + r) * out.token_stride + (int64_t)head * out.head_stride + 8 * c) = make_uint4(v[0], v[1], v[2], v[3]);
+        }
+        tc::bar_sync(barrier, THREADS);
+    }
+}
+
 // log2 of a head's decay: at most 0; -256 makes every power but the zeroth 0 in FP32 and keeps 0 * log a number
 __device__ __forceinline__ float log2_decay(float log_decay) { return fmaxf(fminf(log_decay * 1.4426950408889634f, 0.f), -256.f); }
 

@@ -164,8 +164,18 @@ __device__ __forceinline__ void tma_rows(uint32_t dst, const CUtensorMap *map, i
                  "r"(col), "r"(head), "r"(token), "r"(bar)
                  : "memory");
 }
-__device__ __forceinline__ void tma_prefetch_map(const CUtensorMap *map) {
-    asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+// ... and back: what lies outside the array is not written
+__device__ __forceinline__ void tma_store_rows(const CUtensorMap *map, uint32_t src, int col, int head, int token) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(map), "r"(col), "r"(head), "r"(token), "r"(src)
+                 : "memory");
+}
+__device__ __forceinline__ void tma_store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void tma_store_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }   // sources read
+__device__ __forceinline__ void tma_store_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }         // written
+// whole warps
+__device__ __forceinline__ void bar_sync(int id, int threads) {
+    __syncwarp();
+    asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
 
 }   // namespace tc
