@@ -65,10 +65,6 @@ __device__ __forceinline__ void state_row(const uint32_t (&r)[32], float *dst, b
             if (j < wb && c0 + c < wc) *reinterpret_cast<uint4 *>(dst + (int64_t)j * wc + c0 + c) = make_uint4(r[c], r[c + 1], r[c + 2], r[c + 3]);
     }
 }
-__device__ __forceinline__ void sts16(uint32_t at, const uint32_t (&w)[4]) {
-    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
-}
-
 // Row j of a tile of B, times f, as a sum of 16-bit parts: 16-byte chunks [c0, c1) of its blocks; the first part stays in place.  j >= rows: zeros.
 template <typename T, int PARTS>
 __device__ __forceinline__ void split_rows(uint32_t head, uint32_t tail, uint32_t rest, int j, bool in, f32x2 f, int c0, int c1) {
@@ -99,12 +95,6 @@ __device__ __forceinline__ void split_rows(uint32_t head, uint32_t tail, uint32_
         if (PARTS == 3) sts16(rest + at, z);
     }
 }
-// Chunks [c0, c1) of row j of a tile become zero: tokens of the next sequence meet no weight, not even a weight of zero
-__device__ __forceinline__ void clear_row(uint32_t tile, int j, int c0, int c1) {
-    const uint32_t zero[4] = {0u, 0u, 0u, 0u};
-    for (int i = c0; i < c1; i++) sts16(tile + (i >> 3) * DK_BLOCK + tc::swz(j, i & 7), zero);
-}
-
 template <typename T, int PARTS>
 __global__ void __launch_bounds__(DK_THREADS, 1) decay_tiles(const __grid_constant__ DecayKernel p) {
     extern __shared__ unsigned char raw[];
@@ -282,7 +272,7 @@ __global__ void __launch_bounds__(DK_THREADS, 1) decay_tiles(const __grid_consta
             }
             tc::fence_before_sync();
             tc::mbar_arrive(b_read);
-            store_rows<128>(p.mo, a.out, c_tile(s), h, e.x + e.z, m, nc, a.width_c, i, 1);
+            store_rows<128>(p.mo, a.out, c_tile(s), h, e.x + e.z, m, 0, nc, a.width_c, i, 1);
             if (i == 0) tc::mbar_arrive(b_free + 8 * s);
         }
         if (i == 0) tc::tma_store_wait_all();

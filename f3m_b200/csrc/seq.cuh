@@ -11,11 +11,14 @@ constexpr int SEQ_TILE = F3M_SEQ_TILE;
 
 // The table of a packed batch, as int4: three orders of the tiles {first row of the sequence, its length, first token of the tile, sequence}
 // -- by place, by the tokens before the tile (the rows of late tiles see the most keys) and by the tokens from it on (the keys of early
-// tiles are seen most), the heaviest first in both -- and behind them the sequences {first row, length, first tile, tiles}.
+// tiles are seen most), the heaviest first in both -- behind them the sequences {first row, length, first tile, tiles}, and behind those every other
+// tile of each sequence, from its first on, in the second order.
 __host__ __device__ __forceinline__ size_t seq_by_place(const f3m_seqs &, int i) { return (size_t)i; }
 __host__ __device__ __forceinline__ size_t seq_by_past(const f3m_seqs &s, int i) { return (size_t)s.tiles + i; }
 __host__ __device__ __forceinline__ size_t seq_by_future(const f3m_seqs &s, int i) { return 2 * (size_t)s.tiles + i; }
 __host__ __device__ __forceinline__ size_t seq_of(const f3m_seqs &s, int i) { return 3 * (size_t)s.tiles + i; }
+
+__host__ __device__ __forceinline__ size_t seq_pair_by_past(const f3m_seqs &s, int i) { return 3 * (size_t)s.tiles + s.sequences + i; }
 
 template <typename T> struct Half;
 template <> struct Half<__nv_bfloat16> {
@@ -122,17 +125,26 @@ struct Waits {
     }
 };
 
-// Rows 0 .. m of a swizzled tile in shared memory to tokens token .. token + m, by THREADS threads (t) that have each written rows of it;
+__device__ __forceinline__ void sts16(uint32_t at, const uint32_t (&w)[4]) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+}
+// Chunks [c0, c1) of row j of a tile become zero: tokens of the next sequence meet no weight, not even a weight of zero
+__device__ __forceinline__ void clear_row(uint32_t tile, int j, int c0, int c1) {
+    const uint32_t zero[4] = {0u, 0u, 0u, 0u};
+    for (int i = c0; i < c1; i++) sts16(tile + (i >> 3) * SEQ_TILE * 128 + tc::swz(j, i & 7), zero);
+}
+
+// Rows 0 .. m of a swizzled tile in shared memory, columns from col0 on, to tokens token .. token + m, by THREADS threads (t) that have each written rows of it;
 // on return thread 0 knows that the tile has been read.  A whole tile leaves as bulk copies; one that ends inside would write over the
 // next sequence's rows, so its rows are written one by one.
 template <int THREADS>
-__device__ __forceinline__ void store_rows(const CUtensorMap &map, const f3m_rows &out, uint32_t tile, int head, int token, int m, int blocks, int width,
-                                           int t, int barrier) {
+__device__ __forceinline__ void store_rows(const CUtensorMap &map, const f3m_rows &out, uint32_t tile, int head, int token, int m, int col0, int blocks,
+                                           int width, int t, int barrier) {
     if (m == SEQ_TILE) {
         tc::fence_async_smem();
         tc::bar_sync(barrier, THREADS);
         if (t == 0) {
-            for (int k = 0; k < blocks; k++) tc::tma_store_rows(&map, tile + k * SEQ_TILE * 128, 64 * k, head, token);
+            for (int k = 0; k < blocks; k++) tc::tma_store_rows(&map, tile + k * SEQ_TILE * 128, col0 + 64 * k, head, token);
             tc::tma_store_commit();
             tc::tma_store_wait_read();
         }
@@ -142,8 +154,8 @@ __device__ __forceinline__ void store_rows(const CUtensorMap &map, const f3m_row
             const int r = i / (8 * blocks), c = i % (8 * blocks);
             uint32_t v[4];
             asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(tile + (c >> 3) * SEQ_TILE * 128 + tc::swz(r, c & 7)) : "memory");
-            if (8 * c < width)
-                *reinterpret_cast<uint4 *>(reinterpret_cast<uint16_t *>(out.data) + (int64_t)(token + r) * out.token_stride + (int64_t)head * out.head_stride + 8 * c) = make_uint4(v[0], v[1], v[2], v[3]);
+            if (col0 + 8 * c < width)
+                *reinterpret_cast<uint4 *>(reinterpret_cast<uint16_t *>(out.data) + (int64_t)(token + r) * out.token_stride + (int64_t)head * out.head_stride + col0 + 8 * c) = make_uint4(v[0], v[1], v[2], v[3]);
         }
         tc::bar_sync(barrier, THREADS);
     }

@@ -78,7 +78,7 @@ void check_heads(int heads, int kv_heads) {
 }
 void check_seqs(const f3m_seqs *s) {
     F3M_REQUIRE(s, F3M_ERR_ARG, "null pointer argument");
-    F3M_REQUIRE(s->sequences >= 0 && s->tiles >= 0 && s->tokens >= 0 && s->tokens <= F3M_SEQ_MAX_TOKENS, F3M_ERR_ARG, "counts of the sequences were not filled by f3m_seqs_layout");
+    F3M_REQUIRE(s->sequences >= 0 && s->tiles >= 0 && s->pairs >= 0 && s->tokens >= 0 && s->tokens <= F3M_SEQ_MAX_TOKENS, F3M_ERR_ARG, "counts of the sequences were not filled by f3m_seqs_layout");
     F3M_REQUIRE(s->sequences == 0 || (s->table && (uintptr_t)s->table % 16 == 0), F3M_ERR_ARG, "the table of the sequences is missing or not 16-byte aligned");
 }
 // tokens == 0: the array may be absent
@@ -120,22 +120,24 @@ extern "C" {
 int f3m_seqs_layout(const int32_t *lengths, int32_t n, f3m_seqs *seqs, int32_t *table) {
     return guarded([&] {
         F3M_REQUIRE(seqs && n >= 0 && (lengths || n == 0), F3M_ERR_ARG, "bad argument to f3m_seqs_layout");
-        int64_t tokens = 0, tiles = 0;
+        int64_t tokens = 0, tiles = 0, pairs = 0;
         int32_t longest = 0;
         for (int i = 0; i < n; i++) {
             F3M_REQUIRE(lengths[i] >= 0, F3M_ERR_ARG, "length %d of sequence %d", lengths[i], i);
             tokens += lengths[i];
             tiles += ((int64_t)lengths[i] + SEQ_TILE - 1) / SEQ_TILE;
+            pairs += ((int64_t)lengths[i] + 2 * SEQ_TILE - 1) / (2 * SEQ_TILE);
             longest = std::max(longest, lengths[i]);
         }
         F3M_REQUIRE(tokens <= F3M_SEQ_MAX_TOKENS, F3M_ERR_OVERFLOW, "%lld tokens do not fit in 31 bits", (long long)tokens);
-        F3M_REQUIRE(4 * (3 * tiles + n) <= 0x7fffffff, F3M_ERR_OVERFLOW, "the table of %d sequences does not fit in 31 bits", n);
+        F3M_REQUIRE(4 * (3 * tiles + n + pairs) <= 0x7fffffff, F3M_ERR_OVERFLOW, "the table of %d sequences does not fit in 31 bits", n);
         seqs->table = nullptr;
         seqs->tokens = tokens;
         seqs->sequences = n;
         seqs->tiles = (int32_t)tiles;
         seqs->longest = longest;
-        seqs->table_words = (int32_t)(4 * (3 * tiles + n));
+        seqs->pairs = (int32_t)pairs;
+        seqs->table_words = (int32_t)(4 * (3 * tiles + n + pairs));
         if (!table) return;
         int32_t *t = table, *sq = table + 12 * tiles;
         int32_t first = 0, tile = 0;
@@ -155,6 +157,9 @@ int f3m_seqs_layout(const int32_t *lengths, int32_t n, f3m_seqs *seqs, int32_t *
             });
             for (int64_t k = 0; k < tiles; k++) memcpy(table + 4 * (which * tiles + k), table + 4 * (size_t)order[k], 16);
         }
+        int32_t *pr = sq + 4 * (int64_t)n;
+        for (int64_t k = tiles; k < 2 * tiles; k++)
+            if (table[4 * k + 2] / SEQ_TILE % 2 == 0) { memcpy(pr, table + 4 * k, 16); pr += 4; }
     });
 }
 

@@ -24,14 +24,16 @@ def test_layout(lengths):
     assert (s.tokens, s.sequences, s.longest) == (sum(lengths), len(lengths), max(lengths))
     first = np.cumsum(lengths) - lengths
     tiles = [(first[i], n, a, i) for i, n in enumerate(lengths) for a in range(0, n, 128)]
-    assert s.tiles == len(tiles) and len(t) == 3 * len(tiles) + len(lengths)
+    assert s.tiles == len(tiles) and len(t) == 3 * len(tiles) + len(lengths) + s.pairs
     by = [t[k * s.tiles:(k + 1) * s.tiles] for k in range(3)]
     assert by[0].tolist() == [list(map(int, x)) for x in tiles]
     for b in by[1:]:
         assert sorted(b.tolist()) == sorted(by[0].tolist())
     assert (np.diff(by[1][:, 2]) <= 0).all() and (np.diff(by[2][:, 1] - by[2][:, 2]) <= 0).all()
     at = 0
-    for i, row in enumerate(t[3 * s.tiles:].tolist()):
+    even = [r for r in by[1].tolist() if r[2] % 256 == 0]
+    assert s.pairs == len(even) == sum(-(-n // 256) for n in lengths) and t[3 * s.tiles + len(lengths):].tolist() == even
+    for i, row in enumerate(t[3 * s.tiles:3 * s.tiles + len(lengths)].tolist()):
         n = -(-lengths[i] // 128)
         assert row == [first[i], lengths[i], at, n]
         at += n
@@ -70,7 +72,7 @@ def test_argument_checks_of_the_entries():
     assert window(q=Rows(base + 2, 128, 64)) == 1 and window(k=Rows(base, 132, 64)) == 1 and window(v=Rows(base, 128, -64)) == 1
     assert window(out=Rows(base, 64, 64)) == 1 and b"overlap" in L.f3m_last_error()
     assert window(out=Rows(base, 128, 0)) == 1
-    bad = Seqs(None, 130, 2, 3, 100, 0)
+    bad = Seqs(None, 130, 2, 3, 2, 100, 0)
     assert window(seqs=bad) == 1
 
     def grad(ws=base, have=1 << 20, dk=ok):
