@@ -56,7 +56,7 @@ struct WindowArgs {
     f3m_rows q, k, v, out;
     float *lse;
     f3m_rows dout, dq, dk, dv;   // gradients only
-    float *delta;                // (heads, tokens): rows of dout . out
+    float *delta;                // workspace: 2 x (heads, tokens)
 };
 void window_forward(int type, const WindowArgs &a, cudaStream_t s);
 void window_backward(int type, const WindowArgs &a, cudaStream_t s);

@@ -111,7 +111,7 @@ void check_workspace(const void *ws, size_t have, size_t need) {
 }
 void check_state(const float *p, const char *what) { F3M_REQUIRE((uintptr_t)p % 16 == 0, F3M_ERR_ARG, "%s is not 16-byte aligned", what); }
 
-size_t grad_workspace(const f3m_seqs &s, int heads) { return (size_t)s.tokens * heads * sizeof(float); }
+size_t grad_workspace(const f3m_seqs &s, int heads) { return 2 * (size_t)s.tokens * heads * sizeof(float); }
 
 }  // namespace
 

@@ -19,92 +19,6 @@ __device__ __forceinline__ float dot_rows(const T *a, const T *b, int width, int
 template <typename T>
 __device__ __forceinline__ T *row_of(const f3m_rows &r, int64_t t, int h) { return reinterpret_cast<T *>(r.data) + t * r.token_stride + h * r.head_stride; }
 
-// A warp per (query, head), the running maximum and sum of its softmax in registers.
-template <typename T, bool GRAD>
-__global__ void __launch_bounds__(128) window_rows(WindowArgs a) {
-    const int lane = threadIdx.x & 31, row = (blockIdx.x * 128 + threadIdx.x) >> 5, h = blockIdx.y, hk = h / (a.heads / a.kv_heads);
-    const int4 e = reinterpret_cast<const int4 *>(a.s.table)[row / SEQ_TILE];
-    const int i = e.z + row % SEQ_TILE;
-    if (i >= e.y) return;
-    const T *q = row_of<T>(a.q, e.x + i, h);
-    float2 acc[2] = {};
-    float top = -INFINITY, sum = 0.f, lse = 0.f, delta = 0.f;
-    if (GRAD) {
-        lse = a.lse[(int64_t)h * a.s.tokens + e.x + i];
-        delta = dot_rows(row_of<T>(a.out, e.x + i, h), row_of<T>(a.dout, e.x + i, h), a.width, lane);
-        if (lane == 0) a.delta[(int64_t)h * a.s.tokens + e.x + i] = delta;
-    }
-    const int lo = max(0, i - a.window + 1);
-    for (int j = 0; j <= i; j++) {
-        if (j < lo && j >= a.sinks) j = lo;
-        const T *k = row_of<T>(a.k, e.x + j, hk), *v = row_of<T>(a.v, e.x + j, hk);
-        const float s = a.scale * dot_rows(q, k, a.width, lane);
-        float w, scale_acc = 1.f;
-        if (GRAD) {
-            w = expf(s - lse) * (dot_rows(row_of<T>(a.dout, e.x + i, h), v, a.width, lane) - delta) * a.scale;
-        } else {
-            const float t = fmaxf(top, s);
-            scale_acc = expf(top - t);
-            w = expf(s - t);
-            top = t;
-            sum = sum * scale_acc + w;
-        }
-        const T *src = GRAD ? k : v;
-#pragma unroll
-        for (int p = 0; p < 2; p++) {
-            const int c = 2 * lane + 64 * p;
-            if (c < a.width) {
-                const float2 x = Half<T>::unpack(*reinterpret_cast<const uint32_t *>(src + c));
-                acc[p].x = acc[p].x * scale_acc + w * x.x;
-                acc[p].y = acc[p].y * scale_acc + w * x.y;
-            }
-        }
-    }
-    const float inv = GRAD ? 1.f : 1.f / sum;
-#pragma unroll
-    for (int p = 0; p < 2; p++) {
-        const int c = 2 * lane + 64 * p;
-        if (c < a.width) *reinterpret_cast<uint32_t *>(row_of<T>(GRAD ? a.dq : a.out, e.x + i, h) + c) = Half<T>::pack(acc[p].x * inv, acc[p].y * inv);
-    }
-    if (!GRAD && lane == 0) a.lse[(int64_t)h * a.s.tokens + e.x + i] = top + logf(sum);
-}
-
-// A warp per (key, key head): dk and dv are sums over the queries that see the key, of all heads that share it.
-template <typename T>
-__global__ void __launch_bounds__(128) window_cols(WindowArgs a) {
-    const int lane = threadIdx.x & 31, row = (blockIdx.x * 128 + threadIdx.x) >> 5, hk = blockIdx.y, group = a.heads / a.kv_heads;
-    const int4 e = reinterpret_cast<const int4 *>(a.s.table)[row / SEQ_TILE];
-    const int j = e.z + row % SEQ_TILE;
-    if (j >= e.y) return;
-    const T *k = row_of<T>(a.k, e.x + j, hk), *v = row_of<T>(a.v, e.x + j, hk);
-    float2 gk[2] = {}, gv[2] = {};
-    const int hi = j < a.sinks ? e.y : (int)min((int64_t)e.y, (int64_t)j + a.window);
-    for (int h = hk * group; h < (hk + 1) * group; h++)
-        for (int i = j; i < hi; i++) {
-            const T *q = row_of<T>(a.q, e.x + i, h), *g = row_of<T>(a.dout, e.x + i, h);
-            const int64_t at = (int64_t)h * a.s.tokens + e.x + i;
-            const float p = expf(a.scale * dot_rows(q, k, a.width, lane) - a.lse[at]);
-            const float ds = p * (dot_rows(g, v, a.width, lane) - a.delta[at]) * a.scale;
-#pragma unroll
-            for (int r = 0; r < 2; r++) {
-                const int c = 2 * lane + 64 * r;
-                if (c < a.width) {
-                    const float2 x = Half<T>::unpack(*reinterpret_cast<const uint32_t *>(q + c)), y = Half<T>::unpack(*reinterpret_cast<const uint32_t *>(g + c));
-                    gk[r].x = fmaf(ds, x.x, gk[r].x); gk[r].y = fmaf(ds, x.y, gk[r].y);
-                    gv[r].x = fmaf(p, y.x, gv[r].x); gv[r].y = fmaf(p, y.y, gv[r].y);
-                }
-            }
-        }
-#pragma unroll
-    for (int r = 0; r < 2; r++) {
-        const int c = 2 * lane + 64 * r;
-        if (c < a.width) {
-            *reinterpret_cast<uint32_t *>(row_of<T>(a.dk, e.x + j, hk) + c) = Half<T>::pack(gk[r].x, gk[r].y);
-            *reinterpret_cast<uint32_t *>(row_of<T>(a.dv, e.x + j, hk) + c) = Half<T>::pack(gv[r].x, gv[r].y);
-        }
-    }
-}
-
 // ---- forward --------------------------------------------------------------------------------------------------------------
 // A CTA, one per SM, walks over items; an item is two tiles of 128 query rows that read the same keys: two heads of a group, or, where a group has
 // an odd number of heads, two neighbouring tiles of one head.  Tile by tile of 128 keys, S = Q K^T goes to tensor memory; a thread has one
@@ -419,11 +333,450 @@ static void forward_t(const WindowArgs &a, cudaStream_t s) {
     window_tiles<T><<<std::min(p.items, NUM_SMS_HINT), WF_THREADS, bytes, s>>>(p);
     F3M_LAUNCH_CHECK();
 }
+// ---- gradients ------------------------------------------------------------------------------------------------------------
+// P = 2^(c s - lse), dS = P (scale dP - scale delta) with dP = dout V^T: dV = P^T dout, dK = dS^T Q, dQ = dS K.  dK and dV are sums over queries, dQ
+// over keys: two kernels, one that holds a tile of keys and walks over the queries that see it, of all heads that share it, and one that
+// holds a tile of queries.  S and dP are computed in both, seven products where five would do, but nothing is added across CTAs: sums have one order.
+// P and dS are rounded to 16 bits where they become operands, and go through tensor memory over the scores they come from.
+
+// lse2 = lse log2(e) and delta = scale dout.out, rows (heads, tokens)
+template <typename T>
+__global__ void __launch_bounds__(256) window_rows_sum(WindowArgs a, float *lse2, float *delta) {
+    const int64_t row = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 4, t = row / a.heads;
+    const int h = (int)(row % a.heads), c = 8 * (threadIdx.x & 15);
+    float s = 0.f;
+    if (t < a.s.tokens && c < a.width) {
+        const uint4 x = *reinterpret_cast<const uint4 *>(row_of<T>(a.out, t, h) + c), y = *reinterpret_cast<const uint4 *>(row_of<T>(a.dout, t, h) + c);
+        const uint32_t u[4] = {x.x, x.y, x.z, x.w}, v[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            const float2 f = Half<T>::unpack(u[q]), g = Half<T>::unpack(v[q]);
+            s = fmaf(f.x, g.x, fmaf(f.y, g.y, s));
+        }
+    }
+#pragma unroll
+    for (int o = 8; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (t < a.s.tokens && c == 0) {
+        const int64_t at = h * a.s.tokens + t;
+        delta[at] = a.scale * s;
+        lse2[at] = 1.4426950408889634f * a.lse[at];
+    }
+}
+
+constexpr int WG_COPY = 8, WG_PRODUCTS = 9, WG_THREADS = 320, WG_KEY_BLOCKS = 12;
+// Two threads share a row of scores, 64 columns each, and write their 16-bit operands over the first of their own: step k of the contraction
+// (16 elements, 8 columns) begins at this column
+__device__ __forceinline__ uint32_t operand_col(int k) { return 8 * (k & 3) + 64 * (k >> 2); }
+struct GradKernel {
+    WindowArgs a;
+    CUtensorMap mq, mk, mv, mg, m0, m1;   // q, k, v, dout; the outputs: dk and dv, or dq
+    float c;                              // scale log2(e)
+    const float *lse2, *delta;
+    int *err;
+};
+
+// A CTA has a tile of 128 keys (rows of tensor memory) and walks over tiles of 128 queries (columns).  Of the products of query tile n,
+//     S^T = K Q^T (n + 1)  follows  dV += P^T dout (n),     dP^T = V dout^T (n + 1)  follows  dK += dS^T Q (n),
+// so that the weights of n + 1 are taken while the second pair runs, and dS while the first does.
+template <typename T>
+__global__ void __launch_bounds__(WG_THREADS, 1) window_grad_keys(const __grid_constant__ GradKernel p) {
+    extern __shared__ unsigned char raw[];
+    __shared__ __align__(8) uint64_t bars[2 * 4 + 6];
+    __shared__ uint32_t tmem_s;
+    __shared__ int gave_up_s;
+    __shared__ __align__(16) float lse_s[2][SEQ_TILE], delta_s[2][SEQ_TILE];
+    const WindowArgs &a = p.a;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, nb = (a.width + 63) / 64, group = a.heads / a.kv_heads;
+    const int stages = min(4, (WG_KEY_BLOCKS - 2 * nb) / (2 * nb));
+    const uint32_t smem = (tc::smem_u32(raw) + 1023) & ~1023u, k_tile = smem, v_tile = smem + nb * WF_BLOCK;
+    auto q_tile = [&](int s) { return smem + (2 + 2 * s) * nb * WF_BLOCK; };
+    auto g_tile = [&](int s) { return smem + (3 + 2 * s) * nb * WF_BLOCK; };
+    const int4 e = reinterpret_cast<const int4 *>(a.s.table)[seq_by_future(a.s, blockIdx.x / a.kv_heads)];
+    const int hk = blockIdx.x % a.kv_heads, key = e.z;
+    // queries from the key's own tile on, to the end of the window, or of the sequence where the tile holds sinks
+    const int q0 = key / SEQ_TILE, q1 = (key < a.sinks ? e.y - 1 : (int)min((int64_t)e.y - 1, (int64_t)key + SEQ_TILE - 2 + a.window)) / SEQ_TILE;
+    const int per_head = q1 - q0 + 1, tiles = per_head * group;
+
+    if (warp == WG_COPY) tc::tmem_alloc(tc::smem_u32(&tmem_s), 512);
+    if (tid == 0) {
+        for (int i = 0; i < 12; i++) tc::mbar_init(tc::smem_u32(&bars[i]), 1);    // landed, free (by stage); keys landed, S ready, dP ready, all done
+        tc::mbar_init(tc::smem_u32(&bars[12]), 256);                              // P written
+        tc::mbar_init(tc::smem_u32(&bars[13]), 256);                              // dS written
+        tc::fence_mbar_init();
+        gave_up_s = 0;
+    }
+    tc::fence_before_sync();
+    __syncthreads();
+    tc::fence_after_sync();
+    const Waits wait{&gave_up_s, p.err};
+    const uint32_t tmem = tmem_s, t_s = tmem, t_dp = tmem + 128, t_dv = tmem + 256, t_dk = tmem + 384;
+    const uint32_t b_full = tc::smem_u32(&bars[0]), b_free = tc::smem_u32(&bars[4]), b_k = tc::smem_u32(&bars[8]), b_s = tc::smem_u32(&bars[9]),
+                   b_dp = tc::smem_u32(&bars[10]), b_done = tc::smem_u32(&bars[11]), b_p = tc::smem_u32(&bars[12]), b_ds = tc::smem_u32(&bars[13]);
+    if (warp == WG_COPY) {
+        if (lane == 0) {
+            tc::mbar_expect_tx(b_k, 2 * nb * WF_BLOCK);
+            for (int k = 0; k < nb; k++) {
+                tc::tma_rows(k_tile + k * WF_BLOCK, &p.mk, 64 * k, hk, e.x + key, b_k);
+                tc::tma_rows(v_tile + k * WF_BLOCK, &p.mv, 64 * k, hk, e.x + key, b_k);
+            }
+            int n = 0;
+            for (; n < tiles && !gave_up_s; n++) {
+                const int s = n % stages, h = hk * group + n / per_head, q = (q0 + n % per_head) * SEQ_TILE;
+                if (n >= stages) wait(b_free + 8 * s, (n / stages - 1) & 1);
+                if (gave_up_s) break;
+                tc::mbar_expect_tx(b_full + 8 * s, 2 * nb * WF_BLOCK);
+                for (int k = 0; k < nb; k++) {
+                    tc::tma_rows(q_tile(s) + k * WF_BLOCK, &p.mq, 64 * k, h, e.x + q, b_full + 8 * s);
+                    tc::tma_rows(g_tile(s) + k * WF_BLOCK, &p.mg, 64 * k, h, e.x + q, b_full + 8 * s);
+                }
+            }
+            wait.drain(b_k, 0);
+            for (int s = 0; s < stages; s++)
+                if (n > s) wait.drain(b_full + 8 * s, ((n - 1 - s) / stages) & 1);
+        }
+    } else if (warp == WG_PRODUCTS) {
+        if (lane == 0) {
+            constexpr bool bf = Half<T>::type == F3M_TYPE_BF16;
+            const uint32_t i_s = tc::idesc_f16(bf, 128, 128, false, false), i_d = tc::idesc_f16(bf, 128, 64 * nb, false, true);
+            auto rows = [&](uint32_t d, uint32_t x, uint32_t y, uint32_t bar) {   // x y^T
+                for (int k = 0; k < 4 * nb; k++)
+                    tc::mma_f16(d, tc::desc_k(x + (k >> 2) * WF_BLOCK + (k & 3) * 32), tc::desc_k(y + (k >> 2) * WF_BLOCK + (k & 3) * 32), i_s, k > 0);
+                tc::mma_commit(bar);
+            };
+            wait(b_k, 0);
+            wait(b_full, 0);
+            tc::fence_after_sync();
+            rows(t_s, k_tile, q_tile(0), b_s);
+            rows(t_dp, v_tile, g_tile(0), b_dp);
+            for (int n = 0; n < tiles; n++) {
+                const int s = n % stages, sn = (n + 1) % stages;
+                const bool more = n + 1 < tiles;
+                wait(b_p, n & 1);
+                tc::fence_after_sync();
+                for (int k = 0; k < 8; k++) tc::mma_f16_ta(t_dv, t_s + operand_col(k), tc::desc_mn(g_tile(s) + k * 2048, WF_BLOCK), i_d, n > 0 || k > 0);
+                if (more) {
+                    wait(b_full + 8 * sn, ((n + 1) / stages) & 1);
+                    tc::fence_after_sync();
+                    rows(t_s, k_tile, q_tile(sn), b_s);
+                }
+                wait(b_ds, n & 1);
+                tc::fence_after_sync();
+                for (int k = 0; k < 8; k++) tc::mma_f16_ta(t_dk, t_dp + operand_col(k), tc::desc_mn(q_tile(s) + k * 2048, WF_BLOCK), i_d, n > 0 || k > 0);
+                tc::mma_commit(b_free + 8 * s);
+                if (more) rows(t_dp, v_tile, g_tile(sn), b_dp);
+            }
+            tc::mma_commit(b_done);
+        }
+    } else {
+        // threads r and r + 128 have key row r, half of the queries each
+        const int r = tid & 127, half = tid >> 7, j = key + r;
+        const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
+        const f32x2 cc = pack2(p.c, p.c), scale = pack2(a.scale, a.scale), minus = pack2(-1.f, -1.f);
+        auto row_sum = [&](int n) {   // lse2 (threads of the first half) or delta of a query of tile n
+            const int h = hk * group + n / per_head, i = (q0 + n % per_head) * SEQ_TILE + r;
+            return i < e.y ? (half ? p.delta : p.lse2)[h * a.s.tokens + e.x + i] : 0.f;
+        };
+        float next = row_sum(0);
+        for (int n = 0; n < tiles; n++) {
+            const int q = (q0 + n % per_head) * SEQ_TILE, s = n % stages;
+            (half ? delta_s : lse_s)[n & 1][r] = next;
+            tc::bar_sync(1, 256);
+            if (n + 1 < tiles) next = row_sum(n + 1);
+            if (q + SEQ_TILE > e.y) {   // queries of the next sequence: their rows meet no weight, not even a weight of zero
+                wait(b_full + 8 * s, (n / stages) & 1);
+                wait(b_s, n & 1);
+                wait(b_dp, n & 1);
+                if (q + r >= e.y) clear_row(half ? g_tile(s) : q_tile(s), r, 0, 8 * nb);
+                tc::fence_async_smem();
+            }
+            // seen: query q + c sees key j if j <= q + c, q + c - j < window or j is a sink, and the query is one
+            const bool sink = j < a.sinks;
+            const int low = j - q, up = min(sink ? SEQ_TILE - 1 : j - q + a.window - 1, e.y - 1 - q);
+            const int i0 = key + 32 * (warp & 3);   // the warp's first key
+            const bool whole = i0 + 31 <= q && (q + SEQ_TILE - 1 - i0 < a.window || i0 + 32 <= a.sinks) && q + SEQ_TILE <= e.y;
+            wait(b_s, n & 1);
+            __syncwarp();
+            tc::fence_after_sync();
+            float pr[2][32];
+#pragma unroll
+            for (int b = 0; b < 2; b++) {
+                uint32_t x[32], w[16];
+                tc::tmem_ld32(t_s + lanes + 64 * half + 32 * b, x);
+                tc::tmem_ld_wait(x);
+#pragma unroll
+                for (int c = 0; c < 32; c += 4) {
+                    const ulonglong2 l = *reinterpret_cast<const ulonglong2 *>(&lse_s[n & 1][64 * half + 32 * b + c]);
+                    unpack2(fma2(pack2(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), cc, mul2(l.x, minus)), pr[b][c], pr[b][c + 1]);
+                    unpack2(fma2(pack2(__uint_as_float(x[c + 2]), __uint_as_float(x[c + 3])), cc, mul2(l.y, minus)), pr[b][c + 2], pr[b][c + 3]);
+                }
+#pragma unroll
+                for (int c = 0; c < 32; c++) pr[b][c] = ex2_approx(pr[b][c]);
+                if (!whole)
+#pragma unroll
+                    for (int c = 0; c < 32; c++) {
+                        const int at = 64 * half + 32 * b + c;
+                        if (at < low || at > up) pr[b][c] = 0.f;
+                    }
+#pragma unroll
+                for (int c = 0; c < 32; c += 2) w[c >> 1] = Half<T>::pack(pr[b][c], pr[b][c + 1]);
+                tc::tmem_st16(t_s + lanes + 64 * half + 16 * b, w);
+            }
+            tc::tmem_st_wait();
+            tc::fence_before_sync();
+            tc::mbar_arrive(b_p);
+            wait(b_dp, n & 1);
+            __syncwarp();
+            tc::fence_after_sync();
+#pragma unroll
+            for (int b = 0; b < 2; b++) {
+                uint32_t x[32], w[16];
+                tc::tmem_ld32(t_dp + lanes + 64 * half + 32 * b, x);
+                tc::tmem_ld_wait(x);
+#pragma unroll
+                for (int c = 0; c < 32; c += 4) {
+                    const ulonglong2 d = *reinterpret_cast<const ulonglong2 *>(&delta_s[n & 1][64 * half + 32 * b + c]);
+                    float y[4];
+                    unpack2(mul2(pack2(pr[b][c], pr[b][c + 1]), fma2(pack2(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), scale, mul2(d.x, minus))), y[0], y[1]);
+                    unpack2(mul2(pack2(pr[b][c + 2], pr[b][c + 3]), fma2(pack2(__uint_as_float(x[c + 2]), __uint_as_float(x[c + 3])), scale, mul2(d.y, minus))), y[2], y[3]);
+                    if (!whole)
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            const int at = 64 * half + 32 * b + c + k;
+                            if (at < low || at > up) y[k] = 0.f;
+                        }
+                    w[c >> 1] = Half<T>::pack(y[0], y[1]);
+                    w[(c >> 1) + 1] = Half<T>::pack(y[2], y[3]);
+                }
+                tc::tmem_st16(t_dp + lanes + 64 * half + 16 * b, w);
+            }
+            tc::tmem_st_wait();
+            tc::fence_before_sync();
+            tc::mbar_arrive(b_ds);
+        }
+        wait(b_done, 0);
+        __syncwarp();
+        tc::fence_after_sync();
+        // the first half stages and stores dk over K, the second dv over V
+        const uint32_t out = half ? v_tile : k_tile;
+        for (int q = 0; q < 2 * nb; q++) {
+            uint32_t o[32];
+            tc::tmem_ld32((half ? t_dv : t_dk) + lanes + 32 * q, o);
+            tc::tmem_ld_wait(o);
+#pragma unroll
+            for (int c = 0; c < 32; c += 8) {
+                uint32_t y[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) y[k] = Half<T>::pack(__uint_as_float(o[c + 2 * k]), __uint_as_float(o[c + 2 * k + 1]));
+                sts16(out + (q >> 1) * WF_BLOCK + tc::swz(r, 4 * (q & 1) + c / 8), y);
+            }
+        }
+        store_rows<128>(half ? p.m1 : p.m0, half ? a.dv : a.dk, out, hk, e.x + key, min(SEQ_TILE, e.y - key), 0, nb, a.width, r, 3 + half);
+        if (r == 0) tc::tma_store_wait_all();
+    }
+    __syncwarp();
+    tc::fence_before_sync();
+    __syncthreads();
+    if (warp == WG_COPY) tc::tmem_dealloc(tmem, 512);
+}
+
+// A CTA has a tile of 128 queries (rows of tensor memory) and walks over tiles of 128 keys (columns).  S is computed a tile ahead, into one of two
+// places in turn; dP (n + 1) and dQ += dS K (n) run while the weights of n + 1 are taken.
+template <typename T>
+__global__ void __launch_bounds__(WG_THREADS, 1) window_grad_queries(const __grid_constant__ GradKernel p) {
+    extern __shared__ unsigned char raw[];
+    __shared__ __align__(8) uint64_t bars[2 * 8 + 6];
+    __shared__ uint32_t tmem_s;
+    __shared__ int gave_up_s;
+    const WindowArgs &a = p.a;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, nb = (a.width + 63) / 64, group = a.heads / a.kv_heads;
+    const int slots = min(8, (WF_BLOCKS - 2 * nb) / nb);   // 5 at two blocks, 8 at one
+    const uint32_t smem = (tc::smem_u32(raw) + 1023) & ~1023u, q_tile = smem, g_tile = smem + nb * WF_BLOCK;
+    auto slot_tile = [&](int s) { return smem + (2 + s) * nb * WF_BLOCK; };
+    const int4 e = reinterpret_cast<const int4 *>(a.s.table)[seq_by_past(a.s, blockIdx.x / a.heads)];
+    const int h = blockIdx.x % a.heads, hk = h / group, start = e.z;
+    const int first = max(0, start - a.window + 1) / SEQ_TILE, sinks = (int)min(((int64_t)a.sinks + SEQ_TILE - 1) / SEQ_TILE, (int64_t)first);
+    const int tiles = sinks + start / SEQ_TILE - first + 1;
+    auto key_of = [&](int n) { return SEQ_TILE * (n < sinks ? n : first + n - sinks); };
+
+    if (warp == WG_COPY) tc::tmem_alloc(tc::smem_u32(&tmem_s), 512);
+    if (tid == 0) {
+        for (int i = 0; i < 21; i++) tc::mbar_init(tc::smem_u32(&bars[i]), 1);    // slot landed, free; queries landed, S ready (two), dP ready, all done
+        tc::mbar_init(tc::smem_u32(&bars[21]), 256);                              // dS written
+        tc::fence_mbar_init();
+        gave_up_s = 0;
+    }
+    tc::fence_before_sync();
+    __syncthreads();
+    tc::fence_after_sync();
+    const Waits wait{&gave_up_s, p.err};
+    const uint32_t tmem = tmem_s, t_dp = tmem + 256, t_dq = tmem + 384;   // S at tmem and tmem + 128
+    const uint32_t b_full = tc::smem_u32(&bars[0]), b_free = tc::smem_u32(&bars[8]), b_q = tc::smem_u32(&bars[16]), b_s = tc::smem_u32(&bars[17]),
+                   b_dp = tc::smem_u32(&bars[19]), b_done = tc::smem_u32(&bars[20]), b_ds = tc::smem_u32(&bars[21]);
+    if (warp == WG_COPY) {
+        if (lane == 0) {
+            tc::mbar_expect_tx(b_q, 2 * nb * WF_BLOCK);
+            for (int k = 0; k < nb; k++) {
+                tc::tma_rows(q_tile + k * WF_BLOCK, &p.mq, 64 * k, h, e.x + start, b_q);
+                tc::tma_rows(g_tile + k * WF_BLOCK, &p.mg, 64 * k, h, e.x + start, b_q);
+            }
+            int x = 0;
+            for (; x < 2 * tiles && !gave_up_s; x++) {   // K and V in turn
+                const int s = x % slots;
+                if (x >= slots) wait(b_free + 8 * s, (x / slots - 1) & 1);
+                if (gave_up_s) break;
+                tc::mbar_expect_tx(b_full + 8 * s, nb * WF_BLOCK);
+                for (int k = 0; k < nb; k++) tc::tma_rows(slot_tile(s) + k * WF_BLOCK, x & 1 ? &p.mv : &p.mk, 64 * k, hk, e.x + key_of(x >> 1), b_full + 8 * s);
+            }
+            wait.drain(b_q, 0);
+            for (int s = 0; s < slots; s++)
+                if (x > s) wait.drain(b_full + 8 * s, ((x - 1 - s) / slots) & 1);
+        }
+    } else if (warp == WG_PRODUCTS) {
+        if (lane == 0) {
+            constexpr bool bf = Half<T>::type == F3M_TYPE_BF16;
+            const uint32_t i_s = tc::idesc_f16(bf, 128, 128, false, false), i_d = tc::idesc_f16(bf, 128, 64 * nb, false, true);
+            auto rows = [&](uint32_t d, uint32_t q, int x, uint32_t bar) {   // q (slot's tile)^T
+                const int s = x % slots;
+                wait(b_full + 8 * s, (x / slots) & 1);
+                tc::fence_after_sync();
+                for (int k = 0; k < 4 * nb; k++)
+                    tc::mma_f16(d, tc::desc_k(q + (k >> 2) * WF_BLOCK + (k & 3) * 32), tc::desc_k(slot_tile(s) + (k >> 2) * WF_BLOCK + (k & 3) * 32), i_s, k > 0);
+                tc::mma_commit(bar);
+            };
+            auto scores = [&](int n) { rows(tmem + 128 * (n & 1), q_tile, 2 * n, b_s + 8 * (n & 1)); };
+            auto values = [&](int n) {
+                rows(t_dp, g_tile, 2 * n + 1, b_dp);
+                tc::mma_commit(b_free + 8 * ((2 * n + 1) % slots));
+            };
+            wait(b_q, 0);
+            scores(0);
+            values(0);
+            if (tiles > 1) scores(1);
+            for (int n = 0; n < tiles; n++) {
+                wait(b_ds, n & 1);
+                tc::fence_after_sync();
+                if (n + 1 < tiles) values(n + 1);
+                const int s = (2 * n) % slots;
+                for (int k = 0; k < 8; k++) tc::mma_f16_ta(t_dq, tmem + 128 * (n & 1) + operand_col(k), tc::desc_mn(slot_tile(s) + k * 2048, WF_BLOCK), i_d, n > 0 || k > 0);
+                tc::mma_commit(b_free + 8 * s);
+                if (n + 2 < tiles) scores(n + 2);
+            }
+            tc::mma_commit(b_done);
+        }
+    } else {
+        const int r = tid & 127, half = tid >> 7, i = start + r, i0 = start + 32 * (warp & 3);
+        const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
+        const int64_t at_row = h * a.s.tokens + e.x + i;
+        const float shift = i < e.y ? -p.lse2[at_row] : 0.f, dl = i < e.y ? -p.delta[at_row] : 0.f;
+        const f32x2 cc = pack2(p.c, p.c), ss = pack2(shift, shift), scale = pack2(a.scale, a.scale), dd = pack2(dl, dl);
+        for (int n = 0; n < tiles; n++) {
+            const int key = key_of(n);
+            const uint32_t t_s = tmem + 128 * (n & 1);
+            const bool whole = key + SEQ_TILE - 1 <= i0 && (i0 + 31 - key < a.window || key + SEQ_TILE <= a.sinks);
+            const int up = i - key, low = i - key - a.window, sink = a.sinks - key;   // seen: c <= up and (c > low or c < sink)
+            wait(b_s + 8 * (n & 1), (n >> 1) & 1);
+            __syncwarp();
+            tc::fence_after_sync();
+            float pr[2][32];
+#pragma unroll
+            for (int b = 0; b < 2; b++) {
+                uint32_t x[32];
+                tc::tmem_ld32(t_s + lanes + 64 * half + 32 * b, x);
+                tc::tmem_ld_wait(x);
+#pragma unroll
+                for (int c = 0; c < 32; c += 2) {
+                    unpack2(fma2(pack2(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), cc, ss), pr[b][c], pr[b][c + 1]);
+                    pr[b][c] = ex2_approx(pr[b][c]);
+                    pr[b][c + 1] = ex2_approx(pr[b][c + 1]);
+                }
+            }
+            if (key + SEQ_TILE > e.y) {   // keys of the next sequence
+                const int x = 2 * n, s = x % slots;
+                wait(b_full + 8 * s, (x / slots) & 1);
+                if (key + r >= e.y) clear_row(slot_tile(s), r, half ? 4 * nb : 0, half ? 8 * nb : 4 * nb);
+                tc::fence_async_smem();
+            }
+            wait(b_dp, n & 1);
+            __syncwarp();
+            tc::fence_after_sync();
+#pragma unroll
+            for (int b = 0; b < 2; b++) {
+                uint32_t x[32], w[16];
+                tc::tmem_ld32(t_dp + lanes + 64 * half + 32 * b, x);
+                tc::tmem_ld_wait(x);
+#pragma unroll
+                for (int c = 0; c < 32; c += 2) {
+                    float y[2];
+                    unpack2(mul2(pack2(pr[b][c], pr[b][c + 1]), fma2(pack2(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), scale, dd)), y[0], y[1]);
+                    if (!whole)
+#pragma unroll
+                        for (int k = 0; k < 2; k++) {
+                            const int at = 64 * half + 32 * b + c + k;
+                            if (!(at <= up && (at > low || at < sink))) y[k] = 0.f;
+                        }
+                    w[c >> 1] = Half<T>::pack(y[0], y[1]);
+                }
+                tc::tmem_st16(t_s + lanes + 64 * half + 16 * b, w);
+            }
+            tc::tmem_st_wait();
+            tc::fence_before_sync();
+            tc::mbar_arrive(b_ds);
+        }
+        wait(b_done, 0);
+        __syncwarp();
+        tc::fence_after_sync();
+        // over Q: the halves take its blocks in turn, at one block half of it each
+        for (int q = half * nb; q < (half + 1) * nb; q++) {
+            uint32_t o[32];
+            tc::tmem_ld32(t_dq + lanes + 32 * q, o);
+            tc::tmem_ld_wait(o);
+#pragma unroll
+            for (int c = 0; c < 32; c += 8) {
+                uint32_t y[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) y[k] = Half<T>::pack(__uint_as_float(o[c + 2 * k]), __uint_as_float(o[c + 2 * k + 1]));
+                sts16(q_tile + (q >> 1) * WF_BLOCK + tc::swz(r, 4 * (q & 1) + c / 8), y);
+            }
+        }
+        store_rows<256>(p.m0, a.dq, q_tile, h, e.x + start, min(SEQ_TILE, e.y - start), 0, nb, a.width, tid, 1);
+        if (tid == 0) tc::tma_store_wait_all();
+    }
+    __syncwarp();
+    tc::fence_before_sync();
+    __syncthreads();
+    if (warp == WG_COPY) tc::tmem_dealloc(tmem, 512);
+}
+
 template <typename T>
 static void backward_t(const WindowArgs &a, cudaStream_t s) {
-    window_rows<T, true><<<dim3(a.s.tiles * 32, a.heads), 128, 0, s>>>(a);
+    constexpr int type = Half<T>::type, bytes = WF_BLOCKS * WF_BLOCK + 1024;
+    const int64_t rows = a.s.tokens * a.heads, n = a.s.tokens;
+    F3M_REQUIRE((int64_t)a.s.tiles * a.heads <= 0x7fffffff && (rows + 15) / 16 <= 0x7fffffff, F3M_ERR_OVERFLOW, "%lld tokens of %d heads do not fit in 31 bits", (long long)n,
+                a.heads);
+    GradKernel p;
+    p.a = a;
+    p.a.window = std::min(a.window, a.s.longest);   // places and their differences stay within 31 bits
+    p.a.sinks = std::min(a.sinks, a.s.longest);
+    float *lse2 = a.delta + rows;
+    p.lse2 = lse2;
+    p.delta = a.delta;
+    window_rows_sum<T><<<(unsigned)((rows + 15) / 16), 256, 0, s>>>(a, lse2, a.delta);
     F3M_LAUNCH_CHECK();
-    window_cols<T><<<dim3(a.s.tiles * 32, a.kv_heads), 128, 0, s>>>(a);
+    p.mq = seq_tensor_map(type, a.q, n, a.heads, a.width);
+    p.mk = seq_tensor_map(type, a.k, n, a.kv_heads, a.width);
+    p.mv = seq_tensor_map(type, a.v, n, a.kv_heads, a.width);
+    p.mg = seq_tensor_map(type, a.dout, n, a.heads, a.width);
+    p.m0 = seq_tensor_map(type, a.dk, n, a.kv_heads, a.width);
+    p.m1 = seq_tensor_map(type, a.dv, n, a.kv_heads, a.width);
+    p.c = a.scale * 1.4426950408889634f;
+    p.err = seq_error_word();
+    constexpr int key_bytes = WG_KEY_BLOCKS * WF_BLOCK + 1024;
+    F3M_CUDA(cudaFuncSetAttribute(window_grad_keys<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, key_bytes));
+    window_grad_keys<T><<<a.s.tiles * a.kv_heads, WG_THREADS, key_bytes, s>>>(p);
+    F3M_LAUNCH_CHECK();
+    p.m0 = seq_tensor_map(type, a.dq, n, a.heads, a.width);
+    F3M_CUDA(cudaFuncSetAttribute(window_grad_queries<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    window_grad_queries<T><<<a.s.tiles * a.heads, WG_THREADS, bytes, s>>>(p);
     F3M_LAUNCH_CHECK();
 }
 void window_forward(int type, const WindowArgs &a, cudaStream_t s) { type == F3M_TYPE_BF16 ? forward_t<__nv_bfloat16>(a, s) : forward_t<__half>(a, s); }
