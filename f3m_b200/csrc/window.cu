@@ -6,17 +6,6 @@
 namespace f3m {
 
 template <typename T>
-__device__ __forceinline__ float dot_rows(const T *a, const T *b, int width, int lane) {
-    float s = 0.f;
-    for (int c = 2 * lane; c < width; c += 64) {
-        const float2 x = Half<T>::unpack(*reinterpret_cast<const uint32_t *>(a + c)), y = Half<T>::unpack(*reinterpret_cast<const uint32_t *>(b + c));
-        s = fmaf(x.x, y.x, fmaf(x.y, y.y, s));
-    }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    return s;
-}
-template <typename T>
 __device__ __forceinline__ T *row_of(const f3m_rows &r, int64_t t, int h) { return reinterpret_cast<T *>(r.data) + t * r.token_stride + h * r.head_stride; }
 
 // ---- forward --------------------------------------------------------------------------------------------------------------
@@ -782,43 +771,216 @@ static void backward_t(const WindowArgs &a, cudaStream_t s) {
 void window_forward(int type, const WindowArgs &a, cudaStream_t s) { type == F3M_TYPE_BF16 ? forward_t<__nv_bfloat16>(a, s) : forward_t<__half>(a, s); }
 void window_backward(int type, const WindowArgs &a, cudaStream_t s) { type == F3M_TYPE_BF16 ? backward_t<__nv_bfloat16>(a, s) : backward_t<__half>(a, s); }
 
-// A warp per (sequence, head) reads the keys that are seen one by one.
+// ---- one new token ----------------------------------------------------------------------------------------------------------
+// The cache is read once, by CTAs that each take a part of the keys of one key head for up to 16 query heads that share it; four warps take 16 keys at a
+// time in turn.  Memory is the bound, 16 operations a byte at eight heads a key head; the products run on mma.sync (m16n8k16), whose
+// fragments come straight from global memory: a contraction does not mind the order of its terms, so lane (g, t) of a warp reads 16 bytes of
+// key g, columns 32 s + 8 t .. + 7, and uses them as its terms of two steps; of the values it reads 16 bytes of keys 2t, 2t + 1, 2t + 8, 2t + 9,
+// columns 64 f + 8 g .. + 7, and output column n of tile j stands for column 64 f + 8 n + j.  Parts are joined by step_join.
+constexpr int ST_THREADS = 128, ST_HEADS = 16;
+
 template <typename T>
-__global__ void __launch_bounds__(32) step_rows(StepArgs a) {
-    const int lane = threadIdx.x, b = blockIdx.x, h = blockIdx.y, hk = h / (a.heads / a.kv_heads);
-    const int len = min(max(a.lengths[b], 0), (int)a.capacity), lo = max(0, len - a.window);
-    const T *q = row_of<T>(a.q, b, h);
-    float2 acc[2] = {};
-    float top = -INFINITY, sum = 0.f;
-    for (int j = 0; j < len; j++) {
-        if (j < lo && j >= a.sinks) j = lo;
-        const T *k = row_of<T>(a.k, j, hk) + b * a.k_seq, *v = row_of<T>(a.v, j, hk) + b * a.v_seq;
-        const float s = a.scale * dot_rows(q, k, a.width, lane), t = fmaxf(top, s), old = expf(top - t), w = expf(s - t);
-        top = t;
-        sum = sum * old + w;
+__device__ __forceinline__ void mma_16x8x16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (Half<T>::type == F3M_TYPE_BF16)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint4 load16(const void *p, bool in) {
+    uint4 v = make_uint4(0u, 0u, 0u, 0u);
+    if (in) asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+
+// DF: halves of 64 columns
+template <typename T, int DF>
+__global__ void __launch_bounds__(ST_THREADS, 3) step_keys(StepArgs a) {
+    __shared__ float stat[2][4][ST_HEADS];
+    __shared__ __align__(16) float sum_s[4][ST_HEADS][64 * DF];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const int group = a.heads / a.kv_heads, blocks = (group + ST_HEADS - 1) / ST_HEADS, hk = blockIdx.y / blocks, hb = blockIdx.y % blocks;
+    const int h0 = hk * group + hb * ST_HEADS, heads = min(ST_HEADS, group - hb * ST_HEADS), part = blockIdx.x;
+    const int64_t b = blockIdx.z;
+    // the keys seen, numbered without a gap: the sinks before the window, then the window
+    const int len = min(max(a.lengths[b], 0), (int)a.capacity), lo = max(0, len - a.window), ns = min(a.sinks, lo), seen = ns + len - lo;
+    const int per = ((seen + a.parts - 1) / a.parts + 63) / 64 * 64, v0 = (int)min((int64_t)part * per, (int64_t)seen), v1 = min(seen, v0 + per);
+    const T *kc = reinterpret_cast<const T *>(a.k.data) + b * a.k_seq + hk * a.k.head_stride, *vc = reinterpret_cast<const T *>(a.v.data) + b * a.v_seq + hk * a.v.head_stride;
+    auto key = [&](int v) { return (int64_t)(v < ns ? v : lo + v - ns); };
+
+    uint4 q[2][2 * DF];
 #pragma unroll
-        for (int p = 0; p < 2; p++) {
-            const int c = 2 * lane + 64 * p;
-            if (c < a.width) {
-                const float2 x = Half<T>::unpack(*reinterpret_cast<const uint32_t *>(v + c));
-                acc[p].x = acc[p].x * old + w * x.x;
-                acc[p].y = acc[p].y * old + w * x.y;
+    for (int r = 0; r < 2; r++)
+#pragma unroll
+        for (int s = 0; s < 2 * DF; s++) {
+            const int h = g + 8 * r, d = 32 * s + 8 * t;
+            q[r][s] = h < heads && d < a.width ? *reinterpret_cast<const uint4 *>(row_of<T>(a.q, b, h0 + h) + d) : make_uint4(0u, 0u, 0u, 0u);
+        }
+    float o[DF][8][4] = {}, top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
+    const float c = a.scale * 1.4426950408889634f;
+    for (int v = v0 + 16 * warp; v < v1; v += 64) {
+        uint4 kf[2][2 * DF], vf[DF][4];
+#pragma unroll
+        for (int n = 0; n < 2; n++) {
+            const int at = v + 8 * n + g;
+            const T *row = kc + key(at) * a.k.token_stride + 8 * t;
+#pragma unroll
+            for (int s = 0; s < 2 * DF; s++) kf[n][s] = load16(row + 32 * s, at < v1 && 32 * s + 8 * t < a.width);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int at = v + 8 * (k >> 1) + 2 * t + (k & 1);
+            const T *row = vc + key(at) * a.v.token_stride + 8 * g;
+#pragma unroll
+            for (int f = 0; f < DF; f++) vf[f][k] = load16(row + 64 * f, at < v1 && 64 * f + 8 * g < a.width);
+        }
+        float x[2][4] = {};
+#pragma unroll
+        for (int n = 0; n < 2; n++)
+#pragma unroll
+            for (int s = 0; s < 2 * DF; s++) {
+                const uint32_t a0[4] = {q[0][s].x, q[1][s].x, q[0][s].y, q[1][s].y}, a1[4] = {q[0][s].z, q[1][s].z, q[0][s].w, q[1][s].w};
+                mma_16x8x16<T>(x[n], a0, kf[n][s].x, kf[n][s].y);
+                mma_16x8x16<T>(x[n], a1, kf[n][s].z, kf[n][s].w);
+            }
+        uint32_t w[4];
+#pragma unroll
+        for (int r = 0; r < 2; r++) {   // heads g and g + 8
+            float high = top[r];
+#pragma unroll
+            for (int n = 0; n < 2; n++)
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    float &y = x[n][2 * r + i];
+                    y = v + 8 * n + 2 * t + i < v1 ? y * c : -INFINITY;
+                    high = fmaxf(high, y);
+                }
+            high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 1));
+            high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 2));
+            if (__any_sync(0xffffffffu, high > top[r])) {
+                const float f = exp2_approx(top[r] - high);   // of -inf, where nothing came before: 0
+                sum[r] *= f;
+                top[r] = high;
+#pragma unroll
+                for (int k = 0; k < DF; k++)
+#pragma unroll
+                    for (int j = 0; j < 8; j++) { o[k][j][2 * r] *= f; o[k][j][2 * r + 1] *= f; }
+            }
+#pragma unroll
+            for (int n = 0; n < 2; n++) {
+                const float y0 = exp2_approx(x[n][2 * r] - high), y1 = exp2_approx(x[n][2 * r + 1] - high);
+                sum[r] += y0 + y1;
+                w[2 * n + r] = Half<T>::pack(y0, y1);
+            }
+        }
+#pragma unroll
+        for (int f = 0; f < DF; f++) {
+            const uint32_t *v0p = reinterpret_cast<const uint32_t *>(&vf[f][0]), *v1p = reinterpret_cast<const uint32_t *>(&vf[f][1]),
+                           *v2p = reinterpret_cast<const uint32_t *>(&vf[f][2]), *v3p = reinterpret_cast<const uint32_t *>(&vf[f][3]);
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const uint32_t sel = j & 1 ? 0x7632 : 0x5410;
+                mma_16x8x16<T>(o[f][j], w, __byte_perm(v0p[j >> 1], v1p[j >> 1], sel), __byte_perm(v2p[j >> 1], v3p[j >> 1], sel));
             }
         }
     }
-    const float inv = len ? 1.f / sum : 0.f;
+    // the warps' sums, scaled to their common maximum
 #pragma unroll
-    for (int p = 0; p < 2; p++) {
-        const int c = 2 * lane + 64 * p;
-        if (c < a.width) *reinterpret_cast<uint32_t *>(row_of<T>(a.out, b, h) + c) = Half<T>::pack(acc[p].x * inv, acc[p].y * inv);
+    for (int r = 0; r < 2; r++) {
+        sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
+        sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
+        if (t == 0) { stat[0][warp][g + 8 * r] = top[r]; stat[1][warp][g + 8 * r] = sum[r]; }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < 2; r++) {
+        const int h = g + 8 * r;
+        const float high = fmaxf(fmaxf(stat[0][0][h], stat[0][1][h]), fmaxf(stat[0][2][h], stat[0][3][h]));
+        const float f = top[r] == -INFINITY ? 0.f : exp2_approx(top[r] - high);
+#pragma unroll
+        for (int k = 0; k < DF; k++)
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+#pragma unroll
+                for (int i = 0; i < 2; i++) sum_s[warp][h][64 * k + 8 * (2 * t + i) + j] = f * o[k][j][2 * r + i];
+    }
+    __syncthreads();
+    for (int x = threadIdx.x; x < heads * a.width / 2; x += ST_THREADS) {
+        const int h = 2 * x / a.width, d = 2 * x % a.width;
+        const float high = fmaxf(fmaxf(stat[0][0][h], stat[0][1][h]), fmaxf(stat[0][2][h], stat[0][3][h]));
+        float total = 0.f;
+        float2 y = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            if (stat[0][w][h] != -INFINITY) total += stat[1][w][h] * exp2_approx(stat[0][w][h] - high);
+            y.x += sum_s[w][h][d];
+            y.y += sum_s[w][h][d + 1];
+        }
+        if (a.parts == 1) {
+            const float inv = total > 0.f ? 1.f / total : 0.f;
+            *reinterpret_cast<uint32_t *>(row_of<T>(a.out, b, h0 + h) + d) = Half<T>::pack(y.x * inv, y.y * inv);
+        } else {
+            const int64_t row = (b * a.heads + h0 + h) * a.parts + part;
+            if (total > 0.f) *reinterpret_cast<float2 *>(a.part + (int64_t)a.n * a.heads * a.parts * 2 + row * a.width + d) = y;
+            if (d == 0) *reinterpret_cast<float2 *>(a.part + 2 * row) = make_float2(high, total);
+        }
     }
 }
-int window_step_parts(int, int, int, int64_t, int, int) { return 1; }
-size_t window_step_part_floats(int, int, int, int) { return 0; }
-void window_step(int type, const StepArgs &a, cudaStream_t s) {
-    if (type == F3M_TYPE_BF16) step_rows<__nv_bfloat16><<<dim3(a.n, a.heads), 32, 0, s>>>(a);
-    else step_rows<__half><<<dim3(a.n, a.heads), 32, 0, s>>>(a);
+
+// A CTA per (sequence, head): the parts' sums, scaled to their common maximum, in the order of the parts.
+template <typename T>
+__global__ void __launch_bounds__(64) step_join(StepArgs a) {
+    __shared__ float w_s[256];
+    const int64_t b = blockIdx.x / a.heads, row = (int64_t)blockIdx.x * a.parts;
+    const int h = blockIdx.x % a.heads, d = 2 * threadIdx.x;
+    const float2 *stat = reinterpret_cast<const float2 *>(a.part) + row;
+    const float *sums = a.part + (int64_t)a.n * a.heads * a.parts * 2 + row * a.width;
+    float high = -INFINITY;
+    for (int i = 0; i < a.parts; i++) high = fmaxf(high, stat[i].x);
+    for (int i = threadIdx.x; i < a.parts; i += 64) w_s[i] = stat[i].y > 0.f ? exp2_approx(stat[i].x - high) : 0.f;
+    __syncthreads();
+    if (d >= a.width) return;
+    float total = 0.f;
+    float2 y = make_float2(0.f, 0.f);
+    for (int i = 0; i < a.parts; i++) {
+        if (w_s[i] == 0.f) continue;   // its sums may not have been written
+        total += w_s[i] * stat[i].y;
+        const float2 x = *reinterpret_cast<const float2 *>(sums + (int64_t)i * a.width + d);
+        y.x = fmaf(w_s[i], x.x, y.x);
+        y.y = fmaf(w_s[i], x.y, y.y);
+    }
+    const float inv = total > 0.f ? 1.f / total : 0.f;
+    *reinterpret_cast<uint32_t *>(row_of<T>(a.out, b, h) + d) = Half<T>::pack(y.x * inv, y.y * inv);
+}
+
+// As many parts as make two waves of CTAs (three to an SM), none below 256 keys; how many keys a sequence has is known on the device only.
+int window_step_parts(int n, int heads, int kv_heads, int64_t capacity, int window, int sinks) {
+    const int64_t most = std::min<int64_t>(capacity, (int64_t)window + sinks), blocks = (heads / kv_heads + ST_HEADS - 1) / ST_HEADS;
+    const int64_t ctas = (int64_t)n * kv_heads * blocks, want = (6 * NUM_SMS_HINT + ctas - 1) / ctas;
+    return (int)std::max<int64_t>(1, std::min<int64_t>({want, (most + 255) / 256, 256}));
+}
+size_t window_step_part_floats(int n, int heads, int width, int parts) { return parts == 1 ? 0 : (size_t)n * heads * parts * (width + 2); }
+
+template <typename T>
+static void step_t(const StepArgs &a, cudaStream_t s) {
+    const int blocks = (a.heads / a.kv_heads + ST_HEADS - 1) / ST_HEADS;
+    F3M_REQUIRE(a.n <= 65535 && (int64_t)a.kv_heads * blocks <= 65535 && (int64_t)a.n * a.heads <= 0x7fffffff, F3M_ERR_UNSUPPORTED, "%d sequences of %d heads in one call", a.n,
+                a.heads);
+    const dim3 grid(a.parts, a.kv_heads * blocks, a.n);
+    if (a.width <= 64) step_keys<T, 1><<<grid, ST_THREADS, 0, s>>>(a);
+    else step_keys<T, 2><<<grid, ST_THREADS, 0, s>>>(a);
     F3M_LAUNCH_CHECK();
+    if (a.parts > 1) {
+        step_join<T><<<a.n * a.heads, 64, 0, s>>>(a);
+        F3M_LAUNCH_CHECK();
+    }
+}
+void window_step(int type, const StepArgs &a, cudaStream_t s) {
+    StepArgs b = a;
+    b.window = (int)std::min<int64_t>(a.window, std::max<int64_t>(a.capacity, 1));   // numbers of keys stay within 31 bits
+    b.sinks = (int)std::min<int64_t>(a.sinks, a.capacity);
+    type == F3M_TYPE_BF16 ? step_t<__nv_bfloat16>(b, s) : step_t<__half>(b, s);
 }
 
 }  // namespace f3m
