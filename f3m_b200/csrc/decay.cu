@@ -95,7 +95,7 @@ __device__ __forceinline__ void split_rows(uint32_t head, uint32_t tail, uint32_
         if (PARTS == 3) sts16(rest + at, z);
     }
 }
-template <typename T, int PARTS>
+template <typename T, int PARTS, int NB>
 __global__ void __launch_bounds__(DK_THREADS, 1) decay_tiles(const __grid_constant__ DecayKernel p) {
     extern __shared__ unsigned char raw[];
     __shared__ __align__(8) uint64_t bars[2 * 4 + 8];
@@ -103,9 +103,9 @@ __global__ void __launch_bounds__(DK_THREADS, 1) decay_tiles(const __grid_consta
     __shared__ int gave_up_s;
     __shared__ __align__(16) float pw[32], pr[32];   // decay^n, decay^(31 - n)
     const DecayArgs &a = p.a;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, h = blockIdx.y;
-    const int nb = (a.width_b + 63) / 64, nc = (a.width_c + 63) / 64;
-    const int stage_blocks = 2 * nb + nc, stages = min(4, (DK_TILES - max(nb, nc)) / stage_blocks);
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, h = blockIdx.y;
+    const int nc = (a.width_c + 63) / 64;
+    const int stage_blocks = 2 * NB + nc, stages = min(4, (DK_TILES - max(NB, nc)) / stage_blocks);
     const uint32_t smem = (tc::smem_u32(raw) + 1023) & ~1023u, state_s = smem + stages * stage_blocks * DK_BLOCK;
     const float l2 = log2_decay(a.log_decay[h]);
     const int first = blockIdx.x * p.per_range, tiles = min(a.s.tiles, first + p.per_range) - first;
@@ -140,8 +140,8 @@ __global__ void __launch_bounds__(DK_THREADS, 1) decay_tiles(const __grid_consta
                    b_moved = tc::smem_u32(&bars[10]), b_done = tc::smem_u32(&bars[11]), b_weights = tc::smem_u32(&bars[12]), b_split = tc::smem_u32(&bars[13]),
                    b_state = tc::smem_u32(&bars[14]), b_read = tc::smem_u32(&bars[15]);
     auto a_tile = [&](int s) { return smem + s * stage_blocks * DK_BLOCK; };
-    auto b_tile = [&](int s) { return a_tile(s) + nb * DK_BLOCK; };
-    auto c_tile = [&](int s) { return a_tile(s) + 2 * nb * DK_BLOCK; };
+    auto b_tile = [&](int s) { return a_tile(s) + NB * DK_BLOCK; };
+    auto c_tile = [&](int s) { return a_tile(s) + 2 * NB * DK_BLOCK; };
     auto all_wait = [&](uint32_t bar, uint32_t parity) {   // a whole warp, which stays together for the instructions that need that
         wait(bar, parity);
         __syncwarp();
@@ -157,7 +157,7 @@ __global__ void __launch_bounds__(DK_THREADS, 1) decay_tiles(const __grid_consta
                 if (n >= stages) wait(b_free + 8 * s, (n / stages - 1) & 1);
                 if (gave_up_s) break;
                 tc::mbar_expect_tx(b_full + 8 * s, stage_blocks * DK_BLOCK);
-                for (int k = 0; k < nb; k++) {
+                for (int k = 0; k < NB; k++) {
                     tc::tma_rows(a_tile(s) + k * DK_BLOCK, &p.ma, 64 * k, h, e.x + e.z, b_full + 8 * s);
                     tc::tma_rows(b_tile(s) + k * DK_BLOCK, &p.mb, 64 * k, h, e.x + e.z, b_full + 8 * s);
                 }
@@ -168,33 +168,36 @@ __global__ void __launch_bounds__(DK_THREADS, 1) decay_tiles(const __grid_consta
         }
     } else if (warp == DK_PRODUCTS) {
         // ---- products ----
-        if (lane == 0) {
-            constexpr bool bf = Half<T>::type == F3M_TYPE_BF16;
-            const uint32_t i_score = tc::idesc_f16(bf, 128, 128, false, false), i_rows = tc::idesc_f16(bf, 128, 64 * nc, false, true),
-                           i_state = tc::idesc_f16(bf, 128, 64 * nc, true, true);
-            for (int n = 0; n < tiles; n++) {
-                const int s = n % stages;
-                wait(b_full + 8 * s, (n / stages) & 1);
-                tc::fence_after_sync();
-                for (int k = 0; k < 4 * nb; k++)
-                    tc::mma_f16(t_score, tc::desc_k(a_tile(s) + (k >> 2) * DK_BLOCK + (k & 3) * 32), tc::desc_k(b_tile(s) + (k >> 2) * DK_BLOCK + (k & 3) * 32), i_score, k > 0);
+        constexpr bool bf = Half<T>::type == F3M_TYPE_BF16;
+        const uint32_t i_score = tc::idesc_f16(bf, 128, 128, false, false), i_rows = tc::idesc_f16(bf, 128, 64 * nc, false, true),
+                       i_state = tc::idesc_f16(bf, 128, 64 * nc, true, true);
+        for (int n = 0; n < tiles; n++) {
+            const int s = n % stages;
+            wait(b_full + 8 * s, (n / stages) & 1);
+            tc::fence_after_sync();
+            if (tc::elect()) {
+                tc::product_rows<NB>(t_score, a_tile(s), b_tile(s), i_score);
                 tc::mma_commit(b_score);
-                if (n) wait(b_read, (n - 1) & 1);
-                wait(b_state, n & 1);
-                tc::fence_after_sync();
-                for (int k = 0; k < 4 * nb; k++)
-                    tc::mma_f16(t_inter, tc::desc_k(a_tile(s) + (k >> 2) * DK_BLOCK + (k & 3) * 32), tc::desc_mn(state_s + k * 2048, DK_BLOCK), i_rows, k > 0);
+            }
+            if (n) wait(b_read, (n - 1) & 1);
+            wait(b_state, n & 1);
+            tc::fence_after_sync();
+            if (tc::elect()) {
+                tc::product_mixed<NB>(t_inter, a_tile(s), state_s, i_rows);
                 tc::mma_commit(b_inter);
-                wait(b_split, n & 1);   // also clears the rows of C that belong to another sequence
-                tc::fence_after_sync();
-                for (int part = 0; part < PARTS; part++) {
-                    const uint32_t rows = part == 0 ? b_tile(s) : part == 1 ? a_tile(s) : state_s;
-                    for (int k = 0; k < 8; k++) tc::mma_f16(t_state, tc::desc_mn(rows + k * 2048, DK_BLOCK), tc::desc_mn(c_tile(s) + k * 2048, DK_BLOCK), i_state, 1);
-                }
+            }
+            wait(b_split, n & 1);   // also clears the rows of C that belong to another sequence
+            tc::fence_after_sync();
+            if (tc::elect()) {
+                tc::product_cols<true>(t_state, b_tile(s), c_tile(s), i_state);
+                tc::product_cols<true>(t_state, a_tile(s), c_tile(s), i_state);
+                if (PARTS == 3) tc::product_cols<true>(t_state, state_s, c_tile(s), i_state);
                 tc::mma_commit(b_moved);
-                wait(b_weights, n & 1);
-                tc::fence_after_sync();
-                for (int k = 0; k < 8; k++) tc::mma_f16_ta(t_intra, t_score + 8 * k, tc::desc_mn(c_tile(s) + k * 2048, DK_BLOCK), i_rows, k > 0);
+            }
+            wait(b_weights, n & 1);
+            tc::fence_after_sync();
+            if (tc::elect()) {
+                tc::product_tmem<false>(t_intra, t_score, c_tile(s), i_rows);
                 tc::mma_commit(b_done);
                 tc::mma_commit(b_free + 8 * s);
             }
@@ -340,7 +343,7 @@ __global__ void __launch_bounds__(DK_THREADS, 1) decay_tiles(const __grid_consta
             all_wait(b_full + 8 * s, (n / stages) & 1);
             all_wait(b_inter, n & 1);   // A, B and the state's operand have been read
             const float f = a.upd * exp2f(l2 * (a.reversed ? j + 1 : max(m - 1 - j, 0)));   // rows behind the sequence: a number, to be times 0
-            split_rows<T, PARTS>(b_tile(s), a_tile(s), state_s, j, j < m, pack2(f, f), 4 * nb * half, 4 * nb * (half + 1));
+            split_rows<T, PARTS>(b_tile(s), a_tile(s), state_s, j, j < m, pack2(f, f), 4 * NB * half, 4 * NB * (half + 1));
             if (j >= m) clear_row(c_tile(s), j, 4 * nc * half, 4 * nc * (half + 1));
             tc::fence_async_smem();
             tc::mbar_arrive(b_split);
@@ -369,17 +372,17 @@ __global__ void __launch_bounds__(DK_THREADS, 1) decay_tiles(const __grid_consta
 // What the range adds to the state of the sequence that runs on into the next range, from zero or from where the sequence begins.  The rows
 // of B are scaled to the end of the range at once, so that the state gathers in tensor memory without being touched between tiles: splitting a
 // tile runs beside the products of the one before.
-template <typename T, int PARTS>
+template <typename T, int PARTS, int NB>
 __global__ void __launch_bounds__(DS_THREADS, 1) decay_states(const __grid_constant__ DecayKernel p) {
     extern __shared__ unsigned char raw[];
     __shared__ __align__(8) uint64_t bars[2 * 4 + 3];
     __shared__ uint32_t tmem_s;
     __shared__ int gave_up_s;
     const DecayArgs &a = p.a;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, h = blockIdx.y;
-    const int nb = (a.width_b + 63) / 64, nc = (a.width_c + 63) / 64, stage_blocks = nb + nc, parts_blocks = (PARTS - 1) * nb;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, h = blockIdx.y;
+    const int nc = (a.width_c + 63) / 64, stage_blocks = NB + nc, parts_blocks = (PARTS - 1) * NB;
     // a product reads 128 columns of B, with one block of them the block behind it too: what it finds there goes to rows of the state that are not used
-    const int stages = min(4, (DK_TILES - parts_blocks - (nb == 1)) / stage_blocks);
+    const int stages = min(4, (DK_TILES - parts_blocks - (NB == 1)) / stage_blocks);
     const uint32_t smem = (tc::smem_u32(raw) + 1023) & ~1023u, parts_s = smem + stages * stage_blocks * DK_BLOCK;
     const float l2 = log2_decay(a.log_decay[h]);
     const int last = min(a.s.tiles, (int)(blockIdx.x + 1) * p.per_range);
@@ -406,7 +409,7 @@ __global__ void __launch_bounds__(DS_THREADS, 1) decay_states(const __grid_const
     const uint32_t b_full = tc::smem_u32(&bars[0]), b_free = tc::smem_u32(&bars[4]), b_split = tc::smem_u32(&bars[8]), b_tails = tc::smem_u32(&bars[9]),
                    b_done = tc::smem_u32(&bars[10]);
     auto b_tile = [&](int s) { return smem + s * stage_blocks * DK_BLOCK; };
-    auto c_tile = [&](int s) { return b_tile(s) + nb * DK_BLOCK; };
+    auto c_tile = [&](int s) { return b_tile(s) + NB * DK_BLOCK; };
     if (warp == 8) {
         if (lane == 0) {
             int n = 0;
@@ -416,29 +419,29 @@ __global__ void __launch_bounds__(DS_THREADS, 1) decay_states(const __grid_const
                 if (n >= stages) wait(b_free + 8 * s, (n / stages - 1) & 1);
                 if (gave_up_s) break;
                 tc::mbar_expect_tx(b_full + 8 * s, stage_blocks * DK_BLOCK);
-                for (int k = 0; k < nb; k++) tc::tma_rows(b_tile(s) + k * DK_BLOCK, &p.mb, 64 * k, h, e.x + e.z, b_full + 8 * s);
+                for (int k = 0; k < NB; k++) tc::tma_rows(b_tile(s) + k * DK_BLOCK, &p.mb, 64 * k, h, e.x + e.z, b_full + 8 * s);
                 for (int k = 0; k < nc; k++) tc::tma_rows(c_tile(s) + k * DK_BLOCK, &p.mc, 64 * k, h, e.x + e.z, b_full + 8 * s);
             }
             for (int s = 0; s < stages; s++)
                 if (n > s) wait.drain(b_full + 8 * s, ((n - 1 - s) / stages) & 1);
         }
     } else if (warp == 9) {
-        if (lane == 0) {
-            const uint32_t i_state = tc::idesc_f16(Half<T>::type == F3M_TYPE_BF16, 128, 64 * nc, true, true);
-            for (int n = 0; n < tiles; n++) {
-                const int s = n % stages;
-                wait(b_full + 8 * s, (n / stages) & 1);
-                wait(b_split, n & 1);
-                tc::fence_after_sync();
-                for (int part = PARTS - 1; part >= 0; part--) {
-                    const uint32_t rows = part == 0 ? b_tile(s) : parts_s + (part - 1) * nb * DK_BLOCK;
-                    for (int k = 0; k < 8; k++)
-                        tc::mma_f16(t_state, tc::desc_mn(rows + k * 2048, DK_BLOCK), tc::desc_mn(c_tile(s) + k * 2048, DK_BLOCK), i_state, n > 0 || part < PARTS - 1 || k > 0);
-                    if (part == 1) tc::mma_commit(b_tails);
-                }
+        const uint32_t i_state = tc::idesc_f16(Half<T>::type == F3M_TYPE_BF16, 128, 64 * nc, true, true);
+        for (int n = 0; n < tiles; n++) {
+            const int s = n % stages;
+            wait(b_full + 8 * s, (n / stages) & 1);
+            wait(b_split, n & 1);
+            tc::fence_after_sync();
+            if (tc::elect()) {
+                const uint32_t last_part = parts_s + (PARTS - 2) * NB * DK_BLOCK;
+                if (n) tc::product_cols<true>(t_state, last_part, c_tile(s), i_state);
+                else tc::product_cols<false>(t_state, last_part, c_tile(s), i_state);
+                if (PARTS == 3) tc::product_cols<true>(t_state, parts_s, c_tile(s), i_state);
+                tc::mma_commit(b_tails);
+                tc::product_cols<true>(t_state, b_tile(s), c_tile(s), i_state);
                 tc::mma_commit(b_free + 8 * s);
+                if (n + 1 == tiles) tc::mma_commit(b_done);
             }
-            tc::mma_commit(b_done);
         }
     } else {
         const int j = tid & 127, half = tid >> 7;
@@ -448,7 +451,7 @@ __global__ void __launch_bounds__(DS_THREADS, 1) decay_states(const __grid_const
             const float f = a.upd * exp2f(l2 * (a.reversed ? e.z + j + 1 - stop : stop - 1 - e.z - j));
             wait(b_full + 8 * s, (n / stages) & 1);
             if (n) wait(b_tails, (n - 1) & 1);
-            split_rows<T, PARTS>(b_tile(s), parts_s, parts_s + nb * DK_BLOCK, j, j < m, pack2(f, f), 4 * nb * half, 4 * nb * (half + 1));
+            split_rows<T, PARTS>(b_tile(s), parts_s, parts_s + NB * DK_BLOCK, j, j < m, pack2(f, f), 4 * NB * half, 4 * NB * (half + 1));
             if (j >= m) clear_row(c_tile(s), j, 4 * nc * half, 4 * nc * (half + 1));
             tc::fence_async_smem();
             tc::mbar_arrive(b_split);
@@ -531,18 +534,18 @@ size_t decay_workspace(const f3m_seqs &s, int heads, int width_b, int width_c) {
     return r == 1 ? 0 : (size_t)r * heads * width_b * width_c * sizeof(float);
 }
 
-template <typename T, int PARTS>
+template <typename T, int PARTS, int NB>
 static void launch_parts(const DecayKernel &p, cudaStream_t s) {
     constexpr int bytes = DK_TILES * DK_BLOCK + 1024;
     if (p.ranges > 1) {
-        F3M_CUDA(cudaFuncSetAttribute(decay_states<T, PARTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-        decay_states<T, PARTS><<<dim3(p.ranges - 1, p.a.heads), DS_THREADS, bytes, s>>>(p);
+        F3M_CUDA(cudaFuncSetAttribute(decay_states<T, PARTS, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+        decay_states<T, PARTS, NB><<<dim3(p.ranges - 1, p.a.heads), DS_THREADS, bytes, s>>>(p);
         F3M_LAUNCH_CHECK();
         decay_join<<<dim3((p.a.width_b * p.a.width_c / 4 + 255) / 256, p.a.heads), 256, 0, s>>>(p);
         F3M_LAUNCH_CHECK();
     }
-    F3M_CUDA(cudaFuncSetAttribute(decay_tiles<T, PARTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-    decay_tiles<T, PARTS><<<dim3(p.ranges, p.a.heads), DK_THREADS, bytes, s>>>(p);
+    F3M_CUDA(cudaFuncSetAttribute(decay_tiles<T, PARTS, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    decay_tiles<T, PARTS, NB><<<dim3(p.ranges, p.a.heads), DK_THREADS, bytes, s>>>(p);
     F3M_LAUNCH_CHECK();
 }
 
@@ -566,9 +569,9 @@ static void decay_product_t(const DecayArgs &a, cudaStream_t s) {
     p.err = seq_error_word();
     // a state that is returned in FP32 takes three parts of bf16
     if constexpr (Half<T>::type == F3M_TYPE_BF16) {
-        if (a.state_out) return launch_parts<T, 3>(p, s);
+        if (a.state_out) return a.width_b <= 64 ? launch_parts<T, 3, 1>(p, s) : launch_parts<T, 3, 2>(p, s);
     }
-    launch_parts<T, 2>(p, s);
+    a.width_b <= 64 ? launch_parts<T, 2, 1>(p, s) : launch_parts<T, 2, 2>(p, s);
 }
 void decay_product(int type, const DecayArgs &a, cudaStream_t s) { type == F3M_TYPE_BF16 ? decay_product_t<__nv_bfloat16>(a, s) : decay_product_t<__half>(a, s); }
 

@@ -124,20 +124,63 @@ __host__ __device__ constexpr uint32_t idesc_f16(bool bf16, int M, int N, bool a
     return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((amn ? 1u : 0u) << 15) | ((bmn ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) |
            ((uint32_t)(M >> 4) << 24);
 }
-__device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+template <bool ACC>
+__device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc) {
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "n"(ACC ? 1 : 0)
         : "memory");
 }
 // A from tensor memory: row r in lane r, two consecutive elements of the contraction per 32-bit column
-__device__ __forceinline__ void mma_f16_ta(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+template <bool ACC>
+__device__ __forceinline__ void mma_f16_ta(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc) {
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem), "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem), "r"(a_tmem), "l"(bdesc), "r"(idesc), "n"(ACC ? 1 : 0)
         : "memory");
+}
+// One lane of a whole warp: the values that its instructions take are the warp's, and stay in uniform registers
+__device__ __forceinline__ bool elect() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one;
+}
+// Products of whole tiles (128 rows; blocks of 64 columns, 16384 bytes each), issued by one thread.  A thread issues an instruction every few clocks
+// and a step of a product takes 64: the loops are unrolled and a step's operands are the first one's plus a constant.  ACC: added to D.
+constexpr int BLOCK = 128 * 128;
+// D = A B^T: both contract along their columns, NB blocks of them
+template <int NB, bool ACC = false>
+__device__ __forceinline__ void product_rows(uint32_t d, uint32_t a_tile, uint32_t b_tile, uint32_t idesc) {
+    const uint64_t a = desc_k(a_tile), b = desc_k(b_tile);
+    mma_f16<ACC>(d, a, b, idesc);
+#pragma unroll
+    for (int k = 1; k < 4 * NB; k++) mma_f16<true>(d, a + (k >> 2) * (BLOCK >> 4) + (k & 3) * 2, b + (k >> 2) * (BLOCK >> 4) + (k & 3) * 2, idesc);
+}
+// D = A B: A contracts along its columns, NB blocks of them, B along its rows
+template <int NB, bool ACC = false>
+__device__ __forceinline__ void product_mixed(uint32_t d, uint32_t a_tile, uint32_t b_tile, uint32_t idesc) {
+    const uint64_t a = desc_k(a_tile), b = desc_mn(b_tile, BLOCK);
+    mma_f16<ACC>(d, a, b, idesc);
+#pragma unroll
+    for (int k = 1; k < 4 * NB; k++) mma_f16<true>(d, a + (k >> 2) * (BLOCK >> 4) + (k & 3) * 2, b + k * (2048 >> 4), idesc);
+}
+// D = A^T B: both contract along their rows
+template <bool ACC>
+__device__ __forceinline__ void product_cols(uint32_t d, uint32_t a_tile, uint32_t b_tile, uint32_t idesc) {
+    const uint64_t a = desc_mn(a_tile, BLOCK), b = desc_mn(b_tile, BLOCK);
+    mma_f16<ACC>(d, a, b, idesc);
+#pragma unroll
+    for (int k = 1; k < 8; k++) mma_f16<true>(d, a + k * (2048 >> 4), b + k * (2048 >> 4), idesc);
+}
+// D = A B: A, 128 x 128, from tensor memory, its second 64 elements a row GAP columns behind the first; B contracts along its rows
+template <bool ACC, int GAP = 32>
+__device__ __forceinline__ void product_tmem(uint32_t d, uint32_t a_tmem, uint32_t b_tile, uint32_t idesc) {
+    const uint64_t b = desc_mn(b_tile, BLOCK);
+    mma_f16_ta<ACC>(d, a_tmem, b, idesc);
+#pragma unroll
+    for (int k = 1; k < 8; k++) mma_f16_ta<true>(d, a_tmem + 8 * (k & 3) + GAP * (k >> 2), b + k * (2048 >> 4), idesc);
 }
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
     asm volatile(

@@ -61,19 +61,19 @@ __device__ __forceinline__ WindowItem window_item(const WindowKernel &p, int i) 
     return w;
 }
 
-template <typename T>
+template <typename T, int NB>
 __global__ void __launch_bounds__(WF_THREADS, 1) window_tiles(const __grid_constant__ WindowKernel p) {
     extern __shared__ unsigned char raw[];
     __shared__ __align__(8) uint64_t bars[2 * 8 + 2 + 8];
     __shared__ uint32_t tmem_s;
     __shared__ int gave_up_s;
     const WindowArgs &a = p.a;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, nb = (a.width + 63) / 64;
-    const int slots = min(8, (WF_BLOCKS - 2 * nb - 2) / nb);   // 4 at two blocks, 8 at one
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+    constexpr int slots = NB == 2 ? 4 : 8;
     const uint32_t smem = (tc::smem_u32(raw) + 1023) & ~1023u;
-    auto q_tile = [&](int t) { return smem + t * nb * WF_BLOCK; };
-    auto slot_tile = [&](int s) { return smem + (2 + s) * nb * WF_BLOCK; };
-    const uint32_t stage = smem + (2 + slots) * nb * WF_BLOCK;
+    auto q_tile = [&](int t) { return smem + t * NB * WF_BLOCK; };
+    auto slot_tile = [&](int s) { return smem + (2 + s) * NB * WF_BLOCK; };
+    const uint32_t stage = smem + (2 + slots) * NB * WF_BLOCK;
 
     if (warp == WF_COPY) tc::tmem_alloc(tc::smem_u32(&tmem_s), 512);
     if (tid == 0) {
@@ -102,16 +102,16 @@ __global__ void __launch_bounds__(WF_THREADS, 1) window_tiles(const __grid_const
                 const WindowItem w = window_item(p, it);
                 if (items) wait(b_q_free, (items - 1) & 1);
                 if (gave_up_s) break;
-                tc::mbar_expect_tx(b_q, w.tiles_q * nb * WF_BLOCK);
+                tc::mbar_expect_tx(b_q, w.tiles_q * NB * WF_BLOCK);
                 for (int t = 0; t < w.tiles_q; t++)
-                    for (int k = 0; k < nb; k++)
+                    for (int k = 0; k < NB; k++)
                         tc::tma_rows(q_tile(t) + k * WF_BLOCK, &p.mq, 64 * k, w.head[t], w.row0 + w.start + (p.by_heads ? 0 : t * SEQ_TILE), b_q);
                 for (int j = 0; j < 2 * w.keys && !gave_up_s; j++, x++) {
                     const int s = x % slots;
                     if (x >= slots) wait(b_free + 8 * s, (x / slots - 1) & 1);
                     if (gave_up_s) break;
-                    tc::mbar_expect_tx(b_full + 8 * s, nb * WF_BLOCK);
-                    for (int k = 0; k < nb; k++) tc::tma_rows(slot_tile(s) + k * WF_BLOCK, j & 1 ? &p.mv : &p.mk, 64 * k, w.kv_head, w.row0 + w.key(j >> 1), b_full + 8 * s);
+                    tc::mbar_expect_tx(b_full + 8 * s, NB * WF_BLOCK);
+                    for (int k = 0; k < NB; k++) tc::tma_rows(slot_tile(s) + k * WF_BLOCK, j & 1 ? &p.mv : &p.mk, 64 * k, w.kv_head, w.row0 + w.key(j >> 1), b_full + 8 * s);
                 }
             }
             for (int s = 0; s < slots; s++)   // the last copies
@@ -119,53 +119,54 @@ __global__ void __launch_bounds__(WF_THREADS, 1) window_tiles(const __grid_const
             if (items) wait.drain(b_q, (items - 1) & 1);
         }
     } else if (warp == WF_PRODUCTS) {
-        if (lane == 0) {
-            constexpr bool bf = Half<T>::type == F3M_TYPE_BF16;
-            // a negative scale turns S's sign: bit 13 negates A
-            const uint32_t i_s = tc::idesc_f16(bf, 128, 128, false, false) | (a.scale < 0.f ? 1u << 13 : 0u), i_o = tc::idesc_f16(bf, 128, 64 * nb, false, true);
-            int x = 0, items = 0, np[2] = {0, 0}, no[2] = {0, 0};
-            auto scores = [&](int t, int s) {
-                for (int k = 0; k < 4 * nb; k++)
-                    tc::mma_f16(tmem + 128 * t, tc::desc_k(q_tile(t) + (k >> 2) * WF_BLOCK + (k & 3) * 32), tc::desc_k(slot_tile(s) + (k >> 2) * WF_BLOCK + (k & 3) * 32), i_s, k > 0);
-                tc::mma_commit(b_s + 8 * t);
-            };
-            for (int it = blockIdx.x; it < p.items; it += gridDim.x, items++) {
-                const WindowItem w = window_item(p, it);
-                wait(b_q, items & 1);
-                int sk = x % slots;
-                wait(b_full + 8 * sk, (x / slots) & 1);
-                tc::fence_after_sync();
-                for (int t = 0; t < w.tiles_q; t++) scores(t, sk);
+        constexpr bool bf = Half<T>::type == F3M_TYPE_BF16;
+        // a negative scale turns S's sign: bit 13 negates A
+        const uint32_t i_s = tc::idesc_f16(bf, 128, 128, false, false) | (a.scale < 0.f ? 1u << 13 : 0u), i_o = tc::idesc_f16(bf, 128, 64 * NB, false, true);
+        int x = 0, items = 0, np[2] = {0, 0}, no[2] = {0, 0};
+        for (int it = blockIdx.x; it < p.items; it += gridDim.x, items++) {
+            const WindowItem w = window_item(p, it);
+            wait(b_q, items & 1);
+            int sk = x % slots;
+            wait(b_full + 8 * sk, (x / slots) & 1);
+            tc::fence_after_sync();
+            if (tc::elect()) {
+                for (int t = 0; t < w.tiles_q; t++) {
+                    tc::product_rows<NB>(tmem + 128 * t, q_tile(t), slot_tile(sk), i_s);
+                    tc::mma_commit(b_s + 8 * t);
+                }
                 tc::mma_commit(b_free + 8 * sk);
                 if (w.keys == 1) tc::mma_commit(b_q_free);
-                for (int j = 0; j < w.keys; j++) {
-                    const int xv = x + 2 * j + 1, sv = xv % slots;
-                    const bool more = j + 1 < w.keys;
-                    sk = (xv + 1) % slots;
-                    for (int t = 0; t < w.tiles_q; t++) {
-                        if (t == 0) wait(b_full + 8 * sv, (xv / slots) & 1);
-                        if (j == 0 && no[t]) wait(b_o_read + 8 * t, (no[t] - 1) & 1);
-                        wait(b_p + 8 * t, np[t] & 1);
-                        np[t]++;
-                        tc::fence_after_sync();
-                        for (int k = 0; k < 8; k++) tc::mma_f16_ta(tmem + 256 + 128 * t, tmem + 128 * t + 8 * k, tc::desc_mn(slot_tile(sv) + k * 2048, WF_BLOCK), i_o, j > 0 || k > 0);
+            }
+            for (int j = 0; j < w.keys; j++) {
+                const int xv = x + 2 * j + 1, sv = xv % slots;
+                const bool more = j + 1 < w.keys;
+                sk = (xv + 1) % slots;
+                wait(b_full + 8 * sv, (xv / slots) & 1);
+                if (more) wait(b_full + 8 * sk, ((xv + 1) / slots) & 1);
+                for (int t = 0; t < w.tiles_q; t++) {
+                    if (j == 0 && no[t]) wait(b_o_read + 8 * t, (no[t] - 1) & 1);
+                    wait(b_p + 8 * t, np[t] & 1);
+                    np[t]++;
+                    no[t] += !more;
+                    tc::fence_after_sync();
+                    if (tc::elect()) {
+                        if (j) tc::product_tmem<true>(tmem + 256 + 128 * t, tmem + 128 * t, slot_tile(sv), i_o);
+                        else tc::product_tmem<false>(tmem + 256 + 128 * t, tmem + 128 * t, slot_tile(sv), i_o);
                         if (more) {
-                            if (t == 0) {
-                                wait(b_full + 8 * sk, ((xv + 1) / slots) & 1);
-                                tc::fence_after_sync();
-                            }
-                            scores(t, sk);
+                            tc::product_rows<NB>(tmem + 128 * t, q_tile(t), slot_tile(sk), i_s);
+                            tc::mma_commit(b_s + 8 * t);
                         } else {
                             tc::mma_commit(b_o + 8 * t);
-                            no[t]++;
                         }
                     }
+                }
+                if (tc::elect()) {
                     tc::mma_commit(b_free + 8 * sv);
                     if (more) tc::mma_commit(b_free + 8 * sk);
                     if (j + 2 == w.keys) tc::mma_commit(b_q_free);
                 }
-                x += 2 * w.keys;
             }
+            x += 2 * w.keys;
         }
     } else {
         // ---- weights: thread r of a query tile has its row r ----
@@ -216,7 +217,7 @@ __global__ void __launch_bounds__(WF_THREADS, 1) window_tiles(const __grid_const
                         const float f = rise ? exp2_approx((top - high) * p.c) : 1.f;
                         if (rise) { top = high; sum *= f; }
                         if (j > 0)
-                            for (int q = 0; q < 2 * nb; q++) {
+                            for (int q = 0; q < 2 * NB; q++) {
                                 uint32_t o[32];
                                 tc::tmem_ld32(t_o + 32 * q, o);
                                 tc::tmem_ld_wait(o);
@@ -254,7 +255,7 @@ __global__ void __launch_bounds__(WF_THREADS, 1) window_tiles(const __grid_const
                     if (t == 0 && key + SEQ_TILE > w.len) {   // the sequence ends inside the tile
                         const int xv = x + 2 * j + 1, sv = xv % slots;
                         wait(b_full + 8 * sv, (xv / slots) & 1);
-                        if (key + r >= w.len) clear_row(slot_tile(sv), r, 0, 8 * nb);
+                        if (key + r >= w.len) clear_row(slot_tile(sv), r, 0, 8 * NB);
                         tc::fence_async_smem();
                         __syncwarp();
                     }
@@ -268,12 +269,12 @@ __global__ void __launch_bounds__(WF_THREADS, 1) window_tiles(const __grid_const
                 tc::fence_after_sync();
                 const int m = min(SEQ_TILE, w.len - start);
                 const float inv = 1.f / sum;
-                for (int q = 0; q < 2 * nb; q++) {
+                for (int q = 0; q < 2 * NB; q++) {
                     uint32_t o[32];
                     __syncwarp();
                     tc::tmem_ld32(t_o + 32 * q, o);
                     tc::tmem_ld_wait(o);
-                    if (q + 1 == 2 * nb) {
+                    if (q + 1 == 2 * NB) {
                         tc::fence_before_sync();
                         tc::mbar_arrive(b_o_read + 8 * t);
                     }
@@ -318,8 +319,9 @@ static void forward_t(const WindowArgs &a, cudaStream_t s) {
     p.c = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1e-30f);   // a scale of zero: all weights are one
     p.err = seq_error_word();
     constexpr int bytes = WF_BLOCKS * WF_BLOCK + 1024;
-    F3M_CUDA(cudaFuncSetAttribute(window_tiles<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-    window_tiles<T><<<std::min(p.items, NUM_SMS_HINT), WF_THREADS, bytes, s>>>(p);
+    auto kernel = a.width <= 64 ? window_tiles<T, 1> : window_tiles<T, 2>;
+    F3M_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    kernel<<<std::min(p.items, NUM_SMS_HINT), WF_THREADS, bytes, s>>>(p);
     F3M_LAUNCH_CHECK();
 }
 // ---- gradients ------------------------------------------------------------------------------------------------------------
@@ -353,9 +355,7 @@ __global__ void __launch_bounds__(256) window_rows_sum(WindowArgs a, float *lse2
 }
 
 constexpr int WG_COPY = 8, WG_PRODUCTS = 9, WG_THREADS = 320, WG_KEY_BLOCKS = 12;
-// Two threads share a row of scores, 64 columns each, and write their 16-bit operands over the first of their own: step k of the contraction
-// (16 elements, 8 columns) begins at this column
-__device__ __forceinline__ uint32_t operand_col(int k) { return 8 * (k & 3) + 64 * (k >> 2); }
+// Two threads share a row of scores, 64 columns each, and write their 16-bit operands over the first 32 of their own.
 struct GradKernel {
     WindowArgs a;
     CUtensorMap mq, mk, mv, mg, m0, m1;   // q, k, v, dout; the outputs: dk and dv, or dq
@@ -367,7 +367,7 @@ struct GradKernel {
 // A CTA has a tile of 128 keys (rows of tensor memory) and walks over tiles of 128 queries (columns).  Of the products of query tile n,
 //     S^T = K Q^T (n + 1)  follows  dV += P^T dout (n),     dP^T = V dout^T (n + 1)  follows  dK += dS^T Q (n),
 // so that the weights of n + 1 are taken while the second pair runs, and dS while the first does.
-template <typename T>
+template <typename T, int NB>
 __global__ void __launch_bounds__(WG_THREADS, 1) window_grad_keys(const __grid_constant__ GradKernel p) {
     extern __shared__ unsigned char raw[];
     __shared__ __align__(8) uint64_t bars[2 * 4 + 6];
@@ -375,11 +375,11 @@ __global__ void __launch_bounds__(WG_THREADS, 1) window_grad_keys(const __grid_c
     __shared__ int gave_up_s;
     __shared__ __align__(16) float lse_s[2][SEQ_TILE], delta_s[2][SEQ_TILE];
     const WindowArgs &a = p.a;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, nb = (a.width + 63) / 64, group = a.heads / a.kv_heads;
-    const int stages = min(4, (WG_KEY_BLOCKS - 2 * nb) / (2 * nb));
-    const uint32_t smem = (tc::smem_u32(raw) + 1023) & ~1023u, k_tile = smem, v_tile = smem + nb * WF_BLOCK;
-    auto q_tile = [&](int s) { return smem + (2 + 2 * s) * nb * WF_BLOCK; };
-    auto g_tile = [&](int s) { return smem + (3 + 2 * s) * nb * WF_BLOCK; };
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, group = a.heads / a.kv_heads;
+    constexpr int stages = NB == 2 ? 2 : 4;
+    const uint32_t smem = (tc::smem_u32(raw) + 1023) & ~1023u, k_tile = smem, v_tile = smem + NB * WF_BLOCK;
+    auto q_tile = [&](int s) { return smem + (2 + 2 * s) * NB * WF_BLOCK; };
+    auto g_tile = [&](int s) { return smem + (3 + 2 * s) * NB * WF_BLOCK; };
     const int4 e = reinterpret_cast<const int4 *>(a.s.table)[seq_by_future(a.s, blockIdx.x / a.kv_heads)];
     const int hk = blockIdx.x % a.kv_heads, key = e.z;
     // queries from the key's own tile on, to the end of the window, or of the sequence where the tile holds sinks
@@ -403,8 +403,8 @@ __global__ void __launch_bounds__(WG_THREADS, 1) window_grad_keys(const __grid_c
                    b_dp = tc::smem_u32(&bars[10]), b_done = tc::smem_u32(&bars[11]), b_p = tc::smem_u32(&bars[12]), b_ds = tc::smem_u32(&bars[13]);
     if (warp == WG_COPY) {
         if (lane == 0) {
-            tc::mbar_expect_tx(b_k, 2 * nb * WF_BLOCK);
-            for (int k = 0; k < nb; k++) {
+            tc::mbar_expect_tx(b_k, 2 * NB * WF_BLOCK);
+            for (int k = 0; k < NB; k++) {
                 tc::tma_rows(k_tile + k * WF_BLOCK, &p.mk, 64 * k, hk, e.x + key, b_k);
                 tc::tma_rows(v_tile + k * WF_BLOCK, &p.mv, 64 * k, hk, e.x + key, b_k);
             }
@@ -413,8 +413,8 @@ __global__ void __launch_bounds__(WG_THREADS, 1) window_grad_keys(const __grid_c
                 const int s = n % stages, h = hk * group + n / per_head, q = (q0 + n % per_head) * SEQ_TILE;
                 if (n >= stages) wait(b_free + 8 * s, (n / stages - 1) & 1);
                 if (gave_up_s) break;
-                tc::mbar_expect_tx(b_full + 8 * s, 2 * nb * WF_BLOCK);
-                for (int k = 0; k < nb; k++) {
+                tc::mbar_expect_tx(b_full + 8 * s, 2 * NB * WF_BLOCK);
+                for (int k = 0; k < NB; k++) {
                     tc::tma_rows(q_tile(s) + k * WF_BLOCK, &p.mq, 64 * k, h, e.x + q, b_full + 8 * s);
                     tc::tma_rows(g_tile(s) + k * WF_BLOCK, &p.mg, 64 * k, h, e.x + q, b_full + 8 * s);
                 }
@@ -424,37 +424,44 @@ __global__ void __launch_bounds__(WG_THREADS, 1) window_grad_keys(const __grid_c
                 if (n > s) wait.drain(b_full + 8 * s, ((n - 1 - s) / stages) & 1);
         }
     } else if (warp == WG_PRODUCTS) {
-        if (lane == 0) {
-            constexpr bool bf = Half<T>::type == F3M_TYPE_BF16;
-            const uint32_t i_s = tc::idesc_f16(bf, 128, 128, false, false), i_d = tc::idesc_f16(bf, 128, 64 * nb, false, true);
-            auto rows = [&](uint32_t d, uint32_t x, uint32_t y, uint32_t bar) {   // x y^T
-                for (int k = 0; k < 4 * nb; k++)
-                    tc::mma_f16(d, tc::desc_k(x + (k >> 2) * WF_BLOCK + (k & 3) * 32), tc::desc_k(y + (k >> 2) * WF_BLOCK + (k & 3) * 32), i_s, k > 0);
-                tc::mma_commit(bar);
-            };
-            wait(b_k, 0);
-            wait(b_full, 0);
+        constexpr bool bf = Half<T>::type == F3M_TYPE_BF16;
+        const uint32_t i_s = tc::idesc_f16(bf, 128, 128, false, false), i_d = tc::idesc_f16(bf, 128, 64 * NB, false, true);
+        wait(b_k, 0);
+        wait(b_full, 0);
+        tc::fence_after_sync();
+        if (tc::elect()) {
+            tc::product_rows<NB>(t_s, k_tile, q_tile(0), i_s);
+            tc::mma_commit(b_s);
+            tc::product_rows<NB>(t_dp, v_tile, g_tile(0), i_s);
+            tc::mma_commit(b_dp);
+        }
+        for (int n = 0; n < tiles; n++) {
+            const int s = n % stages, sn = (n + 1) % stages;
+            const bool more = n + 1 < tiles;
+            if (more) wait(b_full + 8 * sn, ((n + 1) / stages) & 1);
+            wait(b_p, n & 1);
             tc::fence_after_sync();
-            rows(t_s, k_tile, q_tile(0), b_s);
-            rows(t_dp, v_tile, g_tile(0), b_dp);
-            for (int n = 0; n < tiles; n++) {
-                const int s = n % stages, sn = (n + 1) % stages;
-                const bool more = n + 1 < tiles;
-                wait(b_p, n & 1);
-                tc::fence_after_sync();
-                for (int k = 0; k < 8; k++) tc::mma_f16_ta(t_dv, t_s + operand_col(k), tc::desc_mn(g_tile(s) + k * 2048, WF_BLOCK), i_d, n > 0 || k > 0);
+            if (tc::elect()) {
+                if (n) tc::product_tmem<true, 64>(t_dv, t_s, g_tile(s), i_d);
+                else tc::product_tmem<false, 64>(t_dv, t_s, g_tile(s), i_d);
                 if (more) {
-                    wait(b_full + 8 * sn, ((n + 1) / stages) & 1);
-                    tc::fence_after_sync();
-                    rows(t_s, k_tile, q_tile(sn), b_s);
+                    tc::product_rows<NB>(t_s, k_tile, q_tile(sn), i_s);
+                    tc::mma_commit(b_s);
                 }
-                wait(b_ds, n & 1);
-                tc::fence_after_sync();
-                for (int k = 0; k < 8; k++) tc::mma_f16_ta(t_dk, t_dp + operand_col(k), tc::desc_mn(q_tile(s) + k * 2048, WF_BLOCK), i_d, n > 0 || k > 0);
-                tc::mma_commit(b_free + 8 * s);
-                if (more) rows(t_dp, v_tile, g_tile(sn), b_dp);
             }
-            tc::mma_commit(b_done);
+            wait(b_ds, n & 1);
+            tc::fence_after_sync();
+            if (tc::elect()) {
+                if (n) tc::product_tmem<true, 64>(t_dk, t_dp, q_tile(s), i_d);
+                else tc::product_tmem<false, 64>(t_dk, t_dp, q_tile(s), i_d);
+                tc::mma_commit(b_free + 8 * s);
+                if (more) {
+                    tc::product_rows<NB>(t_dp, v_tile, g_tile(sn), i_s);
+                    tc::mma_commit(b_dp);
+                } else {
+                    tc::mma_commit(b_done);
+                }
+            }
         }
     } else {
         // threads r and r + 128 have key row r, half of the queries each
@@ -475,7 +482,7 @@ __global__ void __launch_bounds__(WG_THREADS, 1) window_grad_keys(const __grid_c
                 wait(b_full + 8 * s, (n / stages) & 1);
                 wait(b_s, n & 1);
                 wait(b_dp, n & 1);
-                if (q + r >= e.y) clear_row(half ? g_tile(s) : q_tile(s), r, 0, 8 * nb);
+                if (q + r >= e.y) clear_row(half ? g_tile(s) : q_tile(s), r, 0, 8 * NB);
                 tc::fence_async_smem();
             }
             // seen: query q + c sees key j if j <= q + c, q + c - j < window or j is a sink, and the query is one
@@ -547,7 +554,7 @@ __global__ void __launch_bounds__(WG_THREADS, 1) window_grad_keys(const __grid_c
         tc::fence_after_sync();
         // the first half stages and stores dk over K, the second dv over V
         const uint32_t out = half ? v_tile : k_tile;
-        for (int q = 0; q < 2 * nb; q++) {
+        for (int q = 0; q < 2 * NB; q++) {
             uint32_t o[32];
             tc::tmem_ld32((half ? t_dv : t_dk) + lanes + 32 * q, o);
             tc::tmem_ld_wait(o);
@@ -559,7 +566,7 @@ __global__ void __launch_bounds__(WG_THREADS, 1) window_grad_keys(const __grid_c
                 sts16(out + (q >> 1) * WF_BLOCK + tc::swz(r, 4 * (q & 1) + c / 8), y);
             }
         }
-        store_rows<128>(half ? p.m1 : p.m0, half ? a.dv : a.dk, out, hk, e.x + key, min(SEQ_TILE, e.y - key), 0, nb, a.width, r, 3 + half);
+        store_rows<128>(half ? p.m1 : p.m0, half ? a.dv : a.dk, out, hk, e.x + key, min(SEQ_TILE, e.y - key), 0, NB, a.width, r, 3 + half);
         if (r == 0) tc::tma_store_wait_all();
     }
     __syncwarp();
@@ -570,17 +577,17 @@ __global__ void __launch_bounds__(WG_THREADS, 1) window_grad_keys(const __grid_c
 
 // A CTA has a tile of 128 queries (rows of tensor memory) and walks over tiles of 128 keys (columns).  S is computed a tile ahead, into one of two
 // places in turn; dP (n + 1) and dQ += dS K (n) run while the weights of n + 1 are taken.
-template <typename T>
+template <typename T, int NB>
 __global__ void __launch_bounds__(WG_THREADS, 1) window_grad_queries(const __grid_constant__ GradKernel p) {
     extern __shared__ unsigned char raw[];
     __shared__ __align__(8) uint64_t bars[2 * 8 + 6];
     __shared__ uint32_t tmem_s;
     __shared__ int gave_up_s;
     const WindowArgs &a = p.a;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, nb = (a.width + 63) / 64, group = a.heads / a.kv_heads;
-    const int slots = min(8, (WF_BLOCKS - 2 * nb) / nb);   // 5 at two blocks, 8 at one
-    const uint32_t smem = (tc::smem_u32(raw) + 1023) & ~1023u, q_tile = smem, g_tile = smem + nb * WF_BLOCK;
-    auto slot_tile = [&](int s) { return smem + (2 + s) * nb * WF_BLOCK; };
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, group = a.heads / a.kv_heads;
+    constexpr int slots = NB == 2 ? 5 : 8;
+    const uint32_t smem = (tc::smem_u32(raw) + 1023) & ~1023u, q_tile = smem, g_tile = smem + NB * WF_BLOCK;
+    auto slot_tile = [&](int s) { return smem + (2 + s) * NB * WF_BLOCK; };
     const int4 e = reinterpret_cast<const int4 *>(a.s.table)[seq_by_past(a.s, blockIdx.x / a.heads)];
     const int h = blockIdx.x % a.heads, hk = h / group, start = e.z;
     const int first = max(0, start - a.window + 1) / SEQ_TILE, sinks = (int)min(((int64_t)a.sinks + SEQ_TILE - 1) / SEQ_TILE, (int64_t)first);
@@ -603,8 +610,8 @@ __global__ void __launch_bounds__(WG_THREADS, 1) window_grad_queries(const __gri
                    b_dp = tc::smem_u32(&bars[19]), b_done = tc::smem_u32(&bars[20]), b_ds = tc::smem_u32(&bars[21]);
     if (warp == WG_COPY) {
         if (lane == 0) {
-            tc::mbar_expect_tx(b_q, 2 * nb * WF_BLOCK);
-            for (int k = 0; k < nb; k++) {
+            tc::mbar_expect_tx(b_q, 2 * NB * WF_BLOCK);
+            for (int k = 0; k < NB; k++) {
                 tc::tma_rows(q_tile + k * WF_BLOCK, &p.mq, 64 * k, h, e.x + start, b_q);
                 tc::tma_rows(g_tile + k * WF_BLOCK, &p.mg, 64 * k, h, e.x + start, b_q);
             }
@@ -613,44 +620,50 @@ __global__ void __launch_bounds__(WG_THREADS, 1) window_grad_queries(const __gri
                 const int s = x % slots;
                 if (x >= slots) wait(b_free + 8 * s, (x / slots - 1) & 1);
                 if (gave_up_s) break;
-                tc::mbar_expect_tx(b_full + 8 * s, nb * WF_BLOCK);
-                for (int k = 0; k < nb; k++) tc::tma_rows(slot_tile(s) + k * WF_BLOCK, x & 1 ? &p.mv : &p.mk, 64 * k, hk, e.x + key_of(x >> 1), b_full + 8 * s);
+                tc::mbar_expect_tx(b_full + 8 * s, NB * WF_BLOCK);
+                for (int k = 0; k < NB; k++) tc::tma_rows(slot_tile(s) + k * WF_BLOCK, x & 1 ? &p.mv : &p.mk, 64 * k, hk, e.x + key_of(x >> 1), b_full + 8 * s);
             }
             wait.drain(b_q, 0);
             for (int s = 0; s < slots; s++)
                 if (x > s) wait.drain(b_full + 8 * s, ((x - 1 - s) / slots) & 1);
         }
     } else if (warp == WG_PRODUCTS) {
-        if (lane == 0) {
-            constexpr bool bf = Half<T>::type == F3M_TYPE_BF16;
-            const uint32_t i_s = tc::idesc_f16(bf, 128, 128, false, false), i_d = tc::idesc_f16(bf, 128, 64 * nb, false, true);
-            auto rows = [&](uint32_t d, uint32_t q, int x, uint32_t bar) {   // q (slot's tile)^T
-                const int s = x % slots;
-                wait(b_full + 8 * s, (x / slots) & 1);
-                tc::fence_after_sync();
-                for (int k = 0; k < 4 * nb; k++)
-                    tc::mma_f16(d, tc::desc_k(q + (k >> 2) * WF_BLOCK + (k & 3) * 32), tc::desc_k(slot_tile(s) + (k >> 2) * WF_BLOCK + (k & 3) * 32), i_s, k > 0);
-                tc::mma_commit(bar);
-            };
-            auto scores = [&](int n) { rows(tmem + 128 * (n & 1), q_tile, 2 * n, b_s + 8 * (n & 1)); };
-            auto values = [&](int n) {
-                rows(t_dp, g_tile, 2 * n + 1, b_dp);
-                tc::mma_commit(b_free + 8 * ((2 * n + 1) % slots));
-            };
-            wait(b_q, 0);
-            scores(0);
-            values(0);
-            if (tiles > 1) scores(1);
-            for (int n = 0; n < tiles; n++) {
-                wait(b_ds, n & 1);
-                tc::fence_after_sync();
-                if (n + 1 < tiles) values(n + 1);
-                const int s = (2 * n) % slots;
-                for (int k = 0; k < 8; k++) tc::mma_f16_ta(t_dq, tmem + 128 * (n & 1) + operand_col(k), tc::desc_mn(slot_tile(s) + k * 2048, WF_BLOCK), i_d, n > 0 || k > 0);
-                tc::mma_commit(b_free + 8 * s);
-                if (n + 2 < tiles) scores(n + 2);
+        constexpr bool bf = Half<T>::type == F3M_TYPE_BF16;
+        const uint32_t i_s = tc::idesc_f16(bf, 128, 128, false, false), i_d = tc::idesc_f16(bf, 128, 64 * NB, false, true);
+        auto landed = [&](int x) {
+            wait(b_full + 8 * (x % slots), (x / slots) & 1);
+            tc::fence_after_sync();
+        };
+        auto scores = [&](int n) {
+            landed(2 * n);
+            if (tc::elect()) {
+                tc::product_rows<NB>(tmem + 128 * (n & 1), q_tile, slot_tile(2 * n % slots), i_s);
+                tc::mma_commit(b_s + 8 * (n & 1));
             }
-            tc::mma_commit(b_done);
+        };
+        auto values = [&](int n) {
+            landed(2 * n + 1);
+            if (tc::elect()) {
+                tc::product_rows<NB>(t_dp, g_tile, slot_tile((2 * n + 1) % slots), i_s);
+                tc::mma_commit(b_dp);
+                tc::mma_commit(b_free + 8 * ((2 * n + 1) % slots));
+            }
+        };
+        wait(b_q, 0);
+        scores(0);
+        values(0);
+        if (tiles > 1) scores(1);
+        for (int n = 0; n < tiles; n++) {
+            wait(b_ds, n & 1);
+            tc::fence_after_sync();
+            if (n + 1 < tiles) values(n + 1);
+            if (tc::elect()) {
+                if (n) tc::product_tmem<true, 64>(t_dq, tmem + 128 * (n & 1), slot_tile(2 * n % slots), i_d);
+                else tc::product_tmem<false, 64>(t_dq, tmem + 128 * (n & 1), slot_tile(2 * n % slots), i_d);
+                tc::mma_commit(b_free + 8 * (2 * n % slots));
+                if (n + 1 == tiles) tc::mma_commit(b_done);
+            }
+            if (n + 2 < tiles) scores(n + 2);
         }
     } else {
         const int r = tid & 127, half = tid >> 7, i = start + r, i0 = start + 32 * (warp & 3);
@@ -682,7 +695,7 @@ __global__ void __launch_bounds__(WG_THREADS, 1) window_grad_queries(const __gri
             if (key + SEQ_TILE > e.y) {   // keys of the next sequence
                 const int x = 2 * n, s = x % slots;
                 wait(b_full + 8 * s, (x / slots) & 1);
-                if (key + r >= e.y) clear_row(slot_tile(s), r, half ? 4 * nb : 0, half ? 8 * nb : 4 * nb);
+                if (key + r >= e.y) clear_row(slot_tile(s), r, half ? 4 * NB : 0, half ? 8 * NB : 4 * NB);
                 tc::fence_async_smem();
             }
             wait(b_dp, n & 1);
@@ -715,7 +728,7 @@ __global__ void __launch_bounds__(WG_THREADS, 1) window_grad_queries(const __gri
         __syncwarp();
         tc::fence_after_sync();
         // over Q: the halves take its blocks in turn, at one block half of it each
-        for (int q = half * nb; q < (half + 1) * nb; q++) {
+        for (int q = half * NB; q < (half + 1) * NB; q++) {
             uint32_t o[32];
             tc::tmem_ld32(t_dq + lanes + 32 * q, o);
             tc::tmem_ld_wait(o);
@@ -727,7 +740,7 @@ __global__ void __launch_bounds__(WG_THREADS, 1) window_grad_queries(const __gri
                 sts16(q_tile + (q >> 1) * WF_BLOCK + tc::swz(r, 4 * (q & 1) + c / 8), y);
             }
         }
-        store_rows<256>(p.m0, a.dq, q_tile, h, e.x + start, min(SEQ_TILE, e.y - start), 0, nb, a.width, tid, 1);
+        store_rows<256>(p.m0, a.dq, q_tile, h, e.x + start, min(SEQ_TILE, e.y - start), 0, NB, a.width, tid, 1);
         if (tid == 0) tc::tma_store_wait_all();
     }
     __syncwarp();
@@ -760,12 +773,14 @@ static void backward_t(const WindowArgs &a, cudaStream_t s) {
     p.c = a.scale * 1.4426950408889634f;
     p.err = seq_error_word();
     constexpr int key_bytes = WG_KEY_BLOCKS * WF_BLOCK + 1024;
-    F3M_CUDA(cudaFuncSetAttribute(window_grad_keys<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, key_bytes));
-    window_grad_keys<T><<<a.s.tiles * a.kv_heads, WG_THREADS, key_bytes, s>>>(p);
+    auto keys = a.width <= 64 ? window_grad_keys<T, 1> : window_grad_keys<T, 2>;
+    F3M_CUDA(cudaFuncSetAttribute(keys, cudaFuncAttributeMaxDynamicSharedMemorySize, key_bytes));
+    keys<<<a.s.tiles * a.kv_heads, WG_THREADS, key_bytes, s>>>(p);
     F3M_LAUNCH_CHECK();
     p.m0 = seq_tensor_map(type, a.dq, n, a.heads, a.width);
-    F3M_CUDA(cudaFuncSetAttribute(window_grad_queries<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-    window_grad_queries<T><<<a.s.tiles * a.heads, WG_THREADS, bytes, s>>>(p);
+    auto queries = a.width <= 64 ? window_grad_queries<T, 1> : window_grad_queries<T, 2>;
+    F3M_CUDA(cudaFuncSetAttribute(queries, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    queries<<<a.s.tiles * a.heads, WG_THREADS, bytes, s>>>(p);
     F3M_LAUNCH_CHECK();
 }
 void window_forward(int type, const WindowArgs &a, cudaStream_t s) { type == F3M_TYPE_BF16 ? forward_t<__nv_bfloat16>(a, s) : forward_t<__half>(a, s); }
