@@ -1,5 +1,4 @@
 // Linear attention with a decay for each head: the recurrence over packed sequences, and one new token.
-#include "packed.cuh"
 #include "seq.cuh"
 
 namespace f3m {

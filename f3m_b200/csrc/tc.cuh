@@ -182,6 +182,14 @@ __device__ __forceinline__ void product_tmem(uint32_t d, uint32_t a_tmem, uint32
 #pragma unroll
     for (int k = 1; k < 8; k++) mma_f16_ta<true>(d, a_tmem + 8 * (k & 3) + GAP * (k >> 2), b + k * (2048 >> 4), idesc);
 }
+// ... 64 of the 128 elements of its rows
+template <bool ACC>
+__device__ __forceinline__ void product_tmem_half(uint32_t d, uint32_t a_tmem, uint32_t b_tile, uint32_t idesc) {
+    const uint64_t b = desc_mn(b_tile, BLOCK);
+    mma_f16_ta<ACC>(d, a_tmem, b, idesc);
+#pragma unroll
+    for (int k = 1; k < 4; k++) mma_f16_ta<true>(d, a_tmem + 8 * k, b + k * (2048 >> 4), idesc);
+}
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "

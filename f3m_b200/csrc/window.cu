@@ -1,6 +1,5 @@
 // Attention over a window with sinks: forward, gradients, one new token against a cache.
 #include <algorithm>
-#include "packed.cuh"
 #include "seq.cuh"
 
 namespace f3m {
@@ -64,7 +63,7 @@ __device__ __forceinline__ WindowItem window_item(const WindowKernel &p, int i) 
 template <typename T, int NB>
 __global__ void __launch_bounds__(WF_THREADS, 1) window_tiles(const __grid_constant__ WindowKernel p) {
     extern __shared__ unsigned char raw[];
-    __shared__ __align__(8) uint64_t bars[2 * 8 + 2 + 8];
+    __shared__ __align__(8) uint64_t bars[2 * 8 + 2 + 10];
     __shared__ uint32_t tmem_s;
     __shared__ int gave_up_s;
     const WindowArgs &a = p.a;
@@ -80,9 +79,10 @@ __global__ void __launch_bounds__(WF_THREADS, 1) window_tiles(const __grid_const
         for (int i = 0; i < 18; i++) tc::mbar_init(tc::smem_u32(&bars[i]), 1);        // slot landed, free; queries landed, free
         for (int t = 0; t < 2; t++) {
             tc::mbar_init(tc::smem_u32(&bars[18 + t]), 1);      // S ready
-            tc::mbar_init(tc::smem_u32(&bars[20 + t]), 128);    // weights written
+            tc::mbar_init(tc::smem_u32(&bars[20 + t]), 128);    // weights of the first 64 keys written
             tc::mbar_init(tc::smem_u32(&bars[22 + t]), 1);      // O ready
             tc::mbar_init(tc::smem_u32(&bars[24 + t]), 128);    // O read
+            tc::mbar_init(tc::smem_u32(&bars[26 + t]), 128);    // weights of the other 64 written
         }
         tc::fence_mbar_init();
         gave_up_s = 0;
@@ -93,7 +93,7 @@ __global__ void __launch_bounds__(WF_THREADS, 1) window_tiles(const __grid_const
     const Waits wait{&gave_up_s, p.err};
     const uint32_t tmem = tmem_s;
     const uint32_t b_full = tc::smem_u32(&bars[0]), b_free = tc::smem_u32(&bars[8]), b_q = tc::smem_u32(&bars[16]), b_q_free = tc::smem_u32(&bars[17]),
-                   b_s = tc::smem_u32(&bars[18]), b_p = tc::smem_u32(&bars[20]), b_o = tc::smem_u32(&bars[22]), b_o_read = tc::smem_u32(&bars[24]);
+                   b_s = tc::smem_u32(&bars[18]), b_p = tc::smem_u32(&bars[20]), b_o = tc::smem_u32(&bars[22]), b_o_read = tc::smem_u32(&bars[24]), b_p2 = tc::smem_u32(&bars[26]);
 
     if (warp == WF_COPY) {
         if (lane == 0) {
@@ -146,12 +146,17 @@ __global__ void __launch_bounds__(WF_THREADS, 1) window_tiles(const __grid_const
                 for (int t = 0; t < w.tiles_q; t++) {
                     if (j == 0 && no[t]) wait(b_o_read + 8 * t, (no[t] - 1) & 1);
                     wait(b_p + 8 * t, np[t] & 1);
+                    tc::fence_after_sync();
+                    if (tc::elect()) {
+                        if (j) tc::product_tmem_half<true>(tmem + 256 + 128 * t, tmem + 128 * t, slot_tile(sv), i_o);
+                        else tc::product_tmem_half<false>(tmem + 256 + 128 * t, tmem + 128 * t, slot_tile(sv), i_o);
+                    }
+                    wait(b_p2 + 8 * t, np[t] & 1);
                     np[t]++;
                     no[t] += !more;
                     tc::fence_after_sync();
                     if (tc::elect()) {
-                        if (j) tc::product_tmem<true>(tmem + 256 + 128 * t, tmem + 128 * t, slot_tile(sv), i_o);
-                        else tc::product_tmem<false>(tmem + 256 + 128 * t, tmem + 128 * t, slot_tile(sv), i_o);
+                        tc::product_tmem_half<true>(tmem + 256 + 128 * t, tmem + 128 * t + 32, slot_tile(sv) + 64 * 128, i_o);
                         if (more) {
                             tc::product_rows<NB>(tmem + 128 * t, q_tile(t), slot_tile(sk), i_s);
                             tc::mma_commit(b_s + 8 * t);
@@ -172,7 +177,7 @@ __global__ void __launch_bounds__(WF_THREADS, 1) window_tiles(const __grid_const
         // ---- weights: thread r of a query tile has its row r ----
         const int t = warp >> 2, r = tid & 127, wq = warp & 3;
         const uint32_t lanes = (uint32_t)(32 * wq) << 16, t_s = tmem + 128 * t + lanes, t_o = tmem + 256 + 128 * t + lanes;
-        int ns = 0, no = 0, x = 0;
+        int ns = 0, no = 0, x0 = 0;   // x0: key and value tiles of the items before
         for (int it = blockIdx.x; it < p.items; it += gridDim.x) {
             const WindowItem w = window_item(p, it);
             if (t < w.tiles_q) {   // whole warps
@@ -189,32 +194,26 @@ __global__ void __launch_bounds__(WF_THREADS, 1) window_tiles(const __grid_const
                     const bool whole = key + SEQ_TILE - 1 <= i0 && (i0 + 31 - key < a.window || key + SEQ_TILE <= a.sinks);
                     const int up = i - key, low = i - key - a.window, sink = a.sinks - key;   // seen: c <= up and (c > low or c < sink)
                     float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    uint32_t x[2][32];
+                    tc::tmem_ld32(t_s, x[0]);
 #pragma unroll
-                    for (int q = 0; q < 4; q += 2) {
-                        uint32_t s0[32], s1[32];
-                        tc::tmem_ld32(t_s + 32 * q, s0);
-                        tc::tmem_ld32(t_s + 32 * q + 32, s1);
-                        tc::tmem_ld_wait(s0);
-                        tc::tmem_ld_wait(s1);
+                    for (int q = 0; q < 4; q++) {
+                        tc::tmem_ld_wait(x[q & 1]);
+                        if (q < 3) tc::tmem_ld32(t_s + 32 * (q + 1), x[(q + 1) & 1]);
                         if (whole) {
 #pragma unroll
-                            for (int c = 0; c < 32; c++) {
-                                mx[2 * (c & 1)] = fmaxf(mx[2 * (c & 1)], __uint_as_float(s0[c]));
-                                mx[2 * (c & 1) + 1] = fmaxf(mx[2 * (c & 1) + 1], __uint_as_float(s1[c]));
-                            }
+                            for (int c = 0; c < 32; c++) mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(x[q & 1][c]));
                         } else {
 #pragma unroll
-                            for (int c = 0; c < 32; c++) {
-                                const int c0 = 32 * q + c, c1 = c0 + 32;
-                                mx[2 * (c & 1)] = fmaxf(mx[2 * (c & 1)], c0 <= up && (c0 > low || c0 < sink) ? __uint_as_float(s0[c]) : -INFINITY);
-                                mx[2 * (c & 1) + 1] = fmaxf(mx[2 * (c & 1) + 1], c1 <= up && (c1 > low || c1 < sink) ? __uint_as_float(s1[c]) : -INFINITY);
-                            }
+                            for (int c = 0; c < 32; c++)
+                                mx[c & 3] = fmaxf(mx[c & 3], 32 * q + c <= up && (32 * q + c > low || 32 * q + c < sink) ? __uint_as_float(x[q & 1][c]) : -INFINITY);
                         }
                     }
+                    tc::tmem_ld32(t_s, x[0]);   // again
                     const float high = fmaxf(top, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
                     const bool rise = (high - top) * p.c > 8.f;   // also from -inf; not from -inf to -inf
                     if (__any_sync(0xffffffffu, rise)) {
-                        const float f = rise ? exp2_approx((top - high) * p.c) : 1.f;
+                        const float f = rise ? ex2_approx((top - high) * p.c) : 1.f;
                         if (rise) { top = high; sum *= f; }
                         if (j > 0)
                             for (int q = 0; q < 2 * NB; q++) {
@@ -229,39 +228,55 @@ __global__ void __launch_bounds__(WF_THREADS, 1) window_tiles(const __grid_const
                     const float shift = top == -INFINITY ? 0.f : -top * p.c;
                     const f32x2 cc = pack2(p.c, p.c), ss = pack2(shift, shift);
                     f32x2 part[2] = {pack2(sum, 0.f), pack2(0.f, 0.f)};
-#pragma unroll
-                    for (int q = 0; q < 4; q++) {
-                        uint32_t x[32], w16[16];
-                        tc::tmem_ld32(t_s + 32 * q, x);
-                        tc::tmem_ld_wait(x);
-                        if (!whole)
-#pragma unroll
-                            for (int c = 0; c < 32; c++)
-                                if (!(32 * q + c <= up && (32 * q + c > low || 32 * q + c < sink))) x[c] = 0xff800000u;
-#pragma unroll
-                        for (int c = 0; c < 32; c += 2) {
-                            float lo, hi;
-                            unpack2(fma2(pack2(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), cc, ss), lo, hi);
-                            lo = ex2_approx(lo);
-                            hi = ex2_approx(hi);
-                            part[(c >> 1) & 1] = add2(part[(c >> 1) & 1], pack2(lo, hi));
-                            w16[c >> 1] = Half<T>::pack(lo, hi);
-                        }
-                        tc::tmem_st16(t_s + 16 * q, w16);   // over scores that have been read
-                    }
-                    float u, v;
-                    unpack2(add2(part[0], part[1]), u, v);
-                    sum = u + v;
                     if (t == 0 && key + SEQ_TILE > w.len) {   // the sequence ends inside the tile
-                        const int xv = x + 2 * j + 1, sv = xv % slots;
+                        const int xv = x0 + 2 * j + 1, sv = xv % slots;
                         wait(b_full + 8 * sv, (xv / slots) & 1);
                         if (key + r >= w.len) clear_row(slot_tile(sv), r, 0, 8 * NB);
                         tc::fence_async_smem();
                         __syncwarp();
                     }
-                    tc::tmem_st_wait();
-                    tc::fence_before_sync();
-                    tc::mbar_arrive(b_p + 8 * t);
+#pragma unroll
+                    for (int q = 0; q < 4; q++) {
+                        uint32_t w16[16];
+                        tc::tmem_ld_wait(x[q & 1]);
+                        if (q < 3) tc::tmem_ld32(t_s + 32 * (q + 1), x[(q + 1) & 1]);
+                        uint32_t(&y)[32] = x[q & 1];
+                        if (whole) {
+#pragma unroll
+                            for (int c = 0; c < 32; c += 2) {
+                                float lo, hi;
+                                const f32x2 e = fma2(pack2(__uint_as_float(y[c]), __uint_as_float(y[c + 1])), cc, ss);
+                                if (c % 8 == 6) exp2_poly(e, lo, hi);
+                                else {
+                                    unpack2(e, lo, hi);
+                                    lo = ex2_approx(lo);
+                                    hi = ex2_approx(hi);
+                                }
+                                part[(c >> 1) & 1] = add2(part[(c >> 1) & 1], pack2(lo, hi));
+                                w16[c >> 1] = Half<T>::pack(lo, hi);
+                            }
+                        } else {
+#pragma unroll
+                            for (int c = 0; c < 32; c += 2) {
+                                float lo, hi;
+                                unpack2(fma2(pack2(__uint_as_float(y[c]), __uint_as_float(y[c + 1])), cc, ss), lo, hi);
+                                const int c0 = 32 * q + c, c1 = c0 + 1;
+                                lo = c0 <= up && (c0 > low || c0 < sink) ? ex2_approx(lo) : 0.f;
+                                hi = c1 <= up && (c1 > low || c1 < sink) ? ex2_approx(hi) : 0.f;
+                                part[(c >> 1) & 1] = add2(part[(c >> 1) & 1], pack2(lo, hi));
+                                w16[c >> 1] = Half<T>::pack(lo, hi);
+                            }
+                        }
+                        tc::tmem_st16(t_s + 16 * q, w16);   // over scores that have been read
+                        if (q & 1) {
+                            tc::tmem_st_wait();
+                            tc::fence_before_sync();
+                            tc::mbar_arrive((q == 1 ? b_p : b_p2) + 8 * t);
+                        }
+                    }
+                    float u, v;
+                    unpack2(add2(part[0], part[1]), u, v);
+                    sum = u + v;
                 }
                 wait(b_o + 8 * t, no & 1);
                 no++;
@@ -292,7 +307,7 @@ __global__ void __launch_bounds__(WF_THREADS, 1) window_tiles(const __grid_const
                 }
                 if (r < m) a.lse[(int64_t)w.head[t] * a.s.tokens + w.row0 + i] = (top * p.c + log2f(sum)) * 0.69314718055994531f;
             }
-            x += 2 * w.keys;
+            x0 += 2 * w.keys;
         }
         if (r == 0) tc::tma_store_wait_all();
     }
@@ -874,7 +889,7 @@ __global__ void __launch_bounds__(ST_THREADS, 3) step_keys(StepArgs a) {
             high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 1));
             high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 2));
             if (__any_sync(0xffffffffu, high > top[r])) {
-                const float f = exp2_approx(top[r] - high);   // of -inf, where nothing came before: 0
+                const float f = ex2_approx(top[r] - high);   // of -inf, where nothing came before: 0
                 sum[r] *= f;
                 top[r] = high;
 #pragma unroll
@@ -884,7 +899,7 @@ __global__ void __launch_bounds__(ST_THREADS, 3) step_keys(StepArgs a) {
             }
 #pragma unroll
             for (int n = 0; n < 2; n++) {
-                const float y0 = exp2_approx(x[n][2 * r] - high), y1 = exp2_approx(x[n][2 * r + 1] - high);
+                const float y0 = ex2_approx(x[n][2 * r] - high), y1 = ex2_approx(x[n][2 * r + 1] - high);
                 sum[r] += y0 + y1;
                 w[2 * n + r] = Half<T>::pack(y0, y1);
             }
@@ -912,7 +927,7 @@ __global__ void __launch_bounds__(ST_THREADS, 3) step_keys(StepArgs a) {
     for (int r = 0; r < 2; r++) {
         const int h = g + 8 * r;
         const float high = fmaxf(fmaxf(stat[0][0][h], stat[0][1][h]), fmaxf(stat[0][2][h], stat[0][3][h]));
-        const float f = top[r] == -INFINITY ? 0.f : exp2_approx(top[r] - high);
+        const float f = top[r] == -INFINITY ? 0.f : ex2_approx(top[r] - high);
 #pragma unroll
         for (int k = 0; k < DF; k++)
 #pragma unroll
@@ -928,7 +943,7 @@ __global__ void __launch_bounds__(ST_THREADS, 3) step_keys(StepArgs a) {
         float2 y = make_float2(0.f, 0.f);
 #pragma unroll
         for (int w = 0; w < 4; w++) {
-            if (stat[0][w][h] != -INFINITY) total += stat[1][w][h] * exp2_approx(stat[0][w][h] - high);
+            if (stat[0][w][h] != -INFINITY) total += stat[1][w][h] * ex2_approx(stat[0][w][h] - high);
             y.x += sum_s[w][h][d];
             y.y += sum_s[w][h][d + 1];
         }
@@ -953,7 +968,7 @@ __global__ void __launch_bounds__(64) step_join(StepArgs a) {
     const float *sums = a.part + (int64_t)a.n * a.heads * a.parts * 2 + row * a.width;
     float high = -INFINITY;
     for (int i = 0; i < a.parts; i++) high = fmaxf(high, stat[i].x);
-    for (int i = threadIdx.x; i < a.parts; i += 64) w_s[i] = stat[i].y > 0.f ? exp2_approx(stat[i].x - high) : 0.f;
+    for (int i = threadIdx.x; i < a.parts; i += 64) w_s[i] = stat[i].y > 0.f ? ex2_approx(stat[i].x - high) : 0.f;
     __syncthreads();
     if (d >= a.width) return;
     float total = 0.f;
