@@ -53,7 +53,7 @@ class Rows(C.Structure):
 
 
 class Seqs(C.Structure):
-    _fields_ = [("table", C.c_void_p), ("tokens", C.c_int64), ("sequences", C.c_int32), ("tiles", C.c_int32), ("pairs", C.c_int32),
+    _fields_ = [("table", C.c_void_p), ("tokens", C.c_int64), ("sequences", C.c_int32), ("empty", C.c_int32), ("tiles", C.c_int32), ("pairs", C.c_int32),
                 ("longest", C.c_int32), ("table_words", C.c_int32)]
 
 

@@ -516,14 +516,14 @@ __global__ void __launch_bounds__(256) decay_empty(DecayArgs a) {
 }
 
 // How many ranges a head's tiles are cut into.  One CTA of decay_tiles fills an SM.  With one range the SMs without a head idle; with more, B
-// and C are read twice, half as much again: the number that gives the least of (bytes read) / (share of the SMs busy), up to three waves.
+// and C are read twice, half as much again, and two more launches take as long as some four tiles: the least time of a CTA's tiles, up to three waves.
 static int decay_ranges(const f3m_seqs &s, int heads) {
     int best = 1;
     float least = 0.f;
     for (int r = 1; r <= s.tiles && (r == 1 || (int64_t)heads * r <= 3 * NUM_SMS_HINT); r++) {
         const int64_t ctas = (int64_t)heads * r, waves = (ctas + NUM_SMS_HINT - 1) / NUM_SMS_HINT;
         const int per = (s.tiles + r - 1) / r;
-        const float cost = (r == 1 ? 1.f : 1.5f) * (float)(waves * per);
+        const float cost = r == 1 ? (float)(waves * per) : 1.5f * (float)(waves * per) + 4.f;
         if (r == 1 || cost < least) { least = cost; best = r; }
     }
     return best;
@@ -537,20 +537,22 @@ template <typename T, int PARTS, int NB>
 static void launch_parts(const DecayKernel &p, cudaStream_t s) {
     constexpr int bytes = DK_TILES * DK_BLOCK + 1024;
     if (p.ranges > 1) {
-        F3M_CUDA(cudaFuncSetAttribute(decay_states<T, PARTS, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+        static SharedMemory states;
+        states.allow(decay_states<T, PARTS, NB>, bytes);
         decay_states<T, PARTS, NB><<<dim3(p.ranges - 1, p.a.heads), DS_THREADS, bytes, s>>>(p);
         F3M_LAUNCH_CHECK();
         decay_join<<<dim3((p.a.width_b * p.a.width_c / 4 + 255) / 256, p.a.heads), 256, 0, s>>>(p);
         F3M_LAUNCH_CHECK();
     }
-    F3M_CUDA(cudaFuncSetAttribute(decay_tiles<T, PARTS, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    static SharedMemory tiles;
+    tiles.allow(decay_tiles<T, PARTS, NB>, bytes);
     decay_tiles<T, PARTS, NB><<<dim3(p.ranges, p.a.heads), DK_THREADS, bytes, s>>>(p);
     F3M_LAUNCH_CHECK();
 }
 
 template <typename T>
 static void decay_product_t(const DecayArgs &a, cudaStream_t s) {
-    if (a.state_out) {
+    if (a.state_out && a.s.empty) {
         decay_empty<<<a.s.sequences, 256, 0, s>>>(a);
         F3M_LAUNCH_CHECK();
     }

@@ -114,6 +114,20 @@ CUtensorMap seq_tensor_map(int type, const f3m_rows &r, int64_t tokens, int head
 int *seq_error_word();
 void seq_check_error();
 
+// A kernel's leave to use more than 48 KB of shared memory, asked for once on each device
+class SharedMemory {
+    std::atomic<unsigned long long> devices{0};   // the first 64; others ask each time
+public:
+    template <typename K>
+    void allow(K kernel, int bytes) {
+        int d = 0;
+        F3M_CUDA(cudaGetDevice(&d));
+        if (d < 64 && devices.load(std::memory_order_relaxed) >> d & 1) return;
+        F3M_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+        if (d < 64) devices.fetch_or(1ull << d, std::memory_order_relaxed);
+    }
+};
+
 // Waits of a kernel's roles on one another.  None is longer than about two seconds: what expires raises `gave_up`, after which every wait of
 // the block returns at once and the block runs to its end on whatever it finds, inside its buffers.
 struct Waits {

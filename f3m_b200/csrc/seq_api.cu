@@ -121,13 +121,14 @@ int f3m_seqs_layout(const int32_t *lengths, int32_t n, f3m_seqs *seqs, int32_t *
     return guarded([&] {
         F3M_REQUIRE(seqs && n >= 0 && (lengths || n == 0), F3M_ERR_ARG, "bad argument to f3m_seqs_layout");
         int64_t tokens = 0, tiles = 0, pairs = 0;
-        int32_t longest = 0;
+        int32_t longest = 0, empty = 0;
         for (int i = 0; i < n; i++) {
             F3M_REQUIRE(lengths[i] >= 0, F3M_ERR_ARG, "length %d of sequence %d", lengths[i], i);
             tokens += lengths[i];
             tiles += ((int64_t)lengths[i] + SEQ_TILE - 1) / SEQ_TILE;
             pairs += ((int64_t)lengths[i] + 2 * SEQ_TILE - 1) / (2 * SEQ_TILE);
             longest = std::max(longest, lengths[i]);
+            empty += lengths[i] == 0;
         }
         F3M_REQUIRE(tokens <= F3M_SEQ_MAX_TOKENS, F3M_ERR_OVERFLOW, "%lld tokens do not fit in 31 bits", (long long)tokens);
         F3M_REQUIRE(4 * (3 * tiles + n + pairs) <= 0x7fffffff, F3M_ERR_OVERFLOW, "the table of %d sequences does not fit in 31 bits", n);
@@ -136,6 +137,7 @@ int f3m_seqs_layout(const int32_t *lengths, int32_t n, f3m_seqs *seqs, int32_t *
         seqs->sequences = n;
         seqs->tiles = (int32_t)tiles;
         seqs->longest = longest;
+        seqs->empty = empty;
         seqs->pairs = (int32_t)pairs;
         seqs->table_words = (int32_t)(4 * (3 * tiles + n + pairs));
         if (!table) return;

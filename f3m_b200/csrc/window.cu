@@ -335,7 +335,8 @@ static void forward_t(const WindowArgs &a, cudaStream_t s) {
     p.err = seq_error_word();
     constexpr int bytes = WF_BLOCKS * WF_BLOCK + 1024;
     auto kernel = a.width <= 64 ? window_tiles<T, 1> : window_tiles<T, 2>;
-    F3M_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    static SharedMemory allowed[2];
+    allowed[a.width > 64].allow(kernel, bytes);
     kernel<<<std::min(p.items, NUM_SMS_HINT), WF_THREADS, bytes, s>>>(p);
     F3M_LAUNCH_CHECK();
 }
@@ -789,12 +790,13 @@ static void backward_t(const WindowArgs &a, cudaStream_t s) {
     p.err = seq_error_word();
     constexpr int key_bytes = WG_KEY_BLOCKS * WF_BLOCK + 1024;
     auto keys = a.width <= 64 ? window_grad_keys<T, 1> : window_grad_keys<T, 2>;
-    F3M_CUDA(cudaFuncSetAttribute(keys, cudaFuncAttributeMaxDynamicSharedMemorySize, key_bytes));
+    static SharedMemory allowed[2][2];
+    allowed[0][a.width > 64].allow(keys, key_bytes);
     keys<<<a.s.tiles * a.kv_heads, WG_THREADS, key_bytes, s>>>(p);
     F3M_LAUNCH_CHECK();
     p.m0 = seq_tensor_map(type, a.dq, n, a.heads, a.width);
     auto queries = a.width <= 64 ? window_grad_queries<T, 1> : window_grad_queries<T, 2>;
-    F3M_CUDA(cudaFuncSetAttribute(queries, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    allowed[1][a.width > 64].allow(queries, bytes);
     queries<<<a.s.tiles * a.heads, WG_THREADS, bytes, s>>>(p);
     F3M_LAUNCH_CHECK();
 }

@@ -62,30 +62,64 @@ class SequencePlan:
         check(L.f3m_seqs_layout(host.ctypes.data, host.size, C.byref(self._seqs), table.ctypes.data), "f3m_seqs_layout")
         self.table = torch.from_numpy(table).to(self.device)      # pageable memory: the copy has ended when this returns
         self._seqs.table = self.table.data_ptr()
+        self._ref = C.byref(self._seqs)
         self.tokens, self.sequences, self.longest = int(self._seqs.tokens), int(self._seqs.sequences), int(self._seqs.longest)
 
 
-def _stream(device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+class _On:
+    """The device of the arrays made current for a call, where it is not already, and its current stream."""
+    __slots__ = ("index", "guard")
+
+    def __init__(self, device):
+        self.index, self.guard = device.index, None
+
+    def __enter__(self) -> int:
+        if torch.cuda.current_device() != self.index:
+            self.guard = torch.cuda.device(self.index)
+            self.guard.__enter__()
+        return torch._C._cuda_getCurrentRawStream(self.index)
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
 
 
-def _aligned(t: torch.Tensor) -> torch.Tensor:
-    """t, or a dense copy of it where the library could not read it in place."""
-    w = t.dim() - 1
-    if t.stride(w) == 1 and t.data_ptr() % 16 == 0:
-        for i in range(w):
-            if t.shape[i] != 1 and (t.stride(i) % 8 or t.stride(i) < t.shape[w]):
-                break
-        else:
-            return t
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+def _read(t: torch.Tensor) -> Tuple[torch.Tensor, Rows]:
+    """t (tokens, heads, width), or a dense copy of it where the library could not read it in place, and the library's view of that."""
+    (ts, hs, cs), (tokens, heads, width), at = t.stride(), t.shape, t.data_ptr()
+    if tokens == 1:
+        ts = heads * width
+    if heads == 1:
+        hs = width
+    if cs != 1 or (at | 2 * ts | 2 * hs) & 15 or ts < width or hs < width:
+        t = t.contiguous()
+        if t.data_ptr() & 15:
+            t = t.clone()
+        at, ts, hs = t.data_ptr(), heads * width, width
+    return t, Rows(at, ts, hs)
 
 
-def _rows(t: torch.Tensor, token_dim: int = 0) -> Rows:
-    tokens, heads, width = t.shape[token_dim], t.shape[token_dim + 1], t.shape[token_dim + 2]
-    hs = t.stride(token_dim + 1) if heads != 1 else width
-    return Rows(t.data_ptr(), t.stride(token_dim) if tokens != 1 else max(hs * heads, width), hs)
+def _cache(t: torch.Tensor, what: str) -> Tuple[Rows, int]:
+    """The library's view of a cache (n, capacity, heads, width), which is read in place, and the stride of its sequences."""
+    (ss, ts, hs, cs), (n, tokens, heads, width), at = t.stride(), t.shape, t.data_ptr()
+    if t.numel() == 0:
+        return _NO_ROWS, 0
+    if n == 1:
+        ss = 0
+    if tokens == 1:
+        ts = heads * width
+    if heads == 1:
+        hs = width
+    if cs != 1 or (at | 2 * ss | 2 * ts | 2 * hs) & 15 or ts < width or hs < width or (n > 1 and ss < width):
+        raise ValueError(f"{what} is read in place: contiguous columns, strides multiples of 8 elements, data on 16 bytes")
+    return Rows(at, ts, hs), ss
+
+
+def _new(t: torch.Tensor) -> Tuple[torch.Tensor, Rows]:
+    """A dense array like t and the library's view of it."""
+    y = torch.empty_like(t, memory_format=torch.contiguous_format)
+    _, heads, width = y.shape
+    return y, Rows(y.data_ptr(), heads * width, width)
 
 
 def _type_of(q: torch.Tensor, *others: torch.Tensor) -> int:
@@ -139,14 +173,15 @@ def _needs_grad(*tensors) -> bool:
 # window attention
 # ---------------------------------------------------------------------------------------------------------------------
 def _check_qkv(plan, q, k, v):
-    if q.dim() != 3 or k.dim() != 3:
+    qs, ks = q.shape, k.shape
+    if len(qs) != 3 or len(ks) != 3:
         raise ValueError("q, k, v are (tokens, heads, width) arrays")
     _check_plan(plan, q)
-    _check_width(q.shape[2])
-    _shape(k, (q.shape[0], k.shape[1], q.shape[2]), "k")
-    _shape(v, k.shape, "v")
-    if k.shape[1] < 1 or q.shape[1] % k.shape[1]:
-        raise ValueError(f"{q.shape[1]} heads do not share {k.shape[1]} key heads evenly")
+    _check_width(qs[2])
+    if ks[0] != qs[0] or ks[2] != qs[2] or v.shape != ks:
+        raise ValueError(f"q {tuple(qs)}, k {tuple(ks)} and v {tuple(v.shape)} do not match")
+    if ks[1] < 1 or qs[1] % ks[1]:
+        raise ValueError(f"{qs[1]} heads do not share {ks[1]} key heads evenly")
 
 
 def window_attention(plan: SequencePlan, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: int, sinks: int = 0,
@@ -164,12 +199,11 @@ def _window_forward(plan, q, k, v, window, sinks, scale):
     kind = _type_of(q, k, v)
     _check_qkv(plan, q, k, v)
     window, sinks, scale = _window_numbers(q.shape[2], window, sinks, scale)
-    q, k, v = _aligned(q), _aligned(k), _aligned(v)
-    out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-    lse = torch.empty(q.shape[1], q.shape[0], device=q.device, dtype=torch.float32)
-    with torch.cuda.device(q.device):
-        st = _lib.lib().f3m_window_attention(C.byref(plan._seqs), kind, q.shape[1], k.shape[1], q.shape[2], window, sinks, scale, _rows(q),
-                                             _rows(k), _rows(v), _rows(out), lse.data_ptr(), _stream(q.device))
+    tokens, heads, width = q.shape
+    (q, rq), (k, rk), (v, rv), (out, ro) = _read(q), _read(k), _read(v), _new(q)
+    lse = torch.empty((heads, tokens), device=q.device, dtype=torch.float32)
+    with _On(q.device) as stream:
+        st = _lib.lib().f3m_window_attention(plan._ref, kind, heads, k.shape[1], width, window, sinks, scale, rq, rk, rv, ro, lse.data_ptr(), stream)
     check(st, "f3m_window_attention")
     return out, lse
 
@@ -186,15 +220,15 @@ def window_attention_grad(plan: SequencePlan, q: torch.Tensor, k: torch.Tensor, 
     if lse.dtype != torch.float32 or lse.device != q.device:
         raise TypeError("lse must be the float32 array that window_attention returned")
     window, sinks, scale = _window_numbers(q.shape[2], window, sinks, scale)
-    q, k, v, out, dout, lse = _aligned(q), _aligned(k), _aligned(v), _aligned(out), _aligned(dout), lse.contiguous()
-    dq, dk, dv = (torch.empty(x.shape, device=q.device, dtype=q.dtype) for x in (q, k, v))
+    heads, lse = q.shape[1], lse.contiguous()
+    (q, rq), (k, rk), (v, rv), (out, ro), (dout, rg) = _read(q), _read(k), _read(v), _read(out), _read(dout)
+    (dq, wq), (dk, wk), (dv, wv) = _new(q), _new(k), _new(v)
     L = _lib.lib()
-    need = L.f3m_window_attention_grad_workspace_bytes(C.byref(plan._seqs), q.shape[1])
+    need = L.f3m_window_attention_grad_workspace_bytes(plan._ref, heads)
     ws = torch.empty(need, device=q.device, dtype=torch.uint8)
-    with torch.cuda.device(q.device):
-        st = L.f3m_window_attention_grad(C.byref(plan._seqs), kind, q.shape[1], k.shape[1], q.shape[2], window, sinks, scale, _rows(q), _rows(k),
-                                         _rows(v), _rows(out), lse.data_ptr(), _rows(dout), _rows(dq), _rows(dk), _rows(dv), ws.data_ptr(),
-                                         need, _stream(q.device))
+    with _On(q.device) as stream:
+        st = L.f3m_window_attention_grad(plan._ref, kind, heads, k.shape[1], q.shape[2], window, sinks, scale, rq, rk, rv, ro, lse.data_ptr(), rg,
+                                         wq, wk, wv, ws.data_ptr(), need, stream)
     check(st, "f3m_window_attention_grad")
     return dq, dk, dv
 
@@ -237,18 +271,14 @@ def window_attention_step(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
     if _needs_grad(q, k_cache, v_cache):
         raise RuntimeError("window_attention_step has no gradient: call it under torch.no_grad()")
     window, sinks, scale = _window_numbers(width, window, sinks, scale)
-    q, lengths = _aligned(q), lengths.contiguous()
-    for c in (k_cache, v_cache):
-        if n and capacity and _aligned(c) is not c:
-            raise ValueError("a cache is read in place: contiguous columns, strides multiples of 8 elements, data on 16 bytes")
-    out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+    lengths = lengths.contiguous()
+    (q, rq), (out, ro), (rk, sk), (rv, sv) = _read(q), _new(q), _cache(k_cache, "k_cache"), _cache(v_cache, "v_cache")
     L = _lib.lib()
     need = L.f3m_window_attention_step_workspace_bytes(n, heads, kv_heads, width, capacity, window, sinks)
     ws = torch.empty(need, device=q.device, dtype=torch.uint8) if need else None
-    with torch.cuda.device(q.device):
-        st = L.f3m_window_attention_step(n, kind, heads, kv_heads, width, capacity, window, sinks, scale, _rows(q), _rows(k_cache, 1),
-                                         k_cache.stride(0) if n > 1 else 0, _rows(v_cache, 1), v_cache.stride(0) if n > 1 else 0, lengths.data_ptr(), _rows(out),
-                                         ws.data_ptr() if need else None, need, _stream(q.device))
+    with _On(q.device) as stream:
+        st = L.f3m_window_attention_step(n, kind, heads, kv_heads, width, capacity, window, sinks, scale, rq, rk, sk, rv, sv, lengths.data_ptr(), ro,
+                                         _pointer(ws), need, stream)
     check(st, "f3m_window_attention_step")
     return out
 
@@ -295,7 +325,7 @@ def decay_attention(plan: SequencePlan, q: torch.Tensor, k: torch.Tensor, v: tor
 
 
 def _decay_workspace(plan, q, v):
-    need = _lib.lib().f3m_decay_attention_workspace_bytes(C.byref(plan._seqs), q.shape[1], q.shape[2], v.shape[2])
+    need = _lib.lib().f3m_decay_attention_workspace_bytes(plan._ref, q.shape[1], q.shape[2], v.shape[2])
     return need, (torch.empty(need, device=q.device, dtype=torch.uint8) if need else None)
 
 
@@ -305,13 +335,13 @@ def _decay_forward(plan, q, k, v, log_decay, state, scale):
     _check_plan(plan, q)
     state = _check_state(state, plan.sequences, q, v, "state")
     scale = q.shape[2] ** -0.5 if scale is None else float(scale)
-    q, k, v, log_decay = _aligned(q), _aligned(k), _aligned(v), log_decay.contiguous()
-    out = torch.empty(v.shape, device=q.device, dtype=q.dtype)
-    final = torch.empty(plan.sequences, q.shape[1], q.shape[2], v.shape[2], device=q.device, dtype=torch.float32)
+    log_decay, heads = log_decay.contiguous(), q.shape[1]
+    (q, rq), (k, rk), (v, rv), (out, ro) = _read(q), _read(k), _read(v), _new(v)
+    final = torch.empty((plan.sequences, heads, q.shape[2], v.shape[2]), device=q.device, dtype=torch.float32)
     need, ws = _decay_workspace(plan, q, v)
-    with torch.cuda.device(q.device):
-        st = _lib.lib().f3m_decay_attention(C.byref(plan._seqs), kind, q.shape[1], q.shape[2], v.shape[2], log_decay.data_ptr(), scale, _rows(q), _rows(k),
-                                            _rows(v), _pointer(state), _rows(out), final.data_ptr(), _pointer(ws), need, _stream(q.device))
+    with _On(q.device) as stream:
+        st = _lib.lib().f3m_decay_attention(plan._ref, kind, heads, q.shape[2], v.shape[2], log_decay.data_ptr(), scale, rq, rk, rv, _pointer(state), ro,
+                                            final.data_ptr(), _pointer(ws), need, stream)
     check(st, "f3m_decay_attention")
     return out, final
 
@@ -328,14 +358,14 @@ def decay_attention_grad(plan: SequencePlan, q: torch.Tensor, k: torch.Tensor, v
     state = _check_state(state, plan.sequences, q, v, "state")
     dfinal = _check_state(dfinal, plan.sequences, q, v, "dfinal")
     scale = q.shape[2] ** -0.5 if scale is None else float(scale)
-    q, k, v, dout, log_decay = _aligned(q), _aligned(k), _aligned(v), _aligned(dout), log_decay.contiguous()
-    dq, dk, dv = (torch.empty(x.shape, device=q.device, dtype=q.dtype) for x in (q, k, v))
-    dstate = torch.empty(plan.sequences, q.shape[1], q.shape[2], v.shape[2], device=q.device, dtype=torch.float32)
+    log_decay, heads = log_decay.contiguous(), q.shape[1]
+    (q, rq), (k, rk), (v, rv), (dout, rg) = _read(q), _read(k), _read(v), _read(dout)
+    (dq, wq), (dk, wk), (dv, wv) = _new(q), _new(k), _new(v)
+    dstate = torch.empty((plan.sequences, heads, q.shape[2], v.shape[2]), device=q.device, dtype=torch.float32)
     need, ws = _decay_workspace(plan, q, v)
-    with torch.cuda.device(q.device):
-        st = _lib.lib().f3m_decay_attention_grad(C.byref(plan._seqs), kind, q.shape[1], q.shape[2], v.shape[2], log_decay.data_ptr(), scale, _rows(q),
-                                                 _rows(k), _rows(v), _pointer(state), _rows(dout), _pointer(dfinal), _rows(dq), _rows(dk), _rows(dv),
-                                                 dstate.data_ptr(), _pointer(ws), need, _stream(q.device))
+    with _On(q.device) as stream:
+        st = _lib.lib().f3m_decay_attention_grad(plan._ref, kind, heads, q.shape[2], v.shape[2], log_decay.data_ptr(), scale, rq, rk, rv, _pointer(state),
+                                                 rg, _pointer(dfinal), wq, wk, wv, dstate.data_ptr(), _pointer(ws), need, stream)
     check(st, "f3m_decay_attention_grad")
     return dq, dk, dv, dstate
 
@@ -369,11 +399,11 @@ def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_
     if _needs_grad(q, k, v, log_decay, state):
         raise RuntimeError("decay_attention_step has no gradient: call it under torch.no_grad()")
     scale = q.shape[2] ** -0.5 if scale is None else float(scale)
-    q, k, v, log_decay = _aligned(q), _aligned(k), _aligned(v), log_decay.contiguous()
-    out = torch.empty(v.shape, device=q.device, dtype=q.dtype)
-    with torch.cuda.device(q.device):
-        st = _lib.lib().f3m_decay_attention_step(q.shape[0], kind, q.shape[1], q.shape[2], v.shape[2], log_decay.data_ptr(), scale, _rows(q), _rows(k),
-                                                 _rows(v), state.data_ptr(), _rows(out), _stream(q.device))
+    log_decay = log_decay.contiguous()
+    (q, rq), (k, rk), (v, rv), (out, ro) = _read(q), _read(k), _read(v), _new(v)
+    n, heads, width = q.shape
+    with _On(q.device) as stream:
+        st = _lib.lib().f3m_decay_attention_step(n, kind, heads, width, v.shape[2], log_decay.data_ptr(), scale, rq, rk, rv, state.data_ptr(), ro, stream)
     check(st, "f3m_decay_attention_step")
     torch.autograd.graph.increment_version(state)
     return out

@@ -323,7 +323,7 @@ typedef struct f3m_rows {       /* (tokens, heads, width): element (t, h, c) is 
 typedef struct f3m_seqs {
     const int32_t *table;       /* device */
     int64_t tokens;             /* sum of the lengths: rows of every array */
-    int32_t sequences, tiles, pairs, longest;
+    int32_t sequences, empty, tiles, pairs, longest;    /* empty: sequences without tokens */
     int32_t table_words;
 } f3m_seqs;
 int f3m_seqs_layout(const int32_t *lengths, int32_t n, f3m_seqs *seqs, int32_t *table);

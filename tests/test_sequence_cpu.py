@@ -21,7 +21,7 @@ def layout(lengths):
 @pytest.mark.parametrize("lengths", [[1], [0], [128, 129, 0, 1, 5000], [7] * 40])
 def test_layout(lengths):
     s, t = layout(lengths)
-    assert (s.tokens, s.sequences, s.longest) == (sum(lengths), len(lengths), max(lengths))
+    assert (s.tokens, s.sequences, s.empty, s.longest) == (sum(lengths), len(lengths), lengths.count(0), max(lengths))
     first = np.cumsum(lengths) - lengths
     tiles = [(first[i], n, a, i) for i, n in enumerate(lengths) for a in range(0, n, 128)]
     assert s.tiles == len(tiles) and len(t) == 3 * len(tiles) + len(lengths) + s.pairs
@@ -72,7 +72,7 @@ def test_argument_checks_of_the_entries():
     assert window(q=Rows(base + 2, 128, 64)) == 1 and window(k=Rows(base, 132, 64)) == 1 and window(v=Rows(base, 128, -64)) == 1
     assert window(out=Rows(base, 64, 64)) == 1 and b"overlap" in L.f3m_last_error()
     assert window(out=Rows(base, 128, 0)) == 1
-    bad = Seqs(None, 130, 2, 3, 2, 100, 0)
+    bad = Seqs(None, 130, 2, 0, 3, 2, 100, 0)
     assert window(seqs=bad) == 1
 
     def grad(ws=base, have=1 << 20, dk=ok):
