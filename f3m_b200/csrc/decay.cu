@@ -15,28 +15,29 @@ __device__ __forceinline__ float2 unpack2(f32x2 v) {
 //     O = use * ( upd * (L o A B^T) C + diag(decay^steps) A S )        near pairs one by one, far ones through the state
 //     S = decay^m S + (diag(upd * decay^left) B)^T C                   the state moves on by a tile
 //
-// All products run on the tensor cores.  While warps 0-3 turn A B^T into the weights (rounded to 16 bits, written over it in tensor memory),
-// warps 4-11 split the scaled rows of B into a sum of 16-bit parts, in place, over A, and over the state's operand: the state is kept and returned
-// in FP32, and one rounding of what is added to it would leave it 2^-9 off in bf16.  Two parts lose 2^-17 (bf16) or 2^-23 (fp16); a state that is
-// returned takes a third in bf16, one that only serves the tiles behind it does not.  As an operand of A S the state is rounded to 16
-// bits, like the weights.
+// All products run on the tensor cores.  Warps 0-3 turn A B^T into the weights (rounded to 16 bits, written over it in tensor memory) and scale the
+// rows of A S; warps 4-11 split the scaled rows of B into a sum of 16-bit parts, in place, over A, and over the state's operand: the state is kept
+// and returned in FP32, and one rounding of what is added to it would leave it 2^-9 off in bf16.  Two parts lose 2^-17 (bf16) or 2^-23 (fp16); a
+// state that is returned takes a third in bf16, one that only serves the tiles behind it does not.  As an operand of A S the state is rounded to
+// 16 bits, like the weights.
 //
-// What bounds it: tile by tile, the state's way round -- parts written, their products, the state read, rounded and scaled, A S, parts of the next
-// tile.  A B^T, the weights, their product and the outputs run beside it, and so do the copies of the next tile.
+// What bounds it: tile by tile, the state's way round -- products of the parts, the state read, rounded, scaled, A S, the parts put over what that has
+// read.  The arithmetic of the split, A B^T of the next tile, its weights, the outputs and the copies run beside it.
 //
 // A range that does not begin with a sequence needs the state that the ranges before it leave: decay_states computes what each range
 // adds to the state (B and C only), decay_join runs over the ranges, and decay_tiles starts from that.  B and C are then read
 // twice, which is the price of using all SMs when there are fewer heads than SMs.
 constexpr int DK_COPY = 12, DK_PRODUCTS = 13, DK_THREADS = 32 * 14;   // warps: 0-3 weights and outputs, 4-11 operands, copies, products
+constexpr int MAX_RANGES = 3 * NUM_SMS_HINT;
 constexpr int DS_THREADS = 32 * 10;                                   // decay_states: 0-7 operands, copies, products
 constexpr int DK_BLOCK = SEQ_TILE * 128;                     // bytes of a block of 64 columns
 constexpr int DK_TILES = 14;                                 // blocks of 64 columns in shared memory: the tiles of all stages and the state
 
 struct DecayKernel {
     DecayArgs a;
-    CUtensorMap ma, mb, mc, mo;
+    CUtensorMap ma, mb, mc;
     int ranges, per_range;      // per_range tiles each
-    float *carry;               // (ranges, heads, width of b, width of c): the state behind each range
+    float *carry;               // (ranges, heads, width of c, width of b): the state behind each range
     int *err;
 };
 
@@ -52,27 +53,48 @@ __device__ __forceinline__ int tiles_before(const DecayArgs &a, const int4 &e) {
     return a.reversed ? n - 1 - i : i;
 }
 
-// 32 columns of row j of a state, from column c0 on
-__device__ __forceinline__ void state_row(const uint32_t (&r)[32], float *dst, bool transposed, int wb, int wc, int j, int c0) {
+// 16 columns of row j of a state in memory, from column c0 on.  Consecutive threads have consecutive rows: transposed, (width of c, width of b), their
+// accesses join, and so the states between ranges lie; row by row a thread takes 16 bytes at a time.
+__device__ __forceinline__ void load_state(uint32_t (&r)[16], const float *src, bool transposed, int wb, int wc, int j, int c0) {
+#pragma unroll
+    for (int c = 0; c < 16; c++) r[c] = 0u;
+    if (!src || j >= wb) return;
     if (transposed) {
 #pragma unroll
-        for (int c = 0; c < 32; c++)
-            if (j < wb && c0 + c < wc) dst[(int64_t)(c0 + c) * wb + j] = __uint_as_float(r[c]);
+        for (int c = 0; c < 16; c++)
+            if (c0 + c < wc) r[c] = __float_as_uint(src[(c0 + c) * wb + j]);
     } else {
 #pragma unroll
-        for (int c = 0; c < 32; c += 4)
-            if (j < wb && c0 + c < wc) *reinterpret_cast<uint4 *>(dst + (int64_t)j * wc + c0 + c) = make_uint4(r[c], r[c + 1], r[c + 2], r[c + 3]);
+        for (int c = 0; c < 16; c += 4)
+            if (c0 + c < wc) {
+                const uint4 v = *reinterpret_cast<const uint4 *>(src + j * wc + c0 + c);
+                r[c] = v.x; r[c + 1] = v.y; r[c + 2] = v.z; r[c + 3] = v.w;
+            }
     }
 }
-// Row j of a tile of B, times f, as a sum of 16-bit parts: 16-byte chunks [c0, c1) of its blocks; the first part stays in place.  j >= rows: zeros.
-template <typename T, int PARTS>
-__device__ __forceinline__ void split_rows(uint32_t head, uint32_t tail, uint32_t rest, int j, bool in, f32x2 f, int c0, int c1) {
+__device__ __forceinline__ void store_state(const uint32_t (&r)[16], float *dst, bool transposed, int wb, int wc, int j, int c0) {
+    if (j >= wb) return;
+    if (transposed) {
+#pragma unroll
+        for (int c = 0; c < 16; c++)
+            if (c0 + c < wc) dst[(c0 + c) * wb + j] = __uint_as_float(r[c]);
+    } else {
+#pragma unroll
+        for (int c = 0; c < 16; c += 4)
+            if (c0 + c < wc) *reinterpret_cast<uint4 *>(dst + j * wc + c0 + c) = make_uint4(r[c], r[c + 1], r[c + 2], r[c + 3]);
+    }
+}
+
+// Half of row j of a tile of B, times f, as a sum of 16-bit parts: 16-byte chunks [c0, c0 + N) of its blocks.  The first part takes the row's place,
+// the others stay in registers until their places are free.  !in: zeros.
+template <typename T, int PARTS, int N>
+__device__ __forceinline__ void split_row(uint32_t head, int j, bool in, f32x2 f, int c0, uint32_t (&tail)[N][4], uint32_t (&rest)[N][4]) {
     const f32x2 minus = pack2(-1.f, -1.f);
-#pragma unroll 2
-    for (int i = c0; i < c1; i++) {
-        const uint32_t at = (i >> 3) * DK_BLOCK + tc::swz(j, i & 7);
-        uint32_t v[4], w[4], z[4];
-        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(head + at) : "memory");
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const uint32_t at = head + ((c0 + i) >> 3) * DK_BLOCK + tc::swz(j, (c0 + i) & 7);
+        uint32_t v[4];
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(at) : "memory");
 #pragma unroll
         for (int q = 0; q < 4; q++) {
             const float2 u = Half<T>::unpack(in ? v[q] : 0u);
@@ -82,62 +104,56 @@ __device__ __forceinline__ void split_rows(uint32_t head, uint32_t tail, uint32_
             y = Half<T>::unpack(v[q]);
             x = fma2(pack2(y.x, y.y), minus, x);
             y = unpack2(x);
-            w[q] = Half<T>::pack(y.x, y.y);
+            tail[i][q] = Half<T>::pack(y.x, y.y);
             if (PARTS == 3) {
-                y = Half<T>::unpack(w[q]);
+                y = Half<T>::unpack(tail[i][q]);
                 y = unpack2(fma2(pack2(y.x, y.y), minus, x));
-                z[q] = Half<T>::pack(y.x, y.y);
+                rest[i][q] = Half<T>::pack(y.x, y.y);
             }
         }
-        sts16(head + at, v);
-        sts16(tail + at, w);
-        if (PARTS == 3) sts16(rest + at, z);
+        sts16(at, v);
     }
 }
+template <int N>
+__device__ __forceinline__ void put_row(uint32_t tile, int j, int c0, const uint32_t (&v)[N][4]) {
+#pragma unroll
+    for (int i = 0; i < N; i++) sts16(tile + ((c0 + i) >> 3) * DK_BLOCK + tc::swz(j, (c0 + i) & 7), v[i]);
+}
+
 template <typename T, int PARTS, int NB>
 __global__ void __launch_bounds__(DK_THREADS, 1) decay_tiles(const __grid_constant__ DecayKernel p) {
     extern __shared__ unsigned char raw[];
-    __shared__ __align__(8) uint64_t bars[2 * 4 + 8];
+    __shared__ __align__(8) uint64_t bars[2 * 4 + 9];
     __shared__ uint32_t tmem_s;
     __shared__ int gave_up_s;
-    __shared__ __align__(16) float pw[32], pr[32];   // decay^n, decay^(31 - n)
     const DecayArgs &a = p.a;
-    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, h = blockIdx.y;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, h = blockIdx.x, range = blockIdx.y;
     const int nc = (a.width_c + 63) / 64;
     const int stage_blocks = 2 * NB + nc, stages = min(4, (DK_TILES - max(NB, nc)) / stage_blocks);
     const uint32_t smem = (tc::smem_u32(raw) + 1023) & ~1023u, state_s = smem + stages * stage_blocks * DK_BLOCK;
     const float l2 = log2_decay(a.log_decay[h]);
-    const int first = blockIdx.x * p.per_range, tiles = min(a.s.tiles, first + p.per_range) - first;
+    const int first = range * p.per_range, tiles = min(a.s.tiles, first + p.per_range) - first;
 
     if (warp == DK_COPY) tc::tmem_alloc(tc::smem_u32(&tmem_s), 512);
     if (tid == 0) {
         for (int i = 0; i < 4; i++) {
             tc::mbar_init(tc::smem_u32(&bars[i]), 1);                                  // landed (by stage)
-            tc::mbar_init(tc::smem_u32(&bars[4 + i]), 2);                              // free again: products done, outputs on their way
+            tc::mbar_init(tc::smem_u32(&bars[4 + i]), 1);                              // free again
         }
-        tc::mbar_init(tc::smem_u32(&bars[8]), 1);                                      // A B^T done
-        tc::mbar_init(tc::smem_u32(&bars[9]), 1);                                      // A S done
-        tc::mbar_init(tc::smem_u32(&bars[10]), 1);                                     // state done
-        tc::mbar_init(tc::smem_u32(&bars[11]), 1);                                     // outputs done
-        tc::mbar_init(tc::smem_u32(&bars[12]), 128);                                   // weights written
-        tc::mbar_init(tc::smem_u32(&bars[13]), 256);                                   // B split
-        tc::mbar_init(tc::smem_u32(&bars[14]), 256);                                   // state ready as operand and in tensor memory
-        tc::mbar_init(tc::smem_u32(&bars[15]), 128);                                   // outputs read
+        for (int i = 8; i < 12; i++) tc::mbar_init(tc::smem_u32(&bars[i]), 1);         // A B^T, A S, state, outputs done
+        for (int i = 12; i < 15; i++) tc::mbar_init(tc::smem_u32(&bars[i]), 128);      // weights written, A S scaled, outputs read
+        for (int i = 15; i < 17; i++) tc::mbar_init(tc::smem_u32(&bars[i]), 256);      // B split; state ready as operand and in tensor memory
         tc::fence_mbar_init();
         gave_up_s = 0;
-    }
-    if (tid < 32) {
-        pw[tid] = exp2f(l2 * tid);
-        pr[tid] = exp2f(l2 * (31 - tid));
     }
     tc::fence_before_sync();
     __syncthreads();
     tc::fence_after_sync();
     const Waits wait{&gave_up_s, p.err};
-    const uint32_t tmem = tmem_s, t_score = tmem, t_inter = tmem + 128, t_intra = tmem + 256, t_state = tmem + 384;
+    const uint32_t tmem = tmem_s, t_score = tmem, t_out = tmem + 256, t_state = tmem + 384;   // two places for scores, in turn
     const uint32_t b_full = tc::smem_u32(&bars[0]), b_free = tc::smem_u32(&bars[4]), b_score = tc::smem_u32(&bars[8]), b_inter = tc::smem_u32(&bars[9]),
-                   b_moved = tc::smem_u32(&bars[10]), b_done = tc::smem_u32(&bars[11]), b_weights = tc::smem_u32(&bars[12]), b_split = tc::smem_u32(&bars[13]),
-                   b_state = tc::smem_u32(&bars[14]), b_read = tc::smem_u32(&bars[15]);
+                   b_moved = tc::smem_u32(&bars[10]), b_done = tc::smem_u32(&bars[11]), b_weights = tc::smem_u32(&bars[12]), b_scaled = tc::smem_u32(&bars[13]),
+                   b_read = tc::smem_u32(&bars[14]), b_split = tc::smem_u32(&bars[15]), b_state = tc::smem_u32(&bars[16]);
     auto a_tile = [&](int s) { return smem + s * stage_blocks * DK_BLOCK; };
     auto b_tile = [&](int s) { return a_tile(s) + NB * DK_BLOCK; };
     auto c_tile = [&](int s) { return a_tile(s) + 2 * NB * DK_BLOCK; };
@@ -170,45 +186,53 @@ __global__ void __launch_bounds__(DK_THREADS, 1) decay_tiles(const __grid_consta
         constexpr bool bf = Half<T>::type == F3M_TYPE_BF16;
         const uint32_t i_score = tc::idesc_f16(bf, 128, 128, false, false), i_rows = tc::idesc_f16(bf, 128, 64 * nc, false, true),
                        i_state = tc::idesc_f16(bf, 128, 64 * nc, true, true);
-        for (int n = 0; n < tiles; n++) {
+        auto score = [&](int n) {
             const int s = n % stages;
             wait(b_full + 8 * s, (n / stages) & 1);
             tc::fence_after_sync();
             if (tc::elect()) {
-                tc::product_rows<NB>(t_score, a_tile(s), b_tile(s), i_score);
+                tc::product_rows<NB>(t_score + 128 * (n & 1), a_tile(s), b_tile(s), i_score);
                 tc::mma_commit(b_score);
             }
+        };
+        score(0);
+        for (int n = 0; n < tiles; n++) {
+            const int s = n % stages;
             if (n) wait(b_read, (n - 1) & 1);
             wait(b_state, n & 1);
             tc::fence_after_sync();
             if (tc::elect()) {
-                tc::product_mixed<NB>(t_inter, a_tile(s), state_s, i_rows);
+                tc::product_mixed<NB>(t_out, a_tile(s), state_s, i_rows);
                 tc::mma_commit(b_inter);
             }
+            // the next tile's scores beside the split's last step, if it has landed: the state does not wait for a copy
+            const bool more = n + 1 < tiles, early = more && __all_sync(0xffffffffu, tc::mbar_test(b_full + 8 * ((n + 1) % stages), ((n + 1) / stages) & 1));
+            if (early) score(n + 1);
             wait(b_split, n & 1);   // also clears the rows of C that belong to another sequence
             tc::fence_after_sync();
             if (tc::elect()) {
-                tc::product_cols<true>(t_state, b_tile(s), c_tile(s), i_state);
-                tc::product_cols<true>(t_state, a_tile(s), c_tile(s), i_state);
-                if (PARTS == 3) tc::product_cols<true>(t_state, state_s, c_tile(s), i_state);
+#pragma unroll
+                for (int part = 0; part < PARTS; part++) tc::product_cols(t_state, part == 0 ? b_tile(s) : part == 1 ? a_tile(s) : state_s, c_tile(s), i_state, 1);
                 tc::mma_commit(b_moved);
             }
             wait(b_weights, n & 1);
+            wait(b_scaled, n & 1);
             tc::fence_after_sync();
             if (tc::elect()) {
-                tc::product_tmem<false>(t_intra, t_score, c_tile(s), i_rows);
+                tc::product_tmem(t_out, t_score + 128 * (n & 1), c_tile(s), i_rows, 1);
                 tc::mma_commit(b_done);
                 tc::mma_commit(b_free + 8 * s);
             }
+            if (more && !early) score(n + 1);
         }
     } else if (warp < 4) {
         // ---- weights and outputs: thread i has row i ----
         const int i = tid;
         const uint32_t lanes = (uint32_t)(32 * warp) << 16;
         const float coef = a.use * a.upd;
-        for (int n = 0; n < tiles; n++) {
-            const int4 e = tile_at(a, first + n);
-            const int m = tile_rows(e), s = n % stages;
+        const bool wide = rows_wide(a.out);
+        auto weights = [&](int n, int m) {
+            const uint32_t t_s = t_score + 128 * (n & 1) + lanes;
             all_wait(b_score, n & 1);
             tc::fence_after_sync();
 #pragma unroll 1
@@ -217,76 +241,109 @@ __global__ void __launch_bounds__(DK_THREADS, 1) decay_tiles(const __grid_consta
                 const bool near = a.reversed ? cb >= warp : cb <= warp;   // warp-uniform
                 if (near) {
                     uint32_t r[32];
-                    tc::tmem_ld32(t_score + lanes + 32 * cb, r);
+                    tc::tmem_ld32(t_s + 32 * cb, r);
                     tc::tmem_ld_wait(r);
-                    if (cb == warp) {
+                    // the power of the decay by ex2: the unit has nothing else to do here
+                    const float from = a.reversed ? (float)(32 * cb - i) : (float)(i - 32 * cb);
+                    const bool cut = cb == warp || m < SEQ_TILE;
 #pragma unroll
-                        for (int c = 0; c < 32; c += 2) {
-                            float x[2];
+                    for (int c = 0; c < 32; c += 2) {
+                        float x[2];
 #pragma unroll
-                            for (int q = 0; q < 2; q++) {
-                                const int apart = a.reversed ? c + q - lane : lane - c - q;
-                                x[q] = apart >= 0 && 32 * cb + c + q < m ? __uint_as_float(r[c + q]) * (coef * pw[max(apart, 0)]) : 0.f;
-                            }
-                            w[c / 2] = Half<T>::pack(x[0], x[1]);
+                        for (int q = 0; q < 2; q++) {
+                            const float apart = a.reversed ? from + (c + q) : from - (c + q);
+                            x[q] = coef * __uint_as_float(r[c + q]) * ex2_approx(l2 * apart);
+                            if (cut && (apart < 0.f || 32 * cb + c + q >= m)) x[q] = 0.f;
                         }
-                    } else {
-                        const float f = coef * exp2f(l2 * (a.reversed ? 32 * cb - i : i - 32 * cb - 31));
-                        const float *tab = a.reversed ? pw : pr;
-#pragma unroll
-                        for (int c = 0; c < 32; c += 2) {
-                            const float2 t = *reinterpret_cast<const float2 *>(tab + c);
-                            const float x0 = __uint_as_float(r[c]) * (f * t.x), x1 = __uint_as_float(r[c + 1]) * (f * t.y);
-                            w[c / 2] = Half<T>::pack(32 * cb + c < m ? x0 : 0.f, 32 * cb + c + 1 < m ? x1 : 0.f);
-                        }
+                        w[c / 2] = Half<T>::pack(x[0], x[1]);
                     }
                 } else {
 #pragma unroll
                     for (int c = 0; c < 16; c++) w[c] = 0u;
                 }
                 // columns 16 cb .. of the weights lie over scores that this warp has read
-                tc::tmem_st16(t_score + lanes + 16 * cb, w);
+                tc::tmem_st16(t_s + 16 * cb, w);
             }
             tc::tmem_st_wait();
             tc::fence_before_sync();
             tc::mbar_arrive(b_weights);
-
-            all_wait(b_done, n & 1);
+        };
+        int4 e = tile_at(a, first);
+        weights(0, tile_rows(e));
+        for (int n = 0; n < tiles; n++) {
+            const int m = tile_rows(e);
+            const int4 ahead = n + 1 < tiles ? tile_at(a, first + n + 1) : e;
+            const float f = a.use * exp2f(l2 * (a.reversed ? max(m - 1 - i, 0) : i + 1));
+            all_wait(b_inter, n & 1);
             tc::fence_after_sync();
-            // the outputs go over C, which has been read, and leave from there
-            const float f = a.use * exp2f(l2 * (a.reversed ? m - 1 - i : i + 1));
 #pragma unroll 1
             for (int cb = 0; cb < 2 * nc; cb++) {
-                uint32_t x[32], y[32];
-                tc::tmem_ld32(t_inter + lanes + 32 * cb, x);
-                tc::tmem_ld32(t_intra + lanes + 32 * cb, y);
+                uint32_t x[32];
+                tc::tmem_ld32(t_out + lanes + 32 * cb, x);
                 tc::tmem_ld_wait(x);
-                tc::tmem_ld_wait(y);
 #pragma unroll
-                for (int c = 0; c < 32; c += 8) {
-                    uint32_t w[4];
-#pragma unroll
-                    for (int q = 0; q < 4; q++)
-                        w[q] = Half<T>::pack(fmaf(f, __uint_as_float(x[c + 2 * q]), __uint_as_float(y[c + 2 * q])),
-                                             fmaf(f, __uint_as_float(x[c + 2 * q + 1]), __uint_as_float(y[c + 2 * q + 1])));
-                    sts16(c_tile(s) + (cb >> 1) * DK_BLOCK + tc::swz(i, 4 * (cb & 1) + c / 8), w);
-                }
+                for (int c = 0; c < 32; c++) x[c] = __float_as_uint(f * __uint_as_float(x[c]));
+                tc::tmem_st32(t_out + lanes + 32 * cb, x);
             }
+            tc::tmem_st_wait();
             tc::fence_before_sync();
-            tc::mbar_arrive(b_read);
-            store_rows<128>(p.mo, a.out, c_tile(s), h, e.x + e.z, m, 0, nc, a.width_c, i, 1);
-            if (i == 0) tc::mbar_arrive(b_free + 8 * s);
+            tc::mbar_arrive(b_scaled);
+            // the next tile's weights now, if its scores are there, else behind the outputs
+            const bool now = n + 1 < tiles && __all_sync(0xffffffffu, tc::mbar_test(b_score, (n + 1) & 1));
+            if (now) weights(n + 1, tile_rows(ahead));
+            all_wait(b_done, n & 1);
+            tc::fence_after_sync();
+            uint16_t *row = reinterpret_cast<uint16_t *>(a.out.data) + (int64_t)(e.x + e.z + i) * a.out.token_stride + (int64_t)h * a.out.head_stride;
+#pragma unroll 1
+            for (int cb = 0; cb < 2 * nc; cb++) {
+                uint32_t x[32], w[16];
+                tc::tmem_ld32(t_out + lanes + 32 * cb, x);
+                tc::tmem_ld_wait(x);
+                if (cb + 1 == 2 * nc) {
+                    tc::fence_before_sync();
+                    tc::mbar_arrive(b_read);
+                }
+#pragma unroll
+                for (int c = 0; c < 16; c++) w[c] = Half<T>::pack(__uint_as_float(x[2 * c]), __uint_as_float(x[2 * c + 1]));
+                if (i < m) store_row32(row, w, 32 * cb, a.width_c, wide);
+                __syncwarp();
+            }
+            if (n + 1 < tiles && !now) weights(n + 1, tile_rows(ahead));
+            e = ahead;
         }
-        if (i == 0) tc::tma_store_wait_all();
-    } else if (warp < DK_COPY) {
+    } else {
         // ---- operands: threads j and j + 128 have row j of B and C, and row j of the state, half each ----
         const int j = tid & 127, half = (tid - 128) >> 7;
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
         const int64_t plane = (int64_t)a.width_b * a.width_c;
-        int4 e = tile_at(a, first);
-        for (int n = 0; n < tiles; n++) {
+        int4 e = tile_at(a, first), gone = e;
+        for (int n = 0; n <= tiles; n++) {
             const int m = tile_rows(e), s = n % stages;
             const int4 ahead = n + 1 < tiles ? tile_at(a, first + n + 1) : e;
+            uint32_t tail[4 * NB][4], rest[4 * NB][4];
+            if (n < tiles) {
+                all_wait(b_full + 8 * s, (n / stages) & 1);
+                all_wait(b_score, n & 1);   // B has been read
+                const float f = a.upd * exp2f(l2 * (a.reversed ? j + 1 : max(m - 1 - j, 0)));   // rows behind the sequence: a number, to be times 0
+                split_row<T, PARTS, 4 * NB>(b_tile(s), j, j < m, pack2(f, f), 4 * NB * half, tail, rest);
+                if (j >= m) clear_row(c_tile(s), j, 4 * nc * half, 4 * nc * (half + 1));
+            }
+            if (n) {
+                all_wait(b_moved, (n - 1) & 1);
+                tc::fence_after_sync();
+                if (a.state_out && tile_ends(a, gone) && 32 * (warp & 3) < a.width_b) {   // whole warps
+                    float *dst = a.state_out + ((int64_t)gone.w * a.heads + h) * plane;
+#pragma unroll 1
+                    for (int cb = 2 * half * nc; cb < 2 * (half + 1) * nc; cb++) {
+                        uint32_t r[16];
+                        tc::tmem_ld16(t_state + lanes + 16 * cb, r);
+                        tc::tmem_ld_wait(r);
+                        store_state(r, dst, a.transposed, a.width_b, a.width_c, j, 16 * cb);
+                        __syncwarp();
+                    }
+                }
+                if (n == tiles) break;
+            }
             // the state before the tile: from tensor memory, or where a sequence or the range begins
             const bool begins = tile_begins(a, e), fresh = begins || n == 0;
             const float scale = exp2f(l2 * m);
@@ -294,71 +351,39 @@ __global__ void __launch_bounds__(DK_THREADS, 1) decay_tiles(const __grid_consta
             if (begins) {
                 if (a.state_in) src = a.state_in + ((int64_t)e.w * a.heads + h) * plane;
             } else if (n == 0) {
-                src = p.carry + ((int64_t)(blockIdx.x - 1) * a.heads + h) * plane;
+                src = p.carry + ((int64_t)(range - 1) * a.heads + h) * plane;
             }
-            const bool turned = begins && a.transposed;
 #pragma unroll 1
-            for (int cb = half * nc; cb < (half + 1) * nc; cb++) {
-                uint32_t r[32];
+            for (int cb = 2 * half * nc; cb < 2 * (half + 1) * nc; cb++) {   // 16 columns at a time
+                uint32_t r[16];
                 if (!fresh) {
-                    tc::tmem_ld32(t_state + lanes + 32 * cb, r);
+                    tc::tmem_ld16(t_state + lanes + 16 * cb, r);
                     tc::tmem_ld_wait(r);
                 } else {
-#pragma unroll
-                    for (int c = 0; c < 32; c++) r[c] = 0u;
-                    if (src && j < a.width_b) {
-                        if (turned) {
-#pragma unroll
-                            for (int c = 0; c < 32; c++)
-                                if (32 * cb + c < a.width_c) r[c] = __float_as_uint(src[(int64_t)(32 * cb + c) * a.width_b + j]);
-                        } else {
-#pragma unroll
-                            for (int c = 0; c < 32; c += 4)
-                                if (32 * cb + c < a.width_c) {
-                                    const uint4 v = *reinterpret_cast<const uint4 *>(src + (int64_t)j * a.width_c + 32 * cb + c);
-                                    r[c] = v.x; r[c + 1] = v.y; r[c + 2] = v.z; r[c + 3] = v.w;
-                                }
-                        }
-                    }
+                    load_state(r, src, !begins || a.transposed, a.width_b, a.width_c, j, 16 * cb);
+                    __syncwarp();
                 }
-                const uint32_t row = state_s + (cb >> 1) * DK_BLOCK;
 #pragma unroll
-                for (int c = 0; c < 32; c += 8) {
+                for (int c = 0; c < 16; c += 8) {
                     uint32_t w[4];
 #pragma unroll
                     for (int q = 0; q < 4; q++) w[q] = Half<T>::pack(__uint_as_float(r[c + 2 * q]), __uint_as_float(r[c + 2 * q + 1]));
-                    sts16(row + tc::swz(j, 4 * (cb & 1) + c / 8), w);
+                    sts16(state_s + (cb >> 2) * DK_BLOCK + tc::swz(j, 2 * (cb & 3) + c / 8), w);
                 }
 #pragma unroll
-                for (int c = 0; c < 32; c++) r[c] = __float_as_uint(scale * __uint_as_float(r[c]));
-                __syncwarp();
-                tc::tmem_st32(t_state + lanes + 32 * cb, r);
+                for (int c = 0; c < 16; c++) r[c] = __float_as_uint(scale * __uint_as_float(r[c]));
+                tc::tmem_st16(t_state + lanes + 16 * cb, r);
             }
             tc::tmem_st_wait();
             tc::fence_async_smem();
             tc::fence_before_sync();
             tc::mbar_arrive(b_state);
-
-            all_wait(b_full + 8 * s, (n / stages) & 1);
-            all_wait(b_inter, n & 1);   // A, B and the state's operand have been read
-            const float f = a.upd * exp2f(l2 * (a.reversed ? j + 1 : max(m - 1 - j, 0)));   // rows behind the sequence: a number, to be times 0
-            split_rows<T, PARTS>(b_tile(s), a_tile(s), state_s, j, j < m, pack2(f, f), 4 * NB * half, 4 * NB * (half + 1));
-            if (j >= m) clear_row(c_tile(s), j, 4 * nc * half, 4 * nc * (half + 1));
+            all_wait(b_inter, n & 1);   // A and the state's operand have been read
+            put_row(a_tile(s), j, 4 * NB * half, tail);
+            if (PARTS == 3) put_row(state_s, j, 4 * NB * half, rest);
             tc::fence_async_smem();
             tc::mbar_arrive(b_split);
-            all_wait(b_moved, n & 1);
-            tc::fence_after_sync();
-            if (a.state_out && tile_ends(a, e) && 32 * (warp & 3) < a.width_b) {   // whole warps
-                float *dst = a.state_out + ((int64_t)e.w * a.heads + h) * plane;
-#pragma unroll 1
-                for (int cb = half * nc; cb < (half + 1) * nc; cb++) {
-                    uint32_t r[32];
-                    tc::tmem_ld32(t_state + lanes + 32 * cb, r);
-                    tc::tmem_ld_wait(r);
-                    state_row(r, dst, a.transposed, a.width_b, a.width_c, j, 32 * cb);
-                    __syncwarp();
-                }
-            }
+            gone = e;
             e = ahead;
         }
     }
@@ -378,16 +403,16 @@ __global__ void __launch_bounds__(DS_THREADS, 1) decay_states(const __grid_const
     __shared__ uint32_t tmem_s;
     __shared__ int gave_up_s;
     const DecayArgs &a = p.a;
-    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, h = blockIdx.y;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, h = blockIdx.x, range = blockIdx.y;
     const int nc = (a.width_c + 63) / 64, stage_blocks = NB + nc, parts_blocks = (PARTS - 1) * NB;
     // a product reads 128 columns of B, with one block of them the block behind it too: what it finds there goes to rows of the state that are not used
     const int stages = min(4, (DK_TILES - parts_blocks - (NB == 1)) / stage_blocks);
     const uint32_t smem = (tc::smem_u32(raw) + 1023) & ~1023u, parts_s = smem + stages * stage_blocks * DK_BLOCK;
     const float l2 = log2_decay(a.log_decay[h]);
-    const int last = min(a.s.tiles, (int)(blockIdx.x + 1) * p.per_range);
+    const int last = min(a.s.tiles, (range + 1) * p.per_range);
     const int4 end = tile_at(a, last - 1);
     if (tile_ends(a, end)) return;
-    const int first = max((int)blockIdx.x * p.per_range, last - 1 - tiles_before(a, end)), tiles = last - first;
+    const int first = max(range * p.per_range, last - 1 - tiles_before(a, end)), tiles = last - first;
     // token behind the range, as its place in the sequence
     const int stop = a.reversed ? end.z : end.z + SEQ_TILE;
 
@@ -432,12 +457,11 @@ __global__ void __launch_bounds__(DS_THREADS, 1) decay_states(const __grid_const
             wait(b_split, n & 1);
             tc::fence_after_sync();
             if (tc::elect()) {
-                const uint32_t last_part = parts_s + (PARTS - 2) * NB * DK_BLOCK;
-                if (n) tc::product_cols<true>(t_state, last_part, c_tile(s), i_state);
-                else tc::product_cols<false>(t_state, last_part, c_tile(s), i_state);
-                if (PARTS == 3) tc::product_cols<true>(t_state, parts_s, c_tile(s), i_state);
-                tc::mma_commit(b_tails);
-                tc::product_cols<true>(t_state, b_tile(s), c_tile(s), i_state);
+#pragma unroll
+                for (int part = PARTS - 1; part >= 0; part--) {
+                    tc::product_cols(t_state, part ? parts_s + (part - 1) * NB * DK_BLOCK : b_tile(s), c_tile(s), i_state, n > 0 || part < PARTS - 1);
+                    if (part == 1) tc::mma_commit(b_tails);
+                }
                 tc::mma_commit(b_free + 8 * s);
                 if (n + 1 == tiles) tc::mma_commit(b_done);
             }
@@ -448,9 +472,12 @@ __global__ void __launch_bounds__(DS_THREADS, 1) decay_states(const __grid_const
             const int4 e = tile_at(a, first + n);
             const int m = tile_rows(e), s = n % stages;
             const float f = a.upd * exp2f(l2 * (a.reversed ? e.z + j + 1 - stop : stop - 1 - e.z - j));
+            uint32_t tail[4 * NB][4], rest[4 * NB][4];
             wait(b_full + 8 * s, (n / stages) & 1);
+            split_row<T, PARTS, 4 * NB>(b_tile(s), j, j < m, pack2(f, f), 4 * NB * half, tail, rest);
             if (n) wait(b_tails, (n - 1) & 1);
-            split_rows<T, PARTS>(b_tile(s), parts_s, parts_s + NB * DK_BLOCK, j, j < m, pack2(f, f), 4 * NB * half, 4 * NB * (half + 1));
+            put_row(parts_s, j, 4 * NB * half, tail);
+            if (PARTS == 3) put_row(parts_s + NB * DK_BLOCK, j, 4 * NB * half, rest);
             if (j >= m) clear_row(c_tile(s), j, 4 * nc * half, 4 * nc * (half + 1));
             tc::fence_async_smem();
             tc::mbar_arrive(b_split);
@@ -463,18 +490,17 @@ __global__ void __launch_bounds__(DS_THREADS, 1) decay_states(const __grid_const
             const int4 b = tile_at(a, first);
             const float *src = tile_begins(a, b) && a.state_in ? a.state_in + ((int64_t)b.w * a.heads + h) * plane : nullptr;
             const float f = exp2f(l2 * (a.reversed ? min(b.y, b.z + SEQ_TILE) - stop : stop - b.z));
-            float *dst = p.carry + ((int64_t)blockIdx.x * a.heads + h) * plane;
+            float *dst = p.carry + ((int64_t)range * a.heads + h) * plane;
 #pragma unroll 1
-            for (int cb = half * nc; cb < (half + 1) * nc; cb++) {
-                uint32_t r[32];
-                tc::tmem_ld32(t_state + ((uint32_t)(32 * (warp & 3)) << 16) + 32 * cb, r);
+            for (int cb = 2 * half * nc; cb < 2 * (half + 1) * nc; cb++) {
+                uint32_t r[16];
+                tc::tmem_ld16(t_state + ((uint32_t)(32 * (warp & 3)) << 16) + 16 * cb, r);
                 tc::tmem_ld_wait(r);
-                if (src && j < a.width_b)
+                uint32_t b0[16];
+                load_state(b0, src, a.transposed, a.width_b, a.width_c, j, 16 * cb);
 #pragma unroll
-                    for (int c = 0; c < 32; c++)
-                        if (32 * cb + c < a.width_c)
-                            r[c] = __float_as_uint(fmaf(f, src[a.transposed ? (int64_t)(32 * cb + c) * a.width_b + j : (int64_t)j * a.width_c + 32 * cb + c], __uint_as_float(r[c])));
-                state_row(r, dst, false, a.width_b, a.width_c, j, 32 * cb);
+                for (int c = 0; c < 16; c++) r[c] = __float_as_uint(fmaf(f, __uint_as_float(b0[c]), __uint_as_float(r[c])));
+                store_state(r, dst, true, a.width_b, a.width_c, j, 16 * cb);
                 __syncwarp();
             }
         }
@@ -487,23 +513,36 @@ __global__ void __launch_bounds__(DS_THREADS, 1) decay_states(const __grid_const
 
 // Runs over the ranges of a head: where range r is a stretch of one sequence that began before it, the state behind it is what it adds
 // plus the state behind range r - 1, decayed over its tokens.
-__global__ void __launch_bounds__(256) decay_join(const __grid_constant__ DecayKernel p) {
+__global__ void __launch_bounds__(128) decay_join(const __grid_constant__ DecayKernel p) {
     const DecayArgs &a = p.a;
-    const int h = blockIdx.y, plane = a.width_b * a.width_c, at = 4 * (blockIdx.x * 256 + threadIdx.x);
+    __shared__ float keep_s[MAX_RANGES];   // what range r leaves of the state behind range r - 1; -1: it leaves nothing to the next
+    const int h = blockIdx.y, plane = a.width_b * a.width_c, at = 2 * (blockIdx.x * 128 + threadIdx.x);
     const float l2 = log2_decay(a.log_decay[h]);
-    float4 before = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int r = 0; r + 1 < p.ranges; r++) {
-        const int last = (r + 1) * p.per_range;
-        const int4 e = tile_at(a, last - 1), b = tile_at(a, r * p.per_range);
-        if (tile_ends(a, e) || at >= plane) continue;
-        float4 *mine = reinterpret_cast<float4 *>(p.carry + ((int64_t)r * a.heads + h) * plane + at);
-        float4 x = *mine;
-        if (e.w == b.w && !tile_begins(a, b)) {
-            const float f = exp2f(l2 * (a.reversed ? min(b.y, b.z + SEQ_TILE) - e.z : e.z + tile_rows(e) - b.z));
-            x.x = fmaf(f, before.x, x.x); x.y = fmaf(f, before.y, x.y); x.z = fmaf(f, before.z, x.z); x.w = fmaf(f, before.w, x.w);
-            *mine = x;
-        }
-        before = x;
+    for (int r = threadIdx.x; r + 1 < p.ranges; r += 128) {
+        const int4 e = tile_at(a, (r + 1) * p.per_range - 1), b = tile_at(a, r * p.per_range);
+        const bool through = e.w == b.w && !tile_begins(a, b);
+        keep_s[r] = tile_ends(a, e) ? -1.f : through ? exp2f(l2 * (a.reversed ? min(b.y, b.z + SEQ_TILE) - e.z : e.z + tile_rows(e) - b.z)) : 0.f;
+    }
+    __syncthreads();
+    if (at >= plane) return;
+    float2 before = make_float2(0.f, 0.f);
+    constexpr int AHEAD = 8;
+    for (int r0 = 0; r0 + 1 < p.ranges; r0 += AHEAD) {
+        float2 x[AHEAD];
+#pragma unroll
+        for (int k = 0; k < AHEAD; k++)
+            if (r0 + k + 1 < p.ranges && keep_s[r0 + k] >= 0.f) x[k] = *reinterpret_cast<const float2 *>(p.carry + ((int64_t)(r0 + k) * a.heads + h) * plane + at);
+#pragma unroll
+        for (int k = 0; k < AHEAD; k++)
+            if (r0 + k + 1 < p.ranges && keep_s[r0 + k] >= 0.f) {
+                const float f = keep_s[r0 + k];
+                if (f > 0.f) {
+                    x[k].x = fmaf(f, before.x, x[k].x);
+                    x[k].y = fmaf(f, before.y, x[k].y);
+                    *reinterpret_cast<float2 *>(p.carry + ((int64_t)(r0 + k) * a.heads + h) * plane + at) = x[k];
+                }
+                before = x[k];
+            }
     }
 }
 
@@ -520,7 +559,7 @@ __global__ void __launch_bounds__(256) decay_empty(DecayArgs a) {
 static int decay_ranges(const f3m_seqs &s, int heads) {
     int best = 1;
     float least = 0.f;
-    for (int r = 1; r <= s.tiles && (r == 1 || (int64_t)heads * r <= 3 * NUM_SMS_HINT); r++) {
+    for (int r = 1; r <= s.tiles && (r == 1 || (int64_t)heads * r <= MAX_RANGES); r++) {
         const int64_t ctas = (int64_t)heads * r, waves = (ctas + NUM_SMS_HINT - 1) / NUM_SMS_HINT;
         const int per = (s.tiles + r - 1) / r;
         const float cost = r == 1 ? (float)(waves * per) : 1.5f * (float)(waves * per) + 4.f;
@@ -539,14 +578,14 @@ static void launch_parts(const DecayKernel &p, cudaStream_t s) {
     if (p.ranges > 1) {
         static SharedMemory states;
         states.allow(decay_states<T, PARTS, NB>, bytes);
-        decay_states<T, PARTS, NB><<<dim3(p.ranges - 1, p.a.heads), DS_THREADS, bytes, s>>>(p);
+        decay_states<T, PARTS, NB><<<dim3(p.a.heads, p.ranges - 1), DS_THREADS, bytes, s>>>(p);
         F3M_LAUNCH_CHECK();
-        decay_join<<<dim3((p.a.width_b * p.a.width_c / 4 + 255) / 256, p.a.heads), 256, 0, s>>>(p);
+        decay_join<<<dim3((p.a.width_b * p.a.width_c / 2 + 127) / 128, p.a.heads), 128, 0, s>>>(p);
         F3M_LAUNCH_CHECK();
     }
     static SharedMemory tiles;
     tiles.allow(decay_tiles<T, PARTS, NB>, bytes);
-    decay_tiles<T, PARTS, NB><<<dim3(p.ranges, p.a.heads), DK_THREADS, bytes, s>>>(p);
+    decay_tiles<T, PARTS, NB><<<dim3(p.a.heads, p.ranges), DK_THREADS, bytes, s>>>(p);
     F3M_LAUNCH_CHECK();
 }
 
@@ -565,7 +604,6 @@ static void decay_product_t(const DecayArgs &a, cudaStream_t s) {
     p.ranges = decay_ranges(a.s, a.heads);
     p.per_range = (a.s.tiles + p.ranges - 1) / p.ranges;
     p.ranges = (a.s.tiles + p.per_range - 1) / p.per_range;
-    p.mo = seq_tensor_map(Half<T>::type, a.out, a.s.tokens, a.heads, a.width_c);
     p.carry = (float *)a.ws;
     p.err = seq_error_word();
     // a state that is returned in FP32 takes three parts of bf16

@@ -128,28 +128,24 @@ public:
     }
 };
 
-// Waits of a kernel's roles on one another.  None is longer than about two seconds: what expires raises `gave_up`, after which every wait of
-// the block returns at once and the block runs to its end on whatever it finds, inside its buffers.
+// Waits of a kernel's roles on one another.  None is longer than about two seconds (a try lasts two microseconds at most): what expires raises
+// `gave_up`, after which every wait of the block returns at once and the block runs to its end on whatever it finds, inside its buffers. 
+constexpr uint32_t WAIT_TRIES = 1000000;
 struct Waits {
     volatile int *gave_up;
     int *err;
     __device__ __forceinline__ void operator()(uint32_t bar, uint32_t parity) const {
-        if (tc::mbar_try_wait(bar, parity)) return;
-        const long long t0 = clock64();
-        while (!tc::mbar_try_wait(bar, parity)) {
-            if (*gave_up) return;
-            if (clock64() - t0 > 4000000000ll) {
+        uint32_t tries = 0;
+        while (!tc::mbar_try_wait_ns(bar, parity, 2000))
+            if (*gave_up || ++tries > WAIT_TRIES) {
                 *gave_up = 1;
                 *(volatile int *)err = 1;
-                __threadfence_system();
                 return;
             }
-        }
     }
     // also when the block has given up: copies in flight are waited for before it ends
     __device__ __forceinline__ void drain(uint32_t bar, uint32_t parity) const {
-        const long long t0 = clock64();
-        while (!tc::mbar_try_wait(bar, parity) && clock64() - t0 < 4000000000ll) {}
+        for (uint32_t tries = 0; tries < WAIT_TRIES && !tc::mbar_try_wait_ns(bar, parity, 2000); tries++) {}
     }
 };
 
@@ -159,8 +155,26 @@ __device__ __forceinline__ void sts16(uint32_t at, const uint32_t (&w)[4]) {
 // Chunks [c0, c1) of row j of a tile become zero: tokens of the next sequence meet no weight, not even a weight of zero
 __device__ __forceinline__ void clear_row(uint32_t tile, int j, int c0, int c1) {
     const uint32_t zero[4] = {0u, 0u, 0u, 0u};
+#pragma unroll 1
     for (int i = c0; i < c1; i++) sts16(tile + (i >> 3) * SEQ_TILE * 128 + tc::swz(j, i & 7), zero);
 }
+
+// 32 columns of a row, 16 bits each, to memory; `wide`: the row starts on 32 bytes.  Rows go straight from registers: a thread writes whole sectors.
+__device__ __forceinline__ void store_row32(uint16_t *row, const uint32_t (&w)[16], int c0, int width, bool wide) {
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        uint16_t *at = row + c0 + 16 * h;
+        if (wide && c0 + 16 * h + 16 <= width)
+            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(at), "r"(w[8 * h]), "r"(w[8 * h + 1]), "r"(w[8 * h + 2]), "r"(w[8 * h + 3]),
+                         "r"(w[8 * h + 4]), "r"(w[8 * h + 5]), "r"(w[8 * h + 6]), "r"(w[8 * h + 7])
+                         : "memory");
+        else {
+            if (c0 + 16 * h < width) *reinterpret_cast<uint4 *>(at) = make_uint4(w[8 * h], w[8 * h + 1], w[8 * h + 2], w[8 * h + 3]);
+            if (c0 + 16 * h + 8 < width) *reinterpret_cast<uint4 *>(at + 8) = make_uint4(w[8 * h + 4], w[8 * h + 5], w[8 * h + 6], w[8 * h + 7]);
+        }
+    }
+}
+__host__ __device__ __forceinline__ bool rows_wide(const f3m_rows &r) { return (uintptr_t)r.data % 32 == 0 && r.token_stride % 16 == 0 && r.head_stride % 16 == 0; }
 
 // Rows 0 .. m of a swizzled tile in shared memory, columns from col0 on, to tokens token .. token + m, by THREADS threads (t) that have each written rows of it;
 // on return thread 0 knows that the tile has been read.  A whole tile leaves as bulk copies; one that ends inside would write over the
@@ -172,12 +186,14 @@ __device__ __forceinline__ void store_rows(const CUtensorMap &map, const f3m_row
         tc::fence_async_smem();
         tc::bar_sync(barrier, THREADS);
         if (t == 0) {
+#pragma unroll 1
             for (int k = 0; k < blocks; k++) tc::tma_store_rows(&map, tile + k * SEQ_TILE * 128, col0 + 64 * k, head, token);
             tc::tma_store_commit();
             tc::tma_store_wait_read();
         }
     } else {
         tc::bar_sync(barrier, THREADS);
+#pragma unroll 1
         for (int i = t; i < m * 8 * blocks; i += THREADS) {   // 16-byte chunks; consecutive threads along a row
             const int r = i / (8 * blocks), c = i % (8 * blocks);
             uint32_t v[4];

@@ -22,6 +22,30 @@ __device__ __forceinline__ uint32_t mbar_try_wait(uint32_t bar, uint32_t parity)
         : "memory");
     return ok;
 }
+// whether the phase has ended, now
+__device__ __forceinline__ uint32_t mbar_test(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok;
+}
+// a try of at most `ns` nanoseconds
+__device__ __forceinline__ uint32_t mbar_try_wait_ns(uint32_t bar, uint32_t parity, uint32_t ns) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity), "r"(ns)
+        : "memory");
+    return ok;
+}
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void fence_before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -70,6 +94,23 @@ __device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[32]) {
                    "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]),
                    "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]),
                    "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+                 :
+                 : "memory");
+}
+
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                   "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
                  :
                  : "memory");
 }
@@ -124,21 +165,19 @@ __host__ __device__ constexpr uint32_t idesc_f16(bool bf16, int M, int N, bool a
     return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((amn ? 1u : 0u) << 15) | ((bmn ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) |
            ((uint32_t)(M >> 4) << 24);
 }
-template <bool ACC>
-__device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc) {
+__device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "n"(ACC ? 1 : 0)
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
 // A from tensor memory: row r in lane r, two consecutive elements of the contraction per 32-bit column
-template <bool ACC>
-__device__ __forceinline__ void mma_f16_ta(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc) {
+__device__ __forceinline__ void mma_f16_ta(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem), "r"(a_tmem), "l"(bdesc), "r"(idesc), "n"(ACC ? 1 : 0)
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem), "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
 // One lane of a whole warp: the values that its instructions take are the warp's, and stay in uniform registers
@@ -148,47 +187,47 @@ __device__ __forceinline__ bool elect() {
     return one;
 }
 // Products of whole tiles (128 rows; blocks of 64 columns, 16384 bytes each), issued by one thread.  A thread issues an instruction every few clocks
-// and a step of a product takes 64: the loops are unrolled and a step's operands are the first one's plus a constant.  ACC: added to D.
+// and a step of a product takes 64: the loops are unrolled, and a step's operands are the first one's plus a constant.  `acc`: added to D.
 constexpr int BLOCK = 128 * 128;
-// D = A B^T: both contract along their columns, NB blocks of them
-template <int NB, bool ACC = false>
-__device__ __forceinline__ void product_rows(uint32_t d, uint32_t a_tile, uint32_t b_tile, uint32_t idesc) {
-    const uint64_t a = desc_k(a_tile), b = desc_k(b_tile);
-    mma_f16<ACC>(d, a, b, idesc);
+// four steps: 64 of the contraction
+template <int STEP_A, int STEP_B>
+__device__ __forceinline__ void product64(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    mma_f16(d, a, b, idesc, acc);
 #pragma unroll
-    for (int k = 1; k < 4 * NB; k++) mma_f16<true>(d, a + (k >> 2) * (BLOCK >> 4) + (k & 3) * 2, b + (k >> 2) * (BLOCK >> 4) + (k & 3) * 2, idesc);
+    for (int k = 1; k < 4; k++) mma_f16(d, a + k * STEP_A, b + k * STEP_B, idesc, 1);
+}
+// D = A B^T: both contract along their columns, NB blocks of them
+template <int NB>
+__device__ __forceinline__ void product_rows(uint32_t d, uint32_t a_tile, uint32_t b_tile, uint32_t idesc) {
+    uint64_t a = desc_k(a_tile), b = desc_k(b_tile);
+#pragma unroll
+    for (int i = 0; i < NB; i++, a += BLOCK >> 4, b += BLOCK >> 4) product64<2, 2>(d, a, b, idesc, i);
 }
 // D = A B: A contracts along its columns, NB blocks of them, B along its rows
-template <int NB, bool ACC = false>
+template <int NB>
 __device__ __forceinline__ void product_mixed(uint32_t d, uint32_t a_tile, uint32_t b_tile, uint32_t idesc) {
-    const uint64_t a = desc_k(a_tile), b = desc_mn(b_tile, BLOCK);
-    mma_f16<ACC>(d, a, b, idesc);
+    uint64_t a = desc_k(a_tile), b = desc_mn(b_tile, BLOCK);
 #pragma unroll
-    for (int k = 1; k < 4 * NB; k++) mma_f16<true>(d, a + (k >> 2) * (BLOCK >> 4) + (k & 3) * 2, b + k * (2048 >> 4), idesc);
+    for (int i = 0; i < NB; i++, a += BLOCK >> 4, b += 4 * 2048 >> 4) product64<2, 2048 / 16>(d, a, b, idesc, i);
 }
 // D = A^T B: both contract along their rows
-template <bool ACC>
-__device__ __forceinline__ void product_cols(uint32_t d, uint32_t a_tile, uint32_t b_tile, uint32_t idesc) {
-    const uint64_t a = desc_mn(a_tile, BLOCK), b = desc_mn(b_tile, BLOCK);
-    mma_f16<ACC>(d, a, b, idesc);
+__device__ __forceinline__ void product_cols(uint32_t d, uint32_t a_tile, uint32_t b_tile, uint32_t idesc, uint32_t acc) {
+    uint64_t a = desc_mn(a_tile, BLOCK), b = desc_mn(b_tile, BLOCK);
 #pragma unroll
-    for (int k = 1; k < 8; k++) mma_f16<true>(d, a + k * (2048 >> 4), b + k * (2048 >> 4), idesc);
+    for (int i = 0; i < 2; i++, a += 4 * 2048 >> 4, b += 4 * 2048 >> 4) product64<2048 / 16, 2048 / 16>(d, a, b, idesc, acc | i);
 }
-// D = A B: A, 128 x 128, from tensor memory, its second 64 elements a row GAP columns behind the first; B contracts along its rows
-template <bool ACC, int GAP = 32>
-__device__ __forceinline__ void product_tmem(uint32_t d, uint32_t a_tmem, uint32_t b_tile, uint32_t idesc) {
+// D = A B, 64 of the contraction: A from tensor memory, B contracts along its rows
+__device__ __forceinline__ void product_tmem64(uint32_t d, uint32_t a_tmem, uint32_t b_tile, uint32_t idesc, uint32_t acc) {
     const uint64_t b = desc_mn(b_tile, BLOCK);
-    mma_f16_ta<ACC>(d, a_tmem, b, idesc);
+    mma_f16_ta(d, a_tmem, b, idesc, acc);
 #pragma unroll
-    for (int k = 1; k < 8; k++) mma_f16_ta<true>(d, a_tmem + 8 * (k & 3) + GAP * (k >> 2), b + k * (2048 >> 4), idesc);
+    for (int k = 1; k < 4; k++) mma_f16_ta(d, a_tmem + 8 * k, b + k * (2048 >> 4), idesc, 1);
 }
-// ... 64 of the 128 elements of its rows
-template <bool ACC>
-__device__ __forceinline__ void product_tmem_half(uint32_t d, uint32_t a_tmem, uint32_t b_tile, uint32_t idesc) {
-    const uint64_t b = desc_mn(b_tile, BLOCK);
-    mma_f16_ta<ACC>(d, a_tmem, b, idesc);
+// ... all 128; the second 64 of A's rows lie GAP columns behind the first
+template <int GAP = 32>
+__device__ __forceinline__ void product_tmem(uint32_t d, uint32_t a_tmem, uint32_t b_tile, uint32_t idesc, uint32_t acc) {
 #pragma unroll
-    for (int k = 1; k < 4; k++) mma_f16_ta<true>(d, a_tmem + 8 * k, b + k * (2048 >> 4), idesc);
+    for (int i = 0; i < 2; i++, a_tmem += GAP, b_tile += 4 * 2048) product_tmem64(d, a_tmem, b_tile, idesc, acc | i);
 }
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
     asm volatile(

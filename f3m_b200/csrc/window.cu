@@ -148,15 +148,14 @@ __global__ void __launch_bounds__(WF_THREADS, 1) window_tiles(const __grid_const
                     wait(b_p + 8 * t, np[t] & 1);
                     tc::fence_after_sync();
                     if (tc::elect()) {
-                        if (j) tc::product_tmem_half<true>(tmem + 256 + 128 * t, tmem + 128 * t, slot_tile(sv), i_o);
-                        else tc::product_tmem_half<false>(tmem + 256 + 128 * t, tmem + 128 * t, slot_tile(sv), i_o);
+                        tc::product_tmem64(tmem + 256 + 128 * t, tmem + 128 * t, slot_tile(sv), i_o, j);
                     }
                     wait(b_p2 + 8 * t, np[t] & 1);
                     np[t]++;
                     no[t] += !more;
                     tc::fence_after_sync();
                     if (tc::elect()) {
-                        tc::product_tmem_half<true>(tmem + 256 + 128 * t, tmem + 128 * t + 32, slot_tile(sv) + 64 * 128, i_o);
+                        tc::product_tmem64(tmem + 256 + 128 * t, tmem + 128 * t + 32, slot_tile(sv) + 64 * 128, i_o, 1);
                         if (more) {
                             tc::product_rows<NB>(tmem + 128 * t, q_tile(t), slot_tile(sk), i_s);
                             tc::mma_commit(b_s + 8 * t);
@@ -458,8 +457,7 @@ __global__ void __launch_bounds__(WG_THREADS, 1) window_grad_keys(const __grid_c
             wait(b_p, n & 1);
             tc::fence_after_sync();
             if (tc::elect()) {
-                if (n) tc::product_tmem<true, 64>(t_dv, t_s, g_tile(s), i_d);
-                else tc::product_tmem<false, 64>(t_dv, t_s, g_tile(s), i_d);
+                tc::product_tmem<64>(t_dv, t_s, g_tile(s), i_d, n);
                 if (more) {
                     tc::product_rows<NB>(t_s, k_tile, q_tile(sn), i_s);
                     tc::mma_commit(b_s);
@@ -468,8 +466,7 @@ __global__ void __launch_bounds__(WG_THREADS, 1) window_grad_keys(const __grid_c
             wait(b_ds, n & 1);
             tc::fence_after_sync();
             if (tc::elect()) {
-                if (n) tc::product_tmem<true, 64>(t_dk, t_dp, q_tile(s), i_d);
-                else tc::product_tmem<false, 64>(t_dk, t_dp, q_tile(s), i_d);
+                tc::product_tmem<64>(t_dk, t_dp, q_tile(s), i_d, n);
                 tc::mma_commit(b_free + 8 * s);
                 if (more) {
                     tc::product_rows<NB>(t_dp, v_tile, g_tile(sn), i_s);
@@ -674,8 +671,7 @@ __global__ void __launch_bounds__(WG_THREADS, 1) window_grad_queries(const __gri
             tc::fence_after_sync();
             if (n + 1 < tiles) values(n + 1);
             if (tc::elect()) {
-                if (n) tc::product_tmem<true, 64>(t_dq, tmem + 128 * (n & 1), slot_tile(2 * n % slots), i_d);
-                else tc::product_tmem<false, 64>(t_dq, tmem + 128 * (n & 1), slot_tile(2 * n % slots), i_d);
+                tc::product_tmem<64>(t_dq, tmem + 128 * (n & 1), slot_tile(2 * n % slots), i_d, n);
                 tc::mma_commit(b_free + 8 * (2 * n % slots));
                 if (n + 1 == tiles) tc::mma_commit(b_done);
             }
