@@ -29,6 +29,7 @@ __device__ __forceinline__ float2 unpack2(f32x2 v) {
 // twice, which is the price of using all SMs when there are fewer heads than SMs.
 constexpr int DK_COPY = 12, DK_PRODUCTS = 13, DK_THREADS = 32 * 14;   // warps: 0-3 weights and outputs, 4-11 operands, copies, products
 constexpr int MAX_RANGES = 3 * NUM_SMS_HINT;
+constexpr int DK_AHEAD = 1;                                            // tiles brought into L2 before their stage is free
 constexpr int DS_THREADS = 32 * 10;                                   // decay_states: 0-7 operands, copies, products
 constexpr int DK_BLOCK = SEQ_TILE * 128;                     // bytes of a block of 64 columns
 constexpr int DK_TILES = 14;                                 // blocks of 64 columns in shared memory: the tiles of all stages and the state
@@ -123,7 +124,7 @@ __device__ __forceinline__ void put_row(uint32_t tile, int j, int c0, const uint
 template <typename T, int PARTS, int NB>
 __global__ void __launch_bounds__(DK_THREADS, 1) decay_tiles(const __grid_constant__ DecayKernel p) {
     extern __shared__ unsigned char raw[];
-    __shared__ __align__(8) uint64_t bars[2 * 4 + 9];
+    __shared__ __align__(8) uint64_t bars[2 * 4 + 10];
     __shared__ uint32_t tmem_s;
     __shared__ int gave_up_s;
     const DecayArgs &a = p.a;
@@ -142,6 +143,7 @@ __global__ void __launch_bounds__(DK_THREADS, 1) decay_tiles(const __grid_consta
         }
         for (int i = 8; i < 12; i++) tc::mbar_init(tc::smem_u32(&bars[i]), 1);         // A B^T, A S, state, outputs done
         for (int i = 12; i < 15; i++) tc::mbar_init(tc::smem_u32(&bars[i]), 128);      // weights written, A S scaled, outputs read
+        tc::mbar_init(tc::smem_u32(&bars[17]), 1);                                     // A B^T of every other tile
         for (int i = 15; i < 17; i++) tc::mbar_init(tc::smem_u32(&bars[i]), 256);      // B split; state ready as operand and in tensor memory
         tc::fence_mbar_init();
         gave_up_s = 0;
@@ -157,6 +159,8 @@ __global__ void __launch_bounds__(DK_THREADS, 1) decay_tiles(const __grid_consta
     auto a_tile = [&](int s) { return smem + s * stage_blocks * DK_BLOCK; };
     auto b_tile = [&](int s) { return a_tile(s) + NB * DK_BLOCK; };
     auto c_tile = [&](int s) { return a_tile(s) + 2 * NB * DK_BLOCK; };
+    // scores are two tiles ahead of the weights at times: a barrier for even tiles and one for odd
+    auto b_score_of = [&](int n) { return n & 1 ? tc::smem_u32(&bars[17]) : b_score; };
     auto all_wait = [&](uint32_t bar, uint32_t parity) {   // a whole warp, which stays together for the instructions that need that
         wait(bar, parity);
         __syncwarp();
@@ -165,6 +169,16 @@ __global__ void __launch_bounds__(DK_THREADS, 1) decay_tiles(const __grid_consta
     if (warp == DK_COPY) {
         // ---- copies ----
         if (lane == 0) {
+            // two stages are too few to keep memory busy: tiles further ahead are brought into L2
+            auto ahead = [&](int n) {
+                if (n >= tiles) return;
+                const int4 e = tile_at(a, first + n);
+                for (int k = 0; k < NB; k++) {
+                    tc::tma_prefetch_rows(&p.ma, 64 * k, h, e.x + e.z);
+                    tc::tma_prefetch_rows(&p.mb, 64 * k, h, e.x + e.z);
+                }
+                for (int k = 0; k < nc; k++) tc::tma_prefetch_rows(&p.mc, 64 * k, h, e.x + e.z);
+            };
             int n = 0;
             for (; n < tiles && !gave_up_s; n++) {
                 const int s = n % stages;
@@ -177,6 +191,7 @@ __global__ void __launch_bounds__(DK_THREADS, 1) decay_tiles(const __grid_consta
                     tc::tma_rows(b_tile(s) + k * DK_BLOCK, &p.mb, 64 * k, h, e.x + e.z, b_full + 8 * s);
                 }
                 for (int k = 0; k < nc; k++) tc::tma_rows(c_tile(s) + k * DK_BLOCK, &p.mc, 64 * k, h, e.x + e.z, b_full + 8 * s);
+                if (n + 1 >= stages) ahead(n + DK_AHEAD);
             }
             for (int s = 0; s < stages; s++)   // the last copy into each stage
                 if (n > s) wait.drain(b_full + 8 * s, ((n - 1 - s) / stages) & 1);
@@ -192,7 +207,7 @@ __global__ void __launch_bounds__(DK_THREADS, 1) decay_tiles(const __grid_consta
             tc::fence_after_sync();
             if (tc::elect()) {
                 tc::product_rows<NB>(t_score + 128 * (n & 1), a_tile(s), b_tile(s), i_score);
-                tc::mma_commit(b_score);
+                tc::mma_commit(b_score_of(n));
             }
         };
         score(0);
@@ -233,7 +248,7 @@ __global__ void __launch_bounds__(DK_THREADS, 1) decay_tiles(const __grid_consta
         const bool wide = rows_wide(a.out);
         auto weights = [&](int n, int m) {
             const uint32_t t_s = t_score + 128 * (n & 1) + lanes;
-            all_wait(b_score, n & 1);
+            all_wait(b_score_of(n), (n >> 1) & 1);
             tc::fence_after_sync();
 #pragma unroll 1
             for (int cb = 0; cb < 4; cb++) {
@@ -289,7 +304,7 @@ __global__ void __launch_bounds__(DK_THREADS, 1) decay_tiles(const __grid_consta
             tc::fence_before_sync();
             tc::mbar_arrive(b_scaled);
             // the next tile's weights now, if its scores are there, else behind the outputs
-            const bool now = n + 1 < tiles && __all_sync(0xffffffffu, tc::mbar_test(b_score, (n + 1) & 1));
+            const bool now = n + 1 < tiles && __all_sync(0xffffffffu, tc::mbar_test(b_score_of(n + 1), ((n + 1) >> 1) & 1));
             if (now) weights(n + 1, tile_rows(ahead));
             all_wait(b_done, n & 1);
             tc::fence_after_sync();
@@ -323,7 +338,7 @@ __global__ void __launch_bounds__(DK_THREADS, 1) decay_tiles(const __grid_consta
             uint32_t tail[4 * NB][4], rest[4 * NB][4];
             if (n < tiles) {
                 all_wait(b_full + 8 * s, (n / stages) & 1);
-                all_wait(b_score, n & 1);   // B has been read
+                all_wait(b_score_of(n), (n >> 1) & 1);   // B has been read
                 const float f = a.upd * exp2f(l2 * (a.reversed ? j + 1 : max(m - 1 - j, 0)));   // rows behind the sequence: a number, to be times 0
                 split_row<T, PARTS, 4 * NB>(b_tile(s), j, j < m, pack2(f, f), 4 * NB * half, tail, rest);
                 if (j >= m) clear_row(c_tile(s), j, 4 * nc * half, 4 * nc * (half + 1));
@@ -436,6 +451,12 @@ __global__ void __launch_bounds__(DS_THREADS, 1) decay_states(const __grid_const
     auto c_tile = [&](int s) { return b_tile(s) + NB * DK_BLOCK; };
     if (warp == 8) {
         if (lane == 0) {
+            auto ahead = [&](int n) {
+                if (n >= tiles) return;
+                const int4 e = tile_at(a, first + n);
+                for (int k = 0; k < NB; k++) tc::tma_prefetch_rows(&p.mb, 64 * k, h, e.x + e.z);
+                for (int k = 0; k < nc; k++) tc::tma_prefetch_rows(&p.mc, 64 * k, h, e.x + e.z);
+            };
             int n = 0;
             for (; n < tiles && !gave_up_s; n++) {
                 const int s = n % stages;
@@ -445,6 +466,7 @@ __global__ void __launch_bounds__(DS_THREADS, 1) decay_states(const __grid_const
                 tc::mbar_expect_tx(b_full + 8 * s, stage_blocks * DK_BLOCK);
                 for (int k = 0; k < NB; k++) tc::tma_rows(b_tile(s) + k * DK_BLOCK, &p.mb, 64 * k, h, e.x + e.z, b_full + 8 * s);
                 for (int k = 0; k < nc; k++) tc::tma_rows(c_tile(s) + k * DK_BLOCK, &p.mc, 64 * k, h, e.x + e.z, b_full + 8 * s);
+                if (n + 1 >= stages) ahead(n + DK_AHEAD);
             }
             for (int s = 0; s < stages; s++)
                 if (n > s) wait.drain(b_full + 8 * s, ((n - 1 - s) / stages) & 1);

@@ -254,6 +254,10 @@ __device__ __forceinline__ void tma_rows(uint32_t dst, const CUtensorMap *map, i
                  "r"(col), "r"(head), "r"(token), "r"(bar)
                  : "memory");
 }
+// ... into L2 only
+__device__ __forceinline__ void tma_prefetch_rows(const CUtensorMap *map, int col, int head, int token) {
+    asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global.tile [%0, {%1, %2, %3}];" ::"l"(map), "r"(col), "r"(head), "r"(token) : "memory");
+}
 // ... and back: what lies outside the array is not written
 __device__ __forceinline__ void tma_store_rows(const CUtensorMap *map, uint32_t src, int col, int head, int token) {
     asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(map), "r"(col), "r"(head), "r"(token), "r"(src)

@@ -243,6 +243,25 @@ def test_decay_attention_step(n, heads, width_k, width_v, dtype, cuda):
     ref.assert_within(out, (o, ref.half_step(dtype) * o.abs() + 1e-6 * mass + ref.tiny(dtype)), "out")
 
 
+def test_many_calls_in_a_row(cuda):
+    """The roles of a kernel's warps run apart from one another in ways that differ from call to call: the bits do not, and no wait runs out."""
+    from f3m_b200 import sequence as sq
+    tokens, h = 20011, 4
+    lengths = [tokens - 300, 299, 1]
+    q, k, v, do = (normal(i, tokens, h, 128, dtype=torch.bfloat16) for i in range(4))
+    ld = torch.tensor([-0.001, -0.03, -0.2, 0.0], device="cuda")
+    plan = sq.SequencePlan(lengths)
+
+    def calls():
+        out, lse = sq.window_attention(plan, q, k[:, :2], v[:, :2], 300, 5)
+        return (out, lse) + sq.window_attention_grad(plan, q, k[:, :2], v[:, :2], out, lse, do, 300, 5) + sq.decay_attention(plan, q, k, v, ld) + sq.decay_attention_grad(plan, q, k, v, ld, do)
+
+    first = calls()
+    for _ in range(150):
+        again = calls()
+        assert all(torch.equal(x, y) for x, y in zip(again, first))
+
+
 def test_steps_continue_a_prompt(cuda):
     """A prompt, then its answer token by token, as a model runs it: the same outputs as reading all of it at once."""
     from f3m_b200 import sequence as sq
