@@ -132,6 +132,7 @@ __global__ void __launch_bounds__(DK_THREADS, 1) decay_tiles(const __grid_consta
     const int nc = (a.width_c + 63) / 64;
     const int stage_blocks = 2 * NB + nc, stages = min(4, (DK_TILES - max(NB, nc)) / stage_blocks);
     const uint32_t smem = (tc::smem_u32(raw) + 1023) & ~1023u, state_s = smem + stages * stage_blocks * DK_BLOCK;
+    __shared__ __align__(16) float table_s[32];   // decay^(31 - c), from the end decay^c
     const float l2 = log2_decay(a.log_decay[h]);
     const int first = range * p.per_range, tiles = min(a.s.tiles, first + p.per_range) - first;
 
@@ -148,6 +149,7 @@ __global__ void __launch_bounds__(DK_THREADS, 1) decay_tiles(const __grid_consta
         tc::fence_mbar_init();
         gave_up_s = 0;
     }
+    if (tid < 32) table_s[tid] = exp2f(l2 * (a.reversed ? tid : 31 - tid));
     tc::fence_before_sync();
     __syncthreads();
     tc::fence_after_sync();
@@ -258,19 +260,32 @@ __global__ void __launch_bounds__(DK_THREADS, 1) decay_tiles(const __grid_consta
                     uint32_t r[32];
                     tc::tmem_ld32(t_s + 32 * cb, r);
                     tc::tmem_ld_wait(r);
-                    // the power of the decay by ex2: the unit has nothing else to do here
-                    const float from = a.reversed ? (float)(32 * cb - i) : (float)(i - 32 * cb);
-                    const bool cut = cb == warp || m < SEQ_TILE;
+                    if (cb != warp && m == SEQ_TILE) {   // off the diagonal: decay^(to the block's edge) times a table
+                        const float f = coef * exp2f(l2 * (a.reversed ? 32 * cb - i : i - 32 * cb - 31));
+                        const f32x2 ff = pack2(f, f);
+                        const ulonglong2 *tab = reinterpret_cast<const ulonglong2 *>(table_s);
 #pragma unroll
-                    for (int c = 0; c < 32; c += 2) {
-                        float x[2];
-#pragma unroll
-                        for (int q = 0; q < 2; q++) {
-                            const float apart = a.reversed ? from + (c + q) : from - (c + q);
-                            x[q] = coef * __uint_as_float(r[c + q]) * ex2_approx(l2 * apart);
-                            if (cut && (apart < 0.f || 32 * cb + c + q >= m)) x[q] = 0.f;
+                        for (int c = 0; c < 32; c += 4) {
+                            const ulonglong2 t = tab[c >> 2];
+                            float x[4];
+                            unpack2(mul2(pack2(__uint_as_float(r[c]), __uint_as_float(r[c + 1])), mul2(ff, t.x)), x[0], x[1]);
+                            unpack2(mul2(pack2(__uint_as_float(r[c + 2]), __uint_as_float(r[c + 3])), mul2(ff, t.y)), x[2], x[3]);
+                            w[c / 2] = Half<T>::pack(x[0], x[1]);
+                            w[c / 2 + 1] = Half<T>::pack(x[2], x[3]);
                         }
-                        w[c / 2] = Half<T>::pack(x[0], x[1]);
+                    } else {
+                        const float from = a.reversed ? (float)(32 * cb - i) : (float)(i - 32 * cb);
+#pragma unroll
+                        for (int c = 0; c < 32; c += 2) {
+                            float x[2];
+#pragma unroll
+                            for (int q = 0; q < 2; q++) {
+                                const float apart = a.reversed ? from + (c + q) : from - (c + q);
+                                x[q] = coef * __uint_as_float(r[c + q]) * ex2_approx(l2 * apart);
+                                if (apart < 0.f || 32 * cb + c + q >= m) x[q] = 0.f;
+                            }
+                            w[c / 2] = Half<T>::pack(x[0], x[1]);
+                        }
                     }
                 } else {
 #pragma unroll
