@@ -70,10 +70,11 @@ struct WindowArgs {
     f3m_rows q, k, v, out;
     float *lse;
     f3m_rows dout, dq, dk, dv;   // gradients only
-    float *delta;                // workspace: 2 x (heads, tokens)
+    float *delta;                // workspace: 2 x (heads, tokens), and the parts' sums
 };
 void window_forward(int type, const WindowArgs &a, cudaStream_t s);
 void window_backward(int type, const WindowArgs &a, cudaStream_t s);
+size_t window_grad_workspace(const f3m_seqs &s, int heads, int kv_heads, int width, int window, int sinks);
 
 struct StepArgs {
     int n, heads, kv_heads, width, window, sinks;

@@ -111,8 +111,6 @@ void check_workspace(const void *ws, size_t have, size_t need) {
 }
 void check_state(const float *p, const char *what) { F3M_REQUIRE((uintptr_t)p % 16 == 0, F3M_ERR_ARG, "%s is not 16-byte aligned", what); }
 
-size_t grad_workspace(const f3m_seqs &s, int heads) { return 2 * (size_t)s.tokens * heads * sizeof(float); }
-
 }  // namespace
 
 extern "C" {
@@ -180,8 +178,9 @@ int f3m_window_attention(const f3m_seqs *seqs, int32_t type, int32_t heads, int3
     });
 }
 
-size_t f3m_window_attention_grad_workspace_bytes(const f3m_seqs *seqs, int32_t heads) {
-    return seqs && heads > 0 && seqs->tokens > 0 ? grad_workspace(*seqs, heads) : 0;
+size_t f3m_window_attention_grad_workspace_bytes(const f3m_seqs *seqs, int32_t heads, int32_t kv_heads, int32_t width, int32_t window, int32_t sinks) {
+    if (!seqs || seqs->tokens <= 0 || heads < 1 || kv_heads < 1 || heads % kv_heads || width < 8 || window < 1 || sinks < 0) return 0;
+    return window_grad_workspace(*seqs, heads, kv_heads, width, window, sinks);
 }
 
 int f3m_window_attention_grad(const f3m_seqs *seqs, int32_t type, int32_t heads, int32_t kv_heads, int32_t width, int32_t window, int32_t sinks,
@@ -194,8 +193,8 @@ int f3m_window_attention_grad(const f3m_seqs *seqs, int32_t type, int32_t heads,
         check_rows(out, n, heads, width, "out"); check_rows(dout, n, heads, width, "dout");
         check_out(dq, n, heads, width, "dq"); check_out(dk, n, kv_heads, width, "dk"); check_out(dv, n, kv_heads, width, "dv");
         F3M_REQUIRE(n == 0 || lse, F3M_ERR_ARG, "lse: null pointer");
-        check_workspace(workspace, workspace_bytes, grad_workspace(*seqs, heads));
         if (n == 0) return;
+        check_workspace(workspace, workspace_bytes, window_grad_workspace(*seqs, heads, kv_heads, width, window, sinks));
         seq_check_error();
         WindowArgs a{*seqs, heads, kv_heads, width, window, sinks, scale, q, k, v, out, const_cast<float *>(lse), dout, dq, dk, dv, (float *)workspace};
         window_backward(type, a, (cudaStream_t)stream);

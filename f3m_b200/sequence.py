@@ -224,7 +224,7 @@ def window_attention_grad(plan: SequencePlan, q: torch.Tensor, k: torch.Tensor, 
     (q, rq), (k, rk), (v, rv), (out, ro), (dout, rg) = _read(q), _read(k), _read(v), _read(out), _read(dout)
     (dq, wq), (dk, wk), (dv, wv) = _new(q), _new(k), _new(v)
     L = _lib.lib()
-    need = L.f3m_window_attention_grad_workspace_bytes(plan._ref, heads)
+    need = L.f3m_window_attention_grad_workspace_bytes(plan._ref, heads, k.shape[1], q.shape[2], window, sinks)
     ws = torch.empty(need, device=q.device, dtype=torch.uint8)
     with _On(q.device) as stream:
         st = L.f3m_window_attention_grad(plan._ref, kind, heads, k.shape[1], q.shape[2], window, sinks, scale, rq, rk, rv, ro, lse.data_ptr(), rg,

@@ -334,7 +334,8 @@ int f3m_window_attention(const f3m_seqs *seqs, int32_t type, int32_t heads, int3
                          int32_t sinks, float scale, f3m_rows q, f3m_rows k, f3m_rows v, f3m_rows out, float *lse, void *stream);
 /* Gradients of sum(out * dout) by q, k and v, from out and lse of the call above.  dk and dv are sums over the query heads that share
  * them. */
-size_t f3m_window_attention_grad_workspace_bytes(const f3m_seqs *seqs, int32_t heads);
+size_t f3m_window_attention_grad_workspace_bytes(const f3m_seqs *seqs, int32_t heads, int32_t kv_heads, int32_t width, int32_t window,
+                                                 int32_t sinks);
 int f3m_window_attention_grad(const f3m_seqs *seqs, int32_t type, int32_t heads, int32_t kv_heads, int32_t width, int32_t window,
                               int32_t sinks, float scale, f3m_rows q, f3m_rows k, f3m_rows v, f3m_rows out, const float *lse,
                               f3m_rows dout, f3m_rows dq, f3m_rows dk, f3m_rows dv, void *workspace, size_t workspace_bytes,

@@ -78,7 +78,7 @@ def test_argument_checks_of_the_entries():
     def grad(ws=base, have=1 << 20, dk=ok):
         return L.f3m_window_attention_grad(C.byref(s), 1, 2, 2, 64, 4, 0, 0.1, ok, ok, ok, ok, base, ok, ok, dk, ok, ws, have, None)
 
-    need = L.f3m_window_attention_grad_workspace_bytes(C.byref(s), 2)
+    need = L.f3m_window_attention_grad_workspace_bytes(C.byref(s), 2, 2, 64, 4, 0)
     assert need > 0 and grad(have=need - 1) == 7 and grad(ws=None) == 1 and grad(ws=base + 4) == 1 and grad(dk=Rows(base, 8, 64)) == 1
 
     def step(n=2, cap=100, lens=base, ws=base, have=1 << 40, k=ok, seq=12800):

@@ -28,6 +28,8 @@ WINDOWS = [
     ([260], 5, 5, 8, 50, 300),
     ([1030], 2, 2, 104, 1, 1),
     ([900], 16, 2, 96, 384, 0),
+    ([2300, 130, 900], 16, 2, 64, 200, 8),         # key tiles with sinks are cut into parts
+    ([1700], 12, 3, 128, 128, 150),
 ]
 
 
