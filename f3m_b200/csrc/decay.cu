@@ -390,7 +390,7 @@ __global__ void __launch_bounds__(DK_THREADS, 1) decay_tiles(const __grid_consta
                     tc::tmem_ld16(t_state + lanes + 16 * cb, r);
                     tc::tmem_ld_wait(r);
                 } else {
-                    load_state(r, src, !begins || a.transposed, a.width_b, a.width_c, j, 16 * cb);
+                    load_state(r, src, begins ? a.transposed : !a.joined, a.width_b, a.width_c, j, 16 * cb);
                     __syncwarp();
                 }
 #pragma unroll
@@ -612,7 +612,7 @@ size_t decay_workspace(const f3m_seqs &s, int heads, int width_b, int width_c) {
 template <typename T, int PARTS, int NB>
 static void launch_parts(const DecayKernel &p, cudaStream_t s) {
     constexpr int bytes = DK_TILES * DK_BLOCK + 1024;
-    if (p.ranges > 1) {
+    if (p.ranges > 1 && !p.a.joined) {
         static SharedMemory states;
         states.allow(decay_states<T, PARTS, NB>, bytes);
         decay_states<T, PARTS, NB><<<dim3(p.a.heads, p.ranges - 1), DS_THREADS, bytes, s>>>(p);

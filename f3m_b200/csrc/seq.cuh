@@ -99,6 +99,7 @@ struct DecayArgs {
     const float *log_decay;
     float use, upd;
     bool reversed, transposed;
+    bool joined;   // ws holds the states between ranges already, as the same product with b and c exchanged left them
     f3m_rows a, b, c, out;
     const float *state_in;
     float *state_out;

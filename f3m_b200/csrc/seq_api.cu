@@ -252,7 +252,7 @@ int f3m_decay_attention(const f3m_seqs *seqs, int32_t type, int32_t heads, int32
         check_workspace(workspace, workspace_bytes, decay_workspace(*seqs, heads, width_k, width_v));
         if (seqs->sequences == 0) return;
         seq_check_error();
-        decay_product(type, DecayArgs{*seqs, heads, width_k, width_v, log_decay, scale, 1.f, false, false, q, k, v, out, state_in, state_out, workspace}, (cudaStream_t)stream);
+        decay_product(type, DecayArgs{*seqs, heads, width_k, width_v, log_decay, scale, 1.f, false, false, false, q, k, v, out, state_in, state_out, workspace}, (cudaStream_t)stream);
     });
 }
 
@@ -273,9 +273,10 @@ int f3m_decay_attention_grad(const f3m_seqs *seqs, int32_t type, int32_t heads, 
         // dq_i = scale sum_(j <= i) decay^(i-j) (dout_i.v_j) k_j + scale decay^(i+1) S dout_i: the product itself with (dout, v, k), state
         // transposed.  dk and dv come from the adjoint recurrence D_t = scale q_t dout_t^T + decay D_(t+1), dk_t = D_t v_t, dv_t = D_t^T k_t:
         // the product from the end with (v, dout, q) and (k, q, dout).
-        decay_product(type, DecayArgs{*seqs, heads, width_v, width_k, log_decay, scale, 1.f, false, true, dout, v, k, dq, state_in, nullptr, workspace}, (cudaStream_t)stream);
-        decay_product(type, DecayArgs{*seqs, heads, width_v, width_k, log_decay, 1.f, scale, true, true, v, dout, q, dk, dstate_out, nullptr, workspace}, (cudaStream_t)stream);
-        decay_product(type, DecayArgs{*seqs, heads, width_k, width_v, log_decay, 1.f, scale, true, false, k, q, dout, dv, dstate_out, dstate_in, workspace}, (cudaStream_t)stream);
+        // The two have one state, to a transposition: what lies between the ranges is computed once.
+        decay_product(type, DecayArgs{*seqs, heads, width_k, width_v, log_decay, 1.f, scale, true, false, false, k, q, dout, dv, dstate_out, dstate_in, workspace}, (cudaStream_t)stream);
+        decay_product(type, DecayArgs{*seqs, heads, width_v, width_k, log_decay, 1.f, scale, true, true, true, v, dout, q, dk, dstate_out, nullptr, workspace}, (cudaStream_t)stream);
+        decay_product(type, DecayArgs{*seqs, heads, width_v, width_k, log_decay, scale, 1.f, false, true, false, dout, v, k, dq, state_in, nullptr, workspace}, (cudaStream_t)stream);
     });
 }
 

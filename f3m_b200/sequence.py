@@ -38,7 +38,7 @@ _NO_ROWS = Rows(None, 0, 0)
 
 class SequencePlan:
     """Where the sequences of a packed batch lie (f3m_seqs_layout): made from their lengths, a list of whole numbers or a CPU
-    tensor, and kept for any number of products on any stream of the device."""
+    tensor, and kept for any number of products on any stream of the device (as long as any graph that holds one of them)."""
 
     def __init__(self, lengths: Sequence[int], device="cuda:0"):
         host = np.ascontiguousarray(lengths.cpu().numpy() if torch.is_tensor(lengths) else lengths)
@@ -60,24 +60,29 @@ class SequencePlan:
         check(L.f3m_seqs_layout(host.ctypes.data, host.size, C.byref(self._seqs), None), "f3m_seqs_layout")
         table = np.zeros(max(4, self._seqs.table_words), dtype=np.int32)
         check(L.f3m_seqs_layout(host.ctypes.data, host.size, C.byref(self._seqs), table.ctypes.data), "f3m_seqs_layout")
-        self.table = torch.from_numpy(table).to(self.device)      # pageable memory: the copy has ended when this returns
+        self.table = torch.from_numpy(table).to(self.device)      # a copy that blocks: it has ended when this returns
+        self._home = torch.cuda.current_stream(self.device).cuda_stream
         self._seqs.table = self.table.data_ptr()
         self._ref = C.byref(self._seqs)
         self.tokens, self.sequences, self.longest = int(self._seqs.tokens), int(self._seqs.sequences), int(self._seqs.longest)
 
 
 class _On:
-    """The device of the arrays made current for a call, where it is not already, and its current stream."""
-    __slots__ = ("index", "guard")
+    """The device of the arrays made current for a call, where it is not already, and its current stream.  A plan's table belongs to the stream
+    that it was made on: another one's use of it is noted, so that its memory is not handed on before that has ended."""
+    __slots__ = ("index", "guard", "plan")
 
-    def __init__(self, device):
-        self.index, self.guard = device.index, None
+    def __init__(self, device, plan=None):
+        self.index, self.guard, self.plan = device.index, None, plan
 
     def __enter__(self) -> int:
         if torch.cuda.current_device() != self.index:
             self.guard = torch.cuda.device(self.index)
             self.guard.__enter__()
-        return torch._C._cuda_getCurrentRawStream(self.index)
+        stream = torch._C._cuda_getCurrentRawStream(self.index)
+        if self.plan is not None and stream != self.plan._home and not torch.cuda.is_current_stream_capturing():
+            self.plan.table.record_stream(torch.cuda.current_stream(self.index))
+        return stream
 
     def __exit__(self, *exc):
         if self.guard is not None:
@@ -202,7 +207,7 @@ def _window_forward(plan, q, k, v, window, sinks, scale):
     tokens, heads, width = q.shape
     (q, rq), (k, rk), (v, rv), (out, ro) = _read(q), _read(k), _read(v), _new(q)
     lse = torch.empty((heads, tokens), device=q.device, dtype=torch.float32)
-    with _On(q.device) as stream:
+    with _On(q.device, plan) as stream:
         st = _lib.lib().f3m_window_attention(plan._ref, kind, heads, k.shape[1], width, window, sinks, scale, rq, rk, rv, ro, lse.data_ptr(), stream)
     check(st, "f3m_window_attention")
     return out, lse
@@ -226,7 +231,7 @@ def window_attention_grad(plan: SequencePlan, q: torch.Tensor, k: torch.Tensor, 
     L = _lib.lib()
     need = L.f3m_window_attention_grad_workspace_bytes(plan._ref, heads, k.shape[1], q.shape[2], window, sinks)
     ws = torch.empty(need, device=q.device, dtype=torch.uint8)
-    with _On(q.device) as stream:
+    with _On(q.device, plan) as stream:
         st = L.f3m_window_attention_grad(plan._ref, kind, heads, k.shape[1], q.shape[2], window, sinks, scale, rq, rk, rv, ro, lse.data_ptr(), rg,
                                          wq, wk, wv, ws.data_ptr(), need, stream)
     check(st, "f3m_window_attention_grad")
@@ -339,7 +344,7 @@ def _decay_forward(plan, q, k, v, log_decay, state, scale):
     (q, rq), (k, rk), (v, rv), (out, ro) = _read(q), _read(k), _read(v), _new(v)
     final = torch.empty((plan.sequences, heads, q.shape[2], v.shape[2]), device=q.device, dtype=torch.float32)
     need, ws = _decay_workspace(plan, q, v)
-    with _On(q.device) as stream:
+    with _On(q.device, plan) as stream:
         st = _lib.lib().f3m_decay_attention(plan._ref, kind, heads, q.shape[2], v.shape[2], log_decay.data_ptr(), scale, rq, rk, rv, _pointer(state), ro,
                                             final.data_ptr(), _pointer(ws), need, stream)
     check(st, "f3m_decay_attention")
@@ -363,7 +368,7 @@ def decay_attention_grad(plan: SequencePlan, q: torch.Tensor, k: torch.Tensor, v
     (dq, wq), (dk, wk), (dv, wv) = _new(q), _new(k), _new(v)
     dstate = torch.empty((plan.sequences, heads, q.shape[2], v.shape[2]), device=q.device, dtype=torch.float32)
     need, ws = _decay_workspace(plan, q, v)
-    with _On(q.device) as stream:
+    with _On(q.device, plan) as stream:
         st = _lib.lib().f3m_decay_attention_grad(plan._ref, kind, heads, q.shape[2], v.shape[2], log_decay.data_ptr(), scale, rq, rk, rv, _pointer(state),
                                                  rg, _pointer(dfinal), wq, wk, wv, dstate.data_ptr(), _pointer(ws), need, stream)
     check(st, "f3m_decay_attention_grad")

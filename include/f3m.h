@@ -303,9 +303,13 @@ int f3m_rbf_dense_f32_static(const float *X, int64_t N, const float *Y, int64_t 
  * data start on 16 bytes.  Widths are multiples of 8 up to F3M_MAX_WIDTH.  Inputs have to be finite: what is not finite in a
  * token may reach every row of the 128-token tiles that see the token's tile (never another sequence).
  *
+ * In fp16, what becomes an operand of a product has to stay below 65504: in decay attention the entries of the state (S, and in the gradient
+ * its adjoint) and scale q_i.k_j; the outputs everywhere.
+ *
  * These entry points only enqueue work: they neither wait for the stream nor allocate, so they may be captured into a graph, and calls
  * on several streams or host threads need no order among them.  Temporaries lie in the caller's workspace (f3m_*_workspace_bytes; 16-byte
- * aligned), which a call owns until its work has ended.  A repeated call gives the same bits. */
+ * aligned), which a call owns until its work has ended.  A repeated call gives the same bits.  A kernel's roles wait for one another two seconds at
+ * most; should a wait run out, the next call on sequences of the process returns F3M_ERR_INTERNAL. */
 #define F3M_TYPE_BF16 1
 #define F3M_TYPE_F16 2
 #define F3M_MAX_WIDTH 128
