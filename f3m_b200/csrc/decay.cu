@@ -19,7 +19,7 @@ __device__ __forceinline__ float2 unpack2(f32x2 v) {
 // rows of A S; warps 4-11 split the scaled rows of B into a sum of 16-bit parts, in place, over A, and over the state's operand: the state is kept
 // and returned in FP32, and one rounding of what is added to it would leave it 2^-9 off in bf16.  Two parts lose 2^-17 (bf16) or 2^-23 (fp16); a
 // state that is returned takes a third in bf16, one that only serves the tiles behind it does not.  As an operand of A S the state is rounded to
-// 16 bits, like the weights.
+// 16 bits, like the weights.  The tensor cores' FP32 sums round towards zero: a state comes out about 1e-6 off (relative norm), some 0.7e-6 of it short.
 //
 // What bounds it: tile by tile, the state's way round -- products of the parts, the state read, rounded, scaled, A S, the parts put over what that has
 // read.  The arithmetic of the split, A B^T of the next tile, its weights, the outputs and the copies run beside it.
@@ -27,6 +27,8 @@ __device__ __forceinline__ float2 unpack2(f32x2 v) {
 // A range that does not begin with a sequence needs the state that the ranges before it leave: decay_states computes what each range
 // adds to the state (B and C only), decay_join runs over the ranges, and decay_tiles starts from that.  B and C are then read
 // twice, which is the price of using all SMs when there are fewer heads than SMs.
+// 65536 tokens, 8 heads, 128 x 128: 262 us = 65 (states) + 13 (join) + 185, 2.0 TB/s of what has to move and 3.1 of what does; 0.33 of the copy rate
+// while decay_tiles runs, tensor pipe 27 % busy.
 constexpr int DK_COPY = 12, DK_PRODUCTS = 13, DK_THREADS = 32 * 14;   // warps: 0-3 weights and outputs, 4-11 operands, copies, products
 constexpr int MAX_RANGES = 3 * NUM_SMS_HINT;
 constexpr int DK_AHEAD = 1;                                            // tiles brought into L2 before their stage is free
@@ -652,7 +654,7 @@ static void decay_product_t(const DecayArgs &a, cudaStream_t s) {
 void decay_product(int type, const DecayArgs &a, cudaStream_t s) { type == F3M_TYPE_BF16 ? decay_product_t<__nv_bfloat16>(a, s) : decay_product_t<__half>(a, s); }
 
 // A CTA per (sequence, head): 32 threads across the columns, four each, 8 rows of threads down the state.  The state is read and written
-// once, 16 bytes a thread, and that is all the time there is.
+// once, 16 bytes a thread, and that is all the time there is: 64 sequences, 32 heads, 128 x 128 in 45 us, 6.0 TB/s, 92 % of the measured copy.
 template <typename T>
 __global__ void __launch_bounds__(256) decay_step_kernel(int heads, int wk, int wv, const float *log_decay, float scale, f3m_rows q, f3m_rows k,
                                                          f3m_rows v, float *state, f3m_rows out) {

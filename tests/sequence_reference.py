@@ -3,13 +3,15 @@
 Every function returns, for each output, (value, bound): the bound counts half a step of the type (`u`) for each rounding that the
 kernels make -- of the outputs, of the weights that go into a matrix product, of the carried state as an operand -- times the sum of the
 absolute values of what is rounded, and 1e-5 times that sum for arithmetic in FP32 (sums of a few thousand terms and an exponential
-of 2^-22).  Numbers below FP32's smallest normal one, 2^-126, may be flushed or rounded to a multiple of 2^-149.  In fp16 a weight below 2^-14 is off by up to half of 2^-24 instead (`tiny`).
+of 2^-22).  Numbers below FP32's smallest normal one, 2^-126, may be flushed or rounded to a multiple of 2^-149.  In fp16 a weight below 2^-14 is off by up to half of 2^-24 instead (`tiny`).  A weight
+2^x with x below -125 may be taken as 2^-125 (where the exponential is a polynomial, its exponent stays in the normal range): FLOOR.
 """
 import math
 
 import torch
 
 FP32 = 1e-5
+FLOOR = 2.0 ** -125
 
 
 def half_step(t):
@@ -30,7 +32,7 @@ def seen(n, window, sinks, device):
 
 
 def window(q, k, v, lengths, window, sinks, scale=None, dout=None):
-    u, w0, t = half_step(q.dtype), tiny(q.dtype), q.shape[2] ** -0.5 if scale is None else scale
+    u, w0, t = half_step(q.dtype), tiny(q.dtype) + FLOOR, q.shape[2] ** -0.5 if scale is None else scale
     group = q.shape[1] // k.shape[1]
     names = ["out", "lse"] + (["dq", "dk", "dv"] if dout is not None else [])
     got = {n: ([], []) for n in names}
@@ -38,7 +40,8 @@ def window(q, k, v, lengths, window, sinks, scale=None, dout=None):
         qd = qs.double().transpose(0, 1)
         kd, vd = (x.double().transpose(0, 1).repeat_interleave(group, 0) for x in (ks, vs))
         x = (qd @ kd.mT) * t
-        x = x.masked_fill(~seen(qs.shape[0], window, sinks, q.device), -math.inf)
+        m = seen(qs.shape[0], window, sinks, q.device).double()
+        x = x.masked_fill(m == 0, -math.inf)
         lse = torch.logsumexp(x, -1) if x.shape[-1] else x.new_zeros(x.shape[:2])
         p = torch.exp(x - lse[..., None])
         # an exponent is an FP32 sum of products: a weight is off by that, relative to itself
@@ -46,7 +49,7 @@ def window(q, k, v, lengths, window, sinks, scale=None, dout=None):
         o, mass = p @ vd, p @ vd.abs()
         # a weight's error against the row's largest, of which the row sum is at least one
         got["out"][0].append(o.transpose(0, 1))
-        got["out"][1].append((u * o.abs() + (u + fp32) * mass + w0 * ((p > 0).double() @ vd.abs())).transpose(0, 1))
+        got["out"][1].append((u * o.abs() + (u + fp32) * mass + w0 * (m @ vd.abs())).transpose(0, 1))
         got["lse"][0].append(lse)
         got["lse"][1].append(FP32 * (1 + lse.abs() + (qd.abs() @ kd.abs().mT).amax(-1) * abs(t) if x.shape[-1] else lse))
         if dout is None:
@@ -56,8 +59,8 @@ def window(q, k, v, lengths, window, sinks, scale=None, dout=None):
         ds = p * (dp - delta) * t
         # delta is taken from the rounded out; dp and delta are FP32 sums
         slack = p * abs(t) * (u * (g.abs() * (o.abs() + mass)).sum(-1, keepdim=True) + FP32 * (g.abs() @ vd.abs().mT + (g * o).abs().sum(-1, keepdim=True)))
-        e = (u + fp32) * ds.abs() + slack + w0 * (p > 0).double()
-        ep = (u + fp32) * p + w0 * (p > 0).double()
+        e = (u + fp32) * ds.abs() + slack + w0 * m
+        ep = (u + fp32) * p + w0 * m
         shared = lambda y: y.reshape(k.shape[1], group, *y.shape[1:]).sum(1)  # noqa: E731
         for name, val, err in (("dq", ds @ kd, e @ kd.abs()), ("dk", shared(ds.mT @ qd), shared(e.mT @ qd.abs())),
                                ("dv", shared(p.mT @ g), shared(ep.mT @ g.abs()))):

@@ -360,6 +360,71 @@ def test_captured_calls(cuda):
             assert all(torch.equal(x, y) for x, y in zip(f(), res))
 
 
+def test_the_first_call_of_a_process_is_captured(cuda):
+    """What the library makes once per process (its error word, the driver's entry point) may be made while a stream is captured."""
+    import os
+    import subprocess
+    import sys
+    code = """
+import torch
+from f3m_b200 import sequence as sq
+plan = sq.SequencePlan([300])
+q, k, v = (torch.randn(300, 2, 64, device="cuda").half() for _ in range(3))
+ld = torch.tensor([-0.1, -0.01], device="cuda")
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    a, b = sq.window_attention(plan, q, k, v, 100), sq.decay_attention(plan, q, k, v, ld)
+g.replay()
+c, d = sq.window_attention(plan, q, k, v, 100), sq.decay_attention(plan, q, k, v, ld)
+assert all(torch.equal(x, y) for x, y in zip(a + b, c + d))
+print("captured")
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
+
+
+def test_inference_mode_and_a_dropped_plan(cuda):
+    """Under inference mode; and plans dropped while another stream still reads their tables."""
+    from f3m_b200 import sequence as sq
+    q, k, v = (normal(i, 5000, 2, 64, dtype=torch.bfloat16) for i in range(3))
+    ld = torch.tensor([-0.1, -0.01], device="cuda")
+    want = sq.window_attention(sq.SequencePlan([5000]), q, k, v, 700)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    got = []
+    with torch.inference_mode():
+        for _ in range(20):
+            plan = sq.SequencePlan([5000])
+            with torch.cuda.stream(side):
+                got.append(sq.window_attention(plan, q, k, v, 700))
+            del plan
+            torch.full((200, 4), 7, dtype=torch.int32, device="cuda")      # takes the table's memory, were it free
+        state = torch.zeros(3, 2, 64, 64, device="cuda")
+        sq.decay_attention_step(q[:3], k[:3], v[:3], ld, state)
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for g in got for x, y in zip(g, want))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_a_scale_of_zero_and_large_inputs(dtype, cuda):
+    """All weights equal; and exponents of some thousands, where each row has one weight or two."""
+    from f3m_b200 import sequence as sq
+    n, h, w = 333, 2, 64
+    plan = sq.SequencePlan([n])
+    q, k, v, do = (normal(30 + i, n, h, w, dtype=dtype) for i in range(4))
+    for qq, scale in ((q, 0.0), (q * 40, 1.0)):
+        want = ref.window(qq, k, v, [n], 90, 2, scale=scale, dout=do)
+        out, lse = sq.window_attention(plan, qq, k, v, 90, 2, scale=scale)
+        ref.assert_within(out, want["out"], "out")
+        ref.assert_within(lse, want["lse"], "lse")
+        for name, x in zip(("dq", "dk", "dv"), sq.window_attention_grad(plan, qq, k, v, out, lse, do, 90, 2, scale=scale)):
+            if scale == 0.0 or name == "dv":
+                ref.assert_within(x, want[name], name)
+            else:
+                assert torch.isfinite(x).all()
+
+
 def test_autograd_refuses_capture(cuda):
     """Outside a graph it works before and after; nothing has been enqueued when it is refused."""
     from f3m_b200 import sequence as sq
