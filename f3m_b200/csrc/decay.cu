@@ -595,6 +595,7 @@ __global__ void __launch_bounds__(256) decay_empty(DecayArgs a) {
 
 // How many ranges a head's tiles are cut into.  One CTA of decay_tiles fills an SM.  With one range the SMs without a head idle; with more, B
 // and C are read twice, half as much again, and two more launches take as long as some four tiles: the least time of a CTA's tiles, up to three waves.
+// 129 tokens of 8 heads: 11.5 us in one range, 13.5 in two.  65536 tokens of 8 heads, the same arrays again and again: 2204 us in one range, on 8 SMs, 236 in 37.
 static int decay_ranges(const f3m_seqs &s, int heads) {
     int best = 1;
     float least = 0.f;
