@@ -126,7 +126,7 @@ __device__ __forceinline__ void put_row(uint32_t tile, int j, int c0, const uint
 template <typename T, int PARTS, int NB>
 __global__ void __launch_bounds__(DK_THREADS, 1) decay_tiles(const __grid_constant__ DecayKernel p) {
     extern __shared__ unsigned char raw[];
-    __shared__ __align__(8) uint64_t bars[2 * 4 + 10];
+    __shared__ __align__(8) uint64_t bars[2 * 4 + 11];
     __shared__ uint32_t tmem_s;
     __shared__ int gave_up_s;
     const DecayArgs &a = p.a;
@@ -146,7 +146,8 @@ __global__ void __launch_bounds__(DK_THREADS, 1) decay_tiles(const __grid_consta
         }
         for (int i = 8; i < 12; i++) tc::mbar_init(tc::smem_u32(&bars[i]), 1);         // A B^T, A S, state, outputs done
         for (int i = 12; i < 15; i++) tc::mbar_init(tc::smem_u32(&bars[i]), 128);      // weights written, A S scaled, outputs read
-        tc::mbar_init(tc::smem_u32(&bars[17]), 1);                                     // A B^T of every other tile
+        tc::mbar_init(tc::smem_u32(&bars[17]), 1);                                     // A B^T of odd tiles
+        tc::mbar_init(tc::smem_u32(&bars[18]), 128);                                   // weights of odd tiles written
         for (int i = 15; i < 17; i++) tc::mbar_init(tc::smem_u32(&bars[i]), 256);      // B split; state ready as operand and in tensor memory
         tc::fence_mbar_init();
         gave_up_s = 0;
@@ -163,8 +164,11 @@ __global__ void __launch_bounds__(DK_THREADS, 1) decay_tiles(const __grid_consta
     auto a_tile = [&](int s) { return smem + s * stage_blocks * DK_BLOCK; };
     auto b_tile = [&](int s) { return a_tile(s) + NB * DK_BLOCK; };
     auto c_tile = [&](int s) { return a_tile(s) + 2 * NB * DK_BLOCK; };
-    // scores are two tiles ahead of the weights at times: a barrier for even tiles and one for odd
+    // Scores are two tiles ahead of the weights at times, and the weights of a tile may be there before the products have asked for those of the tile
+    // before: a barrier for even tiles and one for odd, each.  A wait names a phase's parity, so no barrier may complete a phase beyond the one that a role
+    // may still be waiting for; every other barrier's next phase needs a step of each role that waits for this one.
     auto b_score_of = [&](int n) { return n & 1 ? tc::smem_u32(&bars[17]) : b_score; };
+    auto b_weights_of = [&](int n) { return n & 1 ? tc::smem_u32(&bars[18]) : b_weights; };
     auto all_wait = [&](uint32_t bar, uint32_t parity) {   // a whole warp, which stays together for the instructions that need that
         wait(bar, parity);
         __syncwarp();
@@ -234,7 +238,7 @@ __global__ void __launch_bounds__(DK_THREADS, 1) decay_tiles(const __grid_consta
                 for (int part = 0; part < PARTS; part++) tc::product_cols(t_state, part == 0 ? b_tile(s) : part == 1 ? a_tile(s) : state_s, c_tile(s), i_state, 1);
                 tc::mma_commit(b_moved);
             }
-            wait(b_weights, n & 1);
+            wait(b_weights_of(n), (n >> 1) & 1);
             wait(b_scaled, n & 1);
             tc::fence_after_sync();
             if (tc::elect()) {
@@ -298,7 +302,7 @@ __global__ void __launch_bounds__(DK_THREADS, 1) decay_tiles(const __grid_consta
             }
             tc::tmem_st_wait();
             tc::fence_before_sync();
-            tc::mbar_arrive(b_weights);
+            tc::mbar_arrive(b_weights_of(n));
         };
         int4 e = tile_at(a, first);
         weights(0, tile_rows(e));
