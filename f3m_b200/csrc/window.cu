@@ -380,11 +380,40 @@ struct GradKernel {
     WindowArgs a;
     CUtensorMap mq, mk, mv, mg, m0, m1;   // q, k, v, dout; the outputs: dk and dv, or dq
     float c;                              // scale log2(e)
-    int parts;                            // CTAs for a tile of keys that holds sinks
-    float *part;                          // their sums: (sequences, tiles with sinks, kv_heads, parts, dk and dv, 128, width)
+    int unit, sink_tiles, slots;          // of the cuts of walks over sinks, below
+    float *part;                          // the parts' sums: (slots, tiles with sinks, kv_heads, dk and dv, 128, width)
     const float *lse2, *delta;
     int *err;
 };
+
+// A tile of keys that holds sinks is seen by the rest of its sequence.  Where its walk is longer than `unit` tiles of queries it is cut into parts of at most
+// that many: a CTA each, whose sums window_grad_sinks adds in order.  A sequence's parts lie from slot 2 group (tiles before it) / unit on: of a walk of x
+// units, x > 1, there are ceil(x) <= floor(2 x) parts, so that neighbours do not meet and 2 group tiles / unit slots hold all.
+struct CutWalk {
+    int4 e;                     // {first row, length, first key, sequence}
+    int all, part, parts;       // tiles of queries; this one of so many parts
+    __device__ __forceinline__ int per() const { return (all + parts - 1) / parts; }
+};
+__device__ __forceinline__ int walk_parts(int all, int unit) { return (all - 1) / unit + 1; }
+// false: the slot holds no part of tile k of keys
+__device__ __forceinline__ bool cut_walk(const GradKernel &p, int slot, int k, CutWalk &w) {
+    const WindowArgs &a = p.a;
+    const int4 *seq = reinterpret_cast<const int4 *>(a.s.table) + seq_of(a.s, 0);
+    const int group = a.heads / a.kv_heads;
+    auto base = [&](int i) { return 2 * (int64_t)group * seq[i].z / p.unit; };
+    int lo = 0, hi = a.s.sequences;   // the last sequence whose slots begin at this one or before
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        (base(mid) <= slot ? lo : hi) = mid;
+    }
+    const int4 q = seq[lo];
+    w.e = make_int4(q.x, q.y, k * SEQ_TILE, lo);
+    w.all = (q.w - k) * group;
+    if (k >= q.w) return false;
+    w.parts = walk_parts(w.all, p.unit);
+    w.part = (int)(slot - base(lo));
+    return w.parts > 1 && w.part < w.parts;
+}
 
 // A CTA has a tile of 128 keys (rows of tensor memory) and walks over tiles of 128 queries (columns).  Of the products of query tile n,
 //     S^T = K Q^T (n + 1)  follows  dV += P^T dout (n),     dP^T = V dout^T (n + 1)  follows  dK += dS^T Q (n),
@@ -402,14 +431,22 @@ __global__ void __launch_bounds__(WG_THREADS, 1) window_grad_keys(const __grid_c
     const uint32_t smem = (tc::smem_u32(raw) + 1023) & ~1023u, k_tile = smem, v_tile = smem + NB * WF_BLOCK;
     auto q_tile = [&](int s) { return smem + (2 + 2 * s) * NB * WF_BLOCK; };
     auto g_tile = [&](int s) { return smem + (3 + 2 * s) * NB * WF_BLOCK; };
-    const int part = blockIdx.x % p.parts, item = blockIdx.x / p.parts;
-    const int4 e = reinterpret_cast<const int4 *>(a.s.table)[seq_by_future(a.s, item / a.kv_heads)];
-    const int hk = item % a.kv_heads, key = e.z;
+    // the parts of walks that are cut come first, then the tiles whose walk is whole
+    const int cut = p.slots * p.sink_tiles * a.kv_heads, hk = ((int)blockIdx.x < cut ? (int)blockIdx.x : (int)blockIdx.x - cut) % a.kv_heads;
+    const bool is_part = (int)blockIdx.x < cut;
+    CutWalk w;
+    if (is_part) {
+        if (!cut_walk(p, blockIdx.x / (p.sink_tiles * a.kv_heads), blockIdx.x / a.kv_heads % p.sink_tiles, w)) return;
+    } else {
+        w.e = reinterpret_cast<const int4 *>(a.s.table)[seq_by_future(a.s, (blockIdx.x - cut) / a.kv_heads)];
+    }
+    const int4 e = w.e;
+    const int key = e.z;
     // queries from the key's own tile on, to the end of the window, or of the sequence where the tile holds sinks
     const int q0 = key / SEQ_TILE, q1 = (key < a.sinks ? e.y - 1 : (int)min((int64_t)e.y - 1, (int64_t)key + SEQ_TILE - 2 + a.window)) / SEQ_TILE;
-    // all the queries of the sequence see a sink: such a tile's walk is cut into parts, which are summed by window_grad_sinks
-    const int per_head = q1 - q0 + 1, all = per_head * group, per = key < a.sinks ? (all + p.parts - 1) / p.parts : all;
-    const int n0 = part * per, tiles = min(all, n0 + per) - n0;
+    const int per_head = q1 - q0 + 1, all = per_head * group;
+    if (!is_part && cut && key < a.sinks && walk_parts(all, p.unit) > 1) return;
+    const int n0 = is_part ? w.part * w.per() : 0, tiles = is_part ? min(all, n0 + w.per()) - n0 : all;
     if (tiles <= 0) return;
 
     if (warp == WG_COPY) tc::tmem_alloc(tc::smem_u32(&tmem_s), 512);
@@ -582,9 +619,8 @@ __global__ void __launch_bounds__(WG_THREADS, 1) window_grad_keys(const __grid_c
         wait(b_done, 0);
         __syncwarp();
         tc::fence_after_sync();
-        if (per < all) {
-            const int ns = (a.sinks + SEQ_TILE - 1) / SEQ_TILE;
-            float *row = p.part + (((((int64_t)e.w * ns + key / SEQ_TILE) * a.kv_heads + hk) * p.parts + part) * 2 + half) * SEQ_TILE * a.width + r * a.width;
+        if (is_part) {
+            float *row = p.part + ((int64_t)blockIdx.x * 2 + half) * SEQ_TILE * a.width + r * a.width;
             for (int q = 0; q < 2 * NB; q++) {
                 uint32_t o[32];
                 tc::tmem_ld32((half ? t_dv : t_dk) + lanes + 32 * q, o);
@@ -619,26 +655,26 @@ __global__ void __launch_bounds__(WG_THREADS, 1) window_grad_keys(const __grid_c
     if (warp == WG_COPY) tc::tmem_dealloc(tmem, 512);
 }
 
-// dk and dv of the tiles that hold sinks: their parts' sums, in order.
+// dk and dv of the tiles of keys whose walk was cut: the parts' sums, in order.  The CTAs of a tile's first part add them.
 template <typename T>
 __global__ void __launch_bounds__(256) window_grad_sinks(const __grid_constant__ GradKernel p) {
     const WindowArgs &a = p.a;
-    const int ns = (a.sinks + SEQ_TILE - 1) / SEQ_TILE, key = blockIdx.x % ns * SEQ_TILE, hk = blockIdx.y;
-    const int4 e = reinterpret_cast<const int4 *>(a.s.table)[seq_of(a.s, blockIdx.x / ns)];
-    if (key >= e.y) return;
-    const int all = ((e.y - 1) / SEQ_TILE - key / SEQ_TILE + 1) * (a.heads / a.kv_heads), per = (all + p.parts - 1) / p.parts, used = (all + per - 1) / per;
-    if (per == all) return;   // written by the one part itself
-    const int rows = min(SEQ_TILE, e.y - key), half_size = SEQ_TILE * a.width;
-    const float *sums = p.part + ((int64_t)blockIdx.x * a.kv_heads + hk) * p.parts * 2 * half_size;
+    const int k = blockIdx.x % p.sink_tiles, slot = blockIdx.x / p.sink_tiles, hk = blockIdx.y;
+    CutWalk w;
+    if (!cut_walk(p, slot, k, w) || w.part) return;
+    const int4 e = w.e;
+    const int used = (w.all + w.per() - 1) / w.per(), rows = min(SEQ_TILE, e.y - e.z), half_size = SEQ_TILE * a.width;
+    const int64_t stride = (int64_t)p.sink_tiles * a.kv_heads * 2 * half_size;   // from part to part
+    const float *sums = p.part + ((int64_t)blockIdx.x * a.kv_heads + hk) * 2 * half_size;
     for (int x = blockIdx.z * 256 + threadIdx.x; x < rows * a.width; x += 16 * 256) {   // pairs of entries: dk, then dv
         const int half = 2 * x >= rows * a.width, at = 2 * x - half * rows * a.width, r = at / a.width, c = at % a.width;
         float2 y = make_float2(0.f, 0.f);
         for (int i = 0; i < used; i++) {
-            const float2 v = *reinterpret_cast<const float2 *>(sums + (2 * i + half) * (int64_t)half_size + at);
+            const float2 v = *reinterpret_cast<const float2 *>(sums + i * stride + half * half_size + at);
             y.x += v.x;
             y.y += v.y;
         }
-        *reinterpret_cast<uint32_t *>(row_of<T>(half ? a.dv : a.dk, e.x + key + r, hk) + c) = Half<T>::pack(y.x, y.y);
+        *reinterpret_cast<uint32_t *>(row_of<T>(half ? a.dv : a.dk, e.x + e.z + r, hk) + c) = Half<T>::pack(y.x, y.y);
     }
 }
 
@@ -819,17 +855,27 @@ __global__ void __launch_bounds__(WG_THREADS, 1) window_grad_queries(const __gri
     if (warp == WG_COPY) tc::tmem_dealloc(tmem, 512);
 }
 
-// Tiles of keys that hold sinks are seen by the whole sequence.  They are cut into parts no longer than the walk of another tile (24 tiles of queries at
-// least): 5 packed documents of up to 3000 tokens, window 512, spent 272 us on the one walk of 96 tiles, and 68 us' worth of work.
-static int grad_parts(const f3m_seqs &s, int group, int window, int sinks) {
-    if (sinks == 0) return 1;
-    const int64_t longest = ((int64_t)s.longest + SEQ_TILE - 1) / SEQ_TILE, other = std::min(longest, ((int64_t)window + SEQ_TILE - 1) / SEQ_TILE + 1);
-    return (int)std::min<int64_t>(16, (longest * group + std::max<int64_t>(24, other * group) - 1) / std::max<int64_t>(24, other * group));
+// Where walks over sinks are cut (CutWalk).  A part is no shorter than the walk of another tile, than 24 tiles of queries, than a sixteenth of the
+// longest walk, and than an SM's share of all walks over sinks, halved: where these fill the SMs by themselves they are not cut, and the parts' sums never take
+// more than 4 x 148 slots, 78 MB at width 128.  5 packed documents of up to 3000 tokens, window 512, spent 272 us on one walk of 96 tiles, and 68 us' worth of work.
+// One of 16384 tokens and 2000 of 64, 32 heads on 8, width 128, window 128, 4 sinks, gradients: 5360 us, 5150 without sinks; with the longest walk's number of
+// parts for every sequence 11000 us and 33.6 GB.
+struct GradCuts {
+    int unit, sink_tiles;
+    int64_t slots;
+};
+static GradCuts grad_cuts(const f3m_seqs &s, int heads, int kv_heads, int window, int sinks) {
+    const int64_t group = heads / kv_heads, longest = ((int64_t)s.longest + SEQ_TILE - 1) / SEQ_TILE, other = std::min(longest, ((int64_t)window + SEQ_TILE - 1) / SEQ_TILE + 1);
+    const int64_t ns = ((int64_t)std::min(sinks, s.longest) + SEQ_TILE - 1) / SEQ_TILE, sms = 2 * NUM_SMS_HINT;
+    const int64_t share = (s.tiles * group * kv_heads + sms - 1) / sms * ns;
+    const int64_t unit = std::max({(int64_t)24, other * group, (longest * group + 15) / 16, share});
+    if (ns == 0 || longest * group <= unit) return {0x7fffffff, (int)ns, 0};
+    return {(int)unit, (int)ns, 2 * group * s.tiles / unit};
 }
+static size_t part_floats(const GradCuts &c, int kv_heads, int width) { return (size_t)c.slots * c.sink_tiles * kv_heads * 2 * SEQ_TILE * width; }
 size_t window_grad_workspace(const f3m_seqs &s, int heads, int kv_heads, int width, int window, int sinks) {
-    const int parts = grad_parts(s, heads / kv_heads, window, sinks);
-    const size_t rows = ((size_t)s.tokens * heads + 3) / 4 * 4, tiles = ((size_t)std::min(sinks, s.longest) + SEQ_TILE - 1) / SEQ_TILE;
-    return (2 * rows + (parts > 1 ? (size_t)s.sequences * tiles * kv_heads * parts * 2 * SEQ_TILE * width : 0)) * sizeof(float);
+    const size_t rows = ((size_t)s.tokens * heads + 3) / 4 * 4;
+    return (2 * rows + part_floats(grad_cuts(s, heads, kv_heads, window, sinks), kv_heads, width)) * sizeof(float);
 }
 
 template <typename T>
@@ -845,10 +891,13 @@ static void backward_t(const WindowArgs &a, cudaStream_t s) {
     float *lse2 = a.delta + (rows + 3) / 4 * 4;
     p.lse2 = lse2;
     p.delta = a.delta;
-    p.parts = grad_parts(a.s, a.heads / a.kv_heads, a.window, a.sinks);
+    const GradCuts cuts = grad_cuts(a.s, a.heads, a.kv_heads, a.window, a.sinks);
+    p.unit = cuts.unit;
+    p.sink_tiles = cuts.sink_tiles;
+    p.slots = (int)cuts.slots;
     p.part = lse2 + (rows + 3) / 4 * 4;
-    F3M_REQUIRE((int64_t)a.s.tiles * a.kv_heads * p.parts <= 0x7fffffff && (int64_t)a.s.sequences * ((p.a.sinks + SEQ_TILE - 1) / SEQ_TILE) <= 0x7fffffff && a.kv_heads <= 65535,
-                F3M_ERR_OVERFLOW, "%d tiles of %d heads do not fit in 31 bits", a.s.tiles, a.heads);
+    const int64_t parts = cuts.slots * cuts.sink_tiles * a.kv_heads;
+    F3M_REQUIRE(a.s.tiles * (int64_t)a.kv_heads + parts <= 0x7fffffff, F3M_ERR_OVERFLOW, "%d tiles of %d heads do not fit in 31 bits", a.s.tiles, a.heads);
     window_rows_sum<T><<<(unsigned)((rows + 15) / 16), 256, 0, s>>>(a, lse2, a.delta);
     F3M_LAUNCH_CHECK();
     p.mq = seq_tensor_map(type, a.q, n, a.heads, a.width);
@@ -863,10 +912,10 @@ static void backward_t(const WindowArgs &a, cudaStream_t s) {
     auto keys = a.width <= 64 ? window_grad_keys<T, 1> : window_grad_keys<T, 2>;
     static SharedMemory allowed[2][2];
     allowed[0][a.width > 64].allow(keys, key_bytes);
-    keys<<<a.s.tiles * a.kv_heads * p.parts, WG_THREADS, key_bytes, s>>>(p);
+    keys<<<(unsigned)(parts + a.s.tiles * (int64_t)a.kv_heads), WG_THREADS, key_bytes, s>>>(p);
     F3M_LAUNCH_CHECK();
-    if (p.parts > 1) {
-        window_grad_sinks<T><<<dim3(a.s.sequences * ((p.a.sinks + SEQ_TILE - 1) / SEQ_TILE), a.kv_heads, 16), 256, 0, s>>>(p);
+    if (parts) {
+        window_grad_sinks<T><<<dim3(p.slots * p.sink_tiles, a.kv_heads, 16), 256, 0, s>>>(p);
         F3M_LAUNCH_CHECK();
     }
     p.m0 = seq_tensor_map(type, a.dq, n, a.heads, a.width);

@@ -101,3 +101,22 @@ def test_cpu_tensors_are_refused():
         sequence.window_attention_step(x, x[:, None], x[:, None], torch.ones(4, dtype=torch.int32), 4)
     with pytest.raises(ValueError):
         sequence.decay_attention_step(x, x, x, torch.zeros(2), torch.zeros(4, 2, 64, 64))
+
+
+def test_gradient_workspace_of_uneven_batches():
+    """Sums of parts of walks over the keys that hold sinks take room where a walk is cut, not for every sequence beside the longest."""
+    L = _lib.lib()
+
+    def need(lengths, heads, kv, width, window, sinks):
+        s, _ = layout(lengths)
+        rows = 2 * 4 * sum(lengths) * heads
+        return L.f3m_window_attention_grad_workspace_bytes(C.byref(s), heads, kv, width, window, sinks) - rows
+
+    # 2 x 148 CTAs' worth of parts and as many again where lengths fall badly, dk and dv of 128 keys each, in FP32
+    most = 4 * 148 * 2 * 128 * 128 * 4 + (1 << 20)
+    assert need([16384] + [64] * 2000, 32, 8, 128, 128, 4) < most
+    assert need([32768] + [64] * 1000, 32, 8, 128, 1024, 16) < most
+    assert need([32768] + [128] * 500, 32, 4, 128, 256, 4) < most
+    assert need([65536], 32, 8, 128, 512, 65536) < most
+    assert need([64] * 5000, 32, 8, 128, 128, 4) < 1 << 20            # no walk is cut
+    assert need([16384] + [64] * 2000, 32, 8, 128, 128, 0) < 1 << 20

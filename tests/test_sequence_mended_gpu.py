@@ -36,3 +36,55 @@ def test_many_calls_of_attention_with_a_decay(width_k, width_v, cuda):
     want = ref.decay(q[:, :1], k[:, :1], v[:, :1], ld[:1].tolist(), lengths, state[:, :1], dout=do[:, :1], dfinal=dfinal[:, :1])
     for name, x in zip(("out", "final", "dq", "dk", "dv", "dstate"), first):
         ref.assert_within(x[:, :1], want[name], name)
+
+
+# lengths, heads, kv_heads, width, window, sinks: walks over sinks that are cut, of few sequences among many, at the front, the end and between
+UNEVEN = [
+    ([3000] + [64] * 60, 8, 2, 64, 128, 8),
+    ([64] * 30 + [3300, 0, 1, 1700] + [130] * 20, 8, 2, 128, 100, 200),
+    ([5, 0, 4100], 12, 1, 32, 129, 300),
+    ([2900, 2900, 64, 3100], 16, 2, 80, 300, 1),
+]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lengths,heads,kv_heads,width,window,sinks", UNEVEN)
+def test_window_gradients_of_uneven_batches(lengths, heads, kv_heads, width, window, sinks, dtype, cuda):
+    from f3m_b200 import sequence as sq
+    n = sum(lengths)
+    q, do = normal(1, n, heads, width, dtype=dtype), normal(2, n, heads, width, dtype=dtype)
+    k, v = normal(3, n, kv_heads, width, dtype=dtype), normal(4, n, kv_heads, width, dtype=dtype)
+    plan = sq.SequencePlan(lengths)
+    want = ref.window(q, k, v, lengths, window, sinks, dout=do)
+    out, lse = sq.window_attention(plan, q, k, v, window, sinks)
+    first = sq.window_attention_grad(plan, q, k, v, out, lse, do, window, sinks)
+    for name, x in zip(("dq", "dk", "dv"), first):
+        ref.assert_within(x, want[name], name)
+    again = sq.window_attention_grad(plan, q, k, v, out, lse, do, window, sinks)
+    assert all(torch.equal(x, y) for x, y in zip(first, again))
+
+
+def test_window_gradients_of_thousands_of_short_sequences(cuda):
+    """One document beside 2000 short ones: a workspace no larger than the arrays, and the gradients that each has by itself."""
+    from f3m_b200 import sequence as sq
+    lengths, h, hk, w, window, sinks = [16384] + [64] * 2000, 32, 8, 128, 128, 4
+    n = sum(lengths)
+    q, do = normal(1, n, h, w, dtype=torch.bfloat16), normal(2, n, h, w, dtype=torch.bfloat16)
+    k, v = normal(3, n, hk, w, dtype=torch.bfloat16), normal(4, n, hk, w, dtype=torch.bfloat16)
+
+    def both(plan, at):
+        x = [y[at] for y in (q, k, v, do)]
+        out, lse = sq.window_attention(plan, *x[:3], window, sinks)
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        held = torch.cuda.memory_allocated()
+        got = sq.window_attention_grad(plan, *x[:3], out, lse, x[3], window, sinks)
+        torch.cuda.synchronize()
+        return got, torch.cuda.max_memory_allocated() - held - sum(y.numel() * 2 for y in got)
+
+    got, room = both(sq.SequencePlan(lengths), slice(0, n))
+    assert room < q.numel() * 2
+    for at, few in ((slice(0, 16384), [16384]), (slice(16384, 16384 + 6400), [64] * 100), (slice(n - 64, n), [64])):
+        want, _ = both(sq.SequencePlan(few), at)
+        for x, y in zip(got, want):     # parts may be cut otherwise: sums in FP32, rounded once
+            assert torch.allclose(x[at].float(), y.float(), rtol=2 ** -7, atol=1e-4)
