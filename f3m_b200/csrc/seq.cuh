@@ -70,7 +70,7 @@ struct WindowArgs {
     f3m_rows q, k, v, out;
     float *lse;
     f3m_rows dout, dq, dk, dv;   // gradients only
-    float *delta;                // workspace: 2 x (heads, tokens), and the parts' sums
+    float *delta;                // workspace: 2 x (heads, tokens), (sequences, kv_heads, 2), and the parts' sums
 };
 void window_forward(int type, const WindowArgs &a, cudaStream_t s);
 void window_backward(int type, const WindowArgs &a, cudaStream_t s);

@@ -343,34 +343,88 @@ static void forward_t(const WindowArgs &a, cudaStream_t s) {
     F3M_LAUNCH_CHECK();
 }
 // ---- gradients ------------------------------------------------------------------------------------------------------------
-// P = 2^(c s - lse), dS = P (scale dP - scale delta) with dP = dout V^T: dV = P^T dout, dK = dS^T Q, dQ = dS K.  dK and dV are sums over queries, dQ
+// P = 2^(c s - lse), dS = P (dP - delta) with dP = dout V^T: dV = P^T dout, dK = scale dS^T Q, dQ = scale dS K.  dK and dV are sums over queries, dQ
 // over keys: two kernels, one that holds a tile of keys and walks over the queries that see it, of all heads that share it, and one that
 // holds a tile of queries.  S and dP are computed in both, seven products where five would do, but nothing is added across CTAs: sums have one order.
 // P and dS are rounded to 16 bits where they become operands, and go through tensor memory over the scores they come from.
 // What bounds it: a tile pair's weights and dS, some 3300 clocks for 256 threads; its products take 2048 (four) and 1536 (three).  2 x 4096 tokens, 8 heads,
 // width 128, window 2048, forward and gradients: 310 us, 0.57 PFLOP/s by the formula's products, 0.74 by those computed; tensor pipe 53 % busy.
 
-// lse2 = lse log2(e) and delta = scale dout.out, rows (heads, tokens)
+// fp16 ends at 2^-24, and dS is far smaller than dout: it would lose its bits where dout still has them (dout of 1e-4: dq and dk were 3 % off).  There P is
+// taken times 2^15 and dS times 2^k, k from the largest |dout_i| and |v_j| of the sequence and the heads that share v: |dP - delta| <= 2 |dout_i| max |v_j|, as out_i
+// is a mean of v_j, and dS stays below 2^15.  The powers of two leave in FP32, where gradients are stored.  bf16 has FP32's range and takes neither.
+template <typename T> constexpr int WG_P_EXP = Half<T>::type == F3M_TYPE_F16 ? 15 : 0;
+struct GradRange {
+    float ds;           // what dP and delta are multiplied by beside P 2^15
+    float out_s, out_v; // what dQ, dK and dV are multiplied by at the end
+};
+// range: squares of the largest finite |dout_i| and |v_j|
 template <typename T>
-__global__ void __launch_bounds__(256) window_rows_sum(WindowArgs a, float *lse2, float *delta) {
-    const int64_t row = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 4, t = row / a.heads;
-    const int h = (int)(row % a.heads), c = 8 * (threadIdx.x & 15);
-    float s = 0.f;
-    if (t < a.s.tokens && c < a.width) {
-        const uint4 x = *reinterpret_cast<const uint4 *>(row_of<T>(a.out, t, h) + c), y = *reinterpret_cast<const uint4 *>(row_of<T>(a.dout, t, h) + c);
+__device__ __forceinline__ GradRange grad_range(const float *range, int kv_heads, int seq, int hk, float scale) {
+    if constexpr (WG_P_EXP<T> == 0) return {1.f, scale, 1.f};
+    const float2 r = reinterpret_cast<const float2 *>(range)[(int64_t)seq * kv_heads + hk];
+    const float most = 2.f * sqrtf(r.x) * sqrtf(r.y);
+    const int k = most > 0.f ? 14 - ((int)(__float_as_uint(most) >> 23) - 127) : 0;   // 2^(14 - k) <= most < 2^(15 - k); -26 <= k <= 62
+    auto power = [](int e) { return __uint_as_float((uint32_t)(e + 127) << 23); };
+    return {power(k - WG_P_EXP<T>), scale * power(-k), power(-WG_P_EXP<T>)};
+}
+// lse2 = lse log2(e), less the power of two of P, and delta = dout.out, rows (heads, tokens); in fp16 the range too.  A CTA has 64 of the
+// rows of a tile of tokens and the query heads that share a key head, 16 threads a row.
+template <typename T>
+__global__ void __launch_bounds__(256) window_rows_sum(const __grid_constant__ WindowArgs a, float *lse2, float *delta, uint32_t *range) {
+    const int group = a.heads / a.kv_heads, hk = blockIdx.x % a.kv_heads, c = 8 * (threadIdx.x & 15);
+    const int4 e = reinterpret_cast<const int4 *>(a.s.table)[seq_by_place(a.s, blockIdx.x / a.kv_heads)];
+    const int64_t t0 = (int64_t)e.x + e.z;
+    const int m = min(SEQ_TILE, e.y - e.z), rows = m * group;
+    auto read = [&](const f3m_rows &r, int64_t t, int h, bool in) { return in ? *reinterpret_cast<const uint4 *>(row_of<T>(r, t, h) + c) : make_uint4(0u, 0u, 0u, 0u); };
+    auto dot = [](const uint4 &x, const uint4 &y) {
         const uint32_t u[4] = {x.x, x.y, x.z, x.w}, v[4] = {y.x, y.y, y.z, y.w};
+        float s = 0.f;
 #pragma unroll
         for (int q = 0; q < 4; q++) {
             const float2 f = Half<T>::unpack(u[q]), g = Half<T>::unpack(v[q]);
             s = fmaf(f.x, g.x, fmaf(f.y, g.y, s));
         }
-    }
+        return s;
+    };
+    auto sum16 = [](float s) {
 #pragma unroll
-    for (int o = 8; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if (t < a.s.tokens && c == 0) {
-        const int64_t at = h * a.s.tokens + t;
-        delta[at] = a.scale * s;
-        lse2[at] = 1.4426950408889634f * a.lse[at];
+        for (int o = 8; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        return s;
+    };
+    uint32_t most[2] = {0u, 0u};
+    auto larger = [](uint32_t &top, float s) {   // of finite numbers, none negative: their bits are in order
+        const uint32_t b = __float_as_uint(s);
+        if (b < 0x7f800000u) top = max(top, b);
+    };
+#pragma unroll 1
+    for (int x0 = 64 * blockIdx.y; x0 < rows; x0 += 64 * gridDim.y) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int x = x0 + 16 * i + (threadIdx.x >> 4), h = hk * group + x % group;
+            const int64_t t = t0 + x / group;
+            const bool in = x < rows && c < a.width;
+            const uint4 o = read(a.out, t, h, in), g = read(a.dout, t, h, in);
+            const float s = sum16(dot(o, g));
+            if constexpr (WG_P_EXP<T> != 0) larger(most[0], sum16(dot(g, g)));
+            if (in && c == 0) {
+                const int64_t at = h * a.s.tokens + t;
+                delta[at] = s;
+                lse2[at] = 1.4426950408889634f * a.lse[at] - WG_P_EXP<T>;
+            }
+        }
+    }
+    if constexpr (WG_P_EXP<T> != 0) {
+        for (int i = 0; i < 4 && blockIdx.y < 2; i++) {
+            const int x = 64 * blockIdx.y + 16 * i + (threadIdx.x >> 4);
+            const uint4 v = read(a.v, t0 + x, hk, x < m && c < a.width);
+            larger(most[1], sum16(dot(v, v)));
+        }
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            most[i] = __reduce_max_sync(0xffffffffu, most[i]);
+            if ((threadIdx.x & 31) == 0 && most[i]) atomicMax(range + 2 * ((int64_t)e.w * a.kv_heads + hk) + i, most[i]);
+        }
     }
 }
 
@@ -382,7 +436,7 @@ struct GradKernel {
     float c;                              // scale log2(e)
     int unit, sink_tiles, slots;          // of the cuts of walks over sinks, below
     float *part;                          // the parts' sums: (slots, tiles with sinks, kv_heads, dk and dv, 128, width)
-    const float *lse2, *delta;
+    const float *lse2, *delta, *range;
     int *err;
 };
 
@@ -528,10 +582,11 @@ __global__ void __launch_bounds__(WG_THREADS, 1) window_grad_keys(const __grid_c
         // threads r and r + 128 have key row r, half of the queries each
         const int r = tid & 127, half = tid >> 7, j = key + r;
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
-        const f32x2 cc = pack2(p.c, p.c), scale = pack2(a.scale, a.scale);
-        auto row_sum = [&](int n) {   // lse2 (threads of the first half) or delta of a query of tile n
+        const float times = grad_range<T>(p.range, a.kv_heads, e.w, hk, a.scale).ds;
+        const f32x2 cc = pack2(p.c, p.c), ds = pack2(times, times);
+        auto row_sum = [&](int n) {   // -lse2 (threads of the first half) or -delta of a query of tile n
             const int h = hk * group + (n0 + n) / per_head, i = (q0 + (n0 + n) % per_head) * SEQ_TILE + r;
-            return i < e.y ? -(half ? p.delta : p.lse2)[h * a.s.tokens + e.x + i] : 0.f;
+            return i < e.y ? (half ? -times : -1.f) * (half ? p.delta : p.lse2)[h * a.s.tokens + e.x + i] : 0.f;
         };
         float next = row_sum(0);
         for (int n = 0; n < tiles; n++) {
@@ -599,8 +654,8 @@ __global__ void __launch_bounds__(WG_THREADS, 1) window_grad_keys(const __grid_c
                 for (int c = 0; c < 32; c += 4) {
                     const ulonglong2 d = *reinterpret_cast<const ulonglong2 *>(&delta_s[n & 1][64 * half + 32 * b + c]);
                     float y[4];
-                    unpack2(mul2(pack2(pr[b][c], pr[b][c + 1]), fma2(pack2(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), scale, d.x)), y[0], y[1]);
-                    unpack2(mul2(pack2(pr[b][c + 2], pr[b][c + 3]), fma2(pack2(__uint_as_float(x[c + 2]), __uint_as_float(x[c + 3])), scale, d.y)), y[2], y[3]);
+                    unpack2(mul2(pack2(pr[b][c], pr[b][c + 1]), fma2(pack2(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), ds, d.x)), y[0], y[1]);
+                    unpack2(mul2(pack2(pr[b][c + 2], pr[b][c + 3]), fma2(pack2(__uint_as_float(x[c + 2]), __uint_as_float(x[c + 3])), ds, d.y)), y[2], y[3]);
                     if (!whole)
 #pragma unroll
                         for (int k = 0; k < 4; k++) {
@@ -633,6 +688,8 @@ __global__ void __launch_bounds__(WG_THREADS, 1) window_grad_keys(const __grid_c
         } else {
             // the first half stages and stores dk over K, the second dv over V
             const uint32_t out = half ? v_tile : k_tile;
+            const GradRange range = grad_range<T>(p.range, a.kv_heads, e.w, hk, a.scale);
+            const float f = half ? range.out_v : range.out_s;
             for (int q = 0; q < 2 * NB; q++) {
                 uint32_t o[32];
                 tc::tmem_ld32((half ? t_dv : t_dk) + lanes + 32 * q, o);
@@ -641,7 +698,7 @@ __global__ void __launch_bounds__(WG_THREADS, 1) window_grad_keys(const __grid_c
                 for (int c = 0; c < 32; c += 8) {
                     uint32_t y[4];
 #pragma unroll
-                    for (int k = 0; k < 4; k++) y[k] = Half<T>::pack(__uint_as_float(o[c + 2 * k]), __uint_as_float(o[c + 2 * k + 1]));
+                    for (int k = 0; k < 4; k++) y[k] = Half<T>::pack(f * __uint_as_float(o[c + 2 * k]), f * __uint_as_float(o[c + 2 * k + 1]));
                     sts16(out + (q >> 1) * WF_BLOCK + tc::swz(r, 4 * (q & 1) + c / 8), y);
                 }
             }
@@ -666,6 +723,7 @@ __global__ void __launch_bounds__(256) window_grad_sinks(const __grid_constant__
     const int used = (w.all + w.per() - 1) / w.per(), rows = min(SEQ_TILE, e.y - e.z), half_size = SEQ_TILE * a.width;
     const int64_t stride = (int64_t)p.sink_tiles * a.kv_heads * 2 * half_size;   // from part to part
     const float *sums = p.part + ((int64_t)blockIdx.x * a.kv_heads + hk) * 2 * half_size;
+    const GradRange range = grad_range<T>(p.range, a.kv_heads, e.w, hk, a.scale);
     for (int x = blockIdx.z * 256 + threadIdx.x; x < rows * a.width; x += 16 * 256) {   // pairs of entries: dk, then dv
         const int half = 2 * x >= rows * a.width, at = 2 * x - half * rows * a.width, r = at / a.width, c = at % a.width;
         float2 y = make_float2(0.f, 0.f);
@@ -674,7 +732,7 @@ __global__ void __launch_bounds__(256) window_grad_sinks(const __grid_constant__
             y.x += v.x;
             y.y += v.y;
         }
-        *reinterpret_cast<uint32_t *>(row_of<T>(half ? a.dv : a.dk, e.x + e.z + r, hk) + c) = Half<T>::pack(y.x, y.y);
+        *reinterpret_cast<uint32_t *>(row_of<T>(half ? a.dv : a.dk, e.x + e.z + r, hk) + c) = Half<T>::pack((half ? range.out_v : range.out_s) * y.x, (half ? range.out_v : range.out_s) * y.y);
     }
 }
 
@@ -771,8 +829,9 @@ __global__ void __launch_bounds__(WG_THREADS, 1) window_grad_queries(const __gri
         const int r = tid & 127, half = tid >> 7, i = start + r, i0 = start + 32 * (warp & 3);
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
         const int64_t at_row = h * a.s.tokens + e.x + i;
-        const float shift = i < e.y ? -p.lse2[at_row] : 0.f, dl = i < e.y ? -p.delta[at_row] : 0.f;
-        const f32x2 cc = pack2(p.c, p.c), ss = pack2(shift, shift), scale = pack2(a.scale, a.scale), dd = pack2(dl, dl);
+        const GradRange range = grad_range<T>(p.range, a.kv_heads, e.w, hk, a.scale);
+        const float shift = i < e.y ? -p.lse2[at_row] : 0.f, dl = i < e.y ? -range.ds * p.delta[at_row] : 0.f;
+        const f32x2 cc = pack2(p.c, p.c), ss = pack2(shift, shift), ds = pack2(range.ds, range.ds), dd = pack2(dl, dl);
         for (int n = 0; n < tiles; n++) {
             const int key = key_of(n);
             const uint32_t t_s = tmem + 128 * (n & 1);
@@ -815,7 +874,7 @@ __global__ void __launch_bounds__(WG_THREADS, 1) window_grad_queries(const __gri
 #pragma unroll
                 for (int c = 0; c < 32; c += 2) {
                     float y[2];
-                    unpack2(mul2(pack2(pr[b][c], pr[b][c + 1]), fma2(pack2(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), scale, dd)), y[0], y[1]);
+                    unpack2(mul2(pack2(pr[b][c], pr[b][c + 1]), fma2(pack2(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), ds, dd)), y[0], y[1]);
                     if (!whole)
 #pragma unroll
                         for (int k = 0; k < 2; k++) {
@@ -842,7 +901,7 @@ __global__ void __launch_bounds__(WG_THREADS, 1) window_grad_queries(const __gri
             for (int c = 0; c < 32; c += 8) {
                 uint32_t y[4];
 #pragma unroll
-                for (int k = 0; k < 4; k++) y[k] = Half<T>::pack(__uint_as_float(o[c + 2 * k]), __uint_as_float(o[c + 2 * k + 1]));
+                for (int k = 0; k < 4; k++) y[k] = Half<T>::pack(range.out_s * __uint_as_float(o[c + 2 * k]), range.out_s * __uint_as_float(o[c + 2 * k + 1]));
                 sts16(q_tile + (q >> 1) * WF_BLOCK + tc::swz(r, 4 * (q & 1) + c / 8), y);
             }
         }
@@ -858,7 +917,7 @@ __global__ void __launch_bounds__(WG_THREADS, 1) window_grad_queries(const __gri
 // Where walks over sinks are cut (CutWalk).  A part is no shorter than the walk of another tile, than 24 tiles of queries, than a sixteenth of the
 // longest walk, and than an SM's share of all walks over sinks, halved: where these fill the SMs by themselves they are not cut, and the parts' sums never take
 // more than 4 x 148 slots, 78 MB at width 128.  5 packed documents of up to 3000 tokens, window 512, spent 272 us on one walk of 96 tiles, and 68 us' worth of work.
-// One of 16384 tokens and 2000 of 64, 32 heads on 8, width 128, window 128, 4 sinks, gradients: 5360 us, 5150 without sinks; with the longest walk's number of
+// One of 16384 tokens and 2000 of 64, 32 heads on 8, width 128, window 128, 4 sinks, gradients: 5460 us, 5250 without sinks; with the longest walk's number of
 // parts for every sequence 11000 us and 33.6 GB.
 struct GradCuts {
     int unit, sink_tiles;
@@ -872,18 +931,18 @@ static GradCuts grad_cuts(const f3m_seqs &s, int heads, int kv_heads, int window
     if (ns == 0 || longest * group <= unit) return {0x7fffffff, (int)ns, 0};
     return {(int)unit, (int)ns, 2 * group * s.tiles / unit};
 }
+static size_t range_floats(const f3m_seqs &s, int kv_heads) { return (2 * (size_t)s.sequences * kv_heads + 3) / 4 * 4; }
 static size_t part_floats(const GradCuts &c, int kv_heads, int width) { return (size_t)c.slots * c.sink_tiles * kv_heads * 2 * SEQ_TILE * width; }
 size_t window_grad_workspace(const f3m_seqs &s, int heads, int kv_heads, int width, int window, int sinks) {
     const size_t rows = ((size_t)s.tokens * heads + 3) / 4 * 4;
-    return (2 * rows + part_floats(grad_cuts(s, heads, kv_heads, window, sinks), kv_heads, width)) * sizeof(float);
+    return (2 * rows + range_floats(s, kv_heads) + part_floats(grad_cuts(s, heads, kv_heads, window, sinks), kv_heads, width)) * sizeof(float);
 }
 
 template <typename T>
 static void backward_t(const WindowArgs &a, cudaStream_t s) {
     constexpr int type = Half<T>::type, bytes = WF_BLOCKS * WF_BLOCK + 1024;
     const int64_t rows = a.s.tokens * a.heads, n = a.s.tokens;
-    F3M_REQUIRE((int64_t)a.s.tiles * a.heads <= 0x7fffffff && (rows + 15) / 16 <= 0x7fffffff, F3M_ERR_OVERFLOW, "%lld tokens of %d heads do not fit in 31 bits", (long long)n,
-                a.heads);
+    F3M_REQUIRE((int64_t)a.s.tiles * a.heads <= 0x7fffffff, F3M_ERR_OVERFLOW, "%lld tokens of %d heads do not fit in 31 bits", (long long)n, a.heads);
     GradKernel p;
     p.a = a;
     p.a.window = std::min(a.window, a.s.longest);   // places and their differences stay within 31 bits
@@ -895,10 +954,13 @@ static void backward_t(const WindowArgs &a, cudaStream_t s) {
     p.unit = cuts.unit;
     p.sink_tiles = cuts.sink_tiles;
     p.slots = (int)cuts.slots;
-    p.part = lse2 + (rows + 3) / 4 * 4;
+    float *range = lse2 + (rows + 3) / 4 * 4;
+    p.range = range;
+    p.part = range + range_floats(a.s, a.kv_heads);
     const int64_t parts = cuts.slots * cuts.sink_tiles * a.kv_heads;
     F3M_REQUIRE(a.s.tiles * (int64_t)a.kv_heads + parts <= 0x7fffffff, F3M_ERR_OVERFLOW, "%d tiles of %d heads do not fit in 31 bits", a.s.tiles, a.heads);
-    window_rows_sum<T><<<(unsigned)((rows + 15) / 16), 256, 0, s>>>(a, lse2, a.delta);
+    if (WG_P_EXP<T>) F3M_CUDA(cudaMemsetAsync(range, 0, range_floats(a.s, a.kv_heads) * sizeof(float), s));
+    window_rows_sum<T><<<dim3(a.s.tiles * a.kv_heads, std::min(2 * (a.heads / a.kv_heads), 65535)), 256, 0, s>>>(a, lse2, a.delta, reinterpret_cast<uint32_t *>(range));
     F3M_LAUNCH_CHECK();
     p.mq = seq_tensor_map(type, a.q, n, a.heads, a.width);
     p.mk = seq_tensor_map(type, a.k, n, a.kv_heads, a.width);

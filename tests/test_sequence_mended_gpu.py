@@ -88,3 +88,54 @@ def test_window_gradients_of_thousands_of_short_sequences(cuda):
         want, _ = both(sq.SequencePlan(few), at)
         for x, y in zip(got, want):     # parts may be cut otherwise: sums in FP32, rounded once
             assert torch.allclose(x[at].float(), y.float(), rtol=2 ** -7, atol=1e-4)
+
+
+def scaled_up(f, dout, up, **also):
+    """What f gives for dout (and dfinal) times `up`, a power of two, scaled back: gradients are linear in them, and so are bounds that do not depend
+    on their size.  What is rounded to fp16 in the end may be subnormal: half of 2^-24."""
+    want = f(dout.double() * up, **{n: x.double() * up for n, x in also.items() if x is not None})
+    return {n: (value / up, bound / up + 2.0 ** -25) for n, (value, bound) in want.items()}
+
+
+@pytest.mark.parametrize("size", [2.0 ** 8, 1.0, 2.0 ** -10, 2.0 ** -13, 2.0 ** -15])
+def test_window_gradients_of_any_size_in_fp16(size, cuda):
+    """dS is a weight times a difference, far below dout: it keeps its bits where dout does, in each sequence by itself."""
+    from f3m_b200 import sequence as sq
+    lengths, h, hk, w, window, sinks = [900, 130, 400], 4, 2, 64, 512, 4
+    n = sum(lengths)
+    q, k, v = (normal(i, n, g, w, dtype=torch.float16) for i, g in enumerate((h, hk, hk)))
+    do = normal(3, n, h, w, dtype=torch.float32)
+    do[:900] *= size
+    do[1030:] *= 64 * size if size < 1 else 1
+    do = do.half()
+    do[900:1030] = 0
+    plan = sq.SequencePlan(lengths)
+    out, lse = sq.window_attention(plan, q, k, v, window, sinks)
+    got = sq.window_attention_grad(plan, q, k, v, out, lse, do, window, sinks)
+    for at, up in ((slice(0, 900), 1 / size), (slice(900, 1030), 1.0), (slice(1030, n), 1 / (64 * size) if size < 1 else 1.0)):
+        q1, k1, v1, d1 = (x[at] for x in (q, k, v, do))
+        want = scaled_up(lambda d: ref.window(q1, k1, v1, [q1.shape[0]], window, sinks, dout=d), d1, up)
+        for name, x in zip(("dq", "dk", "dv"), got):
+            ref.assert_within(x[at], want[name], f"{name} at {size}")
+
+
+def test_captured_gradients_in_fp16_take_their_range_from_each_replay(cuda):
+    from f3m_b200 import sequence as sq
+    lengths, h, w = [333, 129], 2, 64
+    n = sum(lengths)
+    plan = sq.SequencePlan(lengths)
+    q, k, v, do = (normal(i, n, h, w, dtype=torch.float16) for i in range(4))
+
+    def train():
+        out, lse = sq.window_attention(plan, q, k, v, 100, 3)
+        return sq.window_attention_grad(plan, q, k, v, out, lse, do, 100, 3)
+
+    train()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        res = train()
+    for size in (1.0, 2.0 ** 9, 2.0 ** -13, 1.0):
+        do.copy_(normal(9, n, h, w, dtype=torch.float16, scale=size))
+        v.copy_(normal(10, n, h, w, dtype=torch.float16, scale=min(1.0, 1 / size)))
+        g.replay()
+        assert all(torch.equal(x, y) for x, y in zip(train(), res)), size
