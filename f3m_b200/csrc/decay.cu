@@ -17,7 +17,8 @@ __device__ __forceinline__ float2 unpack2(f32x2 v) {
 //
 // All products run on the tensor cores.  Warps 0-3 turn A B^T into the weights (rounded to 16 bits, written over it in tensor memory) and scale the
 // rows of A S; warps 4-11 split the scaled rows of B into a sum of 16-bit parts, in place, over A, and over the state's operand: the state is kept
-// and returned in FP32, and one rounding of what is added to it would leave it 2^-9 off in bf16.  Two parts lose 2^-17 (bf16) or 2^-23 (fp16); a
+// and returned in FP32, and one rounding of what is added to it would leave it 2^-9 off in bf16.  Two parts lose 2^-17 in bf16, and
+// in fp16 2^-23 of rows above 1/4, 2^-25 of smaller ones, whose second part is subnormal (3e-5 of a key of 1e-3); a
 // state that is returned takes a third in bf16, one that only serves the tiles behind it does not.  As an operand of A S the state is rounded to
 // 16 bits, like the weights.  The tensor cores' FP32 sums round towards zero: a state comes out about 1e-6 off (relative norm), some 0.7e-6 of it short.
 //

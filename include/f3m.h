@@ -304,8 +304,10 @@ int f3m_rbf_dense_f32_static(const float *X, int64_t N, const float *Y, int64_t 
  * token may reach every row of the 128-token tiles that see the token's tile (never another sequence).
  *
  * In fp16, what becomes an operand of a product has to stay below 65504: in decay attention the entries of the state (S, and in the gradient
- * its adjoint) and scale q_i.k_j; the outputs everywhere.  The gradients of window attention
- * are taken times powers of two that are chosen for each sequence, and are as exact for a small dout as for one of 1.
+ * its adjoint) and scale q_i.k_j; the outputs everywhere.  The same operands are rounded to
+ * multiples of 2^-24 where they are below 2^-14: the gradients of decay attention are 3e-4 off (relative norm) with dout of 1, 5e-4 with 1e-4, 2e-3 with 3e-5,
+ * where dout itself is subnormal; and a state is off by up to 2^-25 of a value for each of its tokens, 3e-5 of what a key of 1e-3 adds.  The gradients of
+ * window attention are taken times powers of two that are chosen for each sequence, and are as exact for a small dout as for one of 1.
  *
  * These entry points only enqueue work: they neither wait for the stream nor allocate, so they may be captured into a graph, and calls
  * on several streams or host threads need no order among them.  Temporaries lie in the caller's workspace (f3m_*_workspace_bytes; 16-byte

@@ -139,3 +139,29 @@ def test_captured_gradients_in_fp16_take_their_range_from_each_replay(cuda):
         v.copy_(normal(10, n, h, w, dtype=torch.float16, scale=min(1.0, 1 / size)))
         g.replay()
         assert all(torch.equal(x, y) for x, y in zip(train(), res)), size
+
+
+@pytest.mark.parametrize("carried", [False, True])
+@pytest.mark.parametrize("size", [2.0 ** 6, 1.0, 2.0 ** -10, 2.0 ** -13, 2.0 ** -15])
+def test_decay_gradients_of_any_size_in_fp16(size, carried, cuda):
+    """Weights and states that small gradients go into keep their bits where these do, in each sequence and head by itself; in one range and in several."""
+    from f3m_b200 import sequence as sq
+    h, wk, wv, lengths = 2, 64, 80, [2500, 0, 300]
+    n, log_decay = sum(lengths), [-0.02, -0.4]
+    ld = torch.tensor(log_decay, device="cuda")
+    q, k, v, do = normal(1, n, h, wk, dtype=torch.float16), normal(2, n, h, wk, dtype=torch.float16), normal(3, n, h, wv, dtype=torch.float16), normal(4, n, h, wv, dtype=torch.float32)
+    state = normal(5, 3, h, wk, wv, dtype=torch.float32) if carried else None
+    dfinal = normal(6, 3, h, wk, wv, dtype=torch.float32) * size if carried else None
+    do[:, 0] *= size
+    do[:, 1] *= size * 2 ** 4
+    do = do.half()
+    if carried:
+        dfinal[:, 1] *= 2 ** 4
+    plan = sq.SequencePlan(lengths)
+    got = sq.decay_attention_grad(plan, q, k, v, ld, do, state, dfinal)
+    for a in range(h):
+        one = slice(a, a + 1)
+        want = scaled_up(lambda d, dfinal=None: ref.decay(q[:, one], k[:, one], v[:, one], log_decay[one], lengths, None if state is None else state[:, one], dout=d, dfinal=dfinal),
+                         do[:, one], 1 / (size * 2 ** (4 * a)), dfinal=None if dfinal is None else dfinal[:, one])
+        for name, x in zip(("dq", "dk", "dv", "dstate"), got):
+            ref.assert_within(x[:, one], want[name], f"{name}, head {a} at {size}")
