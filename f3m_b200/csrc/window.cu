@@ -21,6 +21,7 @@ __device__ __forceinline__ T *row_of(const f3m_rows &r, int64_t t, int h) { retu
 // left is a tile's chain -- scores 1250 clocks, maximum 370, exponentials 1300 -- of which two run side by side.  16384 tokens, 16 heads on 4, width 128,
 // window 4096: 514-525 us, 0.92-0.94 PFLOP/s, 57 % of measured; tensor pipe 49 % busy, issue slots 44 %.
 constexpr int WF_COPY = 8, WF_PRODUCTS = 9, WF_THREADS = 320, WF_BLOCK = SEQ_TILE * 128;
+constexpr float NO_SUM = 0x1p60f;  // no sum of 2^31 weights comes near: some exponent was not a number (exp2_poly)
 constexpr int WF_BLOCKS = 14;      // blocks of 64 columns: two query tiles, a ring of key and value tiles, two to stage outputs
 
 struct WindowKernel {
@@ -216,7 +217,7 @@ __global__ void __launch_bounds__(WF_THREADS, 1) window_tiles(const __grid_const
                     const bool rise = (high - top) * p.c > 8.f;   // also from -inf; not from -inf to -inf
                     if (__any_sync(0xffffffffu, rise)) {
                         const float f = rise ? ex2_approx((top - high) * p.c) : 1.f;
-                        if (rise) { top = high; sum *= f; }
+                        if (rise) { top = high; sum = sum < NO_SUM ? sum * f : NAN; }
                         if (j > 0)
                             for (int q = 0; q < 2 * NB; q++) {
                                 uint32_t o[32];
@@ -248,7 +249,7 @@ __global__ void __launch_bounds__(WF_THREADS, 1) window_tiles(const __grid_const
                             for (int c = 0; c < 32; c += 2) {
                                 float lo, hi;
                                 const f32x2 e = fma2(pack2(__uint_as_float(y[c]), __uint_as_float(y[c + 1])), cc, ss);
-                                if (c % 8 == 6) exp2_poly(e, lo, hi);
+                                if (c % 8 == 6) exp2_poly<false>(e, lo, hi);
                                 else {
                                     unpack2(e, lo, hi);
                                     lo = ex2_approx(lo);
@@ -285,6 +286,7 @@ __global__ void __launch_bounds__(WF_THREADS, 1) window_tiles(const __grid_const
                 __syncwarp();
                 tc::fence_after_sync();
                 const int m = min(SEQ_TILE, w.len - start);
+                if (!isfinite(top) || !(sum < NO_SUM)) sum = NAN;
                 const float inv = 1.f / sum;
                 for (int q = 0; q < 2 * NB; q++) {
                     uint32_t o[32];
@@ -622,7 +624,7 @@ __global__ void __launch_bounds__(WG_THREADS, 1) window_grad_keys(const __grid_c
                     pr[b][c] = ex2_approx(pr[b][c]);
                     pr[b][c + 1] = ex2_approx(pr[b][c + 1]);
                     const f32x2 e2 = fma2(pack2(__uint_as_float(x[c + 2]), __uint_as_float(x[c + 3])), cc, l.y);
-                    if (c & 4) exp2_poly(e2, pr[b][c + 2], pr[b][c + 3]);
+                    if (c & 4) exp2_poly<true>(e2, pr[b][c + 2], pr[b][c + 3]);
                     else {
                         unpack2(e2, pr[b][c + 2], pr[b][c + 3]);
                         pr[b][c + 2] = ex2_approx(pr[b][c + 2]);
@@ -849,7 +851,7 @@ __global__ void __launch_bounds__(WG_THREADS, 1) window_grad_queries(const __gri
 #pragma unroll
                 for (int c = 0; c < 32; c += 2) {
                     const f32x2 y = fma2(pack2(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), cc, ss);
-                    if (c % 8 == 6) exp2_poly(y, pr[b][c], pr[b][c + 1]);
+                    if (c % 8 == 6) exp2_poly<true>(y, pr[b][c], pr[b][c + 1]);
                     else {
                         unpack2(y, pr[b][c], pr[b][c + 1]);
                         pr[b][c] = ex2_approx(pr[b][c]);

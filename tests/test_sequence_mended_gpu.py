@@ -165,3 +165,25 @@ def test_decay_gradients_of_any_size_in_fp16(size, carried, cuda):
                          do[:, one], 1 / (size * 2 ** (4 * a)), dfinal=None if dfinal is None else dfinal[:, one])
         for name, x in zip(("dq", "dk", "dv", "dstate"), got):
             ref.assert_within(x[:, one], want[name], f"{name}, head {a} at {size}")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_a_key_that_is_not_a_number_reaches_all_that_see_it(dtype, cuda):
+    """Wherever the key stands in its tile, and in tiles that are seen whole."""
+    from f3m_b200 import sequence as sq
+    n, h, w, window = 512, 1, 64, 300
+    plan = sq.SequencePlan([n])
+    q, k, v, do = (normal(40 + i, n, h, w, dtype=dtype) for i in range(4))
+    out, lse = sq.window_attention(plan, q, k, v, window)
+    i = torch.arange(n, device="cuda")
+    for j in (*range(128, 144), 255):
+        bad = k.clone()
+        bad[j] = float("nan")
+        sees = (i >= j) & (i - j < window)
+        got = sq.window_attention(plan, q, bad, v, window)
+        assert got[0][sees].isnan().all() and got[1][0, sees].isnan().all(), j
+        dq, dk, dv = sq.window_attention_grad(plan, q, bad, v, out, lse, do, window)
+        assert dq[sees].isnan().all() and dk[j].isnan().all() and dv[j].isnan().all(), j
+    inf = k.clone()
+    inf[:] = float("inf")
+    assert not torch.isfinite(sq.window_attention(plan, q.abs() * -1, inf, v, window)[0]).any()      # every exponent -inf: no row is a mean of values
