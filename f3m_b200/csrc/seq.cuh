@@ -217,7 +217,10 @@ __device__ __forceinline__ void store_rows(const CUtensorMap &map, const f3m_row
     }
 }
 
-// log2 of a head's decay: at most 0; -256 makes every power but the zeroth 0 in FP32 and keeps 0 * log a number
-__device__ __forceinline__ float log2_decay(float log_decay) { return fmaxf(fminf(log_decay * 1.4426950408889634f, 0.f), -256.f); }
+// log2 of a head's decay: at most 0; -256 makes every power but the zeroth 0 in FP32 and keeps 0 * log a number.  What is not a number stays that.
+__device__ __forceinline__ float log2_decay(float log_decay) {
+    const float x = log_decay * 1.4426950408889634f;
+    return x > 0.f ? 0.f : x < -256.f ? -256.f : x;
+}
 
 }  // namespace f3m

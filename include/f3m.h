@@ -357,7 +357,8 @@ int f3m_window_attention_step(int32_t n, int32_t type, int32_t heads, int32_t kv
                               f3m_rows v_cache, int64_t v_seq_stride, const int32_t *lengths, f3m_rows out, void *workspace,
                               size_t workspace_bytes, void *stream);
 
-/* log_decay (DEVICE, heads) float32: log of each head's decay, at most 0 (larger values are taken as 0, -inf is no memory at all).
+/* log_decay (DEVICE, heads) float32: log of each head's decay, at most 0 (larger values are taken as 0, -inf is no memory at all;
+ * NaN makes what the head's tokens give NaN).
  * q, k (tokens, heads, width_k), v, out (tokens, heads, width_v).  state_in, state_out (sequences, heads, width_k, width_v)
  * float32, dense, 16-byte aligned: the state before the first token (NULL: zeros) and behind the last one (NULL: not wanted; another
  * array than state_in). */

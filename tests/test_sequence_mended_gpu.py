@@ -187,3 +187,21 @@ def test_a_key_that_is_not_a_number_reaches_all_that_see_it(dtype, cuda):
     inf = k.clone()
     inf[:] = float("inf")
     assert not torch.isfinite(sq.window_attention(plan, q.abs() * -1, inf, v, window)[0]).any()      # every exponent -inf: no row is a mean of values
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_a_decay_that_is_not_a_number_is_not_one(dtype, cuda):
+    from f3m_b200 import sequence as sq
+    lengths, h, w = [300, 20], 2, 64
+    n = sum(lengths)
+    plan = sq.SequencePlan(lengths)
+    q, k, v, do = (normal(50 + i, n, h, w, dtype=dtype) for i in range(4))
+    good = torch.tensor([-0.1, -0.1], device="cuda")
+    ld = torch.tensor([float("nan"), -0.1], device="cuda")
+    got = sq.decay_attention(plan, q, k, v, ld) + sq.decay_attention_grad(plan, q, k, v, ld, do)
+    want = sq.decay_attention(plan, q, k, v, good) + sq.decay_attention_grad(plan, q, k, v, good, do)
+    for x, y in zip(got, want):
+        assert x[:, 0].isnan().all() and torch.equal(x[:, 1], y[:, 1])
+    s = normal(60, 3, h, w, w, dtype=torch.float32)
+    out = sq.decay_attention_step(q[:3], k[:3], v[:3], ld, s)
+    assert out[:, 0].isnan().all() and s[:, 0].isnan().all() and torch.isfinite(out[:, 1]).all() and torch.isfinite(s[:, 1]).all()
