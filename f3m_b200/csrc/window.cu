@@ -1134,22 +1134,23 @@ __global__ void __launch_bounds__(ST_THREADS, 3) step_keys(StepArgs a) {
         float2 y = make_float2(0.f, 0.f);
 #pragma unroll
         for (int w = 0; w < 4; w++) {
-            if (stat[0][w][h] != -INFINITY) total += stat[1][w][h] * ex2_approx(stat[0][w][h] - high);
+            if (stat[1][w][h] != 0.f) total += stat[1][w][h] * ex2_approx(stat[0][w][h] - high);   // of a warp without keys: 0
             y.x += sum_s[w][h][d];
             y.y += sum_s[w][h][d + 1];
         }
         if (a.parts == 1) {
-            const float inv = total > 0.f ? 1.f / total : 0.f;
+            const float inv = total != 0.f ? 1.f / total : 0.f;   // no keys at all: 0; what is not a number stays that
             *reinterpret_cast<uint32_t *>(row_of<T>(a.out, b, h0 + h) + d) = Half<T>::pack(y.x * inv, y.y * inv);
         } else {
             const int64_t row = (b * a.heads + h0 + h) * a.parts + part;
-            if (total > 0.f) *reinterpret_cast<float2 *>(a.part + (int64_t)a.n * a.heads * a.parts * 2 + row * a.width + d) = y;
+            if (total != 0.f) *reinterpret_cast<float2 *>(a.part + (int64_t)a.n * a.heads * a.parts * 2 + row * a.width + d) = y;
             if (d == 0) *reinterpret_cast<float2 *>(a.part + 2 * row) = make_float2(high, total);
         }
     }
 }
 
-// A CTA per (sequence, head): the parts' sums, scaled to their common maximum, in the order of the parts.
+// A CTA per (sequence, head): the parts' sums, scaled to their common maximum, in the order of the parts.  A part without keys has a sum of 0, any other
+// one of 1 or more, or one that is not a number.
 template <typename T>
 __global__ void __launch_bounds__(64) step_join(StepArgs a) {
     __shared__ float w_s[256];
@@ -1159,19 +1160,19 @@ __global__ void __launch_bounds__(64) step_join(StepArgs a) {
     const float *sums = a.part + (int64_t)a.n * a.heads * a.parts * 2 + row * a.width;
     float high = -INFINITY;
     for (int i = 0; i < a.parts; i++) high = fmaxf(high, stat[i].x);
-    for (int i = threadIdx.x; i < a.parts; i += 64) w_s[i] = stat[i].y > 0.f ? ex2_approx(stat[i].x - high) : 0.f;
+    for (int i = threadIdx.x; i < a.parts; i += 64) w_s[i] = ex2_approx(stat[i].x - high);
     __syncthreads();
     if (d >= a.width) return;
     float total = 0.f;
     float2 y = make_float2(0.f, 0.f);
     for (int i = 0; i < a.parts; i++) {
-        if (w_s[i] == 0.f) continue;   // its sums may not have been written
+        if (stat[i].y == 0.f) continue;   // its sums have not been written
         total += w_s[i] * stat[i].y;
         const float2 x = *reinterpret_cast<const float2 *>(sums + (int64_t)i * a.width + d);
         y.x = fmaf(w_s[i], x.x, y.x);
         y.y = fmaf(w_s[i], x.y, y.y);
     }
-    const float inv = total > 0.f ? 1.f / total : 0.f;
+    const float inv = total != 0.f ? 1.f / total : 0.f;
     *reinterpret_cast<uint32_t *>(row_of<T>(a.out, b, h) + d) = Half<T>::pack(y.x * inv, y.y * inv);
 }
 

@@ -205,3 +205,25 @@ def test_a_decay_that_is_not_a_number_is_not_one(dtype, cuda):
     s = normal(60, 3, h, w, w, dtype=torch.float32)
     out = sq.decay_attention_step(q[:3], k[:3], v[:3], ld, s)
     assert out[:, 0].isnan().all() and s[:, 0].isnan().all() and torch.isfinite(out[:, 1]).all() and torch.isfinite(s[:, 1]).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("capacity", [200, 5000])
+def test_a_step_does_not_lose_what_is_not_a_number(capacity, dtype, cuda):
+    """A seen key or value that is not a number, among finite ones, in a part of its own, and as a part's only keys; in a cache taken whole and in parts."""
+    from f3m_b200 import sequence as sq
+    h, w = 4, 64
+    q = normal(1, 1, h, w, dtype=dtype)
+    kc, vc = normal(2, 1, capacity, 2, w, dtype=dtype), normal(3, 1, capacity, 2, w, dtype=dtype)
+    lens = torch.tensor([capacity], dtype=torch.int32, device="cuda")
+    assert torch.isfinite(sq.window_attention_step(q, kc, vc, lens, capacity)).all()
+    for at in (slice(0, 1), slice(capacity - 1, capacity), slice(capacity // 2, capacity // 2 + 3), slice(0, capacity // 2), slice(0, capacity)):
+        for which in (0, 1):
+            x = [kc.clone(), vc.clone()]
+            x[which][:, at, 0] = float("nan")
+            got = sq.window_attention_step(q, *x, lens, capacity)
+            assert got[:, :2].isnan().all() and torch.isfinite(got[:, 2:]).all(), (at, which)
+    far = kc.clone()
+    far[:, :64] = float("nan")         # and where what is finite weighs far more
+    far[:, 64:] = 60 * q[:, :1].sign()
+    assert sq.window_attention_step(q[:, :1].repeat(1, 4, 1), far, vc, lens, capacity, scale=1.0).isnan().all()
