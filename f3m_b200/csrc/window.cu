@@ -36,6 +36,11 @@ struct WindowItem {
     int row0, len, start, head[2], kv_head, tiles_q;   // tile t: tokens from start + (by_heads ? 0 : 128 t) on
     int sinks, first, keys;                            // tiles of keys: the first `sinks` of the sequence, then those from tile `first` on; `keys` in all
     __device__ __forceinline__ int key(int j) const { return SEQ_TILE * (j < sinks ? j : first + j - sinks); }
+    // Whether some query of the tile from `from` on sees some key of the tile from k on.  Of two neighbouring tiles one may not: its weights are zeros, and stay out
+    // of its product, as a zero times what is not finite is no zero.
+    __device__ __forceinline__ bool sees(const WindowArgs &a, int from, int k) const {
+        return k < from + SEQ_TILE && (k < a.sinks || from - k - (SEQ_TILE - 1) < a.window);
+    }
 };
 __device__ __forceinline__ WindowItem window_item(const WindowKernel &p, int i) {
     const WindowArgs &a = p.a;
@@ -141,6 +146,7 @@ __global__ void __launch_bounds__(WF_THREADS, 1) window_tiles(const __grid_const
                 tc::mma_commit(b_free + 8 * sk);
                 if (w.keys == 1) tc::mma_commit(b_q_free);
             }
+            bool begun[2] = {false, false};
             for (int j = 0; j < w.keys; j++) {
                 const int xv = x + 2 * j + 1, sv = xv % slots;
                 const bool more = j + 1 < w.keys;
@@ -148,18 +154,19 @@ __global__ void __launch_bounds__(WF_THREADS, 1) window_tiles(const __grid_const
                 wait(b_full + 8 * sv, (xv / slots) & 1);
                 if (more) wait(b_full + 8 * sk, ((xv + 1) / slots) & 1);
                 for (int t = 0; t < w.tiles_q; t++) {
+                    const bool seen = p.by_heads || w.sees(a, w.start + t * SEQ_TILE, w.key(j));
                     if (j == 0 && no[t]) wait(b_o_read + 8 * t, (no[t] - 1) & 1);
                     wait(b_p + 8 * t, np[t] & 1);
                     tc::fence_after_sync();
-                    if (tc::elect()) {
-                        tc::product_tmem64(tmem + 256 + 128 * t, tmem + 128 * t, slot_tile(sv), i_o, j);
+                    if (seen && tc::elect()) {
+                        tc::product_tmem64(tmem + 256 + 128 * t, tmem + 128 * t, slot_tile(sv), i_o, begun[t]);
                     }
                     wait(b_p2 + 8 * t, np[t] & 1);
                     np[t]++;
                     no[t] += !more;
                     tc::fence_after_sync();
                     if (tc::elect()) {
-                        tc::product_tmem64(tmem + 256 + 128 * t, tmem + 128 * t + 32, slot_tile(sv) + 64 * 128, i_o, 1);
+                        if (seen) tc::product_tmem64(tmem + 256 + 128 * t, tmem + 128 * t + 32, slot_tile(sv) + 64 * 128, i_o, 1);
                         if (more) {
                             tc::product_rows<NB>(tmem + 128 * t, q_tile(t), slot_tile(sk), i_s);
                             tc::mma_commit(b_s + 8 * t);
@@ -167,6 +174,7 @@ __global__ void __launch_bounds__(WF_THREADS, 1) window_tiles(const __grid_const
                             tc::mma_commit(b_o + 8 * t);
                         }
                     }
+                    begun[t] |= seen;
                 }
                 if (tc::elect()) {
                     tc::mma_commit(b_free + 8 * sv);

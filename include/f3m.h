@@ -301,7 +301,7 @@ int f3m_rbf_dense_f32_static(const float *X, int64_t N, const float *Y, int64_t 
  * Sequences are packed: row t of an array is token t of all sequences laid end to end.  Data are 16-bit floats of one type
  * (F3M_TYPE_*), sums and states float32.  Columns are contiguous; token and head strides are in elements, multiples of 8, and
  * data start on 16 bytes.  Widths are multiples of 8 up to F3M_MAX_WIDTH.  Inputs have to be finite: what is not finite in a
- * token may reach every row of the 128-token tiles that see the token's tile (never another sequence).
+ * token may reach every row of the 128-token tiles that see the token's tile, and in gradients those that such tiles see (never another sequence).
  *
  * In fp16, what becomes an operand of a product has to stay below 65504: in decay attention the entries of the state (S, and in the gradient
  * its adjoint) and scale q_i.k_j; the outputs everywhere.  The same operands are rounded to

@@ -227,3 +227,26 @@ def test_a_step_does_not_lose_what_is_not_a_number(capacity, dtype, cuda):
     far[:, :64] = float("nan")         # and where what is finite weighs far more
     far[:, 64:] = 60 * q[:, :1].sign()
     assert sq.window_attention_step(q[:, :1].repeat(1, 4, 1), far, vc, lens, capacity, scale=1.0).isnan().all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv_heads", [(1, 1), (3, 1), (4, 2), (2, 2)])
+def test_what_is_not_finite_stays_with_the_tiles_that_see_it(heads, kv_heads, dtype, cuda):
+    """Tiles of 128 queries whose window ends before a token's tile, or begins behind it, do not notice what it holds."""
+    from f3m_b200 import sequence as sq
+    n, w, window, sinks = 900, 64, 130, 3
+    plan = sq.SequencePlan([n])
+    q, k, v = normal(1, n, heads, w, dtype=dtype), normal(2, n, kv_heads, w, dtype=dtype), normal(3, n, kv_heads, w, dtype=dtype)
+    want, lse = sq.window_attention(plan, q, k, v, window, sinks)
+    i = torch.arange(n, device="cuda")
+    for t in range(1, 7):       # tile 0 holds the sinks: it is seen by all
+        for worst in (float("nan"), float("inf")):
+            kk, vv = k.clone(), v.clone()
+            vv[128 * t + 5] = worst
+            kk[128 * t + 77] = worst
+            got, l = sq.window_attention(plan, q, kk, vv, window, sinks)
+            # a tile of queries sees tile t of keys if one of its queries, from 128 tile to 128 tile + 127, sees one of its keys
+            tile = i // 128
+            sees = (tile >= t) & (128 * tile - (128 * t + 127) < window)
+            assert torch.equal(got[~sees], want[~sees]) and torch.equal(l[:, ~sees], lse[:, ~sees]), t
+            assert got[128 * t + 77].isnan().all()
