@@ -1034,7 +1034,7 @@ __global__ void __launch_bounds__(ST_THREADS, 3) step_keys(StepArgs a) {
     const int64_t b = blockIdx.z;
     // the keys seen, numbered without a gap: the sinks before the window, then the window
     const int len = min(max(a.lengths[b], 0), (int)a.capacity), lo = max(0, len - a.window), ns = min(a.sinks, lo), seen = ns + len - lo;
-    const int per = ((seen + a.parts - 1) / a.parts + 63) / 64 * 64, v0 = (int)min((int64_t)part * per, (int64_t)seen), v1 = min(seen, v0 + per);
+    const int per = ((seen + a.parts - 1) / a.parts + 63) / 64 * 64, v0 = (int)min((int64_t)part * per, (int64_t)seen), v1 = (int)min((int64_t)v0 + per, (int64_t)seen);
     const T *kc = reinterpret_cast<const T *>(a.k.data) + b * a.k_seq + hk * a.k.head_stride, *vc = reinterpret_cast<const T *>(a.v.data) + b * a.v_seq + hk * a.v.head_stride;
     auto key = [&](int v) { return (int64_t)(v < ns ? v : lo + v - ns); };
 

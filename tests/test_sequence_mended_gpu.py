@@ -250,3 +250,19 @@ def test_what_is_not_finite_stays_with_the_tiles_that_see_it(heads, kv_heads, dt
             sees = (tile >= t) & (128 * tile - (128 * t + 127) < window)
             assert torch.equal(got[~sees], want[~sees]) and torch.equal(l[:, ~sees], lse[:, ~sees]), t
             assert got[128 * t + 77].isnan().all()
+
+
+def test_a_step_at_the_end_of_the_longest_cache(cuda):
+    """Numbers of keys whose sum with a part's length passes 2^31: the last part's keys, which weigh all."""
+    from f3m_b200 import sequence as sq
+    cap, w, last, dtype = 0x7fffff00, 8, 100, torch.bfloat16
+    cache = torch.zeros(1, cap, 1, w, device="cuda", dtype=dtype)          # keys and values are the same
+    cache[0, -last:, 0] = 2 + normal(1, last, w, dtype=dtype, scale=0.25)
+    q = torch.full((1, 1, w), 8.0, device="cuda", dtype=dtype)
+    got = sq.window_attention_step(q, cache, cache, torch.tensor([cap], dtype=torch.int32, device="cuda"), cap)
+    kd = cache[0, -last:, 0].double()
+    weights = torch.exp(kd @ q[0, 0].double() * w ** -0.5 - 40)            # the others have exp(-40) each
+    want = weights @ kd / (weights.sum() + (cap - last) * torch.exp(torch.tensor(-40.0, dtype=torch.float64, device="cuda")))
+    del cache
+    # the weights and the output are rounded to 16 bits; the row sum adds 2^31 numbers in FP32, which may fall below its last place
+    ref.assert_within(got[0, 0], (want, (3 * ref.half_step(dtype) + 1e-4) * want.abs()))
