@@ -109,6 +109,7 @@ SIGNATURES = {
     "f3m_plan_last_pairs_by_form": (C.c_int, [_P, C.POINTER(_I64)]),
     "f3m_launch_count": (C.c_longlong, []),
     "f3m_seqs_layout": (C.c_int, [_P, _I32, C.POINTER(Seqs), _P]),
+    "f3m_seqs_error_word": (C.POINTER(C.c_int), []),
     "f3m_window_attention": (C.c_int, [C.POINTER(Seqs), _I32, _I32, _I32, _I32, _I32, _I32, _F32, Rows, Rows, Rows, Rows, _P, _P]),
     "f3m_window_attention_grad_workspace_bytes": (C.c_size_t, [C.POINTER(Seqs), _I32, _I32, _I32, _I32, _I32]),
     "f3m_window_attention_grad": (C.c_int, [C.POINTER(Seqs), _I32, _I32, _I32, _I32, _I32, _I32, _F32, Rows, Rows, Rows, Rows, _P, Rows,

@@ -163,6 +163,12 @@ int f3m_seqs_layout(const int32_t *lengths, int32_t n, f3m_seqs *seqs, int32_t *
     });
 }
 
+int *f3m_seqs_error_word(void) {
+    int *word = nullptr;
+    guarded([&] { word = seq_error_word(); });
+    return word;
+}
+
 int f3m_window_attention(const f3m_seqs *seqs, int32_t type, int32_t heads, int32_t kv_heads, int32_t width, int32_t window, int32_t sinks,
                          float scale, f3m_rows q, f3m_rows k, f3m_rows v, f3m_rows out, float *lse, void *stream) {
     return guarded([&] {
@@ -225,6 +231,7 @@ int f3m_window_attention_step(int32_t n, int32_t type, int32_t heads, int32_t kv
         StepArgs a{n, heads, kv_heads, width, window, sinks, capacity, scale, q, k_cache, v_cache, out, k_seq_stride, v_seq_stride, lengths, 1, (float *)workspace};
         a.parts = window_step_parts(n, heads, kv_heads, capacity, window, sinks);
         check_workspace(workspace, workspace_bytes, window_step_part_floats(n, heads, width, a.parts) * sizeof(float));
+        seq_check_error();
         window_step(type, a, (cudaStream_t)stream);
     });
 }
@@ -289,6 +296,7 @@ int f3m_decay_attention_step(int32_t n, int32_t type, int32_t heads, int32_t wid
         check_rows(q, n, heads, width_k, "q"); check_rows(k, n, heads, width_k, "k"); check_rows(v, n, heads, width_v, "v");
         check_out(out, n, heads, width_v, "out"); check_state(state, "state");
         if (n == 0) return;
+        seq_check_error();
         decay_step(type, n, heads, width_k, width_v, log_decay, scale, q, k, v, state, out, (cudaStream_t)stream);
     });
 }

@@ -312,7 +312,8 @@ int f3m_rbf_dense_f32_static(const float *X, int64_t N, const float *Y, int64_t 
  * These entry points only enqueue work: they neither wait for the stream nor allocate, so they may be captured into a graph, and calls
  * on several streams or host threads need no order among them.  Temporaries lie in the caller's workspace (f3m_*_workspace_bytes; 16-byte
  * aligned), which a call owns until its work has ended.  A repeated call gives the same bits.  A kernel's roles wait for one another two seconds at
- * most; should a wait run out, the next call on sequences of the process returns F3M_ERR_INTERNAL. */
+ * most; should a wait run out, the next call on sequences of the process, of whatever kind, thread, stream or device, returns F3M_ERR_INTERNAL and enqueues
+ * nothing.  A program that has to know of its own or its last call waits for its work and reads f3m_seqs_error_word. */
 #define F3M_TYPE_BF16 1
 #define F3M_TYPE_F16 2
 #define F3M_MAX_WIDTH 128
@@ -334,6 +335,9 @@ typedef struct f3m_seqs {
     int32_t table_words;
 } f3m_seqs;
 int f3m_seqs_layout(const int32_t *lengths, int32_t n, f3m_seqs *seqs, int32_t *table);
+/* HOST address of the word that a kernel sets to 1 when a wait of its has run out; the next call's F3M_ERR_INTERNAL sets it back to 0, and so may the
+ * program.  NULL, and f3m_last_error, where there is no device. */
+int *f3m_seqs_error_word(void);
 
 /* out (tokens, heads, width), lse (heads, tokens) float32: log of the row sums sum_j w_ij.  heads is a multiple of kv_heads; query head h
  * reads key head h / (heads / kv_heads).  window >= 1, sinks >= 0. */

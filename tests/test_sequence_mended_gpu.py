@@ -266,3 +266,28 @@ def test_a_step_at_the_end_of_the_longest_cache(cuda):
     del cache
     # the weights and the output are rounded to 16 bits; the row sum adds 2^31 numbers in FP32, which may fall below its last place
     ref.assert_within(got[0, 0], (want, (3 * ref.half_step(dtype) + 1e-4) * want.abs()))
+
+
+def test_every_call_reports_a_wait_that_ran_out(cuda):
+    """The word that a kernel would set, set by hand: the next call is refused, whichever it is, enqueues nothing, and the one behind it runs."""
+    from f3m_b200 import _lib, sequence as sq
+    word = _lib.lib().f3m_seqs_error_word()
+    n, h, w = 40, 2, 64
+    plan, ld = sq.SequencePlan([n]), torch.tensor([-0.1, -0.2], device="cuda")
+    x = normal(1, n, h, w, dtype=torch.bfloat16)
+    lens, state = torch.full((n,), 1, dtype=torch.int32, device="cuda"), torch.ones(n, h, w, w, device="cuda")
+    out, lse = sq.window_attention(plan, x, x, x, 10)
+    calls = [lambda: sq.window_attention(plan, x, x, x, 10), lambda: sq.window_attention_grad(plan, x, x, x, out, lse, x, 10),
+             lambda: sq.window_attention_step(x, x[:, None], x[:, None], lens, 10), lambda: sq.decay_attention(plan, x, x, x, ld),
+             lambda: sq.decay_attention_grad(plan, x, x, x, ld, x), lambda: sq.decay_attention_step(x, x, x, ld, state)]
+    for call in calls:
+        torch.cuda.synchronize()
+        assert word[0] == 0
+        word[0] = 1
+        with pytest.raises(_lib.F3MError, match="gave up"):
+            call()
+        assert word[0] == 0 and bool((state == 1).all())
+    for call in calls:
+        call()
+    torch.cuda.synchronize()
+    assert word[0] == 0
