@@ -19,7 +19,7 @@ and data on 16 bytes -- views of a joint projection are; anything else is copied
 
 `window_attention` and `decay_attention` are differentiable by q, k, v (and the states) when autograd is on.  Autograd's bookkeeping of a
 leaf belongs to the stream that first used it, so a graph that is differentiated by autograd is not captured: the two refuse that, and a
-captured training step calls the gradient functions itself.
+captured training step calls the gradient functions itself.  Forward-mode derivatives are refused.
 """
 from __future__ import annotations
 
@@ -28,6 +28,7 @@ from typing import Optional, Sequence, Tuple
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import Rows, Seqs, check
@@ -170,6 +171,11 @@ def _refuse_capture(what: str):
                            "that need no gradient")
 
 
+def _refuse_tangents(*tensors):
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError("the products over sequences have no forward-mode derivatives")
+
+
 def _needs_grad(*tensors) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
@@ -194,6 +200,7 @@ def window_attention(plan: SequencePlan, q: torch.Tensor, k: torch.Tensor, v: to
     """Token i of a sequence sees token j <= i if i - j < window or j < sinks: out_i = sum_j w_ij v_j / sum_j w_ij, w_ij = exp(scale q_i.k_j).
     q (tokens, heads, width), k and v (tokens, kv_heads, width) with heads a multiple of kv_heads; scale is 1/sqrt(width) unless given.
     Returns out like q and lse (heads, tokens) float32, the logs of the row sums."""
+    _refuse_tangents(q, k, v)
     if _needs_grad(q, k, v):
         _refuse_capture("window_attention")
         return _WindowAttention.apply(plan, q, k, v, window, sinks, scale)
@@ -217,6 +224,7 @@ def window_attention_grad(plan: SequencePlan, q: torch.Tensor, k: torch.Tensor, 
                           dout: torch.Tensor, window: int, sinks: int = 0, scale: Optional[float] = None
                           ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """Gradients (dq, dk, dv) of sum(out * dout), from what window_attention returned for the same arguments."""
+    _refuse_tangents(q, k, v, out, lse, dout)
     kind = _type_of(q, k, v, out, dout)
     _check_qkv(plan, q, k, v)
     _shape(out, q.shape, "out")
@@ -261,6 +269,7 @@ def window_attention_step(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
     """One new token for each of n sequences.  q (n, heads, width); k_cache, v_cache (n, capacity, kv_heads, width) hold the tokens so far,
     the new one at lengths - 1 among them; lengths (n) int32 on the device, taken as 0..capacity.  Returns out like q; a sequence of length
     0 gets zeros."""
+    _refuse_tangents(q, k_cache, v_cache)
     kind = _type_of(q, k_cache, v_cache)
     if q.dim() != 3 or k_cache.dim() != 4:
         raise ValueError("q is a (n, heads, width) array, k_cache and v_cache are (n, capacity, kv_heads, width) arrays")
@@ -321,6 +330,7 @@ def decay_attention(plan: SequencePlan, q: torch.Tensor, k: torch.Tensor, v: tor
     """S_t = exp(log_decay) S_(t-1) + k_t v_t^T, out_t = scale q_t S_t along every sequence.  q, k (tokens, heads, width_k), v (tokens, heads,
     width_v), log_decay (heads) float32, at most 0; state (sequences, heads, width_k, width_v) float32 is the state before the first token
     (zeros unless given); scale is 1/sqrt(width_k) unless given.  Returns out like v and the state behind the last token, as a new array."""
+    _refuse_tangents(q, k, v, log_decay, state)
     if _needs_grad(q, k, v, log_decay, state):
         if log_decay.requires_grad:
             raise RuntimeError("decay_attention has no gradient by log_decay: the decay is a constant")
@@ -356,6 +366,7 @@ def decay_attention_grad(plan: SequencePlan, q: torch.Tensor, k: torch.Tensor, v
                          ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
     """Gradients (dq, dk, dv, dstate) of sum(out * dout) + sum(final * dfinal) for (out, final) = decay_attention(plan, q, k, v, log_decay,
     state, scale); dfinal is zero unless given."""
+    _refuse_tangents(q, k, v, log_decay, dout, state, dfinal)
     kind = _type_of(q, k, v, dout)
     _check_decay(q, k, v, log_decay)
     _check_plan(plan, q)
@@ -396,6 +407,7 @@ def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_
                          scale: Optional[float] = None) -> torch.Tensor:
     """One new token for each of n sequences: q, k (n, heads, width_k), v (n, heads, width_v); state (n, heads, width_k, width_v) float32,
     contiguous, is updated in place.  Returns out like v."""
+    _refuse_tangents(q, k, v, log_decay, state)
     kind = _type_of(q, k, v)
     _check_decay(q, k, v, log_decay)
     _shape(state, (q.shape[0], q.shape[1], q.shape[2], v.shape[2]), "state")

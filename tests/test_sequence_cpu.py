@@ -120,3 +120,27 @@ def test_gradient_workspace_of_uneven_batches():
     assert need([65536], 32, 8, 128, 512, 65536) < most
     assert need([64] * 5000, 32, 8, 128, 128, 4) < 1 << 20            # no walk is cut
     assert need([16384] + [64] * 2000, 32, 8, 128, 128, 0) < 1 << 20
+
+
+def test_forward_mode_derivatives_are_refused():
+    """A tangent would be dropped without a word: the library takes addresses."""
+    from torch.autograd import forward_ad
+    x, ld, state = torch.ones(4, 2, 64, dtype=torch.bfloat16), torch.zeros(2), torch.zeros(4, 2, 64, 64)
+    lens, lse = torch.ones(4, dtype=torch.int32), torch.zeros(2, 4)
+    calls = [lambda d: sequence.window_attention(None, x, d, x, 4), lambda d: sequence.window_attention_grad(None, x, x, x, x, lse, d, 4),
+             lambda d: sequence.window_attention_step(d, x[:, None], x[:, None], lens, 4), lambda d: sequence.decay_attention(None, x, x, d, ld),
+             lambda d: sequence.decay_attention_grad(None, d, x, x, ld, x), lambda d: sequence.decay_attention_step(x, d, x, ld, state)]
+    with forward_ad.dual_level():
+        dual, plain = forward_ad.make_dual(x, torch.ones_like(x)), 0
+        for call in calls:
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call(dual)
+            with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+                call(dual)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            sequence.decay_attention(None, x, x, x, ld, forward_ad.make_dual(state, state))
+        for call in calls:                      # without a tangent it is the CPU that is refused, as ever
+            with pytest.raises((ValueError, RuntimeError)) as e:
+                call(x)
+            plain += "forward-mode" not in str(e.value)
+        assert plain == len(calls)
