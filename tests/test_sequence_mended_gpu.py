@@ -291,3 +291,76 @@ def test_every_call_reports_a_wait_that_ran_out(cuda):
         call()
     torch.cuda.synchronize()
     assert word[0] == 0
+
+
+def test_calls_from_several_host_threads(cuda):
+    """Each thread on its own stream, all at once: the bits of the calls alone."""
+    import threading
+    from f3m_b200 import sequence as sq
+    lengths, h, w = [2500, 17, 400], 4, 64
+    n = sum(lengths)
+    ld = torch.tensor([-0.01, -0.1, -0.3, 0.0], device="cuda")
+    plan = sq.SequencePlan(lengths)
+    kc, vc = normal(8, 2, 3000, 2, w, dtype=torch.float16), normal(9, 2, 3000, 2, w, dtype=torch.float16)
+    lens = torch.tensor([3000, 2000], dtype=torch.int32, device="cuda")
+
+    def calls(seed):
+        q, k, v, do = (normal(seed + i, n, h, w, dtype=torch.float16) for i in range(4))
+        out, lse = sq.window_attention(plan, q, k[:, :2], v[:, :2], 300, 5)
+        a = sq.window_attention_grad(plan, q, k[:, :2], v[:, :2], out, lse, do, 300, 5)
+        s = normal(seed, 2, h, w, w, dtype=torch.float32)
+        step = sq.decay_attention_step(q[:2], k[:2], v[:2], ld, s)
+        return (out, lse, s, step) + a + sq.decay_attention(plan, q, k, v, ld) + sq.decay_attention_grad(plan, q, k, v, ld, do) + (sq.window_attention_step(q[:2], kc, vc, lens, 2500, 3),)
+
+    want = {seed: calls(seed) for seed in range(100, 140, 10)}
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(seed):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    got = calls(seed)
+                    torch.cuda.current_stream().synchronize()
+                    if not all(torch.equal(x, y) for x, y in zip(got, want[seed])):
+                        wrong.append(seed)
+        except Exception as e:      # noqa: BLE001  (a thread's failure has to reach the test)
+            wrong.append(e)
+
+    threads = [threading.Thread(target=work, args=(s,)) for s in want]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not wrong, wrong
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16])
+def test_prompts_and_gradients_behind_two_billion_elements(dtype, cuda):
+    """The last sequence of arrays of more than 2^31 elements: the bits it has by itself."""
+    from f3m_b200 import sequence as sq
+    w, h, last = 128, 16, 300
+    n = 2 ** 31 // (h * w) + 4000
+    plan, alone = sq.SequencePlan([n - last, last]), sq.SequencePlan([last])
+    q = torch.zeros(n, h, w, device="cuda", dtype=dtype)
+    k, v = (torch.zeros(n, 1, w, device="cuda", dtype=dtype) for _ in range(2))
+    q[-last:], k[-last:], v[-last:] = (normal(i, last, x.shape[1], w, dtype=dtype) for i, x in enumerate((q, k, v)))
+    do = q.flip(2)
+    t = [x[-last:].clone() for x in (q, k, v, do)]
+    want, wl = sq.window_attention(alone, *t[:3], 100, 3)
+    wg = sq.window_attention_grad(alone, *t[:3], want, wl, t[3], 100, 3)
+    out, lse = sq.window_attention(plan, q, k, v, 100, 3)
+    assert torch.equal(out[-last:], want) and torch.equal(lse[:, -last:], wl) and not out[:-last].any()
+    got = sq.window_attention_grad(plan, q, k, v, out, lse, do, 100, 3)
+    for x, y in zip(got, wg):
+        ref.assert_within(x[-last:], (y.double(), y.double().abs() * 2 ** -7 + 1e-5))      # walks over sinks may be cut otherwise
+    del got, out, lse, k, v
+    ld = -torch.arange(1, h + 1, device="cuda", dtype=torch.float32) / 50
+    state = normal(7, 2, h, w, w, dtype=torch.float32)
+    want, wf = sq.decay_attention(alone, t[0], t[0], t[3], ld, state[1:])
+    out, final = sq.decay_attention(plan, q, q, do, ld, state)
+    u = ref.half_step(dtype)
+    ref.assert_within(out[-last:], (want.double(), 2 * u * want.double().abs() + 4 * u * want.double().abs().max()))       # states may be joined between ranges
+    ref.assert_within(final[1:], (wf.double(), 1e-5 * wf.double().abs().max().expand_as(wf)))
+    del out
+    got = sq.decay_attention_grad(plan, q, q, do, ld, do, state)
+    for x, y in zip(got[:3], sq.decay_attention_grad(alone, t[0], t[0], t[3], ld, t[3], state[1:])[:3]):
+        ref.assert_within(x[-last:], (y.double(), 2 * u * y.double().abs() + 4 * u * y.double().abs().max()))
