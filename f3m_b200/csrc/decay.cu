@@ -127,7 +127,7 @@ __device__ __forceinline__ void put_row(uint32_t tile, int j, int c0, const uint
 template <typename T, int PARTS, int NB>
 __global__ void __launch_bounds__(DK_THREADS, 1) decay_tiles(const __grid_constant__ DecayKernel p) {
     extern __shared__ unsigned char raw[];
-    __shared__ __align__(8) uint64_t bars[2 * 4 + 11];
+    __shared__ __align__(8) uint64_t bars[2 * 4 + 12];
     __shared__ uint32_t tmem_s;
     __shared__ int gave_up_s;
     const DecayArgs &a = p.a;
@@ -149,6 +149,7 @@ __global__ void __launch_bounds__(DK_THREADS, 1) decay_tiles(const __grid_consta
         for (int i = 12; i < 15; i++) tc::mbar_init(tc::smem_u32(&bars[i]), 128);      // weights written, A S scaled, outputs read
         tc::mbar_init(tc::smem_u32(&bars[17]), 1);                                     // A B^T of odd tiles
         tc::mbar_init(tc::smem_u32(&bars[18]), 128);                                   // weights of odd tiles written
+        tc::mbar_init(tc::smem_u32(&bars[19]), 1);                                     // no products in flight
         for (int i = 15; i < 17; i++) tc::mbar_init(tc::smem_u32(&bars[i]), 256);      // B split; state ready as operand and in tensor memory
         tc::fence_mbar_init();
         gave_up_s = 0;
@@ -249,6 +250,7 @@ __global__ void __launch_bounds__(DK_THREADS, 1) decay_tiles(const __grid_consta
             }
             if (more && !early) score(n + 1);
         }
+        wait.drain_products(tc::smem_u32(&bars[19]));
     } else if (warp < 4) {
         // ---- weights and outputs: thread i has row i ----
         const int i = tid;
@@ -436,7 +438,7 @@ __global__ void __launch_bounds__(DK_THREADS, 1) decay_tiles(const __grid_consta
 template <typename T, int PARTS, int NB>
 __global__ void __launch_bounds__(DS_THREADS, 1) decay_states(const __grid_constant__ DecayKernel p) {
     extern __shared__ unsigned char raw[];
-    __shared__ __align__(8) uint64_t bars[2 * 4 + 3];
+    __shared__ __align__(8) uint64_t bars[2 * 4 + 4];
     __shared__ uint32_t tmem_s;
     __shared__ int gave_up_s;
     const DecayArgs &a = p.a;
@@ -459,6 +461,7 @@ __global__ void __launch_bounds__(DS_THREADS, 1) decay_states(const __grid_const
         tc::mbar_init(tc::smem_u32(&bars[8]), 256);                             // B split
         tc::mbar_init(tc::smem_u32(&bars[9]), 1);                               // tail and rest have been read
         tc::mbar_init(tc::smem_u32(&bars[10]), 1);                              // all done
+        tc::mbar_init(tc::smem_u32(&bars[11]), 1);                              // no products in flight
         tc::fence_mbar_init();
         gave_up_s = 0;
     }
@@ -510,6 +513,7 @@ __global__ void __launch_bounds__(DS_THREADS, 1) decay_states(const __grid_const
                 if (n + 1 == tiles) tc::mma_commit(b_done);
             }
         }
+        wait.drain_products(tc::smem_u32(&bars[11]));
     } else {
         const int j = tid & 127, half = tid >> 7;
         for (int n = 0; n < tiles; n++) {

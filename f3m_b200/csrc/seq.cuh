@@ -158,6 +158,14 @@ struct Waits {
     __device__ __forceinline__ void drain(uint32_t bar, uint32_t parity) const {
         for (uint32_t tries = 0; tries < WAIT_TRIES && !tc::mbar_try_wait_ns(bar, parity, 2000); tries++) {}
     }
+    // by the warp that issues the block's products, behind the last of them: where the block has given up, nobody else may have waited for those in flight, and the
+    // tensor memory that they write is about to be another block's
+    __device__ __forceinline__ void drain_products(uint32_t bar) const {
+        if (tc::elect()) {
+            tc::mma_commit(bar);
+            drain(bar, 0);
+        }
+    }
 };
 
 __device__ __forceinline__ void sts16(uint32_t at, const uint32_t (&w)[4]) {

@@ -72,7 +72,7 @@ __device__ __forceinline__ WindowItem window_item(const WindowKernel &p, int i) 
 template <typename T, int NB>
 __global__ void __launch_bounds__(WF_THREADS, 1) window_tiles(const __grid_constant__ WindowKernel p) {
     extern __shared__ unsigned char raw[];
-    __shared__ __align__(8) uint64_t bars[2 * 8 + 2 + 10];
+    __shared__ __align__(8) uint64_t bars[2 * 8 + 2 + 11];
     __shared__ uint32_t tmem_s;
     __shared__ int gave_up_s;
     const WindowArgs &a = p.a;
@@ -93,6 +93,7 @@ __global__ void __launch_bounds__(WF_THREADS, 1) window_tiles(const __grid_const
             tc::mbar_init(tc::smem_u32(&bars[24 + t]), 128);    // O read
             tc::mbar_init(tc::smem_u32(&bars[26 + t]), 128);    // weights of the other 64 written
         }
+        tc::mbar_init(tc::smem_u32(&bars[28]), 1);              // no products in flight
         tc::fence_mbar_init();
         gave_up_s = 0;
     }
@@ -184,6 +185,7 @@ __global__ void __launch_bounds__(WF_THREADS, 1) window_tiles(const __grid_const
             }
             x += 2 * w.keys;
         }
+        wait.drain_products(tc::smem_u32(&bars[28]));
     } else {
         // ---- weights: thread r of a query tile has its row r ----
         const int t = warp >> 2, r = tid & 127, wq = warp & 3;
@@ -485,7 +487,7 @@ __device__ __forceinline__ bool cut_walk(const GradKernel &p, int slot, int k, C
 template <typename T, int NB>
 __global__ void __launch_bounds__(WG_THREADS, 1) window_grad_keys(const __grid_constant__ GradKernel p) {
     extern __shared__ unsigned char raw[];
-    __shared__ __align__(8) uint64_t bars[2 * 4 + 6];
+    __shared__ __align__(8) uint64_t bars[2 * 4 + 7];
     __shared__ uint32_t tmem_s;
     __shared__ int gave_up_s;
     __shared__ __align__(16) float lse_s[2][SEQ_TILE], delta_s[2][SEQ_TILE];
@@ -518,6 +520,7 @@ __global__ void __launch_bounds__(WG_THREADS, 1) window_grad_keys(const __grid_c
         for (int i = 0; i < 12; i++) tc::mbar_init(tc::smem_u32(&bars[i]), 1);    // landed, free (by stage); keys landed, S ready, dP ready, all done
         tc::mbar_init(tc::smem_u32(&bars[12]), 256);                              // P written
         tc::mbar_init(tc::smem_u32(&bars[13]), 256);                              // dS written
+        tc::mbar_init(tc::smem_u32(&bars[14]), 1);                                // no products in flight
         tc::fence_mbar_init();
         gave_up_s = 0;
     }
@@ -588,6 +591,7 @@ __global__ void __launch_bounds__(WG_THREADS, 1) window_grad_keys(const __grid_c
                 }
             }
         }
+        wait.drain_products(tc::smem_u32(&bars[14]));
     } else {
         // threads r and r + 128 have key row r, half of the queries each
         const int r = tid & 127, half = tid >> 7, j = key + r;
@@ -751,7 +755,7 @@ __global__ void __launch_bounds__(256) window_grad_sinks(const __grid_constant__
 template <typename T, int NB>
 __global__ void __launch_bounds__(WG_THREADS, 1) window_grad_queries(const __grid_constant__ GradKernel p) {
     extern __shared__ unsigned char raw[];
-    __shared__ __align__(8) uint64_t bars[2 * 8 + 6];
+    __shared__ __align__(8) uint64_t bars[2 * 8 + 7];
     __shared__ uint32_t tmem_s;
     __shared__ int gave_up_s;
     const WindowArgs &a = p.a;
@@ -769,6 +773,7 @@ __global__ void __launch_bounds__(WG_THREADS, 1) window_grad_queries(const __gri
     if (tid == 0) {
         for (int i = 0; i < 21; i++) tc::mbar_init(tc::smem_u32(&bars[i]), 1);    // slot landed, free; queries landed, S ready (two), dP ready, all done
         tc::mbar_init(tc::smem_u32(&bars[21]), 256);                              // dS written
+        tc::mbar_init(tc::smem_u32(&bars[22]), 1);                                // no products in flight
         tc::fence_mbar_init();
         gave_up_s = 0;
     }
@@ -835,6 +840,7 @@ __global__ void __launch_bounds__(WG_THREADS, 1) window_grad_queries(const __gri
             }
             if (n + 2 < tiles) scores(n + 2);
         }
+        wait.drain_products(tc::smem_u32(&bars[22]));
     } else {
         const int r = tid & 127, half = tid >> 7, i = start + r, i0 = start + 32 * (warp & 3);
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
