@@ -19,7 +19,11 @@ __device__ __forceinline__ T *row_of(const f3m_rows &r, int64_t t, int h) { retu
 // What bounds it: 128 x 128 exponentials a tile at 16 a clock and SM take 1024 clocks, its two products at width 128 as many.  A quarter of the
 // exponentials goes to the FMA pipe (an eighth: 522 us, half: 544), and the values' product begins at the first half of the weights; what is
 // left is a tile's chain -- scores 1250 clocks, maximum 370, exponentials 1300 -- of which two run side by side.  16384 tokens, 16 heads on 4, width 128,
-// window 4096: 514-525 us, 0.92-0.94 PFLOP/s, 57 % of measured; tensor pipe 49 % busy, issue slots 44 %.
+// window 4096: 505-535 us from box to box, 0.90-0.95 PFLOP/s, 56 % of measured; tensor pipe 49 % busy, issue slots 44 %.
+//
+// Here and in the other kernels one thread issues a block's products, and a product that overwrites scores follows the one that reads its weights
+// from their columns with no wait between.  PTX promises the order of products of one accumulator and shape; that others too run one behind the other is
+// relied on, and what repeated calls' equal bits are tested for.
 constexpr int WF_COPY = 8, WF_PRODUCTS = 9, WF_THREADS = 320, WF_BLOCK = SEQ_TILE * 128;
 constexpr float NO_SUM = 0x1p60f;  // no sum of 2^31 weights comes near: some exponent was not a number (exp2_poly)
 constexpr int WF_BLOCKS = 14;      // blocks of 64 columns: two query tiles, a ring of key and value tiles, two to stage outputs
@@ -203,7 +207,7 @@ __global__ void __launch_bounds__(WF_THREADS, 1) window_tiles(const __grid_const
                     __syncwarp();
                     tc::fence_after_sync();
                     // a row sees the keys j <= i of the window, i - j < window, and the sinks; most tiles are seen whole.  S is read twice,
-                    // for the maximum and for the weights: 128 scores and their weights do not fit in the registers beside the rest.
+                    // for the maximum and for the weights, 32 columns at a time (146 registers); 128 scores held between the two were not tried.
                     const bool whole = key + SEQ_TILE - 1 <= i0 && (i0 + 31 - key < a.window || key + SEQ_TILE <= a.sinks);
                     const int up = i - key, low = i - key - a.window, sink = a.sinks - key;   // seen: c <= up and (c > low or c < sink)
                     float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -360,7 +364,7 @@ static void forward_t(const WindowArgs &a, cudaStream_t s) {
 // holds a tile of queries.  S and dP are computed in both, seven products where five would do, but nothing is added across CTAs: sums have one order.
 // P and dS are rounded to 16 bits where they become operands, and go through tensor memory over the scores they come from.
 // What bounds it: a tile pair's weights and dS, some 3300 clocks for 256 threads; its products take 2048 (four) and 1536 (three).  2 x 4096 tokens, 8 heads,
-// width 128, window 2048, forward and gradients: 310 us, 0.57 PFLOP/s by the formula's products, 0.74 by those computed; tensor pipe 53 % busy.
+// width 128, window 2048, forward and gradients: 305-320 us, 0.55 PFLOP/s by the formula's products, 0.72 by those computed; tensor pipe 53 % busy.
 
 // fp16 ends at 2^-24, and dS is far smaller than dout: it would lose its bits where dout still has them (dout of 1e-4: dq and dk were 3 % off).  There P is
 // taken times 2^15 and dS times 2^k, k from the largest |dout_i| and |v_j| of the sequence and the heads that share v: |dP - delta| <= 2 |dout_i| max |v_j|, as out_i
@@ -1011,7 +1015,8 @@ void window_backward(int type, const WindowArgs &a, cudaStream_t s) { type == F3
 // fragments come straight from global memory: a contraction does not mind the order of its terms, so lane (g, t) of a warp reads 16 bytes of
 // key g, columns 32 s + 8 t .. + 7, and uses them as its terms of two steps; of the values it reads 16 bytes of keys 2t, 2t + 1, 2t + 8, 2t + 9,
 // columns 64 f + 8 g .. + 7, and output column n of tile j stands for column 64 f + 8 n + j.  Parts are joined by step_join.
-// 32 sequences of up to 16384 tokens, 32 heads on 8, width 128, window 4096: 96 us, 4.7 TB/s, 72 % of the measured copy.
+// 32 sequences of up to 16384 tokens, 32 heads on 8, width 128, window 4096: 97-99 us, 4.6 TB/s, 70 % of the measured copy.
+// At width 128 three CTAs an SM leave 168 registers a thread, of which 116 bytes are spilled (100 read back): loads of the next keys have no place beside these.
 constexpr int ST_THREADS = 128, ST_HEADS = 16;
 
 template <typename T>
