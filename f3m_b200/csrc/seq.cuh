@@ -161,7 +161,7 @@ struct Waits {
     // by the warp that issues the block's products, behind the last of them: where the block has given up, nobody else may have waited for those in flight, and the
     // tensor memory that they write is about to be another block's
     __device__ __forceinline__ void drain_products(uint32_t bar) const {
-        if (tc::elect()) {
+        if (__any_sync(0xffffffffu, *gave_up) && tc::elect()) {
             tc::mma_commit(bar);
             drain(bar, 0);
         }

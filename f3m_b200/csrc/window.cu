@@ -413,26 +413,32 @@ __global__ void __launch_bounds__(256) window_rows_sum(const __grid_constant__ W
         const uint32_t b = __float_as_uint(s);
         if (b < 0x7f800000u) top = max(top, b);
     };
+    auto row = [&](int x0) {   // of 16 threads
+        const int x = x0 + (threadIdx.x >> 4), h = hk * group + x % group;
+        const int64_t t = t0 + x / group;
+        const bool in = x < rows && c < a.width;
+        const uint4 o = read(a.out, t, h, in), g = read(a.dout, t, h, in);
+        const float s = sum16(dot(o, g));
+        if constexpr (WG_P_EXP<T> != 0) larger(most[0], sum16(dot(g, g)));
+        if (in && c == 0) {
+            const int64_t at = h * a.s.tokens + t;
+            delta[at] = s;
+            lse2[at] = 1.4426950408889634f * a.lse[at] - WG_P_EXP<T>;
+        }
+    };
 #pragma unroll 1
     for (int x0 = 64 * blockIdx.y; x0 < rows; x0 += 64 * gridDim.y) {
+        if (x0 + 64 <= rows) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int x = x0 + 16 * i + (threadIdx.x >> 4), h = hk * group + x % group;
-            const int64_t t = t0 + x / group;
-            const bool in = x < rows && c < a.width;
-            const uint4 o = read(a.out, t, h, in), g = read(a.dout, t, h, in);
-            const float s = sum16(dot(o, g));
-            if constexpr (WG_P_EXP<T> != 0) larger(most[0], sum16(dot(g, g)));
-            if (in && c == 0) {
-                const int64_t at = h * a.s.tokens + t;
-                delta[at] = s;
-                lse2[at] = 1.4426950408889634f * a.lse[at] - WG_P_EXP<T>;
-            }
+            for (int i = 0; i < 4; i++) row(x0 + 16 * i);
+        } else {
+#pragma unroll 1
+            for (int x = x0; x < rows; x += 16) row(x);
         }
     }
     if constexpr (WG_P_EXP<T> != 0) {
-        for (int i = 0; i < 4 && blockIdx.y < 2; i++) {
-            const int x = 64 * blockIdx.y + 16 * i + (threadIdx.x >> 4);
+        for (int x0 = 64 * blockIdx.y; x0 < min(m, 64 * ((int)blockIdx.y + 1)); x0 += 16) {
+            const int x = x0 + (threadIdx.x >> 4);
             const uint4 v = read(a.v, t0 + x, hk, x < m && c < a.width);
             larger(most[1], sum16(dot(v, v)));
         }
@@ -937,7 +943,7 @@ __global__ void __launch_bounds__(WG_THREADS, 1) window_grad_queries(const __gri
 // Where walks over sinks are cut (CutWalk).  A part is no shorter than the walk of another tile, than 24 tiles of queries, than a sixteenth of the
 // longest walk, and than an SM's share of all walks over sinks, halved: where these fill the SMs by themselves they are not cut, and the parts' sums never take
 // more than 4 x 148 slots, 78 MB at width 128.  5 packed documents of up to 3000 tokens, window 512, spent 272 us on one walk of 96 tiles, and 68 us' worth of work.
-// One of 16384 tokens and 2000 of 64, 32 heads on 8, width 128, window 128, 4 sinks, gradients: 5460 us, 5250 without sinks; with the longest walk's number of
+// One of 16384 tokens and 2000 of 64, 32 heads on 8, width 128, window 128, 4 sinks, gradients: 5350 us, some 200 less without sinks; with the longest walk's number of
 // parts for every sequence 11000 us and 33.6 GB.
 struct GradCuts {
     int unit, sink_tiles;
@@ -980,7 +986,8 @@ static void backward_t(const WindowArgs &a, cudaStream_t s) {
     const int64_t parts = cuts.slots * cuts.sink_tiles * a.kv_heads;
     F3M_REQUIRE(a.s.tiles * (int64_t)a.kv_heads + parts <= 0x7fffffff, F3M_ERR_OVERFLOW, "%d tiles of %d heads do not fit in 31 bits", a.s.tiles, a.heads);
     if (WG_P_EXP<T>) F3M_CUDA(cudaMemsetAsync(range, 0, range_floats(a.s, a.kv_heads) * sizeof(float), s));
-    window_rows_sum<T><<<dim3(a.s.tiles * a.kv_heads, std::min(2 * (a.heads / a.kv_heads), 65535)), 256, 0, s>>>(a, lse2, a.delta, reinterpret_cast<uint32_t *>(range));
+    const int most_rows = std::min(a.s.longest, SEQ_TILE) * (a.heads / a.kv_heads);
+    window_rows_sum<T><<<dim3(a.s.tiles * a.kv_heads, std::min((most_rows + 63) / 64, 65535)), 256, 0, s>>>(a, lse2, a.delta, reinterpret_cast<uint32_t *>(range));
     F3M_LAUNCH_CHECK();
     p.mq = seq_tensor_map(type, a.q, n, a.heads, a.width);
     p.mk = seq_tensor_map(type, a.k, n, a.kv_heads, a.width);
