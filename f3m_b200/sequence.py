@@ -266,7 +266,7 @@ class _WindowAttention(torch.autograd.Function):
 
 def window_attention_step(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, lengths: torch.Tensor, window: int, sinks: int = 0,
                           scale: Optional[float] = None) -> torch.Tensor:
-    """One new token for each of n sequences.  q (n, heads, width); k_cache, v_cache (n, capacity, kv_heads, width) hold the tokens so far,
+    """One new token for each of n sequences, 65535 at most.  q (n, heads, width); k_cache, v_cache (n, capacity, kv_heads, width) hold the tokens so far,
     the new one at lengths - 1 among them; lengths (n) int32 on the device, taken as 0..capacity.  Returns out like q; a sequence of length
     0 gets zeros."""
     _refuse_tangents(q, k_cache, v_cache)

@@ -351,7 +351,7 @@ int f3m_window_attention_grad(const f3m_seqs *seqs, int32_t type, int32_t heads,
                               int32_t sinks, float scale, f3m_rows q, f3m_rows k, f3m_rows v, f3m_rows out, const float *lse,
                               f3m_rows dout, f3m_rows dq, f3m_rows dk, f3m_rows dv, void *workspace, size_t workspace_bytes,
                               void *stream);
-/* One new token for each of n sequences against its cache: q, out (n, heads, width); k_cache, v_cache (n, capacity, kv_heads, width),
+/* One new token for each of n sequences, 65535 at most, against its cache: q, out (n, heads, width); k_cache, v_cache (n, capacity, kv_heads, width),
  * element (b, t, h, c) at data[b * seq_stride + t * token_stride + h * head_stride + c].  lengths (DEVICE, n): tokens in
  * the cache, the new one, at length - 1, among them; values outside 0..capacity are taken as the nearest of these.  Length 0: a row of zeros. */
 size_t f3m_window_attention_step_workspace_bytes(int32_t n, int32_t heads, int32_t kv_heads, int32_t width, int64_t capacity,

@@ -364,3 +364,79 @@ def test_prompts_and_gradients_behind_two_billion_elements(dtype, cuda):
     got = sq.decay_attention_grad(plan, q, q, do, ld, do, state)
     for x, y in zip(got[:3], sq.decay_attention_grad(alone, t[0], t[0], t[3], ld, t[3], state[1:])[:3]):
         ref.assert_within(x[-last:], (y.double(), 2 * u * y.double().abs() + 4 * u * y.double().abs().max()))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("width", [128, 72])
+def test_outputs_between_other_data(width, dtype, cuda):
+    """The C entries write rows that lie between others, heads before tokens or behind them, and nothing else: the bits of dense outputs.  States that are not
+    asked for are not needed."""
+    from f3m_b200 import _lib, sequence as sq
+    from f3m_b200._lib import Rows, check
+    L, kind, lengths, h, hk, w = _lib.lib(), {torch.bfloat16: 1, torch.float16: 2}[dtype], [300, 0, 131, 1], 4, 2, width
+    n, scale, stream = sum(lengths), width ** -0.5, torch.cuda.current_stream().cuda_stream
+    plan, ld = sq.SequencePlan(lengths), torch.tensor([-0.1, -0.01, 0.0, -2.0], device="cuda")
+    q, do = normal(1, n, h, w, dtype=dtype), normal(2, n, h, w, dtype=dtype)
+    k, v = normal(3, n, h, w, dtype=dtype), normal(4, n, h, w, dtype=dtype)
+    k2, v2 = k[:, :hk], v[:, :hk]
+    lens, state0 = torch.tensor([200, 17, 0], dtype=torch.int32, device="cuda"), normal(5, 3, h, w, w, dtype=torch.float32)
+    cache = normal(6, 3, 256, hk, w, dtype=dtype)
+    rows = lambda t: Rows(t.data_ptr(), t.stride(0), t.stride(1))  # noqa: E731
+    held = []
+
+    def place(tokens, heads, order):
+        """(tokens, heads, w) rows inside a larger array of sevens"""
+        if order:
+            a = torch.full((heads + 1, tokens + 3, w + 24), 7.0, device="cuda", dtype=dtype)
+            x = a[:heads, 2:2 + tokens, 8:8 + w].transpose(0, 1)
+        else:
+            a = torch.full((tokens + 2, 3, heads, w + 8), 7.0, device="cuda", dtype=dtype)
+            x = a[1:1 + tokens, 1, :, :w]
+        held.append((a, x))
+        return x
+
+    def work(n):
+        return torch.empty(max(n, 16), device="cuda", dtype=torch.uint8)
+
+    out, lse = sq.window_attention(plan, q, k2, v2, 100, 3)
+    grads = sq.window_attention_grad(plan, q, k2, v2, out, lse, do, 100, 3)
+    dec, final = sq.decay_attention(plan, q, k, v, ld)
+    step = sq.window_attention_step(q[:3], cache, cache, lens, 150, 2)
+    state = state0.clone()
+    dstep = sq.decay_attention_step(q[:3], k[:3], v[:3], ld, state)
+    for order in (False, True):
+        held.clear()
+        x, l2 = place(n, h, order), torch.empty_like(lse)
+        check(L.f3m_window_attention(plan._ref, kind, h, hk, w, 100, 3, scale, rows(q), rows(k2), rows(v2), rows(x), l2.data_ptr(), stream), "")
+        assert torch.equal(x, out) and torch.equal(l2, lse)
+        d = [place(n, g, order) for g in (h, hk, hk)]
+        need = L.f3m_window_attention_grad_workspace_bytes(plan._ref, h, hk, w, 100, 3)
+        ws = work(need)
+        check(L.f3m_window_attention_grad(plan._ref, kind, h, hk, w, 100, 3, scale, rows(q), rows(k2), rows(v2), rows(x), l2.data_ptr(), rows(do), *map(rows, d),
+                                          ws.data_ptr(), need, stream), "")
+        assert all(torch.equal(a, b) for a, b in zip(d, grads))
+        x, need = place(n, h, order), L.f3m_decay_attention_workspace_bytes(plan._ref, h, w, w)
+        ws, f = work(need), torch.empty_like(final)
+        check(L.f3m_decay_attention(plan._ref, kind, h, w, w, ld.data_ptr(), scale, rows(q), rows(k), rows(v), None, rows(x), f.data_ptr(), ws.data_ptr(), need, stream), "")
+        assert torch.equal(x, dec) and torch.equal(f, final)
+        # without the last state it is carried in two parts, and out may round otherwise
+        x = place(n, h, order)
+        check(L.f3m_decay_attention(plan._ref, kind, h, w, w, ld.data_ptr(), scale, rows(q), rows(k), rows(v), None, rows(x), None, ws.data_ptr(), need, stream), "")
+        want = ref.decay(q, k, v, ld.tolist(), lengths, dout=do)
+        ref.assert_within(x, want["out"])
+        d = [place(n, h, order) for _ in range(3)]
+        check(L.f3m_decay_attention_grad(plan._ref, kind, h, w, w, ld.data_ptr(), scale, rows(q), rows(k), rows(v), None, rows(do), None, *map(rows, d), None,
+                                         ws.data_ptr(), need, stream), "")
+        for name, a in zip(("dq", "dk", "dv"), d):
+            ref.assert_within(a, want[name], name)
+        x, need = place(3, h, order), L.f3m_window_attention_step_workspace_bytes(3, h, hk, w, 256, 150, 2)
+        ws = work(need)
+        check(L.f3m_window_attention_step(3, kind, h, hk, w, 256, 150, 2, scale, rows(q), rows(cache[0]), cache.stride(0), rows(cache[0]), cache.stride(0), lens.data_ptr(),
+                                          rows(x), ws.data_ptr(), need, stream), "")
+        assert torch.equal(x, step)
+        x, s = place(3, h, order), state0.clone()
+        check(L.f3m_decay_attention_step(3, kind, h, w, w, ld.data_ptr(), scale, rows(q), rows(k), rows(v), s.data_ptr(), rows(x), stream), "")
+        assert torch.equal(x, dstep) and torch.equal(s, state)
+        for a, x in held:
+            x.fill_(7.0)
+            assert bool((a == 7.0).all())

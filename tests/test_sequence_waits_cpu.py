@@ -1,4 +1,4 @@
-"""The roles of decay_tiles (csrc/decay.cu) as a model: which of them waits for which, tile by tile, in every order that their speeds allow.
+"""The roles of the kernels in csrc/decay.cu and csrc/window.cu as models: which of them waits for which, tile by tile, in every order that their speeds allow.
 
 A wait names a phase's parity only, so a barrier must not complete phase n + 1 while a role may still be waiting for phase n: the role
 would find the parity of n again and wait until its limit.  The model's steps are those of the kernel, in its order; the tensor
@@ -72,9 +72,162 @@ def roles(tiles, stages, weights_barriers):
     return copy, products, rows, operands
 
 
-def faults(tiles, stages, weights_barriers):
-    """The barriers that some order of the steps leaves a phase ahead of a role that waits for them; 'stuck' where no role can go on."""
-    progs = roles(tiles, stages, weights_barriers)
+class Role(list):
+    def wait(self, name, phase):
+        self.append(("wait", name, phase, None))
+
+    def arrive(self, name):
+        self.append(("arrive", name, None, None))
+
+    def commit(self, name):
+        self.append(("commit", name, None, None))
+
+
+def states_roles(tiles, stages):
+    copy, products, operands = Role(), Role(), Role()
+    for n in range(tiles):
+        if n >= stages:
+            copy.wait(f"free{n % stages}", n // stages - 1)
+        copy.arrive(f"full{n % stages}")
+        products.wait(f"full{n % stages}", n // stages)
+        products.wait("split", n)
+        products.commit("tails")
+        products.commit(f"free{n % stages}")
+        operands.wait(f"full{n % stages}", n // stages)
+        if n:
+            operands.wait("tails", n - 1)
+        operands.arrive("split")
+    products.commit("done")
+    operands.wait("done", 0)
+    return copy, products, operands
+
+
+def grad_keys_roles(tiles, stages, ends):
+    """ends: the tiles that hold the end of a sequence, whose rows behind it the weights' warps clear"""
+    copy, products, rows = Role(), Role(), Role()
+    copy.arrive("keys")
+    products.wait("keys", 0)
+    products.wait("full0", 0)
+    products.commit("s")
+    products.commit("dp")
+    for n in range(tiles):
+        if n >= stages:
+            copy.wait(f"free{n % stages}", n // stages - 1)
+        copy.arrive(f"full{n % stages}")
+        more = n + 1 < tiles
+        if more:
+            products.wait(f"full{(n + 1) % stages}", (n + 1) // stages)
+        products.wait("p", n)
+        if more:
+            products.commit("s")
+        products.wait("ds", n)
+        products.commit(f"free{n % stages}")
+        products.commit("dp" if more else "done")
+        if n in ends:
+            rows.wait(f"full{n % stages}", n // stages)
+            rows.wait("s", n)
+            rows.wait("dp", n)
+        rows.wait("s", n)
+        rows.arrive("p")
+        rows.wait("dp", n)
+        rows.arrive("ds")
+    rows.wait("done", 0)
+    return copy, products, rows
+
+
+def grad_queries_roles(tiles, slots):
+    copy, products, rows = Role(), Role(), Role()
+    copy.arrive("q")
+    for x in range(2 * tiles):
+        if x >= slots:
+            copy.wait(f"free{x % slots}", x // slots - 1)
+        copy.arrive(f"full{x % slots}")
+
+    def scores(n):
+        products.wait(f"full{2 * n % slots}", 2 * n // slots)
+        products.commit(f"s{n % 2}")
+
+    def values(n):
+        x = 2 * n + 1
+        products.wait(f"full{x % slots}", x // slots)
+        products.commit("dp")
+        products.commit(f"free{x % slots}")
+
+    products.wait("q", 0)
+    scores(0)
+    values(0)
+    if tiles > 1:
+        scores(1)
+    for n in range(tiles):
+        products.wait("ds", n)
+        if n + 1 < tiles:
+            values(n + 1)
+        products.commit(f"free{2 * n % slots}")
+        if n + 1 == tiles:
+            products.commit("done")
+        if n + 2 < tiles:
+            scores(n + 2)
+        rows.wait(f"s{n % 2}", n // 2)
+        if n + 1 == tiles:      # the end of the sequence
+            rows.wait(f"full{2 * n % slots}", 2 * n // slots)
+        rows.wait("dp", n)
+        rows.arrive("ds")
+    rows.wait("done", 0)
+    return copy, products, rows
+
+
+def window_roles(items, slots):
+    """items: (tiles of keys, query tiles) of each"""
+    copy, products, rows = Role(), Role(), (Role(), Role())
+    x, done, scored, out = 0, [0, 0], [0, 0], [0, 0]
+    for i, (keys, queries) in enumerate(items):
+        if i:
+            copy.wait("q_free", i - 1)
+        copy.arrive("q")
+        for y in range(x, x + 2 * keys):
+            if y >= slots:
+                copy.wait(f"free{y % slots}", y // slots - 1)
+            copy.arrive(f"full{y % slots}")
+        products.wait("q", i)
+        products.wait(f"full{x % slots}", x // slots)
+        for t in range(queries):
+            products.commit(f"s{t}")
+        products.commit(f"free{x % slots}")
+        if keys == 1:
+            products.commit("q_free")
+        for j in range(keys):
+            v, more = x + 2 * j + 1, j + 1 < keys
+            products.wait(f"full{v % slots}", v // slots)
+            if more:
+                products.wait(f"full{(v + 1) % slots}", (v + 1) // slots)
+            for t in range(queries):
+                if j == 0 and done[t]:
+                    products.wait(f"o_read{t}", done[t] - 1)
+                products.wait(f"p{t}", scored[t])
+                products.wait(f"p2{t}", scored[t])
+                done[t] += not more
+                products.commit(f"s{t}" if more else f"o{t}")
+                rows[t].wait(f"s{t}", scored[t])
+                if t == 0 and not more:
+                    rows[t].wait(f"full{v % slots}", v // slots)
+                rows[t].arrive(f"p{t}")
+                rows[t].arrive(f"p2{t}")
+                scored[t] += 1
+            products.commit(f"free{v % slots}")
+            if more:
+                products.commit(f"free{(v + 1) % slots}")
+            if j + 2 == keys:
+                products.commit("q_free")
+        for t in range(queries):
+            rows[t].wait(f"o{t}", out[t])
+            rows[t].arrive(f"o_read{t}")
+            out[t] += 1
+        x += 2 * keys
+    return copy, products, *rows
+
+
+def faults(progs):
+    """The barriers that some order of the steps leaves a phase ahead of a role that waits for them, or a phase behind; 'stuck' where no role can go on."""
     names = sorted({s[1] for p in progs for s in p})
     at = {n: i for i, n in enumerate(names)}
     start = ((0,) * len(progs), (False,) * len(progs), (0,) * len(names), ())
@@ -96,7 +249,7 @@ def faults(tiles, stages, weights_barriers):
             if need is not None and need != flags[r]:
                 after.append((on, flags, done, queue))
             elif kind == "wait":
-                if done[i] > phase + 1:
+                if done[i] > phase + 1 or done[i] < phase:      # the parity of another phase
                     found.add(name)
                 if done[i] == phase + 1:
                     after.append((on, flags, done, queue))
@@ -117,12 +270,20 @@ def faults(tiles, stages, weights_barriers):
 
 @pytest.mark.parametrize("tiles,stages", [(1, 2), (5, 2), (5, 3), (6, 4)])
 def test_no_barrier_of_decay_tiles_runs_ahead_of_a_role_that_waits(tiles, stages):
-    assert faults(tiles, stages, 2) == set()
+    assert faults(roles(tiles, stages, 2)) == set()
+
+
+@pytest.mark.parametrize("progs", [states_roles(6, 2), states_roles(7, 4), grad_keys_roles(1, 2, {0}), grad_keys_roles(5, 2, {2, 4}), grad_keys_roles(7, 4, {3, 6}),
+                                   grad_queries_roles(1, 5), grad_queries_roles(4, 5), grad_queries_roles(6, 8), window_roles([(1, 2), (2, 2), (1, 1), (3, 2)], 4),
+                                   window_roles([(2, 1), (1, 2), (3, 2)], 8)],
+                         ids=["states-2", "states-4", "keys-1", "keys-2", "keys-4", "queries-1", "queries-5", "queries-8", "window-4", "window-8"])
+def test_no_barrier_of_the_other_kernels_does(progs):
+    assert faults(progs) == set()
 
 
 def test_the_model_sees_one_barrier_for_all_weights_run_ahead():
     """The weights of tile n + 1 need no step of the products behind A S of tile n: one barrier for all tiles would not do."""
-    assert faults(4, 2, 1) >= {"weights0", "stuck"}
+    assert faults(roles(4, 2, 1)) >= {"weights0", "stuck"}
 
 
 def test_the_kernel_has_the_barriers_of_the_model():
