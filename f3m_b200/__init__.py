@@ -5,6 +5,6 @@ from . import _lib
 _lib.lib()   # no fallback: a missing library is an import error
 
 from .FFM_classes import FFM, benchmark_matmul, benchmark_matmul_double, block_FFM_matmul, par_FFM_block  # noqa: E402
-from . import engine, sequence  # noqa: E402
+from . import engine, paged, sequence  # noqa: E402
 
-__all__ = ["FFM", "benchmark_matmul", "benchmark_matmul_double", "block_FFM_matmul", "par_FFM_block", "engine", "sequence"]
+__all__ = ["FFM", "benchmark_matmul", "benchmark_matmul_double", "block_FFM_matmul", "par_FFM_block", "engine", "paged", "sequence"]

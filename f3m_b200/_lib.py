@@ -16,8 +16,10 @@ MATH_FASTMATH = 0
 MATH_IEEE = 1
 FLAG_NEAR_MOMENTS = 1
 FLAG_NEAR_TENSOR_CORES = 2
-TYPE_BF16, TYPE_F16 = 1, 2
+TYPE_BF16, TYPE_F16, TYPE_F32 = 1, 2, 3
 MAX_WIDTH = 128
+MAX_CHANNELS = 0x100000
+TREE_MAX = 256
 
 # array ids of f3m_plan_copy_array
 ARR_SORTED_INDEX, ARR_BOX_OFFSETS, ARR_BOX_CENTERS = 0, 1, 2
@@ -55,6 +57,19 @@ class Rows(C.Structure):
 class Seqs(C.Structure):
     _fields_ = [("table", C.c_void_p), ("tokens", C.c_int64), ("sequences", C.c_int32), ("empty", C.c_int32), ("tiles", C.c_int32), ("pairs", C.c_int32),
                 ("longest", C.c_int32), ("table_words", C.c_int32)]
+
+
+class Pages(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("page_stride", C.c_int64), ("token_stride", C.c_int64), ("head_stride", C.c_int64)]
+
+
+class Cache(C.Structure):
+    _fields_ = [("k", Pages), ("v", Pages), ("pages", C.c_int32), ("page_tokens", C.c_int32), ("kv_heads", C.c_int32), ("width", C.c_int32),
+                ("table", C.c_void_p), ("table_stride", C.c_int64), ("table_pages", C.c_int32), ("sequences", C.c_int32), ("lengths", C.c_void_p)]
+
+
+class RotationTable(C.Structure):
+    _fields_ = [("turns", C.c_void_p), ("columns", C.c_int32), ("interleaved", C.c_int32)]
 
 
 _P = C.c_void_p
@@ -122,6 +137,14 @@ SIGNATURES = {
     "f3m_decay_attention_grad": (C.c_int, [C.POINTER(Seqs), _I32, _I32, _I32, _I32, _P, _F32, Rows, Rows, Rows, _P, Rows, _P, Rows, Rows,
                                            Rows, _P, _P, C.c_size_t, _P]),
     "f3m_decay_attention_step": (C.c_int, [_I32, _I32, _I32, _I32, _I32, _P, _F32, Rows, Rows, Rows, _P, Rows, _P]),
+    "f3m_gated_recurrence_workspace_bytes": (C.c_size_t, [C.POINTER(Seqs), _I32]),
+    "f3m_gated_recurrence": (C.c_int, [C.POINTER(Seqs), _I32, _I32, Rows, Rows, _P, Rows, _P, _P, C.c_size_t, _P]),
+    "f3m_gated_recurrence_grad": (C.c_int, [C.POINTER(Seqs), _I32, _I32, Rows, Rows, Rows, _P, _P, Rows, Rows, _P, _P, C.c_size_t, _P]),
+    "f3m_gated_recurrence_step": (C.c_int, [_I32, _I32, _I32, Rows, Rows, _P, Rows, _P]),
+    "f3m_paged_append": (C.c_int, [C.POINTER(Seqs), _I32, C.POINTER(Cache), Rows, Rows, _P, C.POINTER(RotationTable), _I32, Rows, Rows, _P]),
+    "f3m_paged_attention_workspace_bytes": (C.c_size_t, [C.POINTER(Seqs), C.POINTER(Cache), _I32]),
+    "f3m_paged_attention": (C.c_int, [C.POINTER(Seqs), _I32, C.POINTER(Cache), _I32, _I32, _I32, _F32, _P, Rows, Rows, _P, C.c_size_t, _P]),
+    "f3m_paged_keep": (C.c_int, [_I32, C.POINTER(Cache), _P, _I64, _I32, _P, _P]),
 }
 
 _lib = None

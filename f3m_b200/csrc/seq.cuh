@@ -119,6 +119,64 @@ void decay_product(int type, const DecayArgs &a, cudaStream_t s);
 void decay_step(int type, int n, int heads, int width_k, int width_v, const float *log_decay, float scale, const f3m_rows &q, const f3m_rows &k,
                 const f3m_rows &v, float *state, const f3m_rows &out, cudaStream_t s);
 
+// h_t = a_t h_(t-1) + x_t and its gradients, by channel
+struct RecurrenceArgs {
+    f3m_seqs s;
+    int channels;
+    f3m_rows x, log_decay, out;
+    const float *state_in;
+    float *state_out;
+    f3m_rows dout, dx, dlog_decay;   // gradients only
+    const float *dstate_out;
+    float *dstate_in;
+    void *ws;
+};
+size_t recurrence_workspace(const f3m_seqs &s, int channels);
+void recurrence_forward(int type, const RecurrenceArgs &a, cudaStream_t s);
+void recurrence_backward(int type, const RecurrenceArgs &a, cudaStream_t s);
+void recurrence_step(int type, int n, int channels, const f3m_rows &x, const f3m_rows &log_decay, float *state, const f3m_rows &out, cudaStream_t s);
+
+struct PagedArgs {
+    f3m_seqs s;
+    f3m_cache c;
+    int heads, window, sinks;
+    float scale;
+    const int *parents;
+    f3m_rows q, out;
+    void *ws;
+};
+size_t paged_workspace(const f3m_seqs &s, const f3m_cache &c, int heads);
+void paged_attention(int type, const PagedArgs &a, cudaStream_t s);
+struct AppendArgs {
+    f3m_seqs s;
+    f3m_cache c;
+    f3m_rows k, v;
+    const int *parents;
+    f3m_rotation rotation;   // no columns: none
+    int heads;
+    f3m_rows q, q_out;
+};
+void paged_append(int type, const AppendArgs &a, cudaStream_t s);
+void paged_keep(const f3m_cache &c, const int *kept, int64_t kept_stride, int most, const int *counts, cudaStream_t s);
+
+// Tokens that a sequence of a paged cache holds before the new ones
+__device__ __forceinline__ int64_t paged_capacity(const f3m_cache &c) { return (int64_t)c.table_pages * c.page_tokens; }
+__device__ __forceinline__ int paged_length(const f3m_cache &c, int b) { return (int)min((int64_t)max(c.lengths[b], 0), paged_capacity(c)); }
+// The page of a sequence's token, -1 where it has none
+__device__ __forceinline__ int paged_page(const f3m_cache &c, int b, int64_t slot) {
+    if (slot >= paged_capacity(c)) return -1;
+    const int page = c.table[b * c.table_stride + slot / c.page_tokens];
+    return page >= 0 && page < c.pages ? page : -1;
+}
+__device__ __forceinline__ int64_t paged_at(const f3m_cache &c, const f3m_pages &p, int page, int64_t slot, int head) {
+    return page * p.page_stride + (slot & (c.page_tokens - 1)) * p.token_stride + head * p.head_stride;
+}
+// The parent of new token i, among `parents` of its sequence
+__device__ __forceinline__ int parent_of(const int *parents, int i) {
+    const int p = parents[i];
+    return p >= 0 && p < i ? p : -1;
+}
+
 // A tensor map of (tokens, heads, width) rows whose boxes are 64 columns x 1 head x 128 tokens, swizzled
 CUtensorMap seq_tensor_map(int type, const f3m_rows &r, int64_t tokens, int heads, int width);
 // The word in mapped host memory where a kernel notes that a wait of its ran out; the next call reports it

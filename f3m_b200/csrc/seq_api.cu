@@ -301,4 +301,167 @@ int f3m_decay_attention_step(int32_t n, int32_t type, int32_t heads, int32_t wid
     });
 }
 
+static void check_channels(int type, int channels) {
+    F3M_REQUIRE(type == F3M_TYPE_BF16 || type == F3M_TYPE_F16 || type == F3M_TYPE_F32, F3M_ERR_UNSUPPORTED, "type %d: only bf16, fp16 and fp32 are built", type);
+    F3M_REQUIRE(channels >= 8 && channels <= F3M_MAX_CHANNELS && channels % 8 == 0, F3M_ERR_UNSUPPORTED, "%d channels: not a multiple of 8 in 8..%d", channels, F3M_MAX_CHANNELS);
+}
+static void check_channel_rows(const f3m_rows &r, int64_t tokens, int type, int channels, bool out, const char *what) {
+    if (tokens == 0) return;
+    F3M_REQUIRE(r.data && (uintptr_t)r.data % 16 == 0, F3M_ERR_ARG, "%s is missing or does not start on 16 bytes", what);
+    F3M_REQUIRE(r.token_stride % (type == F3M_TYPE_F32 ? 4 : 8) == 0 && r.token_stride >= 0 && r.token_stride < ((int64_t)1 << 36), F3M_ERR_ARG,
+                "%s: stride %lld is not a multiple of 16 bytes", what, (long long)r.token_stride);
+    F3M_REQUIRE(!out || tokens == 1 || r.token_stride >= channels, F3M_ERR_ARG, "%s: rows overlap (stride %lld)", what, (long long)r.token_stride);
+}
+
+size_t f3m_gated_recurrence_workspace_bytes(const f3m_seqs *seqs, int32_t channels) {
+    return seqs && seqs->tokens > 0 && channels >= 8 && channels <= F3M_MAX_CHANNELS ? recurrence_workspace(*seqs, channels) : 0;
+}
+
+int f3m_gated_recurrence(const f3m_seqs *seqs, int32_t type, int32_t channels, f3m_rows x, f3m_rows log_decay, const float *state_in, f3m_rows out,
+                         float *state_out, void *workspace, size_t workspace_bytes, void *stream) {
+    return guarded([&] {
+        check_seqs(seqs); check_channels(type, channels);
+        const int64_t n = seqs->tokens;
+        check_channel_rows(x, n, type, channels, false, "x"); check_channel_rows(log_decay, n, type, channels, false, "log_decay");
+        check_channel_rows(out, n, type, channels, true, "out");
+        check_state(state_in, "state_in"); check_state(state_out, "state_out");
+        F3M_REQUIRE(!state_in || state_in != state_out, F3M_ERR_ARG, "state_in and state_out are the same array");
+        if (n) check_workspace(workspace, workspace_bytes, recurrence_workspace(*seqs, channels));
+        if (seqs->sequences == 0) return;
+        seq_check_error();
+        RecurrenceArgs a{};
+        a.s = *seqs; a.channels = channels; a.x = x; a.log_decay = log_decay; a.out = out; a.state_in = state_in; a.state_out = state_out; a.ws = workspace;
+        recurrence_forward(type, a, (cudaStream_t)stream);
+    });
+}
+
+int f3m_gated_recurrence_grad(const f3m_seqs *seqs, int32_t type, int32_t channels, f3m_rows log_decay, f3m_rows out, f3m_rows dout, const float *state_in,
+                              const float *dstate_out, f3m_rows dx, f3m_rows dlog_decay, float *dstate_in, void *workspace, size_t workspace_bytes, void *stream) {
+    return guarded([&] {
+        check_seqs(seqs); check_channels(type, channels);
+        const int64_t n = seqs->tokens;
+        check_channel_rows(log_decay, n, type, channels, false, "log_decay"); check_channel_rows(out, n, type, channels, false, "out");
+        check_channel_rows(dout, n, type, channels, false, "dout"); check_channel_rows(dx, n, type, channels, true, "dx");
+        check_channel_rows(dlog_decay, n, type, channels, true, "dlog_decay");
+        check_state(state_in, "state_in"); check_state(dstate_out, "dstate_out"); check_state(dstate_in, "dstate_in");
+        F3M_REQUIRE(!dstate_out || dstate_out != dstate_in, F3M_ERR_ARG, "dstate_out and dstate_in are the same array");
+        if (n) check_workspace(workspace, workspace_bytes, recurrence_workspace(*seqs, channels));
+        if (seqs->sequences == 0) return;
+        seq_check_error();
+        RecurrenceArgs a{};
+        a.s = *seqs; a.channels = channels; a.log_decay = log_decay; a.out = out; a.dout = dout; a.state_in = state_in; a.dstate_out = dstate_out; a.dx = dx;
+        a.dlog_decay = dlog_decay; a.dstate_in = dstate_in; a.ws = workspace;
+        recurrence_backward(type, a, (cudaStream_t)stream);
+    });
+}
+
+int f3m_gated_recurrence_step(int32_t n, int32_t type, int32_t channels, f3m_rows x, f3m_rows log_decay, float *state, f3m_rows out, void *stream) {
+    return guarded([&] {
+        check_channels(type, channels);
+        F3M_REQUIRE(n >= 0 && (n == 0 || state), F3M_ERR_ARG, "null pointer argument");
+        check_channel_rows(x, n, type, channels, false, "x"); check_channel_rows(log_decay, n, type, channels, false, "log_decay");
+        check_channel_rows(out, n, type, channels, true, "out"); check_state(state, "state");
+        if (n == 0) return;
+        seq_check_error();
+        recurrence_step(type, n, channels, x, log_decay, state, out, (cudaStream_t)stream);
+    });
+}
+
+static void check_pages(const f3m_cache &c, const f3m_pages &p, bool out, const char *what) {
+    if (c.pages == 0) return;
+    const int64_t top = (int64_t)1 << 36;
+    F3M_REQUIRE(p.data && (uintptr_t)p.data % 16 == 0, F3M_ERR_ARG, "%s is missing or does not start on 16 bytes", what);
+    F3M_REQUIRE(p.page_stride % 8 == 0 && p.token_stride % 8 == 0 && p.head_stride % 8 == 0 && p.page_stride >= 0 && p.token_stride >= 0 && p.head_stride >= 0 &&
+                    p.page_stride < top && p.token_stride < top && p.head_stride < top,
+                F3M_ERR_ARG, "%s: strides %lld, %lld, %lld are not multiples of 8 elements", what, (long long)p.page_stride, (long long)p.token_stride, (long long)p.head_stride);
+    if (!out) return;
+    // an element's place is its own: each axis of more than one steps over all that the smaller steps reach
+    struct Axis { int64_t stride, n; } axes[3] = {{p.page_stride, c.pages}, {p.token_stride, c.page_tokens}, {p.head_stride, c.kv_heads}};
+    std::sort(axes, axes + 3, [](const Axis &x, const Axis &y) { return x.stride < y.stride; });
+    int64_t reach = c.width;
+    for (const Axis &x : axes) {
+        if (x.n == 1) continue;
+        F3M_REQUIRE(x.stride >= reach, F3M_ERR_ARG, "%s: rows overlap (strides %lld, %lld, %lld)", what, (long long)p.page_stride, (long long)p.token_stride, (long long)p.head_stride);
+        reach += x.stride * (x.n - 1);
+    }
+}
+static void check_cache(int type, const f3m_cache *c, bool written) {
+    check_type(type);
+    F3M_REQUIRE(c, F3M_ERR_ARG, "null pointer argument");
+    check_width(c->width, "width");
+    F3M_REQUIRE(c->kv_heads >= 1 && c->kv_heads <= 65535, F3M_ERR_ARG, "%d key heads", c->kv_heads);
+    F3M_REQUIRE(c->page_tokens >= 8 && (c->page_tokens & (c->page_tokens - 1)) == 0, F3M_ERR_UNSUPPORTED, "pages of %d tokens: not a power of two from 8 on", c->page_tokens);
+    F3M_REQUIRE(c->pages >= 0 && c->table_pages >= 0 && c->sequences >= 0 && c->table_stride >= 0 && (int64_t)c->table_pages * c->page_tokens <= F3M_SEQ_MAX_TOKENS, F3M_ERR_ARG,
+                "%d pages, %d of a sequence of %d tokens each", c->pages, c->table_pages, c->page_tokens);
+    F3M_REQUIRE(c->sequences == 0 || (c->lengths && (c->table || c->table_pages == 0)), F3M_ERR_ARG, "the cache's lengths or its table are missing");
+    check_pages(*c, c->k, written, "k_pages"); check_pages(*c, c->v, written, "v_pages");
+}
+static void check_new_tokens(const f3m_seqs *seqs, const f3m_cache *c, const int32_t *parents) {
+    check_seqs(seqs);
+    F3M_REQUIRE(seqs->sequences == c->sequences, F3M_ERR_ARG, "new tokens of %d sequences, a cache of %d", seqs->sequences, c->sequences);
+    F3M_REQUIRE(!parents || seqs->longest <= F3M_TREE_MAX, F3M_ERR_UNSUPPORTED, "a tree of %d tokens: at most %d", seqs->longest, F3M_TREE_MAX);
+    // positions stay within 31 bits
+    F3M_REQUIRE((int64_t)c->table_pages * c->page_tokens + seqs->longest <= F3M_SEQ_MAX_TOKENS, F3M_ERR_OVERFLOW, "%lld cached and %d new tokens do not fit in 31 bits",
+                (long long)c->table_pages * c->page_tokens, seqs->longest);
+}
+
+int f3m_paged_append(const f3m_seqs *seqs, int32_t type, const f3m_cache *cache, f3m_rows k, f3m_rows v, const int32_t *parents, const f3m_rotation *rotation,
+                     int32_t heads, f3m_rows q, f3m_rows q_out, void *stream) {
+    return guarded([&] {
+        check_cache(type, cache, true);
+        check_new_tokens(seqs, cache, parents);
+        const int64_t n = seqs->tokens;
+        check_rows(k, n, cache->kv_heads, cache->width, "k"); check_rows(v, n, cache->kv_heads, cache->width, "v");
+        F3M_REQUIRE(heads >= 0 && heads <= 65535, F3M_ERR_ARG, "%d heads", heads);
+        if (heads) {
+            check_rows(q, n, heads, cache->width, "q");
+            check_out(q_out, n, heads, cache->width, "q_out");
+            F3M_REQUIRE(q.data != q_out.data || (q.token_stride == q_out.token_stride && q.head_stride == q_out.head_stride), F3M_ERR_ARG, "q_out is q with other strides");
+        }
+        if (rotation) {
+            F3M_REQUIRE(rotation->columns >= 16 && rotation->columns % 16 == 0 && rotation->columns <= cache->width, F3M_ERR_UNSUPPORTED,
+                        "%d rotated columns: not a multiple of 16 up to the width %d", rotation->columns, cache->width);
+            F3M_REQUIRE(rotation->turns && (uintptr_t)rotation->turns % 8 == 0, F3M_ERR_ARG, "the rotation's table is missing or not 8-byte aligned");
+        }
+        if (n == 0) return;
+        seq_check_error();
+        paged_append(type, AppendArgs{*seqs, *cache, k, v, parents, rotation ? *rotation : f3m_rotation{nullptr, 0, 0}, heads, q, q_out}, (cudaStream_t)stream);
+    });
+}
+
+static bool paged_sizes(const f3m_seqs *seqs, const f3m_cache *c, int32_t heads) {
+    return seqs && c && seqs->tokens > 0 && heads >= 1 && c->kv_heads >= 1 && heads % c->kv_heads == 0 && c->width >= 8 && c->width <= F3M_MAX_WIDTH && c->page_tokens > 0 &&
+           c->table_pages >= 0;
+}
+
+size_t f3m_paged_attention_workspace_bytes(const f3m_seqs *seqs, const f3m_cache *cache, int32_t heads) {
+    return paged_sizes(seqs, cache, heads) ? paged_workspace(*seqs, *cache, heads) : 0;
+}
+
+int f3m_paged_attention(const f3m_seqs *seqs, int32_t type, const f3m_cache *cache, int32_t heads, int32_t window, int32_t sinks, float scale, const int32_t *parents,
+                        f3m_rows q, f3m_rows out, void *workspace, size_t workspace_bytes, void *stream) {
+    return guarded([&] {
+        check_cache(type, cache, false);
+        check_new_tokens(seqs, cache, parents);
+        check_heads(heads, cache->kv_heads); check_window(window, sinks, scale);
+        F3M_REQUIRE(heads / cache->kv_heads <= 128, F3M_ERR_UNSUPPORTED, "%d heads share a key head: at most 128", heads / cache->kv_heads);
+        const int64_t n = seqs->tokens;
+        check_rows(q, n, heads, cache->width, "q"); check_out(out, n, heads, cache->width, "out");
+        if (n == 0) return;
+        check_workspace(workspace, workspace_bytes, paged_workspace(*seqs, *cache, heads));
+        seq_check_error();
+        paged_attention(type, PagedArgs{*seqs, *cache, heads, window, sinks, scale, parents, q, out, workspace}, (cudaStream_t)stream);
+    });
+}
+
+int f3m_paged_keep(int32_t type, const f3m_cache *cache, const int32_t *kept, int64_t kept_stride, int32_t most, const int32_t *counts, void *stream) {
+    return guarded([&] {
+        check_cache(type, cache, true);
+        F3M_REQUIRE(most >= 0 && kept_stride >= 0 && (cache->sequences == 0 || (counts && (kept || most == 0))), F3M_ERR_ARG, "bad argument to f3m_paged_keep");
+        if (cache->sequences == 0 || most == 0 || cache->pages == 0) return;
+        seq_check_error();
+        paged_keep(*cache, kept, kept_stride, most, counts, (cudaStream_t)stream);
+    });
+}
+
 }  // extern "C"

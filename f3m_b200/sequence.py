@@ -1,4 +1,5 @@
-"""Kernel products over sequences: attention over a window with sinks, and linear attention with a decay for each head.
+"""Kernel products over sequences: attention over a window with sinks, linear attention with a decay for each head, and a recurrence with a decay
+by token and channel.
 
 They are the engine's two products on a line of positions: `window_attention` sums every pair that is seen (as `engine.rbf_dense`
 does, rows normalised), `decay_attention` sums near pairs one by one and far ones through moments (as `FFM` does, here exactly).
@@ -13,12 +14,16 @@ Definitions, limits and what is asked of the arrays stand in include/f3m.h.
     dq, dk, dv, dstate = decay_attention_grad(plan, q, k, v, log_decay, dout)
     out = decay_attention_step(q, k, v, log_decay, state)                               # state updated in place
 
+    out, state = gated_recurrence(plan, x, log_decay)                                   # (tokens, channels), bf16, fp16 or fp32
+    dx, dlog_decay, dstate = gated_recurrence_grad(plan, log_decay, out, dout)
+    out = gated_recurrence_step(x, log_decay, state)                                    # state updated in place
+
 Prompts and training take packed arrays (tokens, heads, width), bf16 or fp16; a batch (n, tokens, heads, width) of equal lengths is
 `x.flatten(0, 1)` with `SequencePlan([tokens] * n)`.  Columns have to be contiguous, token and head strides multiples of 8 elements
 and data on 16 bytes -- views of a joint projection are; anything else is copied.  No call waits for the GPU.
 
-`window_attention` and `decay_attention` are differentiable by q, k, v (and the states) when autograd is on.  Autograd's bookkeeping of a
-leaf belongs to the stream that first used it, so a graph that is differentiated by autograd is not captured: the two refuse that, and a
+`window_attention` and `decay_attention` are differentiable by q, k, v (and the states) when autograd is on, `gated_recurrence` by all that it takes.  Autograd's
+bookkeeping of a leaf belongs to the stream that first used it, so a graph that is differentiated by autograd is not captured: they refuse that, and a
 captured training step calls the gradient functions itself.  Forward-mode derivatives are refused.
 """
 from __future__ import annotations
@@ -422,5 +427,142 @@ def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_
     with _On(q.device) as stream:
         st = _lib.lib().f3m_decay_attention_step(n, kind, heads, width, v.shape[2], log_decay.data_ptr(), scale, rq, rk, rv, state.data_ptr(), ro, stream)
     check(st, "f3m_decay_attention_step")
+    torch.autograd.graph.increment_version(state)
+    return out
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# gated recurrence
+# ---------------------------------------------------------------------------------------------------------------------
+_CHANNEL_TYPES = {**_TYPES, torch.float32: _lib.TYPE_F32}
+
+
+def _read_channels(t: torch.Tensor) -> Tuple[torch.Tensor, Rows]:
+    """t (tokens, channels), or a dense copy of it where the library could not read it in place, and the library's view of that."""
+    (ts, cs), (tokens, channels), at = t.stride(), t.shape, t.data_ptr()
+    if tokens == 1:
+        ts = channels
+    if cs != 1 or (at | ts * t.element_size()) & 15 or ts < channels:
+        t = t.contiguous()
+        if t.data_ptr() & 15:
+            t = t.clone()
+        at, ts = t.data_ptr(), channels
+    return t, Rows(at, ts, 0)
+
+
+def _new_channels(t: torch.Tensor) -> Tuple[torch.Tensor, Rows]:
+    y = torch.empty_like(t, memory_format=torch.contiguous_format)
+    return y, Rows(y.data_ptr(), y.shape[1], 0)
+
+
+def _check_channels(x: torch.Tensor, *others: Tuple[str, torch.Tensor]) -> int:
+    if not x.is_cuda:
+        raise ValueError("the engine has no CPU path: x must be a CUDA tensor")
+    if x.dtype not in _CHANNEL_TYPES:
+        raise TypeError(f"{x.dtype}: only torch.bfloat16, torch.float16 and torch.float32 are built")
+    if x.dim() != 2:
+        raise ValueError("arrays are (tokens, channels)")
+    if x.shape[1] < 8 or x.shape[1] > _lib.MAX_CHANNELS or x.shape[1] % 8:
+        raise ValueError(f"{x.shape[1]} channels: not a multiple of 8 in 8..{_lib.MAX_CHANNELS}")
+    for what, t in others:
+        _shape(t, x.shape, what)
+        if t.dtype != x.dtype:
+            raise TypeError(f"arrays of {x.dtype} and {t.dtype} in one call")
+        if t.device != x.device:
+            raise ValueError(f"arrays on {x.device} and {t.device} in one call")
+    return _CHANNEL_TYPES[x.dtype]
+
+
+def _check_channel_state(t, n, x, what):
+    if t is None:
+        return None
+    _shape(t, (n, x.shape[1]), what)
+    if t.dtype != torch.float32 or t.device != x.device:
+        raise TypeError(f"{what} must be a float32 array on the device of x")
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _channel_workspace(plan, x):
+    need = _lib.lib().f3m_gated_recurrence_workspace_bytes(plan._ref, x.shape[1])
+    return need, (torch.empty(need, device=x.device, dtype=torch.uint8) if need else None)
+
+
+def gated_recurrence(plan: SequencePlan, x: torch.Tensor, log_decay: torch.Tensor, state: Optional[torch.Tensor] = None
+                     ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """h_t = a_t h_(t-1) + x_t, a_t = exp(min(log_decay_t, 0)), along every sequence, every channel for itself.  x, log_decay (tokens, channels) of one
+    type; state (sequences, channels) float32 is h before the first token (zeros unless given).  Returns h of every token, like x, and the state behind the
+    last one, as a new float32 array."""
+    _refuse_tangents(x, log_decay, state)
+    if _needs_grad(x, log_decay, state):
+        _refuse_capture("gated_recurrence")
+        return _GatedRecurrence.apply(plan, x, log_decay, state)
+    return _recurrence_forward(plan, x, log_decay, state)
+
+
+def _recurrence_forward(plan, x, log_decay, state):
+    kind = _check_channels(x, ("log_decay", log_decay))
+    _check_plan(plan, x)
+    state = _check_channel_state(state, plan.sequences, x, "state")
+    (x, rx), (log_decay, rl), (out, ro) = _read_channels(x), _read_channels(log_decay), _new_channels(x)
+    final = torch.empty((plan.sequences, x.shape[1]), device=x.device, dtype=torch.float32)
+    need, ws = _channel_workspace(plan, x)
+    with _On(x.device, plan) as stream:
+        st = _lib.lib().f3m_gated_recurrence(plan._ref, kind, x.shape[1], rx, rl, _pointer(state), ro, final.data_ptr(), _pointer(ws), need, stream)
+    check(st, "f3m_gated_recurrence")
+    return out, final
+
+
+def gated_recurrence_grad(plan: SequencePlan, log_decay: torch.Tensor, out: torch.Tensor, dout: torch.Tensor, state: Optional[torch.Tensor] = None,
+                          dfinal: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Gradients (dx, dlog_decay, dstate) of sum(out * dout) + sum(final * dfinal) for (out, final) = gated_recurrence(plan, x, log_decay, state);
+    dfinal is zero unless given.  dlog_decay is 0 where log_decay is above 0."""
+    _refuse_tangents(log_decay, out, dout, state, dfinal)
+    kind = _check_channels(log_decay, ("out", out), ("dout", dout))
+    _check_plan(plan, log_decay)
+    state = _check_channel_state(state, plan.sequences, log_decay, "state")
+    dfinal = _check_channel_state(dfinal, plan.sequences, log_decay, "dfinal")
+    (log_decay, rl), (out, ro), (dout, rg) = _read_channels(log_decay), _read_channels(out), _read_channels(dout)
+    (dx, wx), (dl, wl) = _new_channels(log_decay), _new_channels(log_decay)
+    dstate = torch.empty((plan.sequences, out.shape[1]), device=out.device, dtype=torch.float32)
+    need, ws = _channel_workspace(plan, out)
+    with _On(out.device, plan) as stream:
+        st = _lib.lib().f3m_gated_recurrence_grad(plan._ref, kind, out.shape[1], rl, ro, rg, _pointer(state), _pointer(dfinal), wx, wl, dstate.data_ptr(),
+                                                  _pointer(ws), need, stream)
+    check(st, "f3m_gated_recurrence_grad")
+    return dx, dl, dstate
+
+
+class _GatedRecurrence(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, plan, x, log_decay, state):
+        out, final = _recurrence_forward(plan, x, log_decay, state)
+        ctx.save_for_backward(log_decay, out, state)
+        ctx.plan = plan
+        return out, final
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout, dfinal):
+        _refuse_capture("gated_recurrence")
+        log_decay, out, state = ctx.saved_tensors
+        dx, dl, dstate = gated_recurrence_grad(ctx.plan, log_decay, out, dout, state, dfinal)
+        return None, dx, dl, dstate if state is not None else None
+
+
+def gated_recurrence_step(x: torch.Tensor, log_decay: torch.Tensor, state: torch.Tensor) -> torch.Tensor:
+    """One new token for each of n sequences: x, log_decay (n, channels); state (n, channels) float32, contiguous, is updated in place.  Returns h
+    like x."""
+    _refuse_tangents(x, log_decay, state)
+    kind = _check_channels(x, ("log_decay", log_decay))
+    _shape(state, x.shape, "state")
+    if state.dtype != torch.float32 or state.device != x.device or not state.is_contiguous() or state.data_ptr() % 16:
+        raise TypeError("state must be a contiguous float32 array on the device of x that starts on 16 bytes: it is updated in place")
+    if _needs_grad(x, log_decay, state):
+        raise RuntimeError("gated_recurrence_step has no gradient: call it under torch.no_grad()")
+    (x, rx), (log_decay, rl), (out, ro) = _read_channels(x), _read_channels(log_decay), _new_channels(x)
+    with _On(x.device) as stream:
+        st = _lib.lib().f3m_gated_recurrence_step(x.shape[0], kind, x.shape[1], rx, rl, state.data_ptr(), ro, stream)
+    check(st, "f3m_gated_recurrence_step")
     torch.autograd.graph.increment_version(state)
     return out

@@ -380,6 +380,67 @@ int f3m_decay_attention_grad(const f3m_seqs *seqs, int32_t type, int32_t heads, 
 int f3m_decay_attention_step(int32_t n, int32_t type, int32_t heads, int32_t width_k, int32_t width_v, const float *log_decay,
                              float scale, f3m_rows q, f3m_rows k, f3m_rows v, float *state, f3m_rows out, void *stream);
 
+/* The recurrence behind both kinds of sums over a past, with a decay by token and channel that comes from data:
+ *   h_t = a_t h_(t-1) + x_t,  a_t = exp(min(log_decay_t, 0)),  every channel for itself.
+ * x, log_decay, out (tokens, channels): rows of the packed batch, heads = 1 and head_stride unused, of one type: bf16, fp16 or
+ * F3M_TYPE_F32 (strides multiples of 4 elements there).  channels is a multiple of 8 up to F3M_MAX_CHANNELS.  state_in, state_out (sequences, channels) float32, dense, 16-byte
+ * aligned: h before the first token (NULL: zeros) and behind the last one (NULL: not wanted; another array than state_in).  h is kept in float32.  -inf is no
+ * memory at all; log_decay that is not a number makes h that. */
+#define F3M_TYPE_F32 3
+#define F3M_MAX_CHANNELS 0x100000
+size_t f3m_gated_recurrence_workspace_bytes(const f3m_seqs *seqs, int32_t channels);
+int f3m_gated_recurrence(const f3m_seqs *seqs, int32_t type, int32_t channels, f3m_rows x, f3m_rows log_decay, const float *state_in, f3m_rows out,
+                         float *state_out, void *workspace, size_t workspace_bytes, void *stream);
+/* Gradients of sum(out * dout) + sum(state_out * dstate_out) by x, log_decay (0 where that is above 0) and state_in, from out of the call above: with
+ * G_t = dout_t + a_(t+1) G_(t+1), behind the last token dstate_out (NULL: zeros), dx_t = G_t, dlog_decay_t = G_t a_t h_(t-1), dstate_in = a_1 G_1
+ * (NULL: not wanted).  h_(t-1) is read from out, as rounded there. */
+int f3m_gated_recurrence_grad(const f3m_seqs *seqs, int32_t type, int32_t channels, f3m_rows log_decay, f3m_rows out, f3m_rows dout, const float *state_in,
+                              const float *dstate_out, f3m_rows dx, f3m_rows dlog_decay, float *dstate_in, void *workspace, size_t workspace_bytes, void *stream);
+/* One new token for each of n sequences: state (n, channels) float32 is updated in place. */
+int f3m_gated_recurrence_step(int32_t n, int32_t type, int32_t channels, f3m_rows x, f3m_rows log_decay, float *state, f3m_rows out, void *stream);
+
+/* A cache of keys and values in pages.  Token s of sequence b lies in page table[b * table_stride + s / page_tokens], row s % page_tokens; element (p, t, h, c) of
+ * the pages at data[p * page_stride + t * token_stride + h * head_stride + c], columns contiguous, strides multiples of 8 elements, data on 16 bytes.
+ * page_tokens is a power of two, 8 or more.  A number in the table outside 0..pages-1 is no page: what would lie there is not written, and not seen.  lengths (DEVICE,
+ * sequences): tokens in the cache before the call's new ones; values outside 0..table_pages * page_tokens are taken as the nearest of these.  New token
+ * i of sequence b, in the packed order of `seqs`, is token lengths[b] + i of the cache, and where that lies behind the table's last page it is neither written nor seen.
+ *
+ * parents (DEVICE, tokens; NULL: new tokens follow one another): new tokens are a tree, parents[t] the number, among the sequence's new tokens, of the one before
+ * token t, -1 where that is the cache's last one.  A parent comes before its children: values outside -1..i-1 are taken as -1.  At most F3M_TREE_MAX new tokens a sequence.  The
+ * position of a new token is lengths[b] plus its depth: the new tokens above it. */
+#define F3M_TREE_MAX 256
+typedef struct f3m_pages {
+    void *data;
+    int64_t page_stride, token_stride, head_stride;
+} f3m_pages;
+typedef struct f3m_cache {
+    f3m_pages k, v;
+    int32_t pages, page_tokens, kv_heads, width;
+    const int32_t *table;       /* device, (sequences, table_pages) */
+    int64_t table_stride;
+    int32_t table_pages, sequences;
+    const int32_t *lengths;     /* device */
+} f3m_cache;
+/* Rotation of the first `columns` columns, a multiple of 16: pair i turns by position * turns[i] / 2^64 of a whole turn (DEVICE, columns / 2 words): exact for far positions.
+ * Pair i is columns (i, i + columns / 2), or (2 i, 2 i + 1) if interleaved. */
+typedef struct f3m_rotation {
+    const uint64_t *turns;
+    int32_t columns, interleaved;
+} f3m_rotation;
+/* Writes new keys, rotated (rotation NULL: as they are), and values (tokens, kv_heads, width) to their pages; q (tokens, heads, width), where heads > 0, is
+ * rotated into q_out, which may be q.  No two sequences may have new tokens in one place. */
+int f3m_paged_append(const f3m_seqs *seqs, int32_t type, const f3m_cache *cache, f3m_rows k, f3m_rows v, const int32_t *parents, const f3m_rotation *rotation,
+                     int32_t heads, f3m_rows q, f3m_rows q_out, void *stream);
+/* Attention of the new tokens, which the pages hold already.  A new token at position p sees cached token j if p - j < window or j < sinks, and of the new tokens itself
+ * and those above it, at positions p', if p - p' < window or p' < sinks.  q, out (tokens, heads, width), heads / kv_heads at most 128.  A row that sees
+ * nothing (its page is missing) is zeros. */
+size_t f3m_paged_attention_workspace_bytes(const f3m_seqs *seqs, const f3m_cache *cache, int32_t heads);
+int f3m_paged_attention(const f3m_seqs *seqs, int32_t type, const f3m_cache *cache, int32_t heads, int32_t window, int32_t sinks, float scale, const int32_t *parents,
+                        f3m_rows q, f3m_rows out, void *workspace, size_t workspace_bytes, void *stream);
+/* Keeps a path of each tree: new token kept[b * kept_stride + j] of sequence b becomes token lengths[b] + j of the cache, in keys and values, for j < counts[b] (taken
+ * as 0..most).  kept[..j] >= j, as along any path from a root; other values, and pages that are missing, leave the place as it is.  kept, counts: DEVICE. */
+int f3m_paged_keep(int32_t type, const f3m_cache *cache, const int32_t *kept, int64_t kept_stride, int32_t most, const int32_t *counts, void *stream);
+
 /* -------- measurement helpers -------------------------------------------------------------- */
 
 /* Measures the SM's exponential (MUFU.EX2) and FP32 FMA issue peaks with two register-only
