@@ -93,70 +93,664 @@ void paged_append(int type, const AppendArgs &a, cudaStream_t s) {
 }
 
 // ---- attention of new tokens ------------------------------------------------------------------------------------------------
-// A warp has a row, 4 columns a lane, and walks over the keys
-template <typename T>
-__global__ void __launch_bounds__(128) paged_rows(const __grid_constant__ PagedArgs a) {
-    __shared__ uint32_t above_s[4][F3M_TREE_MAX / 32];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, h = blockIdx.y, hk = h / (a.heads / a.c.kv_heads), c = 4 * lane;
-    const int4 e = reinterpret_cast<const int4 *>(a.s.table)[seq_by_place(a.s, blockIdx.x / 32)];
-    const int i = e.z + 4 * (blockIdx.x % 32) + warp;
-    if (i >= e.y) return;
-    const int *parents = a.parents ? a.parents + e.x : nullptr;
-    const int length = paged_length(a.c, e.w);
-    int depth = i;
-    if (parents) {
-        if (lane < F3M_TREE_MAX / 32) above_s[warp][lane] = 0u;
-        __syncwarp();
-        depth = -1;
-        for (int p = i; p >= 0; p = parent_of(parents, p), depth++)
-            if (lane == 0) above_s[warp][p >> 5] |= 1u << (p & 31);
-        __syncwarp();
+// An item is one key head and as many new tokens as make two tiles of 128 rows, (token, head) of the heads that share it; it walks over the tiles of 128
+// keys that some of its rows see.  CTAs, one per SM, share all items' tiles evenly: CTA c of G takes tiles c U / G .. (c + 1) U / G of U, cuts through
+// items where that falls, and paged_join puts the parts together.  How long a sequence is stands on the device only, so that each CTA counts for itself.
+//
+// As in window attention S = Q K^T goes to tensor memory, a thread takes the weights of one row and writes them over S, from where they go into O += P V, and two
+// streams take turns, one's weights while the other's products run.  The streams are the item's two tiles of rows, or, where it has one only (one token, a
+// drafted tree), every other tile of keys: rows of the same lanes, so that at the end each thread adds the two O's itself.
+//
+// Keys that only a part of the item's rows sees (the window's edge, new tokens, a tree, missing pages) go by bits, a word for 32 of them.  A value that is not finite would
+// reach every row there, as zero times it: it is taken out of the tile, and added to the rows that see it when they have been written (poison_row).
+constexpr int PG_COPY = 8, PG_PRODUCTS = 9, PG_THREADS = 320, PG_BLOCK = SEQ_TILE * 128, PG_RING = 4, PG_SLOTS = 10;
+constexpr float PG_NO_SUM = 0x1p60f;   // some exponent was not a number (exp2_poly)
+constexpr int PG_WORDS = F3M_TREE_MAX / 32;
+
+struct PagedItem {
+    int row0, n, b, i0, tokens, length;   // the sequence's first row, new tokens, number; first token of the item, how many; tokens in the cache
+    int kv_head, tiles_q, sinks, first, keys;   // tiles of rows; tiles of keys: the first `sinks` of the sequence, then those from tile `first` on; `keys` in all
+    __device__ __forceinline__ int key(int j) const { return SEQ_TILE * (j < sinks ? j : first + j - sinks); }
+};
+struct PagedPart {   // of an item: tiles of keys j0 .. j1 - 1
+    PagedItem w;
+    int j0, j1, slot;   // slot: where its sums go; -1: all of the item, the outputs themselves
+};
+struct PagedSplit {   // an item whose first part is the last one of a CTA
+    PagedItem w;
+    int parts;   // 0: none
+};
+struct PagedKernel {
+    PagedArgs a;
+    CUtensorMap mq, mk, mv;
+    int group, tokens;     // heads that share a key head; tokens of a tile of rows
+    int subs, entries;     // items of 256 tokens of a sequence, of all sequences
+    int page_shift, box;   // box: tokens of a copy
+    int rows;              // of a part's place in the workspace
+    bool wide;
+    float c;               // |scale| log2(e)
+    float2 *stat;          // (2 G, rows): maximum, sum of weights
+    float *sums;           // (2 G, rows, width)
+    PagedSplit *split;     // (G)
+    int *err;
+};
+
+// Entry e: a sequence's tokens, without a key head; no tokens: none are left
+__device__ __forceinline__ PagedItem paged_item(const PagedKernel &p, int e) {
+    const PagedArgs &a = p.a;
+    const int4 q = reinterpret_cast<const int4 *>(a.s.table)[seq_pair_by_past(a.s, e / p.subs)];
+    PagedItem w;
+    w.row0 = q.x; w.n = q.y; w.b = q.w;
+    const int in = 2 * p.tokens * (e % p.subs);
+    w.i0 = q.z + in;
+    w.tokens = max(0, min(min(2 * p.tokens, 2 * SEQ_TILE - in), w.n - w.i0));
+    w.length = paged_length(a.c, w.b);
+    w.kv_head = 0;
+    w.tiles_q = w.tokens > p.tokens ? 2 : 1;
+    // the first new token that a row may be, by its position: a tree's may be a root
+    w.first = max(0, w.length + (a.parents ? 0 : w.i0) - a.window + 1) / SEQ_TILE;
+    w.sinks = min((a.sinks + SEQ_TILE - 1) / SEQ_TILE, w.first);
+    w.keys = w.tokens ? w.sinks + (w.length + w.i0 + w.tokens - 1) / SEQ_TILE - w.first + 1 : 0;
+    return w;
+}
+// Which of 16 groups of 8 keys of a tile have a page: by a lane each
+__device__ __forceinline__ int page_of_group(const PagedKernel &p, const PagedItem &w, int key, int lane) {
+    const int slot = key + 8 * lane;
+    return lane < SEQ_TILE / 8 ? paged_page(p.a.c, w.b, slot) : -1;
+}
+// Whether all rows of the item see all keys of a tile
+__device__ __forceinline__ bool seen_by_all(const PagedKernel &p, const PagedItem &w, int key, uint32_t there) {
+    const PagedArgs &a = p.a;
+    const int last = w.length + w.i0 + w.tokens - 1;   // the furthest position
+    return there == 0xffffu && key + SEQ_TILE - 1 <= w.length + (a.parents ? -1 : w.i0) && (last - key < a.window || key + SEQ_TILE <= a.sinks);
+}
+__device__ __forceinline__ uint32_t ones(int from, int to) {   // bits from .. to - 1 of a word
+    from = max(from, 0);
+    to = min(to, 32);
+    return to > from ? (0xffffffffu >> (32 - to + from)) << from : 0u;
+}
+// The keys from `at` to at + 31 that a row at position pos sees; `there` of their four groups of 8.  up: its last key but for a tree's; above: a tree's new tokens that it sees
+__device__ __forceinline__ uint32_t seen_keys(const PagedArgs &a, const PagedItem &w, int at, uint32_t there, int pos, int up, const uint32_t *above) {
+    uint32_t m = (ones(pos - a.window + 1 - at, 32) | ones(0, a.sinks - at)) & ones(0, up + 1 - at);
+    if (above) {
+        const int bit = at - w.length, k = bit >> 5;
+        const uint32_t lo = k >= 0 && k < PG_WORDS ? above[k] : 0u, hi = k >= -1 && k + 1 < PG_WORDS ? above[k + 1] : 0u;
+        m |= __funnelshift_r(lo, hi, bit & 31);
     }
-    auto read = [&](const void *p, int64_t at, float (&f)[4]) {
-        uint2 v = make_uint2(0u, 0u);
-        if (c + 4 <= a.c.width) v = *reinterpret_cast<const uint2 *>(reinterpret_cast<const uint16_t *>(p) + at + c);
-        const float2 x = Half<T>::unpack(v.x), y = Half<T>::unpack(v.y);
-        f[0] = x.x; f[1] = x.y; f[2] = y.x; f[3] = y.y;
-    };
-    float q[4], o[4] = {}, top = -INFINITY, sum = 0.f;
-    read(a.q.data, (int64_t)(e.x + i) * a.q.token_stride + (int64_t)h * a.q.head_stride, q);
-    const int64_t pos = (int64_t)length + depth, lo = max((int64_t)0, pos - a.window + 1);
-    for (int64_t j = 0; j <= (int64_t)length + i; j++) {
-        const int64_t m = j - length;   // a new token
-        if (j < lo && j >= a.sinks && m < 0) { j = min(lo, (int64_t)length) - 1; continue; }
-        if (m >= 0 && parents) {
-            if (!(above_s[warp][m >> 5] >> (m & 31) & 1)) continue;
-            int d = 0;
-            for (int p = parent_of(parents, (int)m); p >= 0; p = parent_of(parents, p)) d++;
-            if (depth - d >= a.window && length + d >= a.sinks) continue;
-        } else if (j < lo && j >= a.sinks) continue;
-        const int page = paged_page(a.c, e.w, j);
-        if (page < 0) continue;
-        float k[4], v[4];
-        read(a.c.k.data, paged_at(a.c, a.c.k, page, j, hk), k);
-        read(a.c.v.data, paged_at(a.c, a.c.v, page, j, hk), v);
-        float x = q[0] * k[0] + q[1] * k[1] + q[2] * k[2] + q[3] * k[3];
-        for (int w = 16; w; w >>= 1) x += __shfl_xor_sync(0xffffffffu, x, w);
-        x *= a.scale;
-        const float high = fmaxf(top, x), f = top == high ? 1.f : expf(top - high), w = expf(x - high);
-        top = high;
-        sum = sum * f + w;
-        for (int y = 0; y < 4; y++) o[y] = o[y] * f + w * v[y];
-    }
-    const float inv = sum != 0.f ? 1.f / sum : 0.f;
-    if (c + 4 <= a.c.width)
-        *reinterpret_cast<uint2 *>(reinterpret_cast<uint16_t *>(a.out.data) + (int64_t)(e.x + i) * a.out.token_stride + (int64_t)h * a.out.head_stride + c) =
-            make_uint2(Half<T>::pack(o[0] * inv, o[1] * inv), Half<T>::pack(o[2] * inv, o[3] * inv));
+    const uint32_t groups = (there & 1u) | (there & 2u) << 7 | (there & 4u) << 14 | (there & 8u) << 21;
+    return m & groups * 0xffu;
 }
 
-size_t paged_workspace(const f3m_seqs &, const f3m_cache &, int) { return 0; }
+__device__ __forceinline__ bool finite16(uint32_t v, uint32_t exponent) { return (v & exponent) != exponent; }   // the lower half of a word
 
-void paged_attention(int type, const PagedArgs &a, cudaStream_t s) {
-    const dim3 grid(a.s.tiles * 32, a.heads);
-    if (type == F3M_TYPE_BF16) paged_rows<__nv_bfloat16><<<grid, 128, 0, s>>>(a);
-    else paged_rows<__half><<<grid, 128, 0, s>>>(a);
+// Values that are not finite, of keys in tiles that were cleared of them, to columns c0 .. c1 - 1 of a row that sees them
+template <typename T, typename O>
+__device__ __noinline__ void poison_row(const PagedKernel &p, const PagedPart &part, int pos, int up, const uint32_t *above, O *row, int c0, int c1) {
+    const PagedArgs &a = p.a;
+    const PagedItem &w = part.w;
+    for (int j = part.j0; j < part.j1; j++) {
+        const int key = w.key(j);
+        uint32_t there = 0;
+        for (int g = 0; g < SEQ_TILE / 8; g++) there |= (uint32_t)(page_of_group(p, w, key, g) >= 0) << g;
+        if (seen_by_all(p, w, key, there)) continue;
+        for (int q = 0; q < 4; q++)
+            for (uint32_t m = seen_keys(a, w, key + 32 * q, there >> 4 * q, pos, up, above); m; m &= m - 1) {
+                const int64_t slot = key + 32 * q + __ffs(m) - 1;
+                const uint16_t *v = reinterpret_cast<const uint16_t *>(a.c.v.data) + paged_at(a.c, a.c.v, paged_page(a.c, w.b, slot), slot, w.kv_head);
+                for (int c = c0; c < c1; c++) {
+                    const float x = Half<T>::unpack(v[c]).x;
+                    if (isfinite(x)) continue;
+                    if constexpr (sizeof(O) == 4) row[c] += x;
+                    else row[c] = (O)Half<T>::pack(Half<T>::unpack(row[c]).x + x, 0.f);
+                }
+            }
+    }
+}
+
+template <typename T, int NB>
+__global__ void __launch_bounds__(PG_THREADS, 1) paged_tiles(const __grid_constant__ PagedKernel p) {
+    extern __shared__ unsigned char raw[];
+    __shared__ __align__(8) uint64_t bars[2 * PG_SLOTS + 2 * PG_RING + 13];
+    __shared__ PagedPart ring_s[PG_RING];
+    __shared__ long long warp_s[PG_THREADS / 32], start_s[2];
+    __shared__ uint32_t tmem_s, bad_s[2][2][4];
+    __shared__ float2 stat_s[2][SEQ_TILE];
+    __shared__ int gave_up_s, go_s[2];
+    __shared__ int16_t parent_s[F3M_TREE_MAX], depth_s[F3M_TREE_MAX];
+    const PagedArgs &a = p.a;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+    constexpr int slots = NB == 2 ? 4 : 10;
+    const uint32_t smem = (tc::smem_u32(raw) + 1023) & ~1023u;
+    auto q_tile = [&](int t) { return smem + t * NB * PG_BLOCK; };
+    auto slot_tile = [&](int s) { return smem + (2 + s) * NB * PG_BLOCK; };
+    uint32_t(*above_s)[PG_WORDS] = reinterpret_cast<uint32_t(*)[PG_WORDS]>(raw + (smem - tc::smem_u32(raw)) + (2 + slots) * NB * PG_BLOCK);
+
+    if (warp == PG_COPY) tc::tmem_alloc(tc::smem_u32(&tmem_s), 512);
+    const uint32_t b_full = tc::smem_u32(&bars[0]), b_free = b_full + 8 * PG_SLOTS, b_part = b_free + 8 * PG_SLOTS, b_part_free = b_part + 8 * PG_RING, b_q = b_part_free + 8 * PG_RING,
+                   b_q_free = b_q + 8, b_s = b_q + 16, b_p = b_q + 32, b_p2 = b_q + 48, b_o = b_q + 64, b_o_read = b_q + 80, b_none = b_q + 88;
+    if (tid == 0) {
+        for (int i = 0; i < 2 * PG_SLOTS; i++) tc::mbar_init(b_full + 8 * i, 1);       // landed, free
+        for (int i = 0; i < PG_RING; i++) {
+            tc::mbar_init(b_part + 8 * i, 1);                                          // a part is told
+            tc::mbar_init(b_part_free + 8 * i, 9);                                     // and done with, by nine warps
+        }
+        tc::mbar_init(b_q, 1);
+        tc::mbar_init(b_q_free, 1);
+        for (int t = 0; t < 2; t++) {
+            tc::mbar_init(b_s + 8 * t, 1);       // S ready
+            tc::mbar_init(b_p + 8 * t, 128);     // weights of the first 64 keys written
+            tc::mbar_init(b_p2 + 8 * t, 128);    // of the other 64
+            tc::mbar_init(b_o + 8 * t, 1);       // O ready
+        }
+        tc::mbar_init(b_o_read, 256);            // both read
+        tc::mbar_init(b_none, 1);                // no products in flight
+        tc::fence_mbar_init();
+        gave_up_s = 0;
+    }
+    // tiles of all items, and where this CTA's begin
+    auto tiles_of = [&](int e) { return e < p.entries ? (long long)paged_item(p, e).keys * a.c.kv_heads : 0ll; };
+    auto scan = [&](long long v, long long &all) {   // of the block's threads: the sum up to this one, and of all
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long y = __shfl_up_sync(0xffffffffu, v, o);
+            if (lane >= o) v += y;
+        }
+        __syncthreads();
+        if (lane == 31) warp_s[warp] = v;
+        __syncthreads();
+        all = 0;
+        long long before = 0;
+        for (int i = 0; i < PG_THREADS / 32; i++) {
+            if (i == warp) before = all;
+            all += warp_s[i];
+        }
+        return v + before;
+    };
+    long long total = 0, mine = 0, up_to = 0, sum;
+    for (int e = 0; e < p.entries; e += PG_THREADS) {
+        mine = tiles_of(e + tid);
+        up_to = scan(mine, sum);
+        total += sum;
+    }
+    const int ctas = (int)min((long long)gridDim.x, total), cta = blockIdx.x;   // a tile at least for each
+    const long long u0 = cta < ctas ? cta * total / ctas : total, u1 = cta < ctas ? (cta + 1) * total / ctas : total;
+    long long base = 0;
+    for (int e = 0; e < p.entries; e += PG_THREADS) {
+        if (p.entries > PG_THREADS) {
+            mine = tiles_of(e + tid);
+            up_to = scan(mine, sum);
+        }
+        if (u0 < base + up_to && u0 >= base + up_to - mine) { start_s[0] = e + tid; start_s[1] = u0 - (base + up_to - mine); }
+        base += sum;
+    }
+    tc::fence_before_sync();
+    __syncthreads();
+    tc::fence_after_sync();
+    const Waits wait{&gave_up_s, p.err};
+    const uint32_t tmem = tmem_s;
+
+    if (warp == PG_COPY) {
+        // ---- parts told to the others, copies; a lane has a page of a tile ----
+        int x = 0, queries = 0, parts = 0, e = u0 < u1 ? (int)start_s[0] : 0, j = 0;
+        long long left = u1 - u0;
+        bool stop = false;   // of the whole warp
+        PagedItem w = paged_item(p, e);
+        if (left) { w.kv_head = min((int)(start_s[1] / w.keys), a.c.kv_heads - 1); j = (int)(start_s[1] % w.keys); }
+        PagedSplit split{w, 0};
+        const int boxes = SEQ_TILE / p.box;
+        const uint32_t page_mask = (1u << p.page_shift) - 1;
+        auto wait_all = [&](uint32_t bar, uint32_t parity) {
+            wait(bar, parity);
+            stop = __any_sync(0xffffffffu, gave_up_s);
+        };
+        for (; left > 0; parts++) {
+            PagedPart t{w, j, (int)min((long long)w.keys, j + left), -1};
+            if (t.j0 > 0 || t.j1 < w.keys) t.slot = 2 * cta + (t.j0 == 0);
+            if (t.j0 == 0 && t.j1 < w.keys) {   // the item's last tile is keys - j1 behind this CTA's
+                const long long u = u1 - 1 + w.keys - t.j1;
+                split = {w, (int)(((u + 1) * ctas - 1) / total) - cta + 1};
+            }
+            const int r = parts % PG_RING;
+            if (parts >= PG_RING) wait_all(b_part_free + 8 * r, (parts / PG_RING - 1) & 1);
+            if (stop) break;
+            if (lane == 0) {
+                ring_s[r] = t;
+                tc::mbar_arrive(b_part + 8 * r);
+            }
+            if (parts) wait_all(b_q_free, (parts - 1) & 1);
+            if (stop) break;
+            if (lane == 0) {
+                tc::mbar_expect_tx(b_q, w.tiles_q * NB * p.tokens * p.group * 128);
+                for (int i = 0; i < w.tiles_q; i++)
+                    for (int k = 0; k < NB; k++)
+                        tc::tma_rows(q_tile(i) + k * PG_BLOCK, &p.mq, 64 * k, w.kv_head * p.group, w.row0 + w.i0 + i * p.tokens, b_q);
+            }
+            queries++;
+            auto page_at = [&](int k) { return lane < boxes ? paged_page(a.c, w.b, (int64_t)w.key(k) + lane * p.box) : -1; };
+            int page = page_at(t.j0);
+            for (int k = t.j0; k < t.j1 && !stop; k++) {
+                const int next = k + 1 < t.j1 ? page_at(k + 1) : -1, row = (int)((uint32_t)(w.key(k) + lane * p.box) & page_mask);
+                for (int v = 0; v < 2; v++, x++) {
+                    const int s = x % slots;
+                    if (x >= slots) wait_all(b_free + 8 * s, (x / slots - 1) & 1);
+                    if (stop) break;
+                    if (lane == 0) tc::mbar_expect_tx(b_full + 8 * s, NB * PG_BLOCK);
+                    __syncwarp();
+                    if (lane < boxes)   // of a page that is not there zeros come
+                        for (int i = 0; i < NB; i++)
+                            tc::tma_page(slot_tile(s) + i * PG_BLOCK + lane * p.box * 128, v ? &p.mv : &p.mk, 64 * i, w.kv_head, row, page, b_full + 8 * s);
+                }
+                page = next;
+            }
+            if (stop) break;
+            left -= t.j1 - t.j0;
+            j = 0;
+            if (left && ++w.kv_head == a.c.kv_heads)
+                do {
+                    if (++e == p.entries) left = 0;
+                    else w = paged_item(p, e);
+                } while (left && w.keys == 0);
+        }
+        const int r = parts % PG_RING;
+        if (!stop && parts >= PG_RING) wait_all(b_part_free + 8 * r, (parts / PG_RING - 1) & 1);
+        if (lane == 0) {
+            p.split[cta] = split;
+            if (!stop) {   // no more parts
+                ring_s[r].j1 = 0;
+                tc::mbar_arrive(b_part + 8 * r);
+            }
+            for (int s = 0; s < slots; s++)   // the last copies
+                if (x > s) wait.drain(b_full + 8 * s, ((x - 1 - s) / slots) & 1);
+            if (queries) wait.drain(b_q, (queries - 1) & 1);
+        }
+    } else if (warp == PG_PRODUCTS) {
+        constexpr bool bf = Half<T>::type == F3M_TYPE_BF16;
+        // a negative scale turns S's sign: bit 13 negates A
+        const uint32_t i_s = tc::idesc_f16(bf, 128, 128, false, false) | (a.scale < 0.f ? 1u << 13 : 0u), i_o = tc::idesc_f16(bf, 128, 64 * NB, false, true);
+        int x = 0, np[2] = {0, 0};
+        for (int parts = 0;; parts++) {
+            const int r = parts % PG_RING;
+            wait(b_part + 8 * r, (parts / PG_RING) & 1);
+            if (__any_sync(0xffffffffu, gave_up_s)) break;
+            const int tiles_q = ring_s[r].w.tiles_q, keys = ring_s[r].j1 - ring_s[r].j0, end = ring_s[r].j1;
+            __syncwarp();
+            if (end == 0) break;
+            if (lane == 0) tc::mbar_arrive(b_part_free + 8 * r);
+            const int ahead = tiles_q == 2 ? 1 : 2;   // a stream's next tile of keys
+            auto scores = [&](int t, int k) {   // of tile k: it lies in slot 2 k of this part
+                const int s = (x + 2 * k) % slots;
+                wait(b_full + 8 * s, ((x + 2 * k) / slots) & 1);
+                tc::fence_after_sync();
+                if (tc::elect()) {
+                    tc::product_rows<NB>(tmem + 128 * t, q_tile(tiles_q == 2 ? t : 0), slot_tile(s), i_s);
+                    tc::mma_commit(b_s + 8 * t);
+                    if (tiles_q == 1 || t == 1) tc::mma_commit(b_free + 8 * s);
+                    if (k == keys - 1 && (tiles_q == 1 || t == 1)) tc::mma_commit(b_q_free);
+                }
+            };
+            wait(b_q, parts & 1);
+            scores(0, 0);
+            if (tiles_q == 2) scores(1, 0);
+            else if (keys > 1) scores(1, 1);
+            if (parts) wait(b_o_read, (parts - 1) & 1);
+            for (int k = 0; k < keys; k++) {
+                const int sv = (x + 2 * k + 1) % slots;
+                wait(b_full + 8 * sv, ((x + 2 * k + 1) / slots) & 1);
+                for (int i = 0; i < tiles_q; i++) {
+                    const int t = tiles_q == 2 ? i : k & 1;
+                    const bool begun = k >= ahead, more = k + ahead < keys;
+                    wait(b_p + 8 * t, np[t] & 1);
+                    tc::fence_after_sync();
+                    if (tc::elect()) tc::product_tmem64(tmem + 256 + 128 * t, tmem + 128 * t, slot_tile(sv), i_o, begun);
+                    wait(b_p2 + 8 * t, np[t] & 1);
+                    np[t]++;
+                    tc::fence_after_sync();
+                    if (tc::elect()) {
+                        tc::product_tmem64(tmem + 256 + 128 * t, tmem + 128 * t + 32, slot_tile(sv) + 64 * 128, i_o, 1);
+                        if (i == tiles_q - 1) tc::mma_commit(b_free + 8 * sv);
+                        if (!more) tc::mma_commit(b_o + 8 * t);
+                    }
+                    if (more) scores(t, k + ahead);
+                }
+            }
+            x += 2 * keys;
+        }
+        wait.drain_products(b_none);
+    } else {
+        // ---- weights: thread r of a stream has row r of its tile ----
+        const int t = warp >> 2, r = tid & 127, wq = warp & 3;
+        const uint32_t lanes = (uint32_t)(32 * wq) << 16, t_s = tmem + 128 * t + lanes, t_o = tmem + 256 + lanes;
+        constexpr uint32_t exponent = Half<T>::type == F3M_TYPE_BF16 ? 0x7f80u : 0x7c00u;
+        int ns = 0, no[2] = {0, 0}, x0 = 0, had_b = -1, had_i0 = 0;
+        for (int parts = 0;; parts++) {
+            // whether there is a part is one thread's word to all: they meet at barriers inside
+            const int slot_r = parts % PG_RING;
+            if (warp == 0) {
+                wait(b_part + 8 * slot_r, (parts / PG_RING) & 1);
+                if (lane == 0) go_s[parts & 1] = !gave_up_s && ring_s[slot_r].j1 > 0;
+            }
+            tc::bar_sync(3, 256);
+            if (!go_s[parts & 1]) break;
+            const PagedPart part = ring_s[slot_r];
+            const PagedItem &w = part.w;
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(b_part_free + 8 * slot_r);
+            int scrubs = 0;
+            const bool by_keys = w.tiles_q == 1;
+            if (a.parents && (w.b != had_b || w.i0 != had_i0)) {   // depths of the item's tokens, and which new tokens each sees
+                had_b = w.b; had_i0 = w.i0;
+                for (int m = tid; m < w.i0 + w.tokens; m += 256) parent_s[m] = (int16_t)parent_of(a.parents + w.row0, m);
+                tc::bar_sync(3, 256);
+                if (tid < w.tokens) {
+                    int depth = -1;
+                    for (int m = w.i0 + tid; m >= 0; m = parent_s[m]) depth++;
+                    depth_s[tid] = (int16_t)depth;
+                    for (int k = 0; k < PG_WORDS; k++) above_s[tid][k] = 0u;
+                    int d = depth;
+                    for (int m = w.i0 + tid; m >= 0; m = parent_s[m], d--)
+                        if (depth - d < a.window || w.length + d < a.sinks) above_s[tid][m >> 5] |= 1u << (m & 31);
+                }
+                tc::bar_sync(3, 256);
+            }
+            const int in = r / p.group, token = by_keys ? in : t * p.tokens + in;   // of the item
+            const bool row = in < p.tokens && token < w.tokens, some = __any_sync(0xffffffffu, row);
+            const int i = w.i0 + token, pos = w.length + (a.parents ? (row ? depth_s[token] : 0) : i), up = row ? (a.parents ? w.length - 1 : i + w.length) : -1;
+            const uint32_t *above = a.parents && row ? above_s[token] : nullptr;
+            const int step = by_keys ? 2 : 1, k0 = by_keys ? part.j0 + t : part.j0;
+            float top = -INFINITY, sum = 0.f;
+            bool bad = false;
+            int page = k0 < part.j1 ? page_of_group(p, w, w.key(k0), lane) : -1;
+            for (int j = k0; j < part.j1; j += step) {
+                const int key = w.key(j);
+                const uint32_t there = __ballot_sync(0xffffffffu, page >= 0) & 0xffffu;
+                const bool whole = seen_by_all(p, w, key, there);
+                if (j + step < part.j1) page = page_of_group(p, w, w.key(j + step), lane);
+                uint32_t seen[4] = {}, bad_keys = 0u;
+                wait(b_s + 8 * t, ns & 1);
+                ns++;
+                __syncwarp();
+                tc::fence_after_sync();
+                if (!whole) {
+                    // Values that are not finite leave the tile.  Scores of this tile tell that the values in this slot before have landed: the wait names a phase's parity only
+                    uint32_t *bads = bad_s[by_keys ? t : 0][scrubs++ & 1];
+                    if (by_keys || t == 0) {
+                        const int xv = x0 + 2 * (j - part.j0) + 1, sv = xv % slots;
+                        wait(b_full + 8 * sv, (xv / slots) & 1);
+                        bool finite = true;
+                        auto chunk = [&](int c, uint32_t (&v)[4]) {
+                            const uint32_t at = slot_tile(sv) + (c >> 3) * PG_BLOCK + tc::swz(r, c & 7);
+                            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(at) : "memory");
+                            return at;
+                        };
+#pragma unroll
+                        for (int c = 0; c < 8 * NB; c++) {
+                            uint32_t v[4];
+                            chunk(c, v);
+#pragma unroll
+                            for (int k = 0; k < 4; k++) finite &= finite16(v[k], exponent) && finite16(v[k] >> 16, exponent);
+                        }
+                        if (!finite) {
+#pragma unroll 1
+                            for (int c = 0; c < 8 * NB; c++) {
+                                uint32_t v[4];
+                                const uint32_t at = chunk(c, v);
+#pragma unroll
+                                for (int k = 0; k < 4; k++) v[k] &= (finite16(v[k], exponent) ? 0xffffu : 0u) | (finite16(v[k] >> 16, exponent) ? 0xffff0000u : 0u);
+                                sts16(at, v);
+                            }
+                            tc::fence_async_smem();
+                        }
+                        const uint32_t b = __ballot_sync(0xffffffffu, !finite);
+                        if (lane == 0) bads[wq] = b;
+                    }
+                    if (by_keys) tc::bar_sync(1 + t, 128);
+                    else tc::bar_sync(3, 256);
+#pragma unroll
+                    for (int q = 0; q < 4; q++) {
+                        seen[q] = seen_keys(a, w, key + 32 * q, there >> 4 * q, pos, up, above);
+                        bad_keys |= seen[q] & bads[q];
+                    }
+                    bad |= bad_keys != 0u;
+                }
+                if (!some) {   // a warp without rows
+                    tc::fence_before_sync();
+                    tc::mbar_arrive(b_p + 8 * t);
+                    tc::mbar_arrive(b_p2 + 8 * t);
+                    continue;
+                }
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                uint32_t x[2][32];
+                tc::tmem_ld32(t_s, x[0]);
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    tc::tmem_ld_wait(x[q & 1]);
+                    if (q < 3) tc::tmem_ld32(t_s + 32 * (q + 1), x[(q + 1) & 1]);
+                    if (whole) {
+#pragma unroll
+                        for (int c = 0; c < 32; c++) mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(x[q & 1][c]));
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < 32; c++) mx[c & 3] = fmaxf(mx[c & 3], seen[q] >> c & 1 ? __uint_as_float(x[q & 1][c]) : -INFINITY);
+                    }
+                }
+                tc::tmem_ld32(t_s, x[0]);   // again
+                const float high = fmaxf(top, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
+                const bool rise = (high - top) * p.c > 8.f;   // also from -inf; not from -inf to -inf
+                if (__any_sync(0xffffffffu, rise)) {
+                    const float f = rise ? ex2_approx((top - high) * p.c) : 1.f;
+                    if (rise) { top = high; sum = sum < PG_NO_SUM ? sum * f : NAN; }
+                    if (j > k0)
+                        for (int q = 0; q < 2 * NB; q++) {
+                            uint32_t o[32];
+                            tc::tmem_ld32(t_o + 128 * t + 32 * q, o);
+                            tc::tmem_ld_wait(o);
+#pragma unroll
+                            for (int c = 0; c < 32; c++) o[c] = __float_as_uint(f * __uint_as_float(o[c]));
+                            tc::tmem_st32(t_o + 128 * t + 32 * q, o);
+                        }
+                }
+                const float shift = top == -INFINITY ? 0.f : -top * p.c;
+                const f32x2 cc = pack2(p.c, p.c), ss = pack2(shift, shift);
+                f32x2 add[2] = {pack2(sum, 0.f), pack2(0.f, 0.f)};
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    uint32_t w16[16];
+                    tc::tmem_ld_wait(x[q & 1]);
+                    if (q < 3) tc::tmem_ld32(t_s + 32 * (q + 1), x[(q + 1) & 1]);
+                    uint32_t(&y)[32] = x[q & 1];
+                    if (whole) {
+#pragma unroll
+                        for (int c = 0; c < 32; c += 2) {
+                            float lo, hi;
+                            const f32x2 e = fma2(pack2(__uint_as_float(y[c]), __uint_as_float(y[c + 1])), cc, ss);
+                            if (c % 8 == 6) exp2_poly<false>(e, lo, hi);
+                            else {
+                                unpack2(e, lo, hi);
+                                lo = ex2_approx(lo);
+                                hi = ex2_approx(hi);
+                            }
+                            add[(c >> 1) & 1] = add2(add[(c >> 1) & 1], pack2(lo, hi));
+                            w16[c >> 1] = Half<T>::pack(lo, hi);
+                        }
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < 32; c += 2) {
+                            float lo, hi;
+                            unpack2(fma2(pack2(__uint_as_float(y[c]), __uint_as_float(y[c + 1])), cc, ss), lo, hi);
+                            lo = seen[q] >> c & 1 ? ex2_approx(lo) : 0.f;
+                            hi = seen[q] >> (c + 1) & 1 ? ex2_approx(hi) : 0.f;
+                            add[(c >> 1) & 1] = add2(add[(c >> 1) & 1], pack2(lo, hi));
+                            w16[c >> 1] = Half<T>::pack(lo, hi);
+                        }
+                    }
+                    tc::tmem_st16(t_s + 16 * q, w16);   // over scores that have been read
+                    if (q & 1) {
+                        tc::tmem_st_wait();
+                        tc::fence_before_sync();
+                        tc::mbar_arrive((q == 1 ? b_p : b_p2) + 8 * t);
+                    }
+                }
+                float u, v;
+                unpack2(add2(add[0], add[1]), u, v);
+                sum = u + v;
+            }
+            if (!(sum < PG_NO_SUM) || top == INFINITY) sum = NAN;
+            // outputs: of a stream's own rows, or half the columns of both streams' sums
+            float f[2] = {t == 0 ? 1.f : 0.f, t == 0 ? 0.f : 1.f};
+            int c0 = 0, c1 = 64 * NB;
+            if (by_keys) {
+                stat_s[t][r] = make_float2(top, bad ? -sum : sum);   // a sum is not negative: its sign is a word from one stream to the other
+                tc::bar_sync(3, 256);
+                const float2 s0 = stat_s[0][r], s1 = stat_s[1][r];
+                top = fmaxf(s0.x, s1.x);
+                f[0] = s0.x == -INFINITY ? 0.f : ex2_approx((s0.x - top) * p.c);
+                f[1] = s1.x == -INFINITY ? 0.f : ex2_approx((s1.x - top) * p.c);
+                sum = f[0] * fabsf(s0.y) + f[1] * fabsf(s1.y);
+                bad = signbit(s0.y) || signbit(s1.y);
+                c0 = 32 * NB * t;
+                c1 = c0 + 32 * NB;
+            }
+            for (int u = 0; u < 2; u++) {
+                if (by_keys && part.j0 + u >= part.j1) continue;   // that stream had no tile
+                if (by_keys || u == t) wait(b_o + 8 * u, no[u] & 1);
+                no[u]++;
+            }
+            __syncwarp();
+            tc::fence_after_sync();
+            const float inv = part.slot >= 0 ? 1.f : sum != 0.f ? 1.f / sum : 0.f;   // nothing seen: 0
+            const float g0 = f[0] * inv, g1 = f[1] * inv;
+            const int64_t place = part.slot >= 0 ? (int64_t)part.slot * p.rows + token * p.group + r % p.group : 0;
+            uint16_t *out = reinterpret_cast<uint16_t *>(a.out.data) + (int64_t)(w.row0 + i) * a.out.token_stride + (int64_t)(w.kv_head * p.group + r % p.group) * a.out.head_stride;
+            float *part_row = p.sums + place * a.c.width;
+            if (some) {
+                for (int c = c0; c < c1; c += 32) {
+                    uint32_t o[32], o1[32];
+                    __syncwarp();
+                    if (by_keys || t == 0) tc::tmem_ld32(t_o + c, o);
+                    if (by_keys || t == 1) tc::tmem_ld32(t_o + 128 + c, o1);
+                    if (by_keys || t == 0) tc::tmem_ld_wait(o);
+                    if (by_keys || t == 1) tc::tmem_ld_wait(o1);
+                    // a stream that had no tile left what it found
+#pragma unroll
+                    for (int k = 0; k < 32; k++)
+                        o[k] = __float_as_uint((f[0] != 0.f ? g0 * __uint_as_float(o[k]) : 0.f) + (f[1] != 0.f ? g1 * __uint_as_float(o1[k]) : 0.f));
+                    if (!row) continue;
+                    if (part.slot >= 0) {
+#pragma unroll
+                        for (int k = 0; k < 32; k += 4)
+                            if (c + k < a.c.width) *reinterpret_cast<uint4 *>(part_row + c + k) = make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+                    } else {
+                        uint32_t y[16];
+#pragma unroll
+                        for (int k = 0; k < 16; k++) y[k] = Half<T>::pack(__uint_as_float(o[2 * k]), __uint_as_float(o[2 * k + 1]));
+                        store_row32(out, y, c, a.c.width, p.wide);
+                    }
+                }
+            }
+            tc::fence_before_sync();
+            tc::mbar_arrive(b_o_read);
+            if (row) {
+                if (part.slot >= 0 && c0 == 0) p.stat[place] = make_float2(top * p.c, sum);
+                if (bad) {
+                    if (part.slot >= 0) poison_row<T>(p, part, pos, up, above, part_row, c0, min(c1, a.c.width));
+                    else poison_row<T>(p, part, pos, up, above, out, c0, min(c1, a.c.width));
+                }
+            }
+            x0 += 2 * (part.j1 - part.j0);
+        }
+    }
+    __syncwarp();
+    tc::fence_before_sync();
+    __syncthreads();
+    if (warp == PG_COPY) tc::tmem_dealloc(tmem, 512);
+}
+
+// Items that were cut: a warp a row, 4 columns a lane.  Parts lie in the CTAs from this one on, scaled here to their common maximum, in their order; one that has seen nothing has a sum of 0.
+template <typename T>
+__global__ void __launch_bounds__(256) paged_join(const __grid_constant__ PagedKernel p) {
+    const PagedSplit s = p.split[blockIdx.x];
+    const int row = 8 * blockIdx.y + (threadIdx.x >> 5), lane = threadIdx.x & 31, c = 4 * lane;
+    if (row >= s.parts * p.rows || row >= s.w.tokens * p.group) return;
+    auto place = [&](int i) { return (int64_t)(2 * ((int)blockIdx.x + i) + (i == 0)) * p.rows + row; };
+    float high = -INFINITY, total = 0.f, o[4] = {};
+    for (int i = lane; i < s.parts; i += 32) high = fmaxf(high, p.stat[place(i)].x);
+#pragma unroll
+    for (int x = 16; x; x >>= 1) high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, x));
+    if (c >= p.a.c.width) return;
+    for (int i = 0; i < s.parts; i++) {
+        const float2 t = p.stat[place(i)];
+        if (t.y == 0.f) continue;
+        const float f = ex2_approx(t.x - high);
+        const float4 x = *reinterpret_cast<const float4 *>(p.sums + place(i) * p.a.c.width + c);
+        total = fmaf(f, t.y, total);
+        o[0] = fmaf(f, x.x, o[0]); o[1] = fmaf(f, x.y, o[1]); o[2] = fmaf(f, x.z, o[2]); o[3] = fmaf(f, x.w, o[3]);
+    }
+    const float inv = total != 0.f ? 1.f / total : 0.f;
+    uint16_t *out = reinterpret_cast<uint16_t *>(p.a.out.data) + (int64_t)(s.w.row0 + s.w.i0 + row / p.group) * p.a.out.token_stride + (int64_t)(s.w.kv_head * p.group + row % p.group) * p.a.out.head_stride;
+    *reinterpret_cast<uint2 *>(out + c) = make_uint2(Half<T>::pack(o[0] * inv, o[1] * inv), Half<T>::pack(o[2] * inv, o[3] * inv));
+}
+
+struct PagedGrid {
+    int group, tokens, subs, ctas, rows;
+    int64_t entries;
+};
+static PagedGrid paged_grid(const f3m_seqs &s, const f3m_cache &c, int heads) {
+    PagedGrid g;
+    g.group = heads / c.kv_heads;
+    g.tokens = SEQ_TILE / g.group;
+    g.subs = (std::min(s.longest, 2 * SEQ_TILE) + 2 * g.tokens - 1) / (2 * g.tokens);
+    g.entries = (int64_t)s.pairs * g.subs;
+    const int64_t most = ((int64_t)c.table_pages * c.page_tokens + s.longest) / SEQ_TILE + 1;   // tiles of keys of an item
+    g.ctas = (int)std::min<int64_t>(NUM_SMS_HINT, std::min<int64_t>(g.entries * c.kv_heads, NUM_SMS_HINT) * most);
+    g.rows = std::min(s.longest, 2 * g.tokens) * g.group;
+    return g;
+}
+static size_t split_bytes(const PagedGrid &g) { return (g.ctas * sizeof(PagedSplit) + 15) / 16 * 16; }
+size_t paged_workspace(const f3m_seqs &s, const f3m_cache &c, int heads) {
+    if (heads / c.kv_heads > SEQ_TILE) return 0;
+    const PagedGrid g = paged_grid(s, c, heads);
+    return split_bytes(g) + 2 * (size_t)g.ctas * ((g.rows + 1) / 2 * 2) * (c.width + 2) * sizeof(float);
+}
+
+template <typename T>
+static void paged_t(const PagedArgs &a, cudaStream_t s) {
+    PagedKernel p;
+    p.a = a;
+    const PagedGrid g = paged_grid(a.s, a.c, a.heads);
+    const int top = (int)std::min<int64_t>((int64_t)a.c.table_pages * a.c.page_tokens + a.s.longest, 0x7fffff00);   // no position is beyond
+    p.a.window = std::min(a.window, std::max(top, 1));
+    p.a.sinks = std::min(a.sinks, top);
+    F3M_REQUIRE(g.entries <= 0x7fffffff - PG_THREADS, F3M_ERR_OVERFLOW, "%lld tiles of new tokens do not fit in 31 bits", (long long)g.entries);
+    p.group = g.group; p.tokens = g.tokens; p.subs = g.subs; p.entries = (int)g.entries;
+    p.rows = (g.rows + 1) / 2 * 2;
+    p.page_shift = 31 - __builtin_clz(a.c.page_tokens);
+    p.box = std::min(a.c.page_tokens, SEQ_TILE);
+    p.wide = rows_wide(a.out);
+    p.c = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1e-30f);   // a scale of zero: all weights are one
+    p.err = seq_error_word();
+    p.split = reinterpret_cast<PagedSplit *>(a.ws);
+    p.sums = reinterpret_cast<float *>(reinterpret_cast<char *>(a.ws) + split_bytes(g));
+    p.stat = reinterpret_cast<float2 *>(p.sums + 2 * (size_t)g.ctas * p.rows * a.c.width);
+    p.mq = seq_tensor_map(Half<T>::type, a.q, a.s.tokens, a.heads, a.c.width, g.group, g.tokens);
+    f3m_cache c = a.c;
+    if (c.pages == 0) {   // no page is read: the maps need an address
+        c.pages = 1;
+        c.k = c.v = f3m_pages{a.q.data, c.width, c.width, c.width};
+    }
+    p.mk = page_tensor_map(Half<T>::type, c, c.k, p.box);
+    p.mv = page_tensor_map(Half<T>::type, c, c.v, p.box);
+    constexpr int blocks[2] = {2 + PG_SLOTS, 2 * (2 + 4)};
+    const int bytes = blocks[a.c.width > 64] * PG_BLOCK + F3M_TREE_MAX * PG_WORDS * 4 + 1024;
+    auto kernel = a.c.width <= 64 ? paged_tiles<T, 1> : paged_tiles<T, 2>;
+    static SharedMemory allowed[2];
+    allowed[a.c.width > 64].allow(kernel, bytes);
+    kernel<<<g.ctas, PG_THREADS, bytes, s>>>(p);
+    F3M_LAUNCH_CHECK();
+    paged_join<T><<<dim3(g.ctas, (g.rows + 7) / 8), 256, 0, s>>>(p);
     F3M_LAUNCH_CHECK();
 }
+
+void paged_attention(int type, const PagedArgs &a, cudaStream_t s) { type == F3M_TYPE_BF16 ? paged_t<__nv_bfloat16>(a, s) : paged_t<__half>(a, s); }
 
 // ---- accepted paths -----------------------------------------------------------------------------------------------------------
 // A thread has 16 bytes of a row of keys or values and takes the places in order, KP_ROWS at a time: read, then written.  A place is read for one in front of it or

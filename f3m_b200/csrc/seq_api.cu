@@ -27,7 +27,8 @@ void seq_check_error() {
     }
 }
 
-CUtensorMap seq_tensor_map(int type, const f3m_rows &r, int64_t tokens, int heads, int width) {
+// dims and box from the columns on, strides in elements from the second axis on
+static CUtensorMap tensor_map(int type, void *data, int axes, const cuuint64_t *dims, const int64_t *strides, const cuuint32_t *box) {
     typedef CUresult (*Encode)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
                                const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
     static Encode encode = [] {
@@ -38,13 +39,27 @@ CUtensorMap seq_tensor_map(int type, const f3m_rows &r, int64_t tokens, int head
         return (Encode)f;
     }();
     CUtensorMap m;
-    const cuuint64_t dims[3] = {(cuuint64_t)width, (cuuint64_t)heads, (cuuint64_t)tokens}, strides[2] = {2ull * r.head_stride, 2ull * r.token_stride};
-    const cuuint32_t box[3] = {64, 1, SEQ_TILE}, step[3] = {1, 1, 1};
-    const CUresult e = encode(&m, type == F3M_TYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, r.data, dims, strides, box, step,
+    cuuint64_t bytes[3];
+    for (int i = 0; i < axes - 1; i++) bytes[i] = 2ull * strides[i];
+    const cuuint32_t step[4] = {1, 1, 1, 1};
+    const CUresult e = encode(&m, type == F3M_TYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, axes, data, dims, bytes, box, step,
                               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    F3M_REQUIRE(e == CUDA_SUCCESS, F3M_ERR_ARG, "no tensor map for %lld tokens, %d heads, width %d, strides %lld, %lld (driver error %d)", (long long)tokens, heads,
-                width, (long long)r.token_stride, (long long)r.head_stride, (int)e);
+    F3M_REQUIRE(e == CUDA_SUCCESS, F3M_ERR_ARG, "no tensor map for width %lld, axes of %lld, %lld (strides %lld, %lld), .. (driver error %d)", (long long)dims[0], (long long)dims[1],
+                (long long)dims[2], (long long)strides[0], (long long)strides[1], (int)e);
     return m;
+}
+CUtensorMap seq_tensor_map(int type, const f3m_rows &r, int64_t tokens, int heads, int width, int box_heads, int box_tokens) {
+    const cuuint64_t dims[3] = {(cuuint64_t)width, (cuuint64_t)heads, (cuuint64_t)tokens};
+    const int64_t strides[2] = {r.head_stride, r.token_stride};
+    const cuuint32_t box[3] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_tokens};
+    return tensor_map(type, r.data, 3, dims, strides, box);
+}
+CUtensorMap page_tensor_map(int type, const f3m_cache &c, const f3m_pages &p, int box_tokens) {
+    const cuuint64_t dims[4] = {(cuuint64_t)c.width, (cuuint64_t)c.kv_heads, (cuuint64_t)c.page_tokens, (cuuint64_t)c.pages};
+    // the stride of an axis of one is not used, and may be anything
+    const int64_t strides[3] = {c.kv_heads == 1 ? c.width : p.head_stride, p.token_stride, c.pages == 1 ? c.width : p.page_stride};
+    const cuuint32_t box[4] = {64, 1, (cuuint32_t)box_tokens, 1};
+    return tensor_map(type, p.data, 4, dims, strides, box);
 }
 
 }  // namespace f3m

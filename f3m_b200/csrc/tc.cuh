@@ -254,6 +254,12 @@ __device__ __forceinline__ void tma_rows(uint32_t dst, const CUtensorMap *map, i
                  "r"(col), "r"(head), "r"(token), "r"(bar)
                  : "memory");
 }
+// 64 columns of one head, rows of one page; a page that is not there reads as zero
+__device__ __forceinline__ void tma_page(uint32_t dst, const CUtensorMap *map, int col, int head, int token, int page, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst), "l"(map),
+                 "r"(col), "r"(head), "r"(token), "r"(page), "r"(bar)
+                 : "memory");
+}
 // ... into L2 only
 __device__ __forceinline__ void tma_prefetch_rows(const CUtensorMap *map, int col, int head, int token) {
     asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global.tile [%0, {%1, %2, %3}];" ::"l"(map), "r"(col), "r"(head), "r"(token) : "memory");
