@@ -103,7 +103,7 @@ void paged_append(int type, const AppendArgs &a, cudaStream_t s) {
 //
 // Keys that only a part of the item's rows sees (the window's edge, new tokens, a tree, missing pages) go by bits, a word for 32 of them.  A value that is not finite would
 // reach every row there, as zero times it: it is taken out of the tile, and added to the rows that see it when they have been written (poison_row).
-constexpr int PG_COPY = 8, PG_PRODUCTS = 9, PG_THREADS = 320, PG_BLOCK = SEQ_TILE * 128, PG_RING = 4, PG_SLOTS = 10;
+constexpr int PG_COPY = 8, PG_PRODUCTS = 9, PG_THREADS = 320, PG_BLOCK = SEQ_TILE * 128, PG_RING = 4, PG_SLOTS = 10, PG_THERE = 8, PG_ITEM = 1;
 constexpr float PG_NO_SUM = 0x1p60f;   // some exponent was not a number (exp2_poly)
 constexpr int PG_WORDS = F3M_TREE_MAX / 32;
 
@@ -111,6 +111,7 @@ struct PagedItem {
     int row0, n, b, i0, tokens, length;   // the sequence's first row, new tokens, number; first token of the item, how many; tokens in the cache
     int kv_head, tiles_q, sinks, first, keys;   // tiles of rows; tiles of keys: the first `sinks` of the sequence, then those from tile `first` on; `keys` in all
     __device__ __forceinline__ int key(int j) const { return SEQ_TILE * (j < sinks ? j : first + j - sinks); }
+    __device__ __forceinline__ int cost() const { return keys ? keys + PG_ITEM : 0; }   // in tiles; what an item takes beside them comes behind its last
 };
 struct PagedPart {   // of an item: tiles of keys j0 .. j1 - 1
     PagedItem w;
@@ -153,12 +154,7 @@ __device__ __forceinline__ PagedItem paged_item(const PagedKernel &p, int e) {
     w.keys = w.tokens ? w.sinks + (w.length + w.i0 + w.tokens - 1) / SEQ_TILE - w.first + 1 : 0;
     return w;
 }
-// Which of 16 groups of 8 keys of a tile have a page: by a lane each
-__device__ __forceinline__ int page_of_group(const PagedKernel &p, const PagedItem &w, int key, int lane) {
-    const int slot = key + 8 * lane;
-    return lane < SEQ_TILE / 8 ? paged_page(p.a.c, w.b, slot) : -1;
-}
-// Whether all rows of the item see all keys of a tile
+// Whether all rows of the item see all keys of a tile; there: which of its 16 groups of 8 keys have a page
 __device__ __forceinline__ bool seen_by_all(const PagedKernel &p, const PagedItem &w, int key, uint32_t there) {
     const PagedArgs &a = p.a;
     const int last = w.length + w.i0 + w.tokens - 1;   // the furthest position
@@ -191,7 +187,7 @@ __device__ __noinline__ void poison_row(const PagedKernel &p, const PagedPart &p
     for (int j = part.j0; j < part.j1; j++) {
         const int key = w.key(j);
         uint32_t there = 0;
-        for (int g = 0; g < SEQ_TILE / 8; g++) there |= (uint32_t)(page_of_group(p, w, key, g) >= 0) << g;
+        for (int g = 0; g < SEQ_TILE / 8; g++) there |= (uint32_t)(paged_page(a.c, w.b, (int64_t)key + 8 * g) >= 0) << g;
         if (seen_by_all(p, w, key, there)) continue;
         for (int q = 0; q < 4; q++)
             for (uint32_t m = seen_keys(a, w, key + 32 * q, there >> 4 * q, pos, up, above); m; m &= m - 1) {
@@ -210,10 +206,10 @@ __device__ __noinline__ void poison_row(const PagedKernel &p, const PagedPart &p
 template <typename T, int NB>
 __global__ void __launch_bounds__(PG_THREADS, 1) paged_tiles(const __grid_constant__ PagedKernel p) {
     extern __shared__ unsigned char raw[];
-    __shared__ __align__(8) uint64_t bars[2 * PG_SLOTS + 2 * PG_RING + 13];
+    __shared__ __align__(8) uint64_t bars[2 * PG_SLOTS + 2 * PG_RING + 14];
     __shared__ PagedPart ring_s[PG_RING];
     __shared__ long long warp_s[PG_THREADS / 32], start_s[2];
-    __shared__ uint32_t tmem_s, bad_s[2][2][4];
+    __shared__ uint32_t tmem_s, bad_s[2][2][4], there_s[PG_THERE];
     __shared__ float2 stat_s[2][SEQ_TILE];
     __shared__ int gave_up_s, go_s[2];
     __shared__ int16_t parent_s[F3M_TREE_MAX], depth_s[F3M_TREE_MAX];
@@ -227,16 +223,16 @@ __global__ void __launch_bounds__(PG_THREADS, 1) paged_tiles(const __grid_consta
 
     if (warp == PG_COPY) tc::tmem_alloc(tc::smem_u32(&tmem_s), 512);
     const uint32_t b_full = tc::smem_u32(&bars[0]), b_free = b_full + 8 * PG_SLOTS, b_part = b_free + 8 * PG_SLOTS, b_part_free = b_part + 8 * PG_RING, b_q = b_part_free + 8 * PG_RING,
-                   b_q_free = b_q + 8, b_s = b_q + 16, b_p = b_q + 32, b_p2 = b_q + 48, b_o = b_q + 64, b_o_read = b_q + 80, b_none = b_q + 88;
+                   b_q_free = b_q + 16, b_s = b_q + 32, b_p = b_q + 48, b_p2 = b_q + 64, b_o = b_q + 80, b_o_read = b_q + 96, b_none = b_q + 104;
     if (tid == 0) {
         for (int i = 0; i < 2 * PG_SLOTS; i++) tc::mbar_init(b_full + 8 * i, 1);       // landed, free
         for (int i = 0; i < PG_RING; i++) {
             tc::mbar_init(b_part + 8 * i, 1);                                          // a part is told
             tc::mbar_init(b_part_free + 8 * i, 9);                                     // and done with, by nine warps
         }
-        tc::mbar_init(b_q, 1);
-        tc::mbar_init(b_q_free, 1);
         for (int t = 0; t < 2; t++) {
+            tc::mbar_init(b_q + 8 * t, 1);       // a tile of rows landed, free
+            tc::mbar_init(b_q_free + 8 * t, 1);
             tc::mbar_init(b_s + 8 * t, 1);       // S ready
             tc::mbar_init(b_p + 8 * t, 128);     // weights of the first 64 keys written
             tc::mbar_init(b_p2 + 8 * t, 128);    // of the other 64
@@ -248,7 +244,7 @@ __global__ void __launch_bounds__(PG_THREADS, 1) paged_tiles(const __grid_consta
         gave_up_s = 0;
     }
     // tiles of all items, and where this CTA's begin
-    auto tiles_of = [&](int e) { return e < p.entries ? (long long)paged_item(p, e).keys * a.c.kv_heads : 0ll; };
+    auto tiles_of = [&](int e) { return e < p.entries ? (long long)paged_item(p, e).cost() * a.c.kv_heads : 0ll; };
     auto scan = [&](long long v, long long &all) {   // of the block's threads: the sum up to this one, and of all
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -291,24 +287,63 @@ __global__ void __launch_bounds__(PG_THREADS, 1) paged_tiles(const __grid_consta
 
     if (warp == PG_COPY) {
         // ---- parts told to the others, copies; a lane has a page of a tile ----
-        int x = 0, queries = 0, parts = 0, e = u0 < u1 ? (int)start_s[0] : 0, j = 0;
+        // Copies of a part come in the order K0 K1 V0 K2 V1 .., without a stop between parts: values are wanted a tile's weights later than keys, and would only hold their place.
+        int x = 0, y = 0, parts = 0, e = u0 < u1 ? (int)start_s[0] : 0, e0 = e, uses0 = 0, uses1 = 0, turn = 0;   // copies, tiles, parts so far; uses of the places for rows
         long long left = u1 - u0;
         bool stop = false;   // of the whole warp
-        PagedItem w = paged_item(p, e);
-        if (left) { w.kv_head = min((int)(start_s[1] / w.keys), a.c.kv_heads - 1); j = (int)(start_s[1] % w.keys); }
-        PagedSplit split{w, 0};
         const int boxes = SEQ_TILE / p.box;
         const uint32_t page_mask = (1u << p.page_shift) - 1;
         auto wait_all = [&](uint32_t bar, uint32_t parity) {
             wait(bar, parity);
             stop = __any_sync(0xffffffffu, gave_up_s);
         };
-        for (; left > 0; parts++) {
-            PagedPart t{w, j, (int)min((long long)w.keys, j + left), -1};
-            if (t.j0 > 0 || t.j1 < w.keys) t.slot = 2 * cta + (t.j0 == 0);
-            if (t.j0 == 0 && t.j1 < w.keys) {   // the item's last tile is keys - j1 behind this CTA's
-                const long long u = u1 - 1 + w.keys - t.j1;
-                split = {w, (int)(((u + 1) * ctas - 1) / total) - cta + 1};
+        // entries are read 32 at a time, a lane each
+        PagedItem held = paged_item(p, min(e + lane, p.entries - 1)), w;
+        auto entry = [&](int i) {
+            if (i - e0 >= 32) {
+                e0 = i;
+                held = paged_item(p, min(i + lane, p.entries - 1));
+            }
+            PagedItem z;
+#define F3M_SAME(m) z.m = __shfl_sync(0xffffffffu, held.m, i - e0)
+            F3M_SAME(row0); F3M_SAME(n); F3M_SAME(b); F3M_SAME(i0); F3M_SAME(tokens); F3M_SAME(length); F3M_SAME(kv_head); F3M_SAME(tiles_q); F3M_SAME(sinks); F3M_SAME(first); F3M_SAME(keys);
+#undef F3M_SAME
+            return z;
+        };
+        auto rows_of = [&](int place, const PagedItem &z, int tile) {
+            int &uses = place ? uses1 : uses0;
+            if (uses && !stop) wait_all(b_q_free + 8 * place, (uses - 1) & 1);
+            if (stop) return;
+            if (lane == 0) {
+                tc::mbar_expect_tx(b_q + 8 * place, NB * p.tokens * p.group * 128);
+                for (int c = 0; c < NB; c++)
+                    tc::tma_rows(q_tile(place) + c * PG_BLOCK, &p.mq, 64 * c, z.kv_head * p.group, z.row0 + z.i0 + tile * p.tokens, b_q + 8 * place);
+            }
+            uses++;
+        };
+        auto page_at = [&](const PagedItem &z, int k) { return lane < boxes ? paged_page(a.c, z.b, (int64_t)z.key(k) + lane * p.box) : -1; };
+        w = entry(e);
+        int j = 0;
+        if (left) { w.kv_head = min((int)(start_s[1] / w.cost()), a.c.kv_heads - 1); j = (int)(start_s[1] % w.cost()); }
+        if (lane == 0) p.split[cta].parts = 0;
+        auto next = [&] {   // the item behind this one
+            left -= min(left, (long long)w.cost() - j);
+            j = 0;
+            if (left && ++w.kv_head == a.c.kv_heads)
+                do {
+                    if (++e == p.entries) left = 0;
+                    else w = entry(e);
+                } while (left && w.keys == 0);
+        };
+        if (left && j >= w.keys) next();
+        int page = left ? page_at(w, j) : -1;
+        while (left > 0) {
+            const PagedItem now = w;
+            PagedPart t{now, j, (int)min((long long)now.keys, j + left), -1};
+            if (t.j0 > 0 || t.j1 < now.keys) t.slot = 2 * cta + (t.j0 == 0);
+            if (t.j0 == 0 && t.j1 < now.keys) {   // the item's last tile is keys - j1 behind this CTA's
+                const long long u = u1 - 1 + now.keys - t.j1;
+                if (lane == 0) p.split[cta] = {now, (int)(((u + 1) * ctas - 1) / total) - cta + 1};
             }
             const int r = parts % PG_RING;
             if (parts >= PG_RING) wait_all(b_part_free + 8 * r, (parts / PG_RING - 1) & 1);
@@ -317,87 +352,94 @@ __global__ void __launch_bounds__(PG_THREADS, 1) paged_tiles(const __grid_consta
                 ring_s[r] = t;
                 tc::mbar_arrive(b_part + 8 * r);
             }
-            if (parts) wait_all(b_q_free, (parts - 1) & 1);
-            if (stop) break;
-            if (lane == 0) {
-                tc::mbar_expect_tx(b_q, w.tiles_q * NB * p.tokens * p.group * 128);
-                for (int i = 0; i < w.tiles_q; i++)
-                    for (int k = 0; k < NB; k++)
-                        tc::tma_rows(q_tile(i) + k * PG_BLOCK, &p.mq, 64 * k, w.kv_head * p.group, w.row0 + w.i0 + i * p.tokens, b_q);
+            parts++;
+            next();
+            const int later = left ? page_at(w, 0) : -1;   // of the next part, whose copies are to follow without a stop
+            if (now.tiles_q == 2) {
+                rows_of(0, now, 0);
+                rows_of(1, now, 1);
+            } else {
+                rows_of(turn, now, 0);
+                turn ^= 1;
             }
-            queries++;
-            auto page_at = [&](int k) { return lane < boxes ? paged_page(a.c, w.b, (int64_t)w.key(k) + lane * p.box) : -1; };
-            int page = page_at(t.j0);
-            for (int k = t.j0; k < t.j1 && !stop; k++) {
-                const int next = k + 1 < t.j1 ? page_at(k + 1) : -1, row = (int)((uint32_t)(w.key(k) + lane * p.box) & page_mask);
-                for (int v = 0; v < 2; v++, x++) {
-                    const int s = x % slots;
-                    if (x >= slots) wait_all(b_free + 8 * s, (x / slots - 1) & 1);
-                    if (stop) break;
-                    if (lane == 0) tc::mbar_expect_tx(b_full + 8 * s, NB * PG_BLOCK);
-                    __syncwarp();
-                    if (lane < boxes)   // of a page that is not there zeros come
-                        for (int i = 0; i < NB; i++)
-                            tc::tma_page(slot_tile(s) + i * PG_BLOCK + lane * p.box * 128, v ? &p.mv : &p.mk, 64 * i, w.kv_head, row, page, b_full + 8 * s);
+            const int all = t.j1 - t.j0;
+            int even = -1, odd = -1, ahead = page;   // pages of the last tiles of keys, of the next
+            for (int i = 0; i < 2 * all && !stop; i++, x++) {
+                const bool values = i && (i % 2 == 0 || (i + 1) / 2 == all);
+                const int k = !values ? (i + 1) / 2 : i % 2 ? all - 1 : i / 2 - 1, s = x % slots, row = (int)((uint32_t)(now.key(t.j0 + k) + lane * p.box) & page_mask);
+                uint32_t there = 0;
+                if (!values) {
+                    (k & 1 ? odd : even) = ahead;
+                    there = __ballot_sync(0xffffffffu, ahead >= 0);
+                    there = __ballot_sync(0xffffffffu, lane < SEQ_TILE / 8 && there >> (8 * lane / p.box) & 1u);   // of 16 groups of 8 keys
+                    ahead = k + 1 < all ? page_at(now, t.j0 + k + 1) : -1;
                 }
-                page = next;
+                if (x >= slots) wait_all(b_free + 8 * s, (x / slots - 1) & 1);
+                if (stop) break;
+                if (lane == 0) {
+                    if (!values) there_s[(y + k) % PG_THERE] = there;
+                    tc::mbar_expect_tx(b_full + 8 * s, NB * PG_BLOCK);
+                }
+                __syncwarp();
+                if (lane < boxes)   // of a page that is not there zeros come
+                    for (int c = 0; c < NB; c++)
+                        tc::tma_page(slot_tile(s) + c * PG_BLOCK + lane * p.box * 128, values ? &p.mv : &p.mk, 64 * c, now.kv_head, row, k & 1 ? odd : even, b_full + 8 * s);
             }
-            if (stop) break;
-            left -= t.j1 - t.j0;
-            j = 0;
-            if (left && ++w.kv_head == a.c.kv_heads)
-                do {
-                    if (++e == p.entries) left = 0;
-                    else w = paged_item(p, e);
-                } while (left && w.keys == 0);
+            y += all;
+            page = later;
         }
         const int r = parts % PG_RING;
         if (!stop && parts >= PG_RING) wait_all(b_part_free + 8 * r, (parts / PG_RING - 1) & 1);
         if (lane == 0) {
-            p.split[cta] = split;
             if (!stop) {   // no more parts
                 ring_s[r].j1 = 0;
                 tc::mbar_arrive(b_part + 8 * r);
             }
             for (int s = 0; s < slots; s++)   // the last copies
                 if (x > s) wait.drain(b_full + 8 * s, ((x - 1 - s) / slots) & 1);
-            if (queries) wait.drain(b_q, (queries - 1) & 1);
+            if (uses0) wait.drain(b_q, (uses0 - 1) & 1);
+            if (uses1) wait.drain(b_q + 8, (uses1 - 1) & 1);
         }
     } else if (warp == PG_PRODUCTS) {
         constexpr bool bf = Half<T>::type == F3M_TYPE_BF16;
         // a negative scale turns S's sign: bit 13 negates A
         const uint32_t i_s = tc::idesc_f16(bf, 128, 128, false, false) | (a.scale < 0.f ? 1u << 13 : 0u), i_o = tc::idesc_f16(bf, 128, 64 * NB, false, true);
-        int x = 0, np[2] = {0, 0};
+        int x = 0, np[2] = {0, 0}, uses[2] = {0, 0}, turn = 0;
         for (int parts = 0;; parts++) {
             const int r = parts % PG_RING;
             wait(b_part + 8 * r, (parts / PG_RING) & 1);
             if (__any_sync(0xffffffffu, gave_up_s)) break;
-            const int tiles_q = ring_s[r].w.tiles_q, keys = ring_s[r].j1 - ring_s[r].j0, end = ring_s[r].j1;
+            const PagedPart &part = ring_s[r];
+            const int tiles_q = part.w.tiles_q, keys = part.j1 - part.j0, end = part.j1;
             __syncwarp();
             if (end == 0) break;
             if (lane == 0) tc::mbar_arrive(b_part_free + 8 * r);
-            const int ahead = tiles_q == 2 ? 1 : 2;   // a stream's next tile of keys
-            auto scores = [&](int t, int k) {   // of tile k: it lies in slot 2 k of this part
-                const int s = (x + 2 * k) % slots;
-                wait(b_full + 8 * s, ((x + 2 * k) / slots) & 1);
+            const bool by_keys = tiles_q == 1;
+            const int ahead = by_keys ? 2 : 1;   // a stream's next tile of keys
+            auto keys_at = [&](int k) { return x + (k ? 2 * k - 1 : 0); };
+            auto values_at = [&](int k) { return x + min(2 * k + 2, 2 * keys - 1); };
+            auto scores = [&](int t, int k) {
+                const int at = keys_at(k), s = at % slots, place = by_keys ? turn : t;
+                wait(b_full + 8 * s, (at / slots) & 1);
                 tc::fence_after_sync();
                 if (tc::elect()) {
-                    tc::product_rows<NB>(tmem + 128 * t, q_tile(tiles_q == 2 ? t : 0), slot_tile(s), i_s);
+                    tc::product_rows<NB>(tmem + 128 * t, q_tile(place), slot_tile(s), i_s);
                     tc::mma_commit(b_s + 8 * t);
-                    if (tiles_q == 1 || t == 1) tc::mma_commit(b_free + 8 * s);
-                    if (k == keys - 1 && (tiles_q == 1 || t == 1)) tc::mma_commit(b_q_free);
+                    if (by_keys || t == 1) tc::mma_commit(b_free + 8 * s);
+                    if (k == keys - 1) tc::mma_commit(b_q_free + 8 * place);
                 }
             };
-            wait(b_q, parts & 1);
+            for (int t = 0; t < 2; t++)
+                if (!by_keys || t == turn) wait(b_q + 8 * t, uses[t]++ & 1);
             scores(0, 0);
-            if (tiles_q == 2) scores(1, 0);
+            if (!by_keys) scores(1, 0);
             else if (keys > 1) scores(1, 1);
             if (parts) wait(b_o_read, (parts - 1) & 1);
             for (int k = 0; k < keys; k++) {
-                const int sv = (x + 2 * k + 1) % slots;
-                wait(b_full + 8 * sv, ((x + 2 * k + 1) / slots) & 1);
+                const int at = values_at(k), sv = at % slots;
+                wait(b_full + 8 * sv, (at / slots) & 1);
                 for (int i = 0; i < tiles_q; i++) {
-                    const int t = tiles_q == 2 ? i : k & 1;
+                    const int t = by_keys ? k & 1 : i;
                     const bool begun = k >= ahead, more = k + ahead < keys;
                     wait(b_p + 8 * t, np[t] & 1);
                     tc::fence_after_sync();
@@ -414,11 +456,12 @@ __global__ void __launch_bounds__(PG_THREADS, 1) paged_tiles(const __grid_consta
                 }
             }
             x += 2 * keys;
+            if (by_keys) turn ^= 1;
         }
         wait.drain_products(b_none);
     } else {
         // ---- weights: thread r of a stream has row r of its tile ----
-        const int t = warp >> 2, r = tid & 127, wq = warp & 3;
+        const int t = warp >> 2, r = tid & 127, wq = warp & 3, in = r / p.group, head = r % p.group;
         const uint32_t lanes = (uint32_t)(32 * wq) << 16, t_s = tmem + 128 * t + lanes, t_o = tmem + 256 + lanes;
         constexpr uint32_t exponent = Half<T>::type == F3M_TYPE_BF16 ? 0x7f80u : 0x7c00u;
         int ns = 0, no[2] = {0, 0}, x0 = 0, had_b = -1, had_i0 = 0;
@@ -431,50 +474,47 @@ __global__ void __launch_bounds__(PG_THREADS, 1) paged_tiles(const __grid_consta
             }
             tc::bar_sync(3, 256);
             if (!go_s[parts & 1]) break;
-            const PagedPart part = ring_s[slot_r];
-            const PagedItem &w = part.w;
-            __syncwarp();
-            if (lane == 0) tc::mbar_arrive(b_part_free + 8 * slot_r);
-            int scrubs = 0;
+            const PagedPart &part = ring_s[slot_r];
+            const PagedItem &w = part.w;   // stays where it is: few of its numbers are worth a register
+            const int j0 = part.j0, j1 = part.j1, length = w.length, tokens = w.tokens;
             const bool by_keys = w.tiles_q == 1;
+            int scrubs = 0;
             if (a.parents && (w.b != had_b || w.i0 != had_i0)) {   // depths of the item's tokens, and which new tokens each sees
                 had_b = w.b; had_i0 = w.i0;
-                for (int m = tid; m < w.i0 + w.tokens; m += 256) parent_s[m] = (int16_t)parent_of(a.parents + w.row0, m);
+                for (int m = tid; m < had_i0 + tokens; m += 256) parent_s[m] = (int16_t)parent_of(a.parents + w.row0, m);
                 tc::bar_sync(3, 256);
-                if (tid < w.tokens) {
+                if (tid < tokens) {
                     int depth = -1;
-                    for (int m = w.i0 + tid; m >= 0; m = parent_s[m]) depth++;
+                    for (int m = had_i0 + tid; m >= 0; m = parent_s[m]) depth++;
                     depth_s[tid] = (int16_t)depth;
                     for (int k = 0; k < PG_WORDS; k++) above_s[tid][k] = 0u;
                     int d = depth;
-                    for (int m = w.i0 + tid; m >= 0; m = parent_s[m], d--)
-                        if (depth - d < a.window || w.length + d < a.sinks) above_s[tid][m >> 5] |= 1u << (m & 31);
+                    for (int m = had_i0 + tid; m >= 0; m = parent_s[m], d--)
+                        if (depth - d < a.window || length + d < a.sinks) above_s[tid][m >> 5] |= 1u << (m & 31);
                 }
                 tc::bar_sync(3, 256);
             }
-            const int in = r / p.group, token = by_keys ? in : t * p.tokens + in;   // of the item
-            const bool row = in < p.tokens && token < w.tokens, some = __any_sync(0xffffffffu, row);
-            const int i = w.i0 + token, pos = w.length + (a.parents ? (row ? depth_s[token] : 0) : i), up = row ? (a.parents ? w.length - 1 : i + w.length) : -1;
+            const int token = by_keys ? in : t * p.tokens + in;   // of the item
+            const bool row = in < p.tokens && token < tokens, some = __any_sync(0xffffffffu, row);
+            const int pos = length + (a.parents ? (row ? depth_s[token] : 0) : w.i0 + token), up = row ? (a.parents ? length - 1 : pos) : -1;
             const uint32_t *above = a.parents && row ? above_s[token] : nullptr;
-            const int step = by_keys ? 2 : 1, k0 = by_keys ? part.j0 + t : part.j0;
+            const int step = by_keys ? 2 : 1, k0 = by_keys ? j0 + t : j0;
             float top = -INFINITY, sum = 0.f;
             bool bad = false;
-            int page = k0 < part.j1 ? page_of_group(p, w, w.key(k0), lane) : -1;
-            for (int j = k0; j < part.j1; j += step) {
+            for (int j = k0; j < j1; j += step) {
                 const int key = w.key(j);
-                const uint32_t there = __ballot_sync(0xffffffffu, page >= 0) & 0xffffu;
-                const bool whole = seen_by_all(p, w, key, there);
-                if (j + step < part.j1) page = page_of_group(p, w, w.key(j + step), lane);
-                uint32_t seen[4] = {}, bad_keys = 0u;
                 wait(b_s + 8 * t, ns & 1);
                 ns++;
                 __syncwarp();
                 tc::fence_after_sync();
+                const uint32_t there = there_s[(x0 / 2 + j - j0) % PG_THERE];
+                const bool whole = seen_by_all(p, w, key, there);
+                uint32_t seen[4] = {};
                 if (!whole) {
                     // Values that are not finite leave the tile.  Scores of this tile tell that the values in this slot before have landed: the wait names a phase's parity only
                     uint32_t *bads = bad_s[by_keys ? t : 0][scrubs++ & 1];
                     if (by_keys || t == 0) {
-                        const int xv = x0 + 2 * (j - part.j0) + 1, sv = xv % slots;
+                        const int xv = x0 + min(2 * (j - j0) + 2, 2 * (j1 - j0) - 1), sv = xv % slots;
                         wait(b_full + 8 * sv, (xv / slots) & 1);
                         bool finite = true;
                         auto chunk = [&](int c, uint32_t (&v)[4]) {
@@ -508,9 +548,8 @@ __global__ void __launch_bounds__(PG_THREADS, 1) paged_tiles(const __grid_consta
 #pragma unroll
                     for (int q = 0; q < 4; q++) {
                         seen[q] = seen_keys(a, w, key + 32 * q, there >> 4 * q, pos, up, above);
-                        bad_keys |= seen[q] & bads[q];
+                        bad |= (seen[q] & bads[q]) != 0u;
                     }
-                    bad |= bad_keys != 0u;
                 }
                 if (!some) {   // a warp without rows
                     tc::fence_before_sync();
@@ -611,16 +650,17 @@ __global__ void __launch_bounds__(PG_THREADS, 1) paged_tiles(const __grid_consta
                 c1 = c0 + 32 * NB;
             }
             for (int u = 0; u < 2; u++) {
-                if (by_keys && part.j0 + u >= part.j1) continue;   // that stream had no tile
+                if (by_keys && j0 + u >= j1) continue;   // that stream had no tile
                 if (by_keys || u == t) wait(b_o + 8 * u, no[u] & 1);
                 no[u]++;
             }
             __syncwarp();
             tc::fence_after_sync();
-            const float inv = part.slot >= 0 ? 1.f : sum != 0.f ? 1.f / sum : 0.f;   // nothing seen: 0
+            const bool cut = part.slot >= 0;
+            const float inv = cut ? 1.f : sum != 0.f ? 1.f / sum : 0.f;   // nothing seen: 0
             const float g0 = f[0] * inv, g1 = f[1] * inv;
-            const int64_t place = part.slot >= 0 ? (int64_t)part.slot * p.rows + token * p.group + r % p.group : 0;
-            uint16_t *out = reinterpret_cast<uint16_t *>(a.out.data) + (int64_t)(w.row0 + i) * a.out.token_stride + (int64_t)(w.kv_head * p.group + r % p.group) * a.out.head_stride;
+            const int64_t place = cut ? (int64_t)part.slot * p.rows + token * p.group + head : 0;
+            uint16_t *out = reinterpret_cast<uint16_t *>(a.out.data) + (int64_t)(w.row0 + w.i0 + token) * a.out.token_stride + (int64_t)(w.kv_head * p.group + head) * a.out.head_stride;
             float *part_row = p.sums + place * a.c.width;
             if (some) {
                 for (int c = c0; c < c1; c += 32) {
@@ -635,7 +675,7 @@ __global__ void __launch_bounds__(PG_THREADS, 1) paged_tiles(const __grid_consta
                     for (int k = 0; k < 32; k++)
                         o[k] = __float_as_uint((f[0] != 0.f ? g0 * __uint_as_float(o[k]) : 0.f) + (f[1] != 0.f ? g1 * __uint_as_float(o1[k]) : 0.f));
                     if (!row) continue;
-                    if (part.slot >= 0) {
+                    if (cut) {
 #pragma unroll
                         for (int k = 0; k < 32; k += 4)
                             if (c + k < a.c.width) *reinterpret_cast<uint4 *>(part_row + c + k) = make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]);
@@ -650,13 +690,15 @@ __global__ void __launch_bounds__(PG_THREADS, 1) paged_tiles(const __grid_consta
             tc::fence_before_sync();
             tc::mbar_arrive(b_o_read);
             if (row) {
-                if (part.slot >= 0 && c0 == 0) p.stat[place] = make_float2(top * p.c, sum);
+                if (cut && c0 == 0) p.stat[place] = make_float2(top * p.c, sum);
                 if (bad) {
-                    if (part.slot >= 0) poison_row<T>(p, part, pos, up, above, part_row, c0, min(c1, a.c.width));
+                    if (cut) poison_row<T>(p, part, pos, up, above, part_row, c0, min(c1, a.c.width));
                     else poison_row<T>(p, part, pos, up, above, out, c0, min(c1, a.c.width));
                 }
             }
-            x0 += 2 * (part.j1 - part.j0);
+            x0 += 2 * (j1 - j0);
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(b_part_free + 8 * slot_r);
         }
     }
     __syncwarp();
