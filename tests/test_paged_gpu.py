@@ -64,6 +64,13 @@ CASES = [
     ([5, 7], [300, 1], 48, 3, 32, 512, 64, 1, True),
     ([77], [3000], 7, 7, 64, 1024, None, 0, True),
     ([2], [20000], 8, 8, 128, 64, None, 0, True),
+    # items cut anywhere, several to a CTA: short ones and long ones, one tile of rows and two side by side
+    ([1] * 40, [(997 * b) % 3100 for b in range(40)], 16, 8, 128, 64, None, 0, False),
+    ([3, 1] * 100, [(89 * b) % 300 for b in range(200)], 8, 4, 64, 16, None, 0, True),
+    ([400, 1, 30, 200], [5000, 3000, 1, 9000], 16, 4, 128, 64, None, 0, False),
+    ([250, 40, 256], [6000, 100, 3000], 8, 4, 64, 32, None, 0, True),
+    ([700], [12000], 12, 4, 96, 128, 4000, 700, False),
+    ([512, 256], [2000, 2300], 8, 8, 128, 128, 1500, 3, False),
 ]
 
 
