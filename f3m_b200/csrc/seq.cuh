@@ -179,6 +179,8 @@ __device__ __forceinline__ int parent_of(const int *parents, int i) {
 
 // A tensor map of (tokens, heads, width) rows whose boxes are 64 columns x box_heads x box_tokens, swizzled
 CUtensorMap seq_tensor_map(int type, const f3m_rows &r, int64_t tokens, int heads, int width, int box_heads = 1, int box_tokens = SEQ_TILE);
+// ... of (tokens, channels) rows, whose boxes are 128 bytes x 128 tokens, row after row
+CUtensorMap channel_tensor_map(int type, const f3m_rows &r, int64_t tokens, int channels);
 // ... and of pages, whose boxes are 64 columns x 1 head x `box` tokens of a page
 CUtensorMap page_tensor_map(int type, const f3m_cache &c, const f3m_pages &p, int box);
 // The word in mapped host memory where a kernel notes that a wait of its ran out; the next call reports it

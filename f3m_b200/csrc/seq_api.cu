@@ -28,7 +28,7 @@ void seq_check_error() {
 }
 
 // dims and box from the columns on, strides in elements from the second axis on
-static CUtensorMap tensor_map(int type, void *data, int axes, const cuuint64_t *dims, const int64_t *strides, const cuuint32_t *box) {
+static CUtensorMap tensor_map(int type, void *data, int axes, const cuuint64_t *dims, const int64_t *strides, const cuuint32_t *box, bool swizzled = true) {
     typedef CUresult (*Encode)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
                                const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
     static Encode encode = [] {
@@ -40,10 +40,11 @@ static CUtensorMap tensor_map(int type, void *data, int axes, const cuuint64_t *
     }();
     CUtensorMap m;
     cuuint64_t bytes[3];
-    for (int i = 0; i < axes - 1; i++) bytes[i] = 2ull * strides[i];
+    for (int i = 0; i < axes - 1; i++) bytes[i] = (type == F3M_TYPE_F32 ? 4ull : 2ull) * strides[i];
     const cuuint32_t step[4] = {1, 1, 1, 1};
-    const CUresult e = encode(&m, type == F3M_TYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, axes, data, dims, bytes, box, step,
-                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    const CUtensorMapDataType data_type = type == F3M_TYPE_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : type == F3M_TYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    const CUresult e = encode(&m, data_type, axes, data, dims, bytes, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzled ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     F3M_REQUIRE(e == CUDA_SUCCESS, F3M_ERR_ARG, "no tensor map for width %lld, axes of %lld, %lld (strides %lld, %lld), .. (driver error %d)", (long long)dims[0], (long long)dims[1],
                 (long long)dims[2], (long long)strides[0], (long long)strides[1], (int)e);
     return m;
@@ -53,6 +54,12 @@ CUtensorMap seq_tensor_map(int type, const f3m_rows &r, int64_t tokens, int head
     const int64_t strides[2] = {r.head_stride, r.token_stride};
     const cuuint32_t box[3] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_tokens};
     return tensor_map(type, r.data, 3, dims, strides, box);
+}
+CUtensorMap channel_tensor_map(int type, const f3m_rows &r, int64_t tokens, int channels) {
+    const cuuint64_t dims[3] = {(cuuint64_t)channels, 1, (cuuint64_t)tokens};
+    const int64_t strides[2] = {channels, r.token_stride};
+    const cuuint32_t box[3] = {type == F3M_TYPE_F32 ? 32u : 64u, 1, SEQ_TILE};
+    return tensor_map(type, r.data, 3, dims, strides, box, false);
 }
 CUtensorMap page_tensor_map(int type, const f3m_cache &c, const f3m_pages &p, int box_tokens) {
     const cuuint64_t dims[4] = {(cuuint64_t)c.width, (cuuint64_t)c.kv_heads, (cuuint64_t)c.page_tokens, (cuuint64_t)c.pages};
