@@ -1,5 +1,6 @@
 // Gated recurrence by channel: forward, gradients, one new token.
 #include <algorithm>
+#include <type_traits>
 #include "seq.cuh"
 
 namespace f3m {
@@ -45,13 +46,15 @@ __device__ __forceinline__ float advance(float h, float ld, float x) {
 // has it, and what leaves it as soon as it knows what entered: the nearest such state goes through the maps in between, always one after the other, so that a call's bits
 // do not depend on how far that was.  Then every run is walked again, from what enters it.  Each array is read and written once.
 //
+// Maps and states are told in words of 8 bytes that are all ones before, which no number here is: a word is there when it is another, and needs no flag and no fence.
+//
 // Gradients are the same from the end, on what flows back between tokens, c_t = a_t G_t: G_t = dout_t + c_(t+1), dx_t = G_t, dlog_decay_t = c_t h_(t-1).
 //
 // Blocks take units from a counter, tiles in order, so that what a tile waits for is always taken by a running block; a ninth warp takes the next one, starts its
 // copies, and looks back.
-constexpr int GR_WARPS = 8, GR_THREADS = 32 * (GR_WARPS + 1), GR_TILE = SEQ_TILE * 128;   // bytes of an array's tile
-template <bool BACK> constexpr int GR_STAGES = BACK ? 2 : 3;
-enum { GR_NOTHING = 0, GR_MAP = 1, GR_STATE = 2 };   // what a tile has told
+constexpr int GR_WARPS = 8, GR_THREADS = 32 * (GR_WARPS + 1), GR_TILE = SEQ_TILE * 128, GR_STAGES = 2;   // bytes of an array's tile
+constexpr int GR_LOOK = 8;   // tiles that are looked over at a time
+constexpr unsigned long long GR_NOTHING = ~0ull;
 
 struct RecurrenceKernel {
     RecurrenceArgs a;
@@ -59,40 +62,61 @@ struct RecurrenceKernel {
     int groups;         // of channels
     int units;
     bool counted;       // tiles look back: units come from the counter
-    int *told;          // the counter, and from word 4 on by unit
-    float4 *maps;       // by unit and lane: multipliers of its two channels, added
-    float2 *states;     // what left
+    unsigned *counter;  // all ones before the first
+    unsigned long long *told;   // by unit and lane: multipliers, added; by unit, lane: states, behind them
+    int64_t states;
     int *err;
 };
 
-// Multipliers: a or, where it is above exp(-1/4), a - 1, which is told by its sign (-0 for a decay of 1).  A decay next to 1 that is rounded to FP32 would leave a sum
-// over thousands of tokens 1e-5 off; a - 1 keeps its bits, as ld (1 + ld / 2 + ld^2 / 6 + ..) to the sixth power, 5e-8 off at most.
-__device__ __forceinline__ f32x2 multiplier(f32x2 ld) {
-    f32x2 y = fma2(ld, pack2(1.f / 720, 1.f / 720), pack2(1.f / 120, 1.f / 120));
-    y = fma2(y, ld, pack2(1.f / 24, 1.f / 24));
-    y = fma2(y, ld, pack2(1.f / 6, 1.f / 6));
-    y = fma2(y, ld, pack2(0.5f, 0.5f));
-    y = mul2(fma2(y, ld, pack2(1.f, 1.f)), ld);
+// exp of two log decays, at most 0: above -1/4 as 1 + ld (..), a polynomial of least maximum relative error (2.5e-7) by Lawson's iteration, so that a decay next to 1 is
+// rounded to the nearest -- the special-function unit's is not, and a sum over thousands of tokens would show it.  Below, that unit's.
+__device__ __forceinline__ f32x2 decay_of(f32x2 ld) {
+    f32x2 y = fma2(ld, pack2(0.037709992f, 0.037709992f), pack2(0.16605508f, 0.16605508f));
+    y = fma2(y, ld, pack2(0.4999693f, 0.4999693f));
+    y = fma2(y, ld, pack2(0.99999976f, 0.99999976f));
+    y = fma2(y, ld, pack2(1.f, 1.f));
     float near[2], far[2], l[2];
     unpack2(y, near[0], near[1]);
     unpack2(ld, l[0], l[1]);
     unpack2(mul2(ld, pack2(1.4426950408889634f, 1.4426950408889634f)), far[0], far[1]);
     return pack2(l[0] > -0.25f ? near[0] : ex2_approx(far[0]), l[1] > -0.25f ? near[1] : ex2_approx(far[1]));   // what is not a number stays that
 }
-// a h + x
-__device__ __forceinline__ f32x2 through(f32x2 h, f32x2 m, f32x2 x) {
-    float hl, hh, ml, mh;
-    unpack2(h, hl, hh);
-    unpack2(m, ml, mh);
-    const f32x2 kept = pack2(__int_as_float(__float_as_int(hl) & __float_as_int(ml) >> 31), __int_as_float(__float_as_int(hh) & __float_as_int(mh) >> 31));
-    return add2(fma2(m, h, x), kept);
+// Multipliers of maps, from sums of log decays below zero: exp or, above -1/4, exp - 1, which is below zero.  A map's multiplier next to 1 that is rounded to FP32 would leave a sum
+// over many tiles off where decays are all alike (3e-8 a tile); exp - 1 keeps its bits, by a polynomial as above (2.5e-9).
+__device__ __forceinline__ f32x2 multiplier(f32x2 ld) {
+    f32x2 y = fma2(ld, pack2(0.0075102216f, 0.0075102216f), pack2(0.041488953f, 0.041488953f));
+    y = fma2(y, ld, pack2(0.16665082f, 0.16665082f));
+    y = fma2(y, ld, pack2(0.4999995f, 0.4999995f));
+    y = mul2(fma2(y, ld, pack2(1.f, 1.f)), ld);
+    float near[2], far[2], l[2];
+    unpack2(y, near[0], near[1]);
+    unpack2(ld, l[0], l[1]);
+    unpack2(mul2(ld, pack2(1.4426950408889634f, 1.4426950408889634f)), far[0], far[1]);
+    return pack2(l[0] > -0.25f ? near[0] : ex2_approx(far[0]), l[1] > -0.25f ? near[1] : ex2_approx(far[1]));
 }
-__device__ __forceinline__ f32x2 held(f32x2 ld) {   // at most -0
+// h through a map
+__device__ __forceinline__ f32x2 through(f32x2 h, f32x2 m, f32x2 x) {
+    float ml, mh, kl, kh;
+    unpack2(m, ml, mh);
+    asm("set.lt.f32.f32 %0, %1, 0f00000000;" : "=f"(kl) : "f"(ml));   // 1 or 0
+    asm("set.lt.f32.f32 %0, %1, 0f00000000;" : "=f"(kh) : "f"(mh));
+    return fma2(m, h, fma2(pack2(kl, kh), h, x));
+}
+constexpr float GR_BELOW_ZERO = -1e-30f;   // where sums of log decays begin: too small to change one
+__device__ __forceinline__ f32x2 held(f32x2 ld) {
     float l, h;
     unpack2(ld, l, h);
-    asm("min.NaN.f32 %0, %0, %1;" : "+f"(l) : "f"(-0.f));
-    asm("min.NaN.f32 %0, %0, %1;" : "+f"(h) : "f"(-0.f));
+    asm("min.NaN.f32 %0, %0, %1;" : "+f"(l) : "f"(0.f));
+    asm("min.NaN.f32 %0, %0, %1;" : "+f"(h) : "f"(0.f));
     return pack2(l, h);
+}
+__device__ __forceinline__ void tell(unsigned long long *at, f32x2 v) {
+    asm volatile("st.relaxed.gpu.global.u64 [%0], %1;" ::"l"(at), "l"(v == GR_NOTHING ? 0x7fffffff7fffffffull : v) : "memory");
+}
+__device__ __forceinline__ f32x2 heard(const unsigned long long *at) {
+    f32x2 v;
+    asm volatile("ld.relaxed.gpu.global.u64 %0, [%1];" : "=l"(v) : "l"(at) : "memory");
+    return v;
 }
 
 // Two channels as they lie in memory
@@ -108,182 +132,198 @@ template <> struct Two<float> {
 };
 
 template <typename T, bool BACK>
-__global__ void __launch_bounds__(GR_THREADS, 2) recurrence_tiles(const __grid_constant__ RecurrenceKernel p) {
+__global__ void __launch_bounds__(GR_THREADS, BACK ? 2 : 3) recurrence_tiles(const __grid_constant__ RecurrenceKernel p) {
     typedef typename Two<T>::Raw Raw;
-    constexpr int ARRAYS = BACK ? 3 : 2, STAGES = GR_STAGES<BACK>, LANES = 128 / sizeof(Raw), RUNS = GR_WARPS * 32 / LANES, RUN = SEQ_TILE / RUNS, CHANNELS = 2 * LANES;
+    constexpr int ARRAYS = BACK ? 3 : 2, LANES = 128 / sizeof(Raw), RUNS = GR_WARPS * 32 / LANES, RUN = SEQ_TILE / RUNS, CHANNELS = 2 * LANES;
     extern __shared__ unsigned char raw[];
-    __shared__ __align__(8) uint64_t bars[STAGES];
-    __shared__ __align__(16) float4 runs_s[RUNS][LANES];   // maps of the runs: sums of log decays, added
-    __shared__ f32x2 enter_s[RUNS][LANES];
-    __shared__ int unit_s[STAGES], gave_up_s;
+    __shared__ __align__(8) uint64_t bars[GR_STAGES];
+    __shared__ f32x2 logs_s[RUNS][LANES], times_s[RUNS][LANES], added_s[RUNS][LANES], enter_s[RUNS][LANES];   // maps of the runs; what enters them
+    __shared__ __align__(16) int4 entry_s[GR_STAGES];   // {first row, length, first token, sequence} of a stage's unit
+    __shared__ int unit_s[GR_STAGES], gave_up_s;
     const RecurrenceArgs &a = p.a;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const unsigned char *base = raw + (-tc::smem_u32(raw) & 127);
     const uint32_t smem = tc::smem_u32(base), b_full = tc::smem_u32(&bars[0]);
-    const f32x2 none = pack2(-0.f, -0.f);   // the log of no decay, summed
+    const f32x2 none = pack2(GR_BELOW_ZERO, GR_BELOW_ZERO);
     if (threadIdx.x == 0) {
-        for (int i = 0; i < STAGES; i++) tc::mbar_init(b_full + 8 * i, 1);
+        for (int i = 0; i < GR_STAGES; i++) tc::mbar_init(b_full + 8 * i, 1);
         tc::fence_mbar_init();
         gave_up_s = 0;
     }
     __syncthreads();
     const Waits wait{&gave_up_s, p.err};
-    auto entry = [&](int u) {   // {first row, length, first token, sequence}
+    // units that the ninth warp's first lane has taken: the next one, known with its entry, and the one behind, asked for
+    int next = (int)blockIdx.x, behind = next, copies = 0;
+    int4 next_e = make_int4(0, 0, 0, 0);
+    auto ask = [&](int u) { return p.counted ? (int)(atomicAdd(p.counter, 1u) + 1u) : u + (int)gridDim.x; };
+    auto known = [&](int u) {
         const int i = u / p.groups;
-        return reinterpret_cast<const int4 *>(a.s.table)[seq_by_place(a.s, BACK ? a.s.tiles - 1 - i : i)];
+        return u < p.units ? reinterpret_cast<const int4 *>(a.s.table)[seq_by_place(a.s, BACK ? a.s.tiles - 1 - i : i)] : make_int4(0, 0, 0, 0);
     };
-    int taken = (int)blockIdx.x - (int)gridDim.x, copies = 0;   // of the ninth warp's first lane
-    auto take = [&](int stage) {   // the next unit, and its copies
-        taken = p.counted ? atomicAdd(p.told, 1) : taken + (int)gridDim.x;
-        unit_s[stage] = min(taken, p.units);
-        if (taken >= p.units) return;
-        const int4 e = entry(taken);
-        tc::mbar_expect_tx(b_full + 8 * stage, ARRAYS * GR_TILE);
-        for (int i = 0; i < ARRAYS; i++)   // of the outputs the tokens before
-            tc::tma_rows(smem + (ARRAYS * stage + i) * GR_TILE, &p.m[i], taken % p.groups * CHANNELS, 0, e.x + e.z - (i == 2), b_full + 8 * stage);
-        copies++;
+    auto start = [&](int stage) {
+        unit_s[stage] = min(next, p.units);
+        entry_s[stage] = next_e;
+        if (next < p.units) {
+            tc::mbar_expect_tx(b_full + 8 * stage, ARRAYS * GR_TILE);
+            for (int i = 0; i < ARRAYS; i++)   // of the outputs the tokens before
+                tc::tma_rows(smem + (ARRAYS * stage + i) * GR_TILE, &p.m[i], next % p.groups * CHANNELS, 0, next_e.x + next_e.z - (i == 2), b_full + 8 * stage);
+            copies++;
+        }
+        next = behind;
+        next_e = known(next);
+        behind = ask(behind);
     };
-    if (threadIdx.x == 32 * GR_WARPS)
-        for (int i = 0; i < STAGES - 1; i++) take(i);
+    if (threadIdx.x == 32 * GR_WARPS) {
+        if (p.counted) next = ask(0);
+        next_e = known(next);
+        behind = ask(next);
+        start(0);
+    }
     for (int n = 0;; n++) {
         __syncthreads();   // the unit is known, and all have done with the one before
-        const int stage = n % STAGES, u = unit_s[stage];
+        const int stage = n % GR_STAGES, u = unit_s[stage];
         if (u >= p.units) break;
-        const int4 e = entry(u);
-        const int g = u % p.groups, count = min(SEQ_TILE, e.y - e.z);
+        const int4 e = entry_s[stage];
+        const int g = u % p.groups;
         if (warp == GR_WARPS) {
-            if (lane == 0) take((n + STAGES - 1) % STAGES);
+            if (lane == 0) start((n + 1) % GR_STAGES);
             __syncwarp();
             const int before = BACK ? (e.y - 1) / SEQ_TILE - e.z / SEQ_TILE : e.z / SEQ_TILE;   // tiles before this one
             const bool last = BACK ? e.z == 0 : e.z + SEQ_TILE >= e.y;
             const int l = lane % LANES, c = g * CHANNELS + 2 * l;
             const float *in = BACK ? a.dstate_out : a.state_in;   // what enters the sequence, and leaves it
             float *out = BACK ? a.dstate_in : a.state_out;
-            const bool mine = lane < LANES && c < a.channels;
             f32x2 h = 0;
             if (before == 0 && in && c < a.channels) h = *reinterpret_cast<const f32x2 *>(in + (int64_t)e.w * a.channels + c);
-            auto run = [&](int i, f32x2 &log, f32x2 &added) {
-                const float4 r = runs_s[BACK ? RUNS - 1 - i : i][l];
-                log = pack2(r.x, r.y);
-                added = pack2(r.z, r.w);
-            };
+            auto run_of = [&](int i) { return BACK ? RUNS - 1 - i : i; };
+            unsigned long long *map = p.told + 2 * ((int64_t)u * LANES + l), *state = p.told + p.states + (int64_t)u * LANES + l;
+            const int64_t step = (int64_t)p.groups * LANES;
             __syncthreads();   // the runs' maps are there
-            f32x2 leaves = 0;   // told to the tiles behind: through the tile's own map, as those do who look over it
+            f32x2 times = 0, sum = 0;   // the tile's
             if (before) {
-                int *told = p.told + 4 + u;
-                f32x2 logs = none, sum = 0;
                 if (!last) {
-#pragma unroll 4
+                    f32x2 logs = none;
+#pragma unroll 8
                     for (int i = 0; i < RUNS; i++) {
-                        f32x2 log, added;
-                        run(i, log, added);
-                        logs = add2(logs, log);
-                        sum = through(sum, multiplier(log), added);
+                        logs = add2(logs, logs_s[run_of(i)][l]);
+                        sum = through(sum, times_s[run_of(i)][l], added_s[run_of(i)][l]);
                     }
-                    float4 map;
-                    unpack2(multiplier(logs), map.x, map.y);
-                    unpack2(sum, map.z, map.w);
-                    if (lane < LANES) __stcg(p.maps + (int64_t)u * LANES + l, map);
-                    __threadfence();
-                    __syncwarp();
-                    if (lane == 0) *(volatile int *)told = GR_MAP;
+                    times = multiplier(logs);
+                    if (lane < LANES) {
+                        tell(map, times);
+                        tell(map + 1, sum);
+                    }
                 }
-                // the nearest tile that has told what left it, with maps told by all in between
-                int near = 0;
+                f32x2 s[GR_LOOK], t[GR_LOOK], b[GR_LOOK];
                 for (uint32_t tries = 0;;) {
-                    const int what = lane < before ? *(volatile int *)(told - (int64_t)p.groups * (1 + lane)) : GR_NOTHING;
-                    const uint32_t has = __ballot_sync(0xffffffffu, what == GR_STATE), nothing = __ballot_sync(0xffffffffu, what == GR_NOTHING);
-                    near = __ffs(has) - 1;
-                    if (has && (nothing & ((1u << near) - 1)) == 0) break;
-                    if (__any_sync(0xffffffffu, gave_up_s) || ++tries > 2 * WAIT_TRIES) {   // a try takes a microsecond, about
+#pragma unroll
+                    for (int d = 1; d <= GR_LOOK; d++) {
+                        s[d - 1] = d <= before ? heard(state - d * step) : GR_NOTHING;
+                        if (d < GR_LOOK) {
+                            t[d - 1] = d < before ? heard(map - 2 * d * step) : GR_NOTHING;
+                            b[d - 1] = d < before ? heard(map - 2 * d * step + 1) : GR_NOTHING;
+                        }
+                    }
+                    // the nearest state that is told, with maps told by all in between
+                    bool there = false, open = true;
+#pragma unroll
+                    for (int d = 0; d < GR_LOOK; d++) {
+                        if (open && s[d] != GR_NOTHING) there = true;
+                        open &= !there && d + 1 < GR_LOOK && t[d] != GR_NOTHING && b[d] != GR_NOTHING;
+                    }
+                    if (__all_sync(0xffffffffu, there)) break;
+                    if (__any_sync(0xffffffffu, gave_up_s) || ++tries > 2 * WAIT_TRIES) {   // a try takes half a microsecond or more
                         if (lane == 0) {
                             gave_up_s = 1;
                             *(volatile int *)p.err = 1;
                         }
-                        near = 0;
                         break;
                     }
-                    __nanosleep(50);
                 }
-                __threadfence();
-                const float2 s = __ldcg(p.states + (int64_t)(u - p.groups * (1 + near)) * LANES + l);
-                h = pack2(s.x, s.y);
-#pragma unroll 4
-                for (int i = near - 1; i >= 0; i--) {
-                    const float4 map = __ldcg(p.maps + (int64_t)(u - p.groups * (1 + i)) * LANES + l);
-                    h = through(h, pack2(map.x, map.y), pack2(map.z, map.w));
+                bool on = false;   // from the nearest state on
+#pragma unroll
+                for (int d = GR_LOOK - 1; d >= 0; d--) {
+                    bool nearer = false;   // whether a nearer one is told
+#pragma unroll
+                    for (int i = 0; i < d; i++) nearer |= s[i] != GR_NOTHING;
+                    if (on) h = through(h, t[d], b[d]);
+                    if (!nearer && s[d] != GR_NOTHING) {
+                        h = s[d];
+                        on = true;
+                    }
                 }
-                leaves = through(h, multiplier(logs), sum);
             }
-#pragma unroll 4
+            f32x2 leaves = h;
+#pragma unroll 8
             for (int i = 0; i < RUNS; i++) {
-                f32x2 log, added;
-                run(i, log, added);
-                if (lane < LANES) enter_s[BACK ? RUNS - 1 - i : i][l] = h;
-                h = through(h, multiplier(log), added);
+                if (lane < LANES) enter_s[run_of(i)][l] = leaves;
+                leaves = through(leaves, times_s[run_of(i)][l], added_s[run_of(i)][l]);
             }
             __syncthreads();   // what enters the runs is there
             if (last) {
-                if (out && mine) *reinterpret_cast<f32x2 *>(out + (int64_t)e.w * a.channels + c) = h;
-            } else {
-                float2 s;
-                unpack2(before ? leaves : h, s.x, s.y);
-                if (lane < LANES) __stcg(p.states + (int64_t)u * LANES + l, s);
-                __threadfence();
-                __syncwarp();
-                if (lane == 0) *(volatile int *)(p.told + 4 + u) = GR_STATE;
+                if (out && lane < LANES && c < a.channels) *reinterpret_cast<f32x2 *>(out + (int64_t)e.w * a.channels + c) = leaves;
+            } else if (lane < LANES) {
+                tell(state, before ? through(h, times, sum) : leaves);   // through the tile's own map, as those do who look over it
             }
         } else {
-            const int run = warp * (32 / LANES) + lane / LANES, l = lane % LANES, r0 = run * RUN, c = g * CHANNELS + 2 * l;
+            const int run = warp * (32 / LANES) + lane / LANES, l = lane % LANES, r0 = run * RUN, c = g * CHANNELS + 2 * l, count = min(SEQ_TILE, e.y - e.z) - r0;
             const unsigned char *tile = base + ARRAYS * stage * GR_TILE + r0 * 128 + l * sizeof(Raw);
             auto raw_of = [&](int array, int i) { return *reinterpret_cast<const Raw *>(tile + array * GR_TILE + i * 128); };
             f32x2 m[RUN], logs = none, sum = 0;
-            Raw x[RUN];   // x, or dout
-            wait(b_full + 8 * stage, (n / STAGES) & 1);
+            wait(b_full + 8 * stage, (n / GR_STAGES) & 1);
+            auto first = [&](auto whole) {   // whether all of the run's tokens are the sequence's
+                const bool all = decltype(whole)::value;
 #pragma unroll
-            for (int k = 0; k < RUN; k++) {
-                const int i = BACK ? RUN - 1 - k : k;
-                x[i] = raw_of(0, i);
-                f32x2 ld = held(Two<T>::open(raw_of(1, i)));
-                if (r0 + i >= count) { x[i] = 0; ld = none; }   // behind the sequence
-                m[i] = multiplier(ld);
-                logs = add2(logs, ld);
-                sum = BACK ? through(add2(sum, Two<T>::open(x[i])), m[i], 0) : through(sum, m[i], Two<T>::open(x[i]));
-            }
-            float4 map;
-            unpack2(logs, map.x, map.y);
-            unpack2(sum, map.z, map.w);
-            runs_s[run][l] = map;
+                for (int k = 0; k < RUN; k++) {
+                    const int i = BACK ? RUN - 1 - k : k;
+                    const f32x2 ld = all || i < count ? held(Two<T>::open(raw_of(1, i))) : 0ull, x = all || i < count ? Two<T>::open(raw_of(0, i)) : 0ull;   // x, or dout
+                    m[i] = decay_of(ld);
+                    logs = add2(logs, ld);
+                    sum = BACK ? mul2(m[i], add2(sum, x)) : fma2(m[i], sum, x);
+                }
+            };
+            if (count >= RUN) first(std::true_type());
+            else first(std::false_type());
+            logs_s[run][l] = logs;
+            times_s[run][l] = multiplier(logs);
+            added_s[run][l] = sum;
             __syncthreads();   // the runs' maps are there
-            __syncthreads();   // what enters the runs is there
-            f32x2 h = enter_s[run][l];
             const int64_t t0 = (int64_t)e.x + e.z + r0;
-            const int rows = c < a.channels ? count - r0 : 0;   // of this run's
             T *y = reinterpret_cast<T *>(BACK ? a.dx.data : a.out.data) + t0 * (BACK ? a.dx.token_stride : a.out.token_stride) + c;
             T *z = BACK ? reinterpret_cast<T *>(a.dlog_decay.data) + t0 * a.dlog_decay.token_stride + c : nullptr;
+            const bool in = c < a.channels;
+            __syncthreads();   // what enters the runs is there
+            f32x2 h = enter_s[run][l];
+            auto second = [&](auto whole) {
+                const bool all = decltype(whole)::value;
 #pragma unroll
-            for (int k = 0; k < RUN; k++) {
-                const int i = BACK ? RUN - 1 - k : k;
-                if constexpr (!BACK) {
-                    h = through(h, m[i], Two<T>::open(x[i]));
-                    if (i < rows) *reinterpret_cast<Raw *>(y + i * a.out.token_stride) = Two<T>::close(h);
-                } else {
-                    const f32x2 d = add2(h, Two<T>::open(x[i]));
-                    h = through(d, m[i], 0);
-                    if (i >= rows) continue;
-                    *reinterpret_cast<Raw *>(y + i * a.dx.token_stride) = Two<T>::close(d);
-                    f32x2 past = Two<T>::open(raw_of(2, i));
-                    if (e.z + r0 + i == 0) past = a.state_in ? *reinterpret_cast<const f32x2 *>(a.state_in + (int64_t)e.w * a.channels + c) : 0;
-                    float ll, lh, dl, dh;
-                    unpack2(Two<T>::open(raw_of(1, i)), ll, lh);
-                    unpack2(mul2(h, past), dl, dh);
-                    *reinterpret_cast<Raw *>(z + i * a.dlog_decay.token_stride) = Two<T>::close(pack2(ll > 0.f ? 0.f : dl, lh > 0.f ? 0.f : dh));
+                for (int k = 0; k < RUN; k++) {
+                    const int i = BACK ? RUN - 1 - k : k;
+                    if (!all && i >= count) continue;
+                    const f32x2 x = Two<T>::open(raw_of(0, i));
+                    if constexpr (!BACK) {
+                        h = fma2(m[i], h, x);
+                        if (in) *reinterpret_cast<Raw *>(y + i * a.out.token_stride) = Two<T>::close(h);
+                    } else {
+                        const f32x2 d = add2(h, x);
+                        h = mul2(m[i], d);
+                        f32x2 past = Two<T>::open(raw_of(2, i));
+                        if (i == 0 && e.z + r0 == 0) past = a.state_in && in ? *reinterpret_cast<const f32x2 *>(a.state_in + (int64_t)e.w * a.channels + c) : 0;
+                        float ll, lh, dl, dh;
+                        unpack2(Two<T>::open(raw_of(1, i)), ll, lh);
+                        unpack2(mul2(h, past), dl, dh);
+                        if (!in) continue;
+                        *reinterpret_cast<Raw *>(y + i * a.dx.token_stride) = Two<T>::close(d);
+                        *reinterpret_cast<Raw *>(z + i * a.dlog_decay.token_stride) = Two<T>::close(pack2(ll > 0.f ? 0.f : dl, lh > 0.f ? 0.f : dh));
+                    }
                 }
-            }
+            };
+            if (count >= RUN) second(std::true_type());
+            else second(std::false_type());
         }
     }
-    if (threadIdx.x == 32 * GR_WARPS && copies)   // copies that nobody waited for, where the block gave up
-        for (int i = max(0, copies - STAGES); i < copies; i++) wait.drain(b_full + 8 * (i % STAGES), (i / STAGES) & 1);
+    if (threadIdx.x == 32 * GR_WARPS)   // copies that nobody waited for, where the block gave up
+        for (int i = max(0, copies - GR_STAGES); i < copies; i++) wait.drain(b_full + 8 * (i % GR_STAGES), (i / GR_STAGES) & 1);
 }
 
 // Sequences without tokens
@@ -316,12 +356,9 @@ __global__ void __launch_bounds__(256) recurrence_step_kernel(int64_t vectors, i
     Vec<T>::store(out.data, t * out.token_stride + c, h);
 }
 
-// the counter and what the tiles have told, maps, states; more than enough for any type
-static size_t told_bytes(const f3m_seqs &s, int channels) { return 16 + ((size_t)s.tiles * ((channels + 31) / 32) * 4 + 15) / 16 * 16; }
+// the counter, and two words of maps and one of states by tile and lane
 static size_t lane_places(const f3m_seqs &s, int channels) { return (size_t)s.tiles * ((channels + 63) / 64) * 32; }
-size_t recurrence_workspace(const f3m_seqs &s, int channels) {
-    return s.longest > SEQ_TILE ? told_bytes(s, channels) + lane_places(s, channels) * (sizeof(float4) + sizeof(float2)) : 0;
-}
+size_t recurrence_workspace(const f3m_seqs &s, int channels) { return s.longest > SEQ_TILE ? 16 + lane_places(s, channels) * 24 : 0; }
 
 template <typename T, bool BACK>
 static void recurrence_t(int type, const RecurrenceArgs &a, cudaStream_t s) {
@@ -337,23 +374,22 @@ static void recurrence_t(int type, const RecurrenceArgs &a, cudaStream_t s) {
     RecurrenceKernel p;
     p.a = a;
     constexpr int channels = 128 / sizeof(T);
-    const int arrays = BACK ? 3 : 2;
     p.groups = (a.channels + channels - 1) / channels;
     F3M_REQUIRE((int64_t)a.s.tiles * p.groups <= 0x7fff0000, F3M_ERR_OVERFLOW, "%d tiles of %d channels do not fit in 31 bits", a.s.tiles, a.channels);
     p.units = a.s.tiles * p.groups;
     p.counted = a.s.longest > SEQ_TILE;
-    p.told = reinterpret_cast<int *>(a.ws);
-    p.maps = reinterpret_cast<float4 *>(reinterpret_cast<char *>(a.ws) + told_bytes(a.s, a.channels));
-    p.states = reinterpret_cast<float2 *>(p.maps + lane_places(a.s, a.channels));
+    p.counter = reinterpret_cast<unsigned *>(a.ws);
+    p.told = reinterpret_cast<unsigned long long *>(reinterpret_cast<char *>(a.ws) + 16);
+    p.states = 2 * (int64_t)lane_places(a.s, a.channels);
     p.err = seq_error_word();
     p.m[0] = channel_tensor_map(type, BACK ? a.dout : a.x, a.s.tokens, a.channels);
     p.m[1] = channel_tensor_map(type, a.log_decay, a.s.tokens, a.channels);
     if (BACK) p.m[2] = channel_tensor_map(type, a.out, a.s.tokens, a.channels);
-    if (p.counted) F3M_CUDA(cudaMemsetAsync(p.told, 0, 16 + 4 * (size_t)p.units, s));
-    const int bytes = GR_STAGES<BACK> * arrays * GR_TILE + 128;
+    if (p.counted) F3M_CUDA(cudaMemsetAsync(a.ws, 0xff, recurrence_workspace(a.s, a.channels), s));
+    const int bytes = GR_STAGES * (BACK ? 3 : 2) * GR_TILE + 128;
     static SharedMemory allowed;
     allowed.allow(recurrence_tiles<T, BACK>, bytes);
-    recurrence_tiles<T, BACK><<<std::min(p.units, 2 * NUM_SMS_HINT), GR_THREADS, bytes, s>>>(p);
+    recurrence_tiles<T, BACK><<<std::min(p.units, (BACK ? 2 : 3) * NUM_SMS_HINT), GR_THREADS, bytes, s>>>(p);
     F3M_LAUNCH_CHECK();
 }
 template <bool BACK>
