@@ -53,7 +53,6 @@ __device__ __forceinline__ float advance(float h, float ld, float x) {
 // Blocks take units from a counter, tiles in order, so that what a tile waits for is always taken by a running block; a ninth warp takes the next one, starts its
 // copies, and looks back.
 constexpr int GR_WARPS = 8, GR_THREADS = 32 * (GR_WARPS + 1), GR_TILE = SEQ_TILE * 128, GR_STAGES = 2;   // bytes of an array's tile
-constexpr int GR_LOOK = 8;   // tiles that are looked over at a time
 constexpr unsigned long long GR_NOTHING = ~0ull;
 
 struct RecurrenceKernel {
@@ -214,42 +213,30 @@ __global__ void __launch_bounds__(GR_THREADS, BACK ? 2 : 3) recurrence_tiles(con
                         tell(map + 1, sum);
                     }
                 }
-                f32x2 s[GR_LOOK], t[GR_LOOK], b[GR_LOOK];
+                // a lane looks at one of the 32 tiles before: the nearest that has told its state, with maps told by all in between
                 for (uint32_t tries = 0;;) {
-#pragma unroll
-                    for (int d = 1; d <= GR_LOOK; d++) {
-                        s[d - 1] = d <= before ? heard(state - d * step) : GR_NOTHING;
-                        if (d < GR_LOOK) {
-                            t[d - 1] = d < before ? heard(map - 2 * d * step) : GR_NOTHING;
-                            b[d - 1] = d < before ? heard(map - 2 * d * step + 1) : GR_NOTHING;
+                    const bool is = lane < before;
+                    const f32x2 s = is ? heard(state - l - (1 + lane) * step) : GR_NOTHING, t = is ? heard(map - 2 * (l + (1 + lane) * step)) : GR_NOTHING;   // its first word
+                    const uint32_t has = __ballot_sync(0xffffffffu, s != GR_NOTHING), maps = __ballot_sync(0xffffffffu, t != GR_NOTHING);
+                    const int near = __ffs(has) - 1;
+                    bool all = has && (~maps & ((1u << near) - 1)) == 0;
+                    if (all) {   // the channels' own words, each of which tells whether it is there
+                        h = heard(state - (1 + near) * step);
+                        all = h != GR_NOTHING;
+#pragma unroll 8
+                        for (int d = near; d > 0; d--) {
+                            const f32x2 times = heard(map - 2 * d * step), added = heard(map - 2 * d * step + 1);
+                            all &= times != GR_NOTHING && added != GR_NOTHING;
+                            h = through(h, times, added);
                         }
                     }
-                    // the nearest state that is told, with maps told by all in between
-                    bool there = false, open = true;
-#pragma unroll
-                    for (int d = 0; d < GR_LOOK; d++) {
-                        if (open && s[d] != GR_NOTHING) there = true;
-                        open &= !there && d + 1 < GR_LOOK && t[d] != GR_NOTHING && b[d] != GR_NOTHING;
-                    }
-                    if (__all_sync(0xffffffffu, there)) break;
+                    if (__all_sync(0xffffffffu, all)) break;
                     if (__any_sync(0xffffffffu, gave_up_s) || ++tries > 2 * WAIT_TRIES) {   // a try takes half a microsecond or more
                         if (lane == 0) {
                             gave_up_s = 1;
                             *(volatile int *)p.err = 1;
                         }
                         break;
-                    }
-                }
-                bool on = false;   // from the nearest state on
-#pragma unroll
-                for (int d = GR_LOOK - 1; d >= 0; d--) {
-                    bool nearer = false;   // whether a nearer one is told
-#pragma unroll
-                    for (int i = 0; i < d; i++) nearer |= s[i] != GR_NOTHING;
-                    if (on) h = through(h, t[d], b[d]);
-                    if (!nearer && s[d] != GR_NOTHING) {
-                        h = s[d];
-                        on = true;
                     }
                 }
             }
