@@ -767,38 +767,38 @@ static void paged_t(const PagedArgs &a, cudaStream_t s) {
 void paged_attention(int type, const PagedArgs &a, cudaStream_t s) { type == F3M_TYPE_BF16 ? paged_t<__nv_bfloat16>(a, s) : paged_t<__half>(a, s); }
 
 // ---- accepted paths -----------------------------------------------------------------------------------------------------------
-// A thread has 16 bytes of a row of keys or values and takes the places in order, KP_ROWS at a time: read, then written.  A place is read for one in front of it or
-// for itself (kept[j] >= j), so that what is written has been read.
-constexpr int KP_ROWS = 8, KP_THREADS = 128;
-__global__ void __launch_bounds__(KP_THREADS) keep_paths(f3m_cache c, const int *kept, int64_t kept_stride, int most, const int *counts) {
-    const int b = blockIdx.x, per = c.width / 8, x = blockIdx.y * KP_THREADS + threadIdx.x;
-    if (x >= 2 * c.kv_heads * per) return;
-    const f3m_pages &p = x < c.kv_heads * per ? c.k : c.v;
-    const int h = x / per % c.kv_heads, col = 8 * (x % per), length = paged_length(c, b), count = min(max(counts[b], 0), most);
+// A CTA has the keys or the values of one head of a sequence, and takes its places in order, KP_ROWS at a time: read, then written.  A place is read for one in front of it or
+// for itself (kept[j] >= j), so that what is written has been read.  64 paths of up to 30 tokens, 8 heads, width 128: three dependent loads and a store, 4.9 us (a thread for all
+// places of 16 bytes, 8 at a time: 17.9).
+constexpr int KP_STEP = 16, KP_EACH = 4, KP_ROWS = KP_STEP * KP_EACH, KP_THREADS = 16 * KP_STEP;
+__global__ void __launch_bounds__(KP_THREADS) keep_paths(const __grid_constant__ f3m_cache c, const int *kept, int64_t kept_stride, int most, const int *counts) {
+    const int b = blockIdx.x, h = blockIdx.y >> 1, col = 8 * (threadIdx.x & 15), length = paged_length(c, b), count = min(max(counts[b], 0), most);
+    const f3m_pages &p = blockIdx.y & 1 ? c.v : c.k;
     uint16_t *data = reinterpret_cast<uint16_t *>(p.data) + col;
     for (int j0 = 0; j0 < count; j0 += KP_ROWS) {
-        uint4 v[KP_ROWS];
-        int64_t to[KP_ROWS];
+        uint4 v[KP_EACH];
+        int64_t to[KP_EACH];
 #pragma unroll
-        for (int r = 0; r < KP_ROWS; r++) {
-            const int j = j0 + r;
+        for (int r = 0; r < KP_EACH; r++) {
+            const int j = j0 + KP_STEP * r + (threadIdx.x >> 4), m = j < count && col < c.width ? kept[b * kept_stride + j] : -1;
             to[r] = -1;
-            if (j >= count) continue;
-            const int m = kept[b * kept_stride + j];
             if (m <= j) continue;   // its place already, or no place of a path
             const int page = paged_page(c, b, (int64_t)length + m), there = paged_page(c, b, (int64_t)length + j);
             if (page < 0 || there < 0) continue;
             to[r] = paged_at(c, p, there, (int64_t)length + j, h);
             v[r] = *reinterpret_cast<const uint4 *>(data + paged_at(c, p, page, (int64_t)length + m, h));
         }
+        __syncthreads();
 #pragma unroll
-        for (int r = 0; r < KP_ROWS; r++)
+        for (int r = 0; r < KP_EACH; r++)
             if (to[r] >= 0) *reinterpret_cast<uint4 *>(data + to[r]) = v[r];
+        __syncthreads();
     }
 }
 
 void paged_keep(const f3m_cache &c, const int *kept, int64_t kept_stride, int most, const int *counts, cudaStream_t s) {
-    keep_paths<<<dim3(c.sequences, (2 * c.kv_heads * (c.width / 8) + KP_THREADS - 1) / KP_THREADS), KP_THREADS, 0, s>>>(c, kept, kept_stride, most, counts);
+    F3M_REQUIRE(c.kv_heads <= 32767, F3M_ERR_UNSUPPORTED, "%d key heads", c.kv_heads);
+    keep_paths<<<dim3(c.sequences, 2 * c.kv_heads), KP_THREADS, 0, s>>>(c, kept, kept_stride, most, counts);
     F3M_LAUNCH_CHECK();
 }
 

@@ -64,30 +64,31 @@ class Rotation:
         self._ref = C.byref(self._table)
 
 
-def _pages(t: torch.Tensor, what: str) -> Pages:
-    (ps, ts, hs, cs), (pages, tokens, heads, width), at = t.stride(), t.shape, t.data_ptr()
-    if t.numel() == 0:
-        return Pages(None, 0, 0, 0)
-    if pages == 1:
+def _pages(t: torch.Tensor, shape, what: str) -> Pages:
+    (ps, ts, hs, cs), (pages, _, heads, width), at = t.stride(), shape, t.data_ptr()
+    if pages < 2:
+        if pages == 0:
+            return Pages(None, 0, 0, 0)
         ps = 0
     if heads == 1:
         hs = 0
-    if cs != 1 or (at | 2 * ps | 2 * ts | 2 * hs) & 15 or ts < width or (heads > 1 and hs < width) or (pages > 1 and ps < width):
+    if cs != 1 or (at | 2 * (ps | ts | hs)) & 15 or ts < width or (hs < width and heads > 1) or (ps < width and pages > 1):
         raise ValueError(f"{what} is used in place: contiguous columns, strides multiples of 8 elements, data on 16 bytes")
     return Pages(at, ps, ts, hs)
 
 
 def _numbers(t: torch.Tensor, shape, device, what: str) -> torch.Tensor:
-    if t.dtype != torch.int32 or tuple(t.shape) != tuple(shape) or t.device != device:
+    if t.dtype is not torch.int32 or t.shape != shape or t.device != device:
         raise TypeError(f"{what} must be an int32 array {tuple(shape)} on {device}")
     return t
 
 
 def _cache(k_pages, v_pages, page_table, lengths):
     """The library's view of a cache, and the arrays that it points to."""
-    if k_pages.dim() != 4 or v_pages.shape != k_pages.shape:
+    shape, device = k_pages.shape, k_pages.device
+    if len(shape) != 4 or v_pages.shape != shape:
         raise ValueError(f"k_pages {tuple(k_pages.shape)} and v_pages {tuple(v_pages.shape)} are (pages, page_tokens, kv_heads, width) arrays")
-    pages, page_tokens, kv_heads, width = k_pages.shape
+    pages, page_tokens, kv_heads, width = shape
     _check_width(width)
     if page_tokens < 8 or page_tokens & (page_tokens - 1):
         raise ValueError(f"pages of {page_tokens} tokens: not a power of two from 8 on")
@@ -95,13 +96,15 @@ def _cache(k_pages, v_pages, page_table, lengths):
         raise ValueError("a cache without key heads")
     if page_table.dim() != 2:
         raise ValueError("page_table is a (sequences, most) array")
-    n, most = page_table.shape
-    page_table = _numbers(page_table, (n, most), k_pages.device, "page_table")
-    if most > 1 and page_table.stride(1) != 1 or n > 1 and page_table.stride(0) < 0:
+    n, most = sizes = page_table.shape
+    _numbers(page_table, sizes, device, "page_table")
+    step, one = page_table.stride()
+    if one != 1 and most > 1:
         page_table = page_table.contiguous()
-    lengths = _numbers(lengths, (n,), k_pages.device, "lengths").contiguous()
-    c = Cache(_pages(k_pages, "k_pages"), _pages(v_pages, "v_pages"), pages, page_tokens, kv_heads, width, page_table.data_ptr(),
-              page_table.stride(0) if n > 1 else most, most, n, lengths.data_ptr())
+        step = most
+    lengths = _numbers(lengths, sizes[:1], device, "lengths").contiguous()
+    c = Cache(_pages(k_pages, shape, "k_pages"), _pages(v_pages, shape, "v_pages"), pages, page_tokens, kv_heads, width, page_table.data_ptr(), step if n > 1 else most, most, n,
+              lengths.data_ptr())
     return c, (page_table, lengths)
 
 

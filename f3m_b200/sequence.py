@@ -182,7 +182,10 @@ def _refuse_tangents(*tensors):
 
 
 def _needs_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            return torch.is_grad_enabled()
+    return False
 
 
 # ---------------------------------------------------------------------------------------------------------------------
