@@ -6,35 +6,17 @@ namespace f3m {
 
 // ---- new tokens to their pages ----------------------------------------------------------------------------------------------
 // A CTA has AP_TOKENS neighbouring tokens of a sequence.  Their places and angles are taken once for all heads: the part of a whole turn is position * turns modulo
-// 2^64, exact for any position, and what is left, in FP32, is at most half a turn.  Then 16-byte vectors, as (token, head, vector); a vector of a half-split
-// rotation brings its partner.  Memory is the bound: every array is read and written once.
-constexpr int AP_TOKENS = 4, AP_THREADS = 256;
+// 2^64, exact for any position, and what is left, in FP32, is at most half a turn.  Then its rows, (token, head) of queries, keys and values, 16 lanes or 8 to a row with 16 bytes
+// each; a lane's partner in a half-split rotation hands its columns over.  Memory is the bound: every array is read and written once.
+constexpr int AP_TOKENS = 2, AP_THREADS = 256;
 
 template <typename T>
-__device__ __forceinline__ void rotate8(uint4 &x, uint4 &y, const float2 *turn, bool interleaved) {
-    uint32_t *xs = reinterpret_cast<uint32_t *>(&x), *ys = reinterpret_cast<uint32_t *>(&y);
-    if (interleaved) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const float2 f = Half<T>::unpack(xs[i]), c = turn[i];
-            xs[i] = Half<T>::pack(f.x * c.x - f.y * c.y, f.x * c.y + f.y * c.x);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const float2 f = Half<T>::unpack(xs[i]), g = Half<T>::unpack(ys[i]), c = turn[2 * i], d = turn[2 * i + 1];
-            xs[i] = Half<T>::pack(f.x * c.x - g.x * c.y, f.y * d.x - g.y * d.y);
-            ys[i] = Half<T>::pack(f.x * c.y + g.x * c.x, f.y * d.y + g.y * d.x);
-        }
-    }
-}
-
-template <typename T>
-__global__ void __launch_bounds__(AP_THREADS) append_tokens(const __grid_constant__ AppendArgs a) {
+__global__ void __launch_bounds__(AP_THREADS, 8) append_tokens(const __grid_constant__ AppendArgs a) {
     __shared__ int slot_s[AP_TOKENS], pos_s[AP_TOKENS], page_s[AP_TOKENS];
-    __shared__ float2 turn_s[AP_TOKENS][F3M_MAX_WIDTH / 2];
+    __shared__ __align__(16) float2 turn_s[AP_TOKENS][F3M_MAX_WIDTH / 2];   // cosines and sines, two pairs of each lane side by side, then the lanes' next two
     const int4 e = reinterpret_cast<const int4 *>(a.s.table)[seq_by_place(a.s, blockIdx.x)];
     const int i0 = e.z + AP_TOKENS * blockIdx.y, m = min(AP_TOKENS, min(e.z + SEQ_TILE, e.y) - i0), half = a.rotation.columns / 2;
+    const int own = a.rotation.interleaved ? 4 : 8, turned = half / own;   // pairs of a lane, lanes with pairs of their own
     if (m <= 0) return;
     if (threadIdx.x < m) {
         const int i = i0 + threadIdx.x, length = paged_length(a.c, e.w);
@@ -54,34 +36,55 @@ __global__ void __launch_bounds__(AP_THREADS) append_tokens(const __grid_constan
         const int64_t part = (int64_t)((uint64_t)pos_s[t] * a.rotation.turns[i]);   // of a whole turn, 2^64; as signed the nearest one
         float s, c;
         sincospif(0x1p-63f * (float)part, &s, &c);
-        turn_s[t][i] = make_float2(c, s);
+        turn_s[t][i % own / 2 * 2 * turned + 2 * (i / own) + (i & 1)] = make_float2(c, s);
     }
     __syncthreads();
-    const int vectors = a.c.width / 8, moved = a.rotation.interleaved ? 0 : half / 8;   // the second half's vectors come with the first's
-    const int turned = vectors - moved, rows = a.heads + a.c.kv_heads, units = rows * turned + a.c.kv_heads * vectors;
-    for (int x = threadIdx.x; x < m * units; x += AP_THREADS) {
-        const int t = x / units, u = x % units;
-        const bool value = u >= rows * turned;
-        const int w = value ? u - rows * turned : u, per = value ? vectors : turned;
-        int h = w / per, c = w % per;
-        const bool query = !value && h < a.heads;
-        if (!value && !query) h -= a.heads;
-        const bool pair = !value && c < moved, rotated = !value && 8 * c < (moved ? half : 2 * half);
-        if (!value && c >= moved) c += moved;   // behind the pairs; of no consequence where moved is 0
-        const f3m_rows &from = query ? a.q : value ? a.v : a.k;
-        const uint16_t *src = reinterpret_cast<const uint16_t *>(from.data) + (int64_t)(e.x + i0 + t) * from.token_stride + (int64_t)h * from.head_stride + 8 * c;
-        uint16_t *dst;
-        if (query) dst = reinterpret_cast<uint16_t *>(a.q_out.data) + (int64_t)(e.x + i0 + t) * a.q_out.token_stride + (int64_t)h * a.q_out.head_stride + 8 * c;
-        else {
-            if (page_s[t] < 0) continue;
-            const f3m_pages &p = value ? a.c.v : a.c.k;
-            dst = reinterpret_cast<uint16_t *>(p.data) + paged_at(a.c, p, page_s[t], slot_s[t], h) + 8 * c;
+    const int lanes = a.c.width > 64 ? 16 : 8, step = AP_THREADS / lanes, c = threadIdx.x & (lanes - 1), per_token = a.heads + 2 * a.c.kv_heads;
+    const bool inside = 8 * c < a.c.width, split = !a.rotation.interleaved, second = 8 * c >= half;
+    const bool turns = 8 * c < 2 * half;
+    const int partner = (threadIdx.x & 31) + (second ? -half : half) / 8, at = 2 * (split && second ? c - turned : c);
+    int t = 0, j = threadIdx.x / lanes;
+    for (int r = 0; r < m * per_token; r += step, j += step) {   // whole warps
+        while (j >= per_token) { j -= per_token; t++; }
+        const bool query = j < a.heads, value = j >= a.heads + a.c.kv_heads;
+        const int h = query ? j : value ? j - a.heads - a.c.kv_heads : j - a.heads;
+        uint16_t *dst = nullptr;
+        uint4 f = make_uint4(0u, 0u, 0u, 0u);
+        if (t < m && inside) {
+            const int64_t row = e.x + i0 + t;
+            if (query) dst = reinterpret_cast<uint16_t *>(a.q_out.data) + row * a.q_out.token_stride + (int64_t)h * a.q_out.head_stride + 8 * c;
+            else if (page_s[t] >= 0) {
+                const f3m_pages &p = value ? a.c.v : a.c.k;
+                dst = reinterpret_cast<uint16_t *>(p.data) + paged_at(a.c, p, page_s[t], slot_s[t], h) + 8 * c;
+            }
+            const f3m_rows &from = query ? a.q : value ? a.v : a.k;
+            f = *reinterpret_cast<const uint4 *>(reinterpret_cast<const uint16_t *>(from.data) + row * from.token_stride + (int64_t)h * from.head_stride + 8 * c);
         }
-        uint4 f = *reinterpret_cast<const uint4 *>(src), g = make_uint4(0u, 0u, 0u, 0u);
-        if (pair) g = *reinterpret_cast<const uint4 *>(src + half);
-        if (rotated) rotate8<T>(f, g, turn_s[t] + (a.rotation.interleaved ? 4 * c : 8 * c), a.rotation.interleaved);
-        *reinterpret_cast<uint4 *>(dst) = f;
-        if (pair) *reinterpret_cast<uint4 *>(dst + half) = g;
+        uint32_t x[4] = {f.x, f.y, f.z, f.w}, y[4];
+        if (split && half)
+#pragma unroll
+            for (int i = 0; i < 4; i++) y[i] = __shfl_sync(0xffffffffu, x[i], partner & 31);
+        if (turns && !value && t < m) {
+            const float4 *turn = reinterpret_cast<const float4 *>(turn_s[t] + at);   // cosine and sine, of two pairs
+            if (split) {   // x cos - y sin, and of the second half x cos + y sin
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float2 v = Half<T>::unpack(x[i]), w = Half<T>::unpack(y[i]);
+                    const float4 p = turn[i * turned];
+                    const float s0 = second ? p.y : -p.y, s1 = second ? p.w : -p.w;
+                    x[i] = Half<T>::pack(v.x * p.x + w.x * s0, v.y * p.z + w.y * s1);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; i += 2) {
+                    const float2 v = Half<T>::unpack(x[i]), w = Half<T>::unpack(x[i + 1]);
+                    const float4 p = turn[i / 2 * turned];
+                    x[i] = Half<T>::pack(v.x * p.x - v.y * p.y, v.x * p.y + v.y * p.x);
+                    x[i + 1] = Half<T>::pack(w.x * p.z - w.y * p.w, w.x * p.w + w.y * p.z);
+                }
+            }
+        }
+        if (dst) *reinterpret_cast<uint4 *>(dst) = make_uint4(x[0], x[1], x[2], x[3]);
     }
 }
 
