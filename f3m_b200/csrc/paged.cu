@@ -211,7 +211,7 @@ template <typename T, int NB, int TILES>
 __global__ void __launch_bounds__(128 * TILES + 64, 3 - TILES) paged_tiles(const __grid_constant__ PagedKernel p) {
     constexpr int ROWS = 128 * TILES, THREADS = ROWS + 64, WARPS = THREADS / 32, COPY = 4 * TILES, PRODUCTS = COPY + 1;
     extern __shared__ unsigned char raw[];
-    __shared__ __align__(8) uint64_t bars[2 * PG_MAX_SLOTS + 2 * PG_RING + 14];
+    __shared__ __align__(8) uint64_t bars[2 * PG_MAX_SLOTS + 2 * PG_RING + 16];
     __shared__ PagedPart ring_s[PG_RING];
     __shared__ long long warp_s[WARPS], start_s[2];
     __shared__ uint32_t tmem_s, bad_s[2][4], there_s[PG_THERE];
@@ -230,7 +230,7 @@ __global__ void __launch_bounds__(128 * TILES + 64, 3 - TILES) paged_tiles(const
 
     if (warp == COPY) tc::tmem_alloc(tc::smem_u32(&tmem_s), 256 * TILES);
     const uint32_t b_full = tc::smem_u32(&bars[0]), b_free = b_full + 8 * PG_MAX_SLOTS, b_part = b_free + 8 * PG_MAX_SLOTS, b_part_free = b_part + 8 * PG_RING, b_q = b_part_free + 8 * PG_RING,
-                   b_q_free = b_q + 16, b_s = b_q + 32, b_p = b_q + 48, b_p2 = b_q + 64, b_o = b_q + 80, b_o_read = b_q + 96, b_none = b_q + 104;
+                   b_q_free = b_q + 16, b_s = b_q + 32, b_p = b_q + 48, b_p2 = b_q + 64, b_o = b_q + 80, b_o_read = b_q + 96, b_none = b_q + 104, b_clear = b_q + 112;
     if (tid == 0) {
         for (int i = 0; i < 2 * PG_MAX_SLOTS; i++) tc::mbar_init(b_full + 8 * i, 1);   // landed, free
         for (int i = 0; i < PG_RING; i++) {
@@ -244,6 +244,7 @@ __global__ void __launch_bounds__(128 * TILES + 64, 3 - TILES) paged_tiles(const
             tc::mbar_init(b_p + 8 * t, 128);     // weights of the first 64 keys written
             tc::mbar_init(b_p2 + 8 * t, 128);    // of the other 64
             tc::mbar_init(b_o + 8 * t, 1);       // O ready
+            tc::mbar_init(b_clear + 8 * t, 4);   // values of a tile that is seen in part are finite, of one such tile and of the next
         }
         tc::mbar_init(b_o_read, ROWS);
         tc::mbar_init(b_none, 1);                // no products in flight
@@ -446,7 +447,7 @@ __global__ void __launch_bounds__(128 * TILES + 64, 3 - TILES) paged_tiles(const
         const uint32_t lanes = (uint32_t)(32 * wq) << 16, t_s = tmem + 128 * t + lanes, t_o = t_out + 128 * t + lanes;
         constexpr uint32_t exponent = Half<T>::type == F3M_TYPE_BF16 ? 0x7f80u : 0x7c00u;
         const bool wide = p.wide;
-        int tile = 0, had_b = -1, had_i0 = 0;   // tiles of keys so far; the tree that is at hand
+        int tile = 0, cleared = 0, had_b = -1, had_i0 = 0;   // tiles of keys so far, those that were seen in part; the tree that is at hand
         for (int parts = 0;; parts++) {
             // whether there is a part is one thread's word to all: they meet at barriers inside
             const int slot_r = parts % PG_RING;
@@ -459,7 +460,6 @@ __global__ void __launch_bounds__(128 * TILES + 64, 3 - TILES) paged_tiles(const
             const PagedPart &part = ring_s[slot_r];
             const PagedItem &w = part.w;   // stays where it is: few of its numbers are worth a register
             const int j0 = part.j0, j1 = part.j1, length = w.length, tokens = w.tokens;
-            int scrubs = 0;
             if (a.parents && (w.b != had_b || w.i0 != had_i0)) {   // depths of the item's tokens, and which new tokens each sees
                 had_b = w.b; had_i0 = w.i0;
                 for (int m = tid; m < had_i0 + tokens; m += ROWS) parent_s[m] = (int16_t)parent_of(a.parents + w.row0, m);
@@ -491,8 +491,10 @@ __global__ void __launch_bounds__(128 * TILES + 64, 3 - TILES) paged_tiles(const
                 const bool whole = by_all && there == 0xffffu;
                 uint32_t seen[4] = {};
                 if (!whole) {
-                    // Values that are not finite leave the tile.  Scores of this tile tell that the values in this slot before have landed: the wait names a phase's parity only
-                    uint32_t *bads = bad_s[scrubs++ & 1];
+                    // Values that are not finite leave the tile, by the first tile of rows' threads, which may be a tile of keys ahead of the second's.  Scores of this tile tell
+                    // that the values in this slot before have landed: the wait names a phase's parity only
+                    uint32_t *bads = bad_s[cleared & 1];
+                    const uint32_t b_this = b_clear + 8 * (cleared & 1), turn = cleared++ >> 1 & 1;
                     if (t == 0) {
                         const int xv = 2 * tile + 1, sv = xv % slots;
                         wait(b_full + 8 * sv, (xv / slots) & 1);
@@ -521,9 +523,13 @@ __global__ void __launch_bounds__(128 * TILES + 64, 3 - TILES) paged_tiles(const
                             tc::fence_async_smem();
                         }
                         const uint32_t b = __ballot_sync(0xffffffffu, !finite);
-                        if (lane == 0) bads[wq] = b;
+                        if (lane == 0) {
+                            bads[wq] = b;
+                            tc::mbar_arrive(b_this);
+                        }
                     }
-                    tc::bar_sync(1, ROWS);
+                    wait(b_this, turn);
+                    __syncwarp();
 #pragma unroll
                     for (int q = 0; q < 4; q++) {
                         seen[q] = seen_keys(a, length, key + 32 * q, there >> 4 * q, pos, up, above);

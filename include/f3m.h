@@ -404,6 +404,8 @@ int f3m_gated_recurrence_step(int32_t n, int32_t type, int32_t channels, f3m_row
  * page_tokens is a power of two, 8 or more.  A number in the table outside 0..pages-1 is no page: what would lie there is not written, and not seen.  lengths (DEVICE,
  * sequences): tokens in the cache before the call's new ones; values outside 0..table_pages * page_tokens are taken as the nearest of these.  New token
  * i of sequence b, in the packed order of `seqs`, is token lengths[b] + i of the cache, and where that lies behind the table's last page it is neither written nor seen.
+ * What places behind a sequence's tokens and pages outside its window hold does not matter, whatever it is; what is not finite in a key or value reaches the rows that see it
+ * and no others.
  *
  * parents (DEVICE, tokens; NULL: new tokens follow one another): new tokens are a tree, parents[t] the number, among the sequence's new tokens, of the one before
  * token t, -1 where that is the cache's last one.  A parent comes before its children: values outside -1..i-1 are taken as -1.  At most F3M_TREE_MAX new tokens a sequence.  The
@@ -431,7 +433,7 @@ typedef struct f3m_rotation {
  * rotated into q_out, which may be q.  No two sequences may have new tokens in one place. */
 int f3m_paged_append(const f3m_seqs *seqs, int32_t type, const f3m_cache *cache, f3m_rows k, f3m_rows v, const int32_t *parents, const f3m_rotation *rotation,
                      int32_t heads, f3m_rows q, f3m_rows q_out, void *stream);
-/* Attention of the new tokens, which the pages hold already.  A new token at position p sees cached token j if p - j < window or j < sinks, and of the new tokens itself
+/* Attention of the new tokens, whose keys and values the pages hold already.  A new token at position p sees cached token j if p - j < window or j < sinks, and of the new tokens itself
  * and those above it, at positions p', if p - p' < window or p' < sinks.  q, out (tokens, heads, width), heads / kv_heads at most 128.  A row that sees
  * nothing (its page is missing) is zeros. */
 size_t f3m_paged_attention_workspace_bytes(const f3m_seqs *seqs, const f3m_cache *cache, int32_t heads);

@@ -461,3 +461,81 @@ def test_refusals(cuda):
             call()
     with pytest.raises(RuntimeError):          # the library's own check
         att(scale=float("inf"))
+
+
+def test_pages_behind_two_billion_elements(cuda):
+    """Sequences whose pages lie at the end of arrays of more than 2^31 elements: the bits that they have in small ones."""
+    from f3m_b200 import paged, sequence as sq
+    new, cached, page, kv, w, dtype = [3, 20], [700, 129], 256, 8, 128, torch.bfloat16
+    plan, rotation, lens = sq.SequencePlan(new), paged.Rotation(w), ints(cached)
+    kp, vp, table = cache(200, cached, new, kv, w, page, dtype, garbage=0.0)
+    pool = (1 << 31) // (page * kv * w) + 5 + kp.shape[0]
+    big = [torch.empty(pool, page, kv, w, device="cuda", dtype=dtype) for _ in range(2)]
+    far = table + (pool - kp.shape[0])
+    for x, y in zip(big, (kp, vp)):
+        x[-kp.shape[0]:] = y
+    k, v, q = normal(201, 23, kv, w, dtype=dtype), normal(202, 23, kv, w, dtype=dtype), normal(203, 23, 32, w, dtype=dtype)
+    parents, kept, counts = trees(204, new), ints([[0, 2], [3, 7]]), ints([2, 2])
+    outs = []
+    for a, b, t in ((kp, vp, table), (*big, far)):
+        qq = paged.paged_append(plan, k, v, a, b, t, lens, rotation, parents, q)
+        outs.append(paged.paged_attention(plan, qq, a, b, t, lens, parents=parents))
+        paged.paged_keep(a, b, t, lens, kept, counts)
+    assert torch.equal(*outs) and all(torch.equal(x[-kp.shape[0]:], y) for x, y in zip(big, (kp, vp)))
+
+
+def test_outputs_between_other_data(cuda):
+    """The C entries turn queries in place, and write rows that lie between others, and nothing else."""
+    import ctypes as C
+
+    from f3m_b200 import _lib, paged, sequence as sq
+    new, cached, page, kv, heads, w, dtype = [5, 40], [300, 64], 64, 2, 6, 64, torch.float16
+    plan, rotation, lens, n = sq.SequencePlan(new), paged.Rotation(w), ints(cached), 45
+    kp, vp, table = cache(210, cached, new, kv, w, page, dtype)
+    k, v, q = normal(211, n, kv, w, dtype=dtype), normal(212, n, kv, w, dtype=dtype), normal(213, n, heads, w, dtype=dtype)
+    want_q = paged.paged_append(plan, k, v, kp, vp, table, lens, rotation, q=q)
+    want = paged.paged_attention(plan, want_q, kp, vp, table, lens)
+    c, held = paged._cache(kp, vp, table, lens)
+    rows = lambda t: _lib.Rows(t.data_ptr(), t.stride(0), t.stride(1))  # noqa: E731
+    L, stream, wide = _lib.lib(), torch.cuda.current_stream().cuda_stream, normal(214, heads + 1, n, 2 * w, dtype=dtype)
+    out = wide[1:, :, w:].transpose(0, 1)
+    before = wide.clone()
+    assert L.f3m_paged_append(plan._ref, 2, C.byref(c), rows(k), rows(v), None, rotation._ref, heads, rows(q), rows(q), stream) == 0
+    need = L.f3m_paged_attention_workspace_bytes(plan._ref, C.byref(c), heads)
+    ws = torch.full((need + 64,), 0xa5, device="cuda", dtype=torch.uint8)
+    assert L.f3m_paged_attention(plan._ref, 2, C.byref(c), heads, 0x7fffffff, 0, w ** -0.5, None, rows(q), rows(out), ws.data_ptr(), need, stream) == 0
+    assert torch.equal(q, want_q) and torch.equal(out, want) and (ws[need:] == 0xa5).all()
+    before[1:, :, w:] = wide[1:, :, w:]
+    assert torch.equal(wide, before)
+
+
+def test_calls_from_several_host_threads(cuda):
+    """Each thread on its own stream, all at once: the bits of the calls alone."""
+    import threading
+
+    from f3m_b200 import paged, sequence as sq
+    new, dtype = [6, 1, 30], torch.bfloat16
+    plan, jobs, got = sq.SequencePlan(new), [], [None] * 4
+    x, ld = normal(225, 5000, 512, dtype=dtype), -normal(226, 5000, 512, dtype=dtype).abs() * 0.1
+    line = sq.SequencePlan([5000])
+    for i in range(4):
+        cached = [500 * (i + 1), 3000, 17 * i]
+        kp, vp, table = cache(220 + i, cached, new, 2, 64, 32, dtype)
+        jobs.append((normal(230 + i, 37, 8, 64, dtype=dtype), kp, vp, table, ints(cached)))
+    want = [paged.paged_attention(plan, *j) for j in jobs]
+    h = sq.gated_recurrence(line, x, ld)
+    torch.cuda.synchronize()
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(30):
+                got[i] = (paged.paged_attention(plan, *jobs[i]), *sq.gated_recurrence(line, x, ld))
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for a, b in zip(got, want):
+        assert torch.equal(a[0], b) and torch.equal(a[1], h[0]) and torch.equal(a[2], h[1])
