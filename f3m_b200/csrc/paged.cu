@@ -7,7 +7,8 @@ namespace f3m {
 // ---- new tokens to their pages ----------------------------------------------------------------------------------------------
 // A CTA has AP_TOKENS neighbouring tokens of a sequence.  Their places and angles are taken once for all heads: the part of a whole turn is position * turns modulo
 // 2^64, exact for any position, and what is left, in FP32, is at most half a turn.  Then its rows, (token, head) of queries, keys and values, 16 lanes or 8 to a row with 16 bytes
-// each; a lane's partner in a half-split rotation hands its columns over.  Memory is the bound: every array is read and written once.
+// each; a lane's partner in a half-split rotation hands its columns over.  Memory is the bound: every array is read and written once.  10121 tokens in 8 chunks, 32 heads and 8, width
+// 128: 52-56 us, 4.8 TB/s, 73 % of the measured copy (four tokens a CTA 64; a thread's vectors found by divisions 62; four of them in flight 92).
 constexpr int AP_TOKENS = 2, AP_THREADS = 256;
 
 template <typename T>
@@ -101,6 +102,9 @@ void paged_append(int type, const AppendArgs &a, cudaStream_t s) {
 // other's copies and products run, also where items are short.  Items of two (chunks of prompts) are arithmetic's: a CTA an SM, two tiles of rows that share each
 // tile of keys.  How long a sequence is stands on the device only, so that each CTA counts for itself: CTA c of G takes the share c U / G .. (c + 1) U / G of all items' U
 // tiles, cuts through items where that falls, and paged_join puts the parts together, in one order.
+//
+// What bounds it: of one token for 32 sequences up to 16384, 32 heads on 8, width 128, memory (181-200 us, 5.2-5.9 TB/s of 6.5); of trees of 32 tokens on the same the chain of a tile
+// (scores, maximum, exponentials, product), 234-252 us; of chunks of 2048 and 1021 tokens, window 4096, that chain too, 330 us, 0.62 PFLOP/s (0.87 where all is seen).
 //
 // As in window attention S = Q K^T goes to tensor memory, a thread takes the weights of one row and writes them over S, from where they go into O += P V.
 //
@@ -777,8 +781,8 @@ void paged_attention(int type, const PagedArgs &a, cudaStream_t s) { type == F3M
 
 // ---- accepted paths -----------------------------------------------------------------------------------------------------------
 // A CTA has the keys or the values of one head of a sequence, and takes its places in order, KP_ROWS at a time: read, then written.  A place is read for one in front of it or
-// for itself (kept[j] >= j), so that what is written has been read.  64 paths of up to 30 tokens, 8 heads, width 128: three dependent loads and a store, 4.9 us (a thread for all
-// places of 16 bytes, 8 at a time: 17.9).
+// for itself (kept[j] >= j), so that what is written has been read.  64 paths of up to 30 tokens, 8 heads, width 128: three dependent loads and a store, 6.2 us (a thread for all
+// places of 16 bytes, 8 at a time: 17.9 in all).
 constexpr int KP_STEP = 16, KP_EACH = 4, KP_ROWS = KP_STEP * KP_EACH, KP_THREADS = 16 * KP_STEP;
 __global__ void __launch_bounds__(KP_THREADS) keep_paths(const __grid_constant__ f3m_cache c, const int *kept, int64_t kept_stride, int most, const int *counts) {
     const int b = blockIdx.x, h = blockIdx.y >> 1, col = 8 * (threadIdx.x & 15), length = paged_length(c, b), count = min(max(counts[b], 0), most);

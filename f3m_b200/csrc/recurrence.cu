@@ -50,6 +50,9 @@ __device__ __forceinline__ float advance(float h, float ld, float x) {
 //
 // Gradients are the same from the end, on what flows back between tokens, c_t = a_t G_t: G_t = dout_t + c_(t+1), dx_t = G_t, dlog_decay_t = c_t h_(t-1).
 //
+// What bounds it: a unit takes 8500 clocks, three of them run on an SM (two of gradients); 1200 go to each walk, 2700 to 5600 to looking back, as the tiles before run at the same time.  65536 tokens,
+// 2048 channels, bf16: 238 us, 3.4 TB/s; 64 sequences of 128 tokens, 4096 channels, where nothing looks back: 43 us, 4.8 TB/s.
+//
 // Blocks take units from a counter, tiles in order, so that what a tile waits for is always taken by a running block; a ninth warp takes the next one, starts its
 // copies, and looks back.
 constexpr int GR_WARPS = 8, GR_THREADS = 32 * (GR_WARPS + 1), GR_TILE = SEQ_TILE * 128, GR_STAGES = 2;   // bytes of an array's tile
