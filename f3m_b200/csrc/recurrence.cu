@@ -50,13 +50,14 @@ __device__ __forceinline__ float advance(float h, float ld, float x) {
 //
 // Gradients are the same from the end, on what flows back between tokens, c_t = a_t G_t: G_t = dout_t + c_(t+1), dx_t = G_t, dlog_decay_t = c_t h_(t-1).
 //
-// What bounds it: a unit takes 8500 clocks, three of them run on an SM (two of gradients); 1200 go to each walk, 2700 to 5600 to looking back, as the tiles before run at the same time.  65536 tokens,
-// 2048 channels, bf16: 238 us, 3.4 TB/s; 64 sequences of 128 tokens, 4096 channels, where nothing looks back: 43 us, 4.8 TB/s.
+// What bounds it: a unit takes some 8000 clocks, three of them run on an SM (two of gradients); 1200 go to each walk, 2000 to 4000 to looking back, as the tiles before run at the same time.  65536 tokens,
+// 2048 channels, bf16: 218 us, 3.7 TB/s; 64 sequences of 128 tokens, 4096 channels, where nothing looks back: 43 us, 4.8 TB/s.
 //
 // Blocks take units from a counter, tiles in order, so that what a tile waits for is always taken by a running block; a ninth warp takes the next one, starts its
 // copies, and looks back.
 constexpr int GR_WARPS = 8, GR_THREADS = 32 * (GR_WARPS + 1), GR_TILE = SEQ_TILE * 128, GR_STAGES = 2;   // bytes of an array's tile
 constexpr unsigned long long GR_NOTHING = ~0ull;
+constexpr int GR_MAPS = 4;   // words of so many tiles on their way at a time: 218 us, one by one 238 (65536 tokens, 2048 channels); eight spill
 
 struct RecurrenceKernel {
     RecurrenceArgs a;
@@ -226,11 +227,21 @@ __global__ void __launch_bounds__(GR_THREADS, BACK ? 2 : 3) recurrence_tiles(con
                     if (all) {   // the channels' own words, each of which tells whether it is there
                         h = heard(state - (1 + near) * step);
                         all = h != GR_NOTHING;
-#pragma unroll 8
-                        for (int d = near; d > 0; d--) {
-                            const f32x2 times = heard(map - 2 * d * step), added = heard(map - 2 * d * step + 1);
-                            all &= times != GR_NOTHING && added != GR_NOTHING;
-                            h = through(h, times, added);
+#pragma unroll 1
+                        for (int d = near; d > 0; d -= GR_MAPS) {   // so many at a time on their way
+                            f32x2 t[GR_MAPS], b[GR_MAPS];
+#pragma unroll
+                            for (int i = 0; i < GR_MAPS; i++)
+                                if (d > i) {
+                                    t[i] = heard(map - 2 * (d - i) * step);
+                                    b[i] = heard(map - 2 * (d - i) * step + 1);
+                                }
+#pragma unroll
+                            for (int i = 0; i < GR_MAPS; i++)
+                                if (d > i) {
+                                    all &= t[i] != GR_NOTHING && b[i] != GR_NOTHING;
+                                    h = through(h, t[i], b[i]);
+                                }
                         }
                     }
                     if (__all_sync(0xffffffffu, all)) break;
@@ -243,6 +254,7 @@ __global__ void __launch_bounds__(GR_THREADS, BACK ? 2 : 3) recurrence_tiles(con
                     }
                 }
             }
+            if (before && !last && lane < LANES) tell(state, through(h, times, sum));   // through the tile's own map, as those do who look over it
             f32x2 leaves = h;
 #pragma unroll 8
             for (int i = 0; i < RUNS; i++) {
@@ -252,8 +264,8 @@ __global__ void __launch_bounds__(GR_THREADS, BACK ? 2 : 3) recurrence_tiles(con
             __syncthreads();   // what enters the runs is there
             if (last) {
                 if (out && lane < LANES && c < a.channels) *reinterpret_cast<f32x2 *>(out + (int64_t)e.w * a.channels + c) = leaves;
-            } else if (lane < LANES) {
-                tell(state, before ? through(h, times, sum) : leaves);   // through the tile's own map, as those do who look over it
+            } else if (before == 0 && lane < LANES) {
+                tell(state, leaves);
             }
         } else {
             const int run = warp * (32 / LANES) + lane / LANES, l = lane % LANES, r0 = run * RUN, c = g * CHANNELS + 2 * l, count = min(SEQ_TILE, e.y - e.z) - r0;
