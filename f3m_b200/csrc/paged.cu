@@ -492,7 +492,7 @@ __global__ void __launch_bounds__(128 * TILES + 64, 3 - TILES) paged_tiles(const
                 __syncwarp();
                 tc::fence_after_sync();
                 const uint32_t there = there_s[tile % PG_THERE];
-                const bool whole = by_all && there == 0xffffu;
+                bool whole = by_all && there == 0xffffu;   // then: for this warp's rows
                 uint32_t seen[4] = {};
                 if (!whole) {
                     // Values that are not finite leave the tile, by the first tile of rows' threads, which may be a tile of keys ahead of the second's.  Scores of this tile tell
@@ -539,6 +539,7 @@ __global__ void __launch_bounds__(128 * TILES + 64, 3 - TILES) paged_tiles(const
                         seen[q] = seen_keys(a, length, key + 32 * q, there >> 4 * q, pos, up, above);
                         bad |= (seen[q] & bads[q]) != 0u;
                     }
+                    whole = __all_sync(0xffffffffu, (seen[0] & seen[1] & seen[2] & seen[3]) == 0xffffffffu);
                 }
                 if (!some) {   // a warp without rows
                     tc::fence_before_sync();
