@@ -103,8 +103,8 @@ void paged_append(int type, const AppendArgs &a, cudaStream_t s) {
 // tile of keys.  How long a sequence is stands on the device only, so that each CTA counts for itself: CTA c of G takes the share c U / G .. (c + 1) U / G of all items' U
 // tiles, cuts through items where that falls, and paged_join puts the parts together, in one order.
 //
-// What bounds it: of one token for 32 sequences up to 16384, 32 heads on 8, width 128, memory (181-200 us, 5.2-5.9 TB/s of 6.5); of trees of 32 tokens on the same the chain of a tile
-// (scores, maximum, exponentials, product), 234-252 us; of chunks of 2048 and 1021 tokens, window 4096, that chain too, 330 us, 0.62 PFLOP/s (0.87 where all is seen).
+// What bounds it: of one token for 32 sequences up to 16384, 32 heads on 8, width 128, memory (187-204 us, 5.1-5.6 TB/s of 6.5); of trees of 32 tokens on the same the chain of a tile
+// (scores, maximum, exponentials, product), 233-246 us; of chunks of 2048 and 1021 tokens, window 4096, that chain too, 326 us, 0.63 PFLOP/s (0.83 where all is seen).
 //
 // As in window attention S = Q K^T goes to tensor memory, a thread takes the weights of one row and writes them over S, from where they go into O += P V.
 //

@@ -459,21 +459,24 @@ def _new_channels(t: torch.Tensor) -> Tuple[torch.Tensor, Rows]:
 
 
 def _check_channels(x: torch.Tensor, *others: Tuple[str, torch.Tensor]) -> int:
-    if not x.is_cuda:
+    kind, shape, device = _CHANNEL_TYPES.get(x.dtype), x.shape, x.device
+    if device.type != "cuda":
         raise ValueError("the engine has no CPU path: x must be a CUDA tensor")
-    if x.dtype not in _CHANNEL_TYPES:
+    if kind is None:
         raise TypeError(f"{x.dtype}: only torch.bfloat16, torch.float16 and torch.float32 are built")
-    if x.dim() != 2:
+    if len(shape) != 2:
         raise ValueError("arrays are (tokens, channels)")
-    if x.shape[1] < 8 or x.shape[1] > _lib.MAX_CHANNELS or x.shape[1] % 8:
-        raise ValueError(f"{x.shape[1]} channels: not a multiple of 8 in 8..{_lib.MAX_CHANNELS}")
+    channels = shape[1]
+    if channels < 8 or channels > _lib.MAX_CHANNELS or channels % 8:
+        raise ValueError(f"{channels} channels: not a multiple of 8 in 8..{_lib.MAX_CHANNELS}")
     for what, t in others:
-        _shape(t, x.shape, what)
-        if t.dtype != x.dtype:
+        if t.shape != shape:
+            _shape(t, shape, what)
+        if t.dtype is not x.dtype:
             raise TypeError(f"arrays of {x.dtype} and {t.dtype} in one call")
-        if t.device != x.device:
-            raise ValueError(f"arrays on {x.device} and {t.device} in one call")
-    return _CHANNEL_TYPES[x.dtype]
+        if t.device != device:
+            raise ValueError(f"arrays on {device} and {t.device} in one call")
+    return kind
 
 
 def _check_channel_state(t, n, x, what):
@@ -558,14 +561,16 @@ def gated_recurrence_step(x: torch.Tensor, log_decay: torch.Tensor, state: torch
     like x."""
     _refuse_tangents(x, log_decay, state)
     kind = _check_channels(x, ("log_decay", log_decay))
-    _shape(state, x.shape, "state")
+    if state.shape != x.shape:
+        _shape(state, x.shape, "state")
     if state.dtype != torch.float32 or state.device != x.device or not state.is_contiguous() or state.data_ptr() % 16:
         raise TypeError("state must be a contiguous float32 array on the device of x that starts on 16 bytes: it is updated in place")
     if _needs_grad(x, log_decay, state):
         raise RuntimeError("gated_recurrence_step has no gradient: call it under torch.no_grad()")
     (x, rx), (log_decay, rl), (out, ro) = _read_channels(x), _read_channels(log_decay), _new_channels(x)
+    n, channels = x.shape
     with _On(x.device) as stream:
-        st = _lib.lib().f3m_gated_recurrence_step(x.shape[0], kind, x.shape[1], rx, rl, state.data_ptr(), ro, stream)
+        st = _lib.lib().f3m_gated_recurrence_step(n, kind, channels, rx, rl, state.data_ptr(), ro, stream)
     check(st, "f3m_gated_recurrence_step")
     torch.autograd.graph.increment_version(state)
     return out
