@@ -104,14 +104,16 @@ void paged_append(int type, const AppendArgs &a, cudaStream_t s) {
 // tiles, cuts through items where that falls, and paged_join puts the parts together, in one order.
 //
 // What bounds it: of one token for 32 sequences up to 16384, 32 heads on 8, width 128, memory (187-204 us, 5.1-5.6 TB/s of 6.5); of trees of 32 tokens on the same the chain of a tile
-// (scores, maximum, exponentials, product), 233-246 us; of chunks of 2048 and 1021 tokens, window 4096, that chain too, 326 us, 0.63 PFLOP/s (0.83 where all is seen).
+// (scores, maximum, exponentials, product), 215-238 us; of chunks of 2048 and 1021 tokens, window 4096, that chain too, 326 us, 0.63 PFLOP/s (0.83 where all is seen).
 //
 // As in window attention S = Q K^T goes to tensor memory, a thread takes the weights of one row and writes them over S, from where they go into O += P V.
 //
 // Keys that only a part of the item's rows sees (the window's edge, new tokens, a tree, missing pages) go by bits, a word for 32 of them.  A value that is not finite would
 // reach every row there, as zero times it: it is taken out of the tile, and added to the rows that see it when they have been written (poison_row).
 constexpr int PG_BLOCK = SEQ_TILE * 128, PG_RING = 4, PG_THERE = 8, PG_MAX_SLOTS = 8;
-constexpr int PG_ITEM = 1;   // what an item takes beside its tiles, in tiles
+// What an item takes beside its tiles of keys, in tiles: of one tile of rows 2 (trees of 32 tokens for 32 sequences 215 us, 235 with 1, 213-216 with 4; 96 single tokens on up to 3800
+// 141-143, 147-154, 147), of two tiles 1 (chunks 340-345 us, 348 with 2, 344-364 with 4).
+template <int TILES> constexpr int PG_ITEM = TILES == 1 ? 2 : 1;
 constexpr float PG_NO_SUM = 0x1p60f;   // some exponent was not a number (exp2_poly)
 constexpr int PG_WORDS = F3M_TREE_MAX / 32;
 
@@ -119,7 +121,7 @@ struct PagedItem {
     int row0, n, b, i0, tokens, length;   // the sequence's first row, new tokens, number; first token of the item, how many; tokens in the cache
     int kv_head, sinks, first, keys;      // tiles of keys: the first `sinks` of the sequence, then those from tile `first` on; `keys` in all
     __device__ __forceinline__ int key(int j) const { return SEQ_TILE * (j < sinks ? j : first + j - sinks); }
-    __device__ __forceinline__ int cost() const { return keys ? keys + PG_ITEM : 0; }   // the item's own comes behind its last tile
+    template <int TILES> __device__ __forceinline__ int cost() const { return keys ? keys + PG_ITEM<TILES> : 0; }   // the item's own comes behind its last tile
 };
 struct PagedPart {   // of an item: tiles of keys j0 .. j1 - 1
     PagedItem w;
@@ -256,7 +258,7 @@ __global__ void __launch_bounds__(128 * TILES + 64, 3 - TILES) paged_tiles(const
         gave_up_s = 0;
     }
     // tiles of all items, and where this CTA's begin
-    auto cost_of = [&](int e) { return e < p.entries ? (long long)paged_item<TILES>(p, e).cost() * a.c.kv_heads : 0ll; };
+    auto cost_of = [&](int e) { return e < p.entries ? (long long)paged_item<TILES>(p, e).template cost<TILES>() * a.c.kv_heads : 0ll; };
     auto scan = [&](long long v, long long &all) {   // of the block's threads: the sum up to this one, and of all
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -321,10 +323,10 @@ __global__ void __launch_bounds__(128 * TILES + 64, 3 - TILES) paged_tiles(const
         auto page_at = [&](const PagedItem &z, int k) { return lane < boxes ? paged_page(a.c, z.b, (int64_t)z.key(k) + lane * p.box) : -1; };
         w = entry(e);
         int j = 0;
-        if (left) { w.kv_head = min((int)(start_s[1] / w.cost()), a.c.kv_heads - 1); j = (int)(start_s[1] % w.cost()); }
+        if (left) { w.kv_head = min((int)(start_s[1] / w.template cost<TILES>()), a.c.kv_heads - 1); j = (int)(start_s[1] % w.template cost<TILES>()); }
         if (lane == 0) p.split[cta].parts = 0;
         auto next = [&] {   // the item behind this one
-            left -= min(left, (long long)w.cost() - j);
+            left -= min(left, (long long)w.template cost<TILES>() - j);
             j = 0;
             if (left && ++w.kv_head == a.c.kv_heads)
                 do {
