@@ -115,6 +115,7 @@ constexpr int PG_BLOCK = SEQ_TILE * 128, PG_RING = 4, PG_THERE = 8, PG_MAX_SLOTS
 // 141-143, 147-154, 147), of two tiles 1 (chunks 340-345 us, 348 with 2, 344-364 with 4).
 template <int TILES> constexpr int PG_ITEM = TILES == 1 ? 2 : 1;
 constexpr float PG_NO_SUM = 0x1p60f;   // some exponent was not a number (exp2_poly)
+constexpr float PG_ALL_LOW = -1.f;     // in the place of a part's sum: it has seen keys, and all their scores are -inf
 constexpr int PG_WORDS = F3M_TREE_MAX / 32;
 
 struct PagedItem {
@@ -486,7 +487,7 @@ __global__ void __launch_bounds__(128 * TILES + 64, 3 - TILES) paged_tiles(const
             const int pos = length + (a.parents ? (row ? depth_s[token] : 0) : w.i0 + token), up = row ? (a.parents ? length - 1 : pos) : -1;
             const uint32_t *above = a.parents && row ? above_s[token] : nullptr;
             float top = -INFINITY, sum = 0.f;
-            bool bad = false;
+            bool bad = false, met = false;   // met: some key is seen
             for (int j = j0; j < j1; j++, tile++) {
                 const int key = w.key(j);
                 const bool by_all = seen_by_all(a, w, key);
@@ -495,6 +496,7 @@ __global__ void __launch_bounds__(128 * TILES + 64, 3 - TILES) paged_tiles(const
                 tc::fence_after_sync();
                 const uint32_t there = there_s[tile % PG_THERE];
                 bool whole = by_all && there == 0xffffu;   // then: for this warp's rows
+                met |= whole;
                 uint32_t seen[4] = {};
                 if (!whole) {
                     // Values that are not finite leave the tile, by the first tile of rows' threads, which may be a tile of keys ahead of the second's.  Scores of this tile tell
@@ -540,6 +542,7 @@ __global__ void __launch_bounds__(128 * TILES + 64, 3 - TILES) paged_tiles(const
                     for (int q = 0; q < 4; q++) {
                         seen[q] = seen_keys(a, length, key + 32 * q, there >> 4 * q, pos, up, above);
                         bad |= (seen[q] & bads[q]) != 0u;
+                        met |= seen[q] != 0u;
                     }
                     whole = __all_sync(0xffffffffu, (seen[0] & seen[1] & seen[2] & seen[3]) == 0xffffffffu);
                 }
@@ -625,8 +628,9 @@ __global__ void __launch_bounds__(128 * TILES + 64, 3 - TILES) paged_tiles(const
                 unpack2(add2(add[0], add[1]), u, v);
                 sum = u + v;
             }
-            if (!(sum < PG_NO_SUM) || top == INFINITY) sum = NAN;
             const bool cut = part.slot >= 0;
+            if (!(sum < PG_NO_SUM) || top == INFINITY) sum = NAN;
+            else if (met && top == -INFINITY) sum = cut ? PG_ALL_LOW : NAN;   // 0 / 0, unless another part has more
             const float inv = cut ? 1.f : sum != 0.f ? 1.f / sum : 0.f;   // nothing seen: 0
             const int64_t place = cut ? (int64_t)part.slot * p.rows + token * p.group + head : 0;
             uint16_t *out = reinterpret_cast<uint16_t *>(a.out.data) + (int64_t)(w.row0 + w.i0 + token) * a.out.token_stride + (int64_t)(w.kv_head * p.group + head) * a.out.head_stride;
@@ -672,7 +676,8 @@ __global__ void __launch_bounds__(128 * TILES + 64, 3 - TILES) paged_tiles(const
     if (warp == COPY) tc::tmem_dealloc(tmem, 256 * TILES);
 }
 
-// Items that were cut: a warp a row, 4 columns a lane.  Parts lie in the CTAs from this one on, scaled here to their common maximum, in their order; one that has seen nothing has a sum of 0.
+// Items that were cut: a warp a row, 4 columns a lane.  Parts lie in the CTAs from this one on, scaled here to their common maximum, in their order; one that has seen nothing has a sum of 0,
+// one whose scores are all -inf weighs nothing beside others, and alone makes the row not a number.
 template <typename T>
 __global__ void __launch_bounds__(256) paged_join(const __grid_constant__ PagedKernel p) {
     const PagedSplit s = p.split[blockIdx.x];
@@ -680,6 +685,7 @@ __global__ void __launch_bounds__(256) paged_join(const __grid_constant__ PagedK
     if (s.parts == 0 || row >= s.w.tokens * p.group) return;
     auto place = [&](int i) { return (int64_t)(2 * ((int)blockIdx.x + i) + (i == 0)) * p.rows + row; };
     float high = -INFINITY, total = 0.f, o[4] = {};
+    bool met = false;
     for (int i = lane; i < s.parts; i += 32) high = fmaxf(high, p.stat[place(i)].x);
 #pragma unroll
     for (int x = 16; x; x >>= 1) high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, x));
@@ -687,12 +693,13 @@ __global__ void __launch_bounds__(256) paged_join(const __grid_constant__ PagedK
     for (int i = 0; i < s.parts; i++) {
         const float2 t = p.stat[place(i)];
         if (t.y == 0.f) continue;
-        const float f = ex2_approx(t.x - high);
+        met = true;
+        const float f = t.y == PG_ALL_LOW ? 0.f : ex2_approx(t.x - high);
         const float4 x = *reinterpret_cast<const float4 *>(p.sums + place(i) * p.a.c.width + c);
         total = fmaf(f, t.y, total);
         o[0] = fmaf(f, x.x, o[0]); o[1] = fmaf(f, x.y, o[1]); o[2] = fmaf(f, x.z, o[2]); o[3] = fmaf(f, x.w, o[3]);
     }
-    const float inv = total != 0.f ? 1.f / total : 0.f;
+    const float inv = total != 0.f ? 1.f / total : met ? NAN : 0.f;
     uint16_t *out = reinterpret_cast<uint16_t *>(p.a.out.data) + (int64_t)(s.w.row0 + s.w.i0 + row / p.group) * p.a.out.token_stride + (int64_t)(s.w.kv_head * p.group + row % p.group) * p.a.out.head_stride;
     *reinterpret_cast<uint2 *>(out + c) = make_uint2(Half<T>::pack(o[0] * inv, o[1] * inv), Half<T>::pack(o[2] * inv, o[3] * inv));
 }
