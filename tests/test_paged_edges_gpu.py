@@ -46,3 +46,84 @@ def test_scores_of_minus_infinity(new, cached, heads, kv, width, page, window, s
         got = run(k2, table)
         assert got[none].isnan().all()
         assert_within(got[~none], tuple(x[~none] for x in want))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_one_bad_value_among_missing_pages(dtype, cuda):
+    """Long caches where each tile of keys has a missing page, so that all are looked through: a value that is not finite costs the tiles next to it, not the whole of a part."""
+    from f3m_b200 import paged, sequence
+    n, kv, width, page, most = 32, 8, 128, 16, 1024
+    kp, vp = normal(20, 256, page, kv, width, dtype=dtype), normal(21, 256, page, kv, width, dtype=dtype)
+    table = (torch.arange(n * most, device="cuda").view(n, most) * 37 % 255).int()      # pages are shared, the last one is one sequence's
+    table[:, 3::8] = -1
+    table[:, most - 1:] = torch.arange(n, device="cuda")[:, None].int()
+    plan, lens = sequence.SequencePlan([1] * n), ints([16 * most - 1] * n)
+    q = normal(22, n, 4 * kv, width, dtype=dtype)
+
+    def timed():
+        times = []
+        for _ in range(5):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            out = paged.paged_attention(plan, q, kp, vp, table, lens)
+            b.record()
+            b.synchronize()
+            times.append(a.elapsed_time(b))
+        return out, min(times)
+
+    clean, fast = timed()
+    assert torch.isfinite(clean).all()
+    table[5, 500], table[9, 0] = 255, 255
+    vp[255, 7, 2, 11], vp[255, 3, 6, 100] = float("nan"), float("-inf")
+    kp[255] = 0.0
+    got, slow = timed()
+    assert got[[5, 9], 8:12, 11].isnan().all() and (got[[5, 9], 24:28, 100] == float("-inf")).all()
+    others = [b for b in range(n) if b not in (5, 9)]
+    assert torch.equal(got[others], clean[others])
+    rest = torch.ones_like(got, dtype=torch.bool)
+    rest[[5, 9], 8:12, 11] = rest[[5, 9], 24:28, 100] = False
+    assert torch.isfinite(got[rest]).all()
+    assert slow < 5 * fast, (slow, fast)
+
+
+# new, cached, heads, kv_heads, width, page, window, sinks, a tree: items cut into parts; two tiles of rows
+BAD = [
+    ([1], [6000], 8, 2, 64, 16, None, 0, False),
+    ([1], [6000], 8, 2, 128, 16, 700, 3, False),
+    ([250], [130], 4, 4, 64, 16, None, 0, False),
+    ([300], [3000], 3, 1, 128, 32, 150, 5, False),
+    ([200], [500], 2, 1, 64, 16, None, 0, True),
+    ([250], [5000], 4, 2, 128, 16, 200, 7, True),
+]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("new,cached,heads,kv,width,page,window,sinks,drafted", BAD)
+def test_bad_values_reach_the_rows_that_see_them(new, cached, heads, kv, width, page, window, sinks, drafted, dtype, cuda):
+    """One value that is not finite, of any kind of key: cached, at the window's edge, new, seen by rows of the second tile only.  Rows that see it have it in its column; all else is as before."""
+    from f3m_b200 import paged, sequence
+    plan, lens, n, c = sequence.SequencePlan(new), ints(cached), new[0], cached[0]
+    kp, vp, table = cache(30, cached, new, kv, width, page, dtype)
+    q, parents = normal(31, n, heads, width, dtype=dtype, scale=0.5), trees(32, new) if drafted else None
+    run = lambda v, t: paged.paged_attention(plan, q, kp, v, t, lens, window, sinks, parents)  # noqa: E731
+    table[0, min(c // page, 20)] = -1           # tiles with a missing page are looked through
+    clean = run(vp, table)
+    assert torch.isfinite(clean).all()
+    depths, above = ref.tree(None if parents is None else parents.tolist(), n)
+    w = window or 1 << 40
+    for s in (0, 2, c - (window or 50) + 1, c - 1, c, c + n // 3, c + n - 1, c + 5 * n // 6, c // 2):
+        if not 0 <= s < c + n or int(table[0, s // page]) < 0:
+            continue
+        pos = s if s < c else c + depths[s - c]
+        sees = torch.tensor([(s < c or s - c in above[i]) and (c + depths[i] - pos < w or pos < sinks) for i in range(n)], device="cuda")
+        partly = not bool(sees.all())
+        for bad in (float("inf"), float("nan")):
+            v2 = vp.clone()
+            v2[table[0, s // page].long(), s % page, kv - 1, 9] = bad
+            got, group = run(v2, table), heads // kv
+            mine = torch.zeros_like(got, dtype=torch.bool)
+            mine[sees, heads - group:, 9] = True
+            assert not torch.isfinite(got[mine]).any(), (s, bad)
+            if partly:
+                assert (got[mine] == bad).all() or got[mine].isnan().all()
+            assert torch.equal(got[~mine], clean[~mine]), (s, bad)
