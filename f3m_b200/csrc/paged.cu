@@ -788,7 +788,7 @@ static void paged_t(const PagedArgs &a, cudaStream_t s) {
     p.page_shift = 31 - __builtin_clz(a.c.page_tokens);
     p.box = std::min(a.c.page_tokens, SEQ_TILE);
     p.wide = rows_wide(a.out);
-    p.c = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1e-30f);   // a scale of zero: all weights are one
+    p.c = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 0x1p-149f);   // a scale of zero: all weights are one, whatever finite number the scores are
     p.err = seq_error_word();
     f3m_cache c = a.c;
     if (c.pages == 0) {   // no page is read: the maps need an address

@@ -127,3 +127,15 @@ def test_bad_values_reach_the_rows_that_see_them(new, cached, heads, kv, width, 
             if partly:
                 assert (got[mine] == bad).all() or got[mine].isnan().all()
             assert torch.equal(got[~mine], clean[~mine]), (s, bad)
+
+
+def test_a_scale_of_zero_weighs_all_alike(cuda):
+    """Also where products of queries and keys are as large as FP32 has them."""
+    from f3m_b200 import paged, sequence
+    dtype, new, cached = torch.bfloat16, [3], [300]
+    kp, vp, table = cache(40, cached, new, 1, 64, 16, dtype)
+    q = normal(41, 3, 2, 64, dtype=dtype) * 1e17
+    plain = ref.attention(q, kp, vp, table, cached, new, scale=0.0)
+    got = paged.paged_attention(sequence.SequencePlan(new), q, kp * 1e17, vp, table, ints(cached), scale=0.0)
+    # the bound counts an exponent's error by the size of the products, which a scale of zero takes out
+    assert_within(got, plain)
