@@ -34,9 +34,11 @@ template <> struct Vec<float> {
 };
 
 // a h + x, a = exp(min(ld, 0)).  Next to 1 a's own rounding, half a step of 2^-24, would be seen in a sum over thousands of tokens: there h keeps what
-// a - 1 does not take.  What is not a number stays that.
+// a - 1 does not take.  What is not a number stays that.  An infinite h has nothing to keep, and a - 1 would turn its sign: it is a's multiple, infinite where a is above 0 as the
+// kernels of whole sequences take it (decay_of).
 __device__ __forceinline__ float advance(float h, float ld, float x) {
     ld = ld > 0.f ? 0.f : ld;
+    if (isinf(h)) return fmaf(ex2_approx(1.4426950408889634f * ld), h, x);
     return ld > -0.5f ? h + fmaf(expm1f(ld), h, x) : fmaf(expf(ld), h, x);
 }
 
