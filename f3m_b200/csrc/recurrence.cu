@@ -99,13 +99,25 @@ __device__ __forceinline__ f32x2 multiplier(f32x2 ld) {
     unpack2(mul2(ld, pack2(1.4426950408889634f, 1.4426950408889634f)), far[0], far[1]);
     return pack2(l[0] > -0.25f ? near[0] : ex2_approx(far[0]), l[1] > -0.25f ? near[1] : ex2_approx(far[1]));
 }
-// h through a map
+// h through a map.  An infinite h comes out as not a number, whatever the map is, and that stays so through all that follow
 __device__ __forceinline__ f32x2 through(f32x2 h, f32x2 m, f32x2 x) {
     float ml, mh, kl, kh;
     unpack2(m, ml, mh);
     asm("set.lt.f32.f32 %0, %1, 0f00000000;" : "=f"(kl) : "f"(ml));   // 1 or 0
     asm("set.lt.f32.f32 %0, %1, 0f00000000;" : "=f"(kh) : "f"(mh));
     return fma2(m, h, fma2(pack2(kl, kh), h, x));
+}
+__device__ __forceinline__ int no_number(f32x2 v) {   // a bit for each of the channels
+    float l, h;
+    unpack2(v, l, h);
+    return (l != l) | (h != h) << 1;
+}
+// v, or w in the channels of `lost`
+__device__ __forceinline__ f32x2 in_place_of(int lost, f32x2 w, f32x2 v) {
+    float a[2], b[2];
+    unpack2(w, a[0], a[1]);
+    unpack2(v, b[0], b[1]);
+    return pack2(lost & 1 ? a[0] : b[0], lost & 2 ? a[1] : b[1]);
 }
 constexpr float GR_BELOW_ZERO = -1e-30f;   // where sums of log decays begin: too small to change one
 __device__ __forceinline__ f32x2 held(f32x2 ld) {
@@ -205,6 +217,7 @@ __global__ void __launch_bounds__(GR_THREADS, BACK ? 2 : 3) recurrence_tiles(con
             const int64_t step = (int64_t)p.groups * LANES;
             __syncthreads();   // the runs' maps are there
             f32x2 times = 0, sum = 0;   // the tile's
+            int near = 0;               // tiles between this one and the nearest that had told its state
             if (before) {
                 if (!last) {
                     f32x2 logs = none;
@@ -224,7 +237,7 @@ __global__ void __launch_bounds__(GR_THREADS, BACK ? 2 : 3) recurrence_tiles(con
                     const bool is = lane < before;
                     const f32x2 s = is ? heard(state - l - (1 + lane) * step) : GR_NOTHING, t = is ? heard(map - 2 * (l + (1 + lane) * step)) : GR_NOTHING;   // its first word
                     const uint32_t has = __ballot_sync(0xffffffffu, s != GR_NOTHING), maps = __ballot_sync(0xffffffffu, t != GR_NOTHING);
-                    const int near = __ffs(has) - 1;
+                    near = __ffs(has) - 1;
                     bool all = has && (~maps & ((1u << near) - 1)) == 0;
                     if (all) {   // the channels' own words, each of which tells whether it is there
                         h = heard(state - (1 + near) * step);
@@ -256,12 +269,42 @@ __global__ void __launch_bounds__(GR_THREADS, BACK ? 2 : 3) recurrence_tiles(con
                     }
                 }
             }
-            if (before && !last && lane < LANES) tell(state, through(h, times, sum));   // through the tile's own map, as those do who look over it
+            const bool told = before && !last && lane < LANES;
+            const f32x2 own = through(h, times, sum);   // through the tile's own map, as those do who look over it
+            if (told && !no_number(own)) tell(state, own);
             f32x2 leaves = h;
 #pragma unroll 8
             for (int i = 0; i < RUNS; i++) {
                 if (lane < LANES) enter_s[run_of(i)][l] = leaves;
                 leaves = through(leaves, times_s[run_of(i)][l], added_s[run_of(i)][l]);
+            }
+            if (const int lost = no_number(leaves) | no_number(own)) {
+                // Something was infinite here, or is not a number: maps do not tell which.  What enters is then what the tile before tells, which is waited for (unless there was
+                // no number farther back already), and goes through the tile token by token, as the definition has it.  65536 tokens with an infinite one in front: 2 ms.
+                if (before) {
+                    f32x2 from = heard(state - (1 + near) * step);
+                    if (near && (no_number(h) & ~no_number(from)))
+                        for (uint32_t tries = 0; (from = heard(state - step)) == GR_NOTHING && !*(volatile int *)&gave_up_s;)
+                            if (++tries > 2 * WAIT_TRIES) {
+                                gave_up_s = 1;
+                                *(volatile int *)p.err = 1;
+                            }
+                    h = in_place_of(no_number(h), from, h);
+                }
+                if (lost & ~no_number(h)) {
+                    wait(b_full + 8 * stage, (n / GR_STAGES) & 1);
+                    const unsigned char *tile = base + ARRAYS * stage * GR_TILE + l * sizeof(Raw);
+                    const int count = min(SEQ_TILE, e.y - e.z);
+#pragma unroll 8
+                    for (int k = 0; k < SEQ_TILE; k++) {
+                        const int i = BACK ? SEQ_TILE - 1 - k : k;
+                        if (k % RUN == 0 && lane < LANES) enter_s[i / RUN][l] = in_place_of(no_number(enter_s[i / RUN][l]), h, enter_s[i / RUN][l]);
+                        const f32x2 m = decay_of(held(Two<T>::open(*reinterpret_cast<const Raw *>(tile + GR_TILE + i * 128)))), x = Two<T>::open(*reinterpret_cast<const Raw *>(tile + i * 128));
+                        if (i < count) h = BACK ? mul2(m, add2(h, x)) : fma2(m, h, x);
+                    }
+                    leaves = in_place_of(no_number(leaves), h, leaves);
+                }
+                if (told) tell(state, in_place_of(lost, leaves, own));
             }
             __syncthreads();   // what enters the runs is there
             if (last) {

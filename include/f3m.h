@@ -385,7 +385,8 @@ int f3m_decay_attention_step(int32_t n, int32_t type, int32_t heads, int32_t wid
  * x, log_decay, out (tokens, channels): rows of the packed batch, heads = 1 and head_stride unused, of one type: bf16, fp16 or
  * F3M_TYPE_F32 (strides multiples of 4 elements there).  channels is a multiple of 8 up to F3M_MAX_CHANNELS.  state_in, state_out (sequences, channels) float32, dense, 16-byte
  * aligned: h before the first token (NULL: zeros) and behind the last one (NULL: not wanted; another array than state_in).  h is kept in float32.  -inf is no
- * memory at all; log_decay that is not a number makes h that. */
+ * memory at all of a finite h; log_decay that is not a number makes h that.  An infinite h stays infinite under any a_t above 0, and is not a number behind an a_t of 0, as 0 times
+ * infinity is not: at -inf, and where a_t is below float32's smallest normal number (log_decay below -87.3).  The same holds for gradients. */
 #define F3M_TYPE_F32 3
 #define F3M_MAX_CHANNELS 0x100000
 size_t f3m_gated_recurrence_workspace_bytes(const f3m_seqs *seqs, int32_t channels);
