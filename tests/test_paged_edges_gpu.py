@@ -139,3 +139,31 @@ def test_a_scale_of_zero_weighs_all_alike(cuda):
     got = paged.paged_attention(sequence.SequencePlan(new), q, kp * 1e17, vp, table, ints(cached), scale=0.0)
     # the bound counts an exponent's error by the size of the products, which a scale of zero takes out
     assert_within(got, plain)
+
+
+def test_every_call_reports_a_wait_that_ran_out(cuda):
+    """The word that a kernel would set, set by hand: the next call is refused, whichever it is, enqueues nothing, and the one behind it runs."""
+    from f3m_b200 import _lib, paged, sequence as sq
+    word = _lib.lib().f3m_seqs_error_word()
+    new, cached = [5, 20], [200, 17]
+    plan, lens, n = sq.SequencePlan(new), ints(cached), 25
+    kp, vp, table = cache(50, cached, new, 2, 64, 16, torch.bfloat16, garbage=0.0)
+    k, q = normal(51, n, 2, 64, dtype=torch.bfloat16), normal(52, n, 4, 64, dtype=torch.bfloat16)
+    x, ld, state = normal(53, n, 16, dtype=torch.float32), -normal(54, n, 16, dtype=torch.float32).abs(), torch.ones(n, 16, device="cuda")
+    out, _ = sq.gated_recurrence(plan, x, ld)
+    calls = [lambda: paged.paged_append(plan, k, k, kp, vp, table, lens), lambda: paged.paged_attention(plan, q, kp, vp, table, lens),
+             lambda: paged.paged_keep(kp, vp, table, lens, ints([[3], [4]]), ints([1, 1])), lambda: sq.gated_recurrence(plan, x, ld), lambda: sq.gated_recurrence_grad(plan, ld, out, x),
+             lambda: sq.gated_recurrence_step(x, ld, state)]
+    before = kp.clone(), vp.clone()
+    for call in calls:
+        torch.cuda.synchronize()
+        assert word[0] == 0
+        word[0] = 1
+        with pytest.raises(_lib.F3MError, match="gave up"):
+            call()
+        torch.cuda.synchronize()
+        assert word[0] == 0 and bool((state == 1).all()) and torch.equal(kp, before[0]) and torch.equal(vp, before[1])
+    for call in calls:
+        call()
+    torch.cuda.synchronize()
+    assert word[0] == 0
