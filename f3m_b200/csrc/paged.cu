@@ -115,6 +115,7 @@ constexpr int PG_BLOCK = SEQ_TILE * 128, PG_RING = 4, PG_THERE = 8, PG_MAX_SLOTS
 // 141-143, 147-154, 147), of two tiles 1 (chunks 340-345 us, 348 with 2, 344-364 with 4).
 template <int TILES> constexpr int PG_ITEM = TILES == 1 ? 2 : 1;
 constexpr float PG_NO_SUM = 0x1p60f;   // some exponent was not a number (exp2_poly)
+constexpr float PG_MET = 0x1p-126f;    // a row's sum is at least this if it has seen a key; of a tile that all see the polynomial's least, 2^-125, comes to more
 constexpr float PG_ALL_LOW = -1.f;     // in the place of a part's sum: it has seen keys, and all their scores are -inf
 constexpr int PG_WORDS = F3M_TREE_MAX / 32;
 
@@ -506,7 +507,6 @@ __global__ void __launch_bounds__(128 * TILES + 64, 3 - TILES) paged_tiles(const
             const uint32_t *above = a.parents && row ? above_s[token] : nullptr;
             float top = -INFINITY, sum = 0.f;
             uint32_t bad = 0;    // tiles with a seen value that is not finite and was taken out
-            bool met = false;    // some key is seen
             for (int j = j0; j < j1; j++, tile++) {
                 const int key = w.key(j);
                 const bool by_all = seen_by_all(a, w, key);
@@ -515,7 +515,6 @@ __global__ void __launch_bounds__(128 * TILES + 64, 3 - TILES) paged_tiles(const
                 tc::fence_after_sync();
                 const uint32_t there = there_s[tile % PG_THERE];
                 bool whole = by_all && there == 0xffffu;   // then: for this warp's rows
-                met |= whole;
                 uint32_t seen[4] = {};
                 if (!whole) {
                     // Values that are not finite leave the tile, by the first tile of rows' threads, which may be a tile of keys ahead of the second's.  Scores of this tile tell
@@ -561,7 +560,6 @@ __global__ void __launch_bounds__(128 * TILES + 64, 3 - TILES) paged_tiles(const
                     for (int q = 0; q < 4; q++) {
                         seen[q] = seen_keys(a, length, key + 32 * q, there >> 4 * q, pos, up, above);
                         if (seen[q] & bads[q]) bad |= 1u << ((j - j0) >> tile_shift(part));
-                        met |= seen[q] != 0u;
                     }
                     whole = __all_sync(0xffffffffu, (seen[0] & seen[1] & seen[2] & seen[3]) == 0xffffffffu);
                 }
@@ -604,7 +602,7 @@ __global__ void __launch_bounds__(128 * TILES + 64, 3 - TILES) paged_tiles(const
                 }
                 const float shift = top == -INFINITY ? 0.f : -top * p.c;
                 const f32x2 cc = pack2(p.c, p.c), ss = pack2(shift, shift);
-                f32x2 add[2] = {pack2(sum, 0.f), pack2(0.f, 0.f)};
+                f32x2 add[2] = {pack2(sum, (seen[0] | seen[1] | seen[2] | seen[3]) ? PG_MET : 0.f), pack2(0.f, 0.f)};
 #pragma unroll
                 for (int q = 0; q < 4; q++) {
                     uint32_t w16[16];
@@ -649,7 +647,7 @@ __global__ void __launch_bounds__(128 * TILES + 64, 3 - TILES) paged_tiles(const
             }
             const bool cut = part.slot >= 0;
             if (!(sum < PG_NO_SUM) || top == INFINITY) sum = NAN;
-            else if (met && top == -INFINITY) sum = cut ? PG_ALL_LOW : NAN;   // 0 / 0, unless another part has more
+            else if (top == -INFINITY && sum != 0.f) sum = cut ? PG_ALL_LOW : NAN;   // 0 / 0, unless another part has more
             const float inv = cut ? 1.f : sum != 0.f ? 1.f / sum : 0.f;   // nothing seen: 0
             const int64_t place = cut ? (int64_t)part.slot * p.rows + token * p.group + head : 0;
             uint16_t *out = reinterpret_cast<uint16_t *>(a.out.data) + (int64_t)(w.row0 + w.i0 + token) * a.out.token_stride + (int64_t)(w.kv_head * p.group + head) * a.out.head_stride;
