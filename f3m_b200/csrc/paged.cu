@@ -103,16 +103,23 @@ void paged_append(int type, const AppendArgs &a, cudaStream_t s) {
 // tile of keys.  How long a sequence is stands on the device only, so that each CTA counts for itself: CTA c of G takes the share c U / G .. (c + 1) U / G of all items' U
 // tiles, cuts through items where that falls, and paged_join puts the parts together, in one order.
 //
-// What bounds it: of one token for 32 sequences up to 16384, 32 heads on 8, width 128, memory (187-204 us, 5.1-5.6 TB/s of 6.5); of trees of 32 tokens on the same the chain of a tile
-// (scores, maximum, exponentials, product), 215-238 us; of chunks of 2048 and 1021 tokens, window 4096, that chain too, 326 us, 0.63 PFLOP/s (0.83 where all is seen).
+// What bounds it: of one token for 32 sequences up to 16384, 32 heads on 8, width 128, memory (176-206 us, 5.1-5.9 TB/s of 6.5); of trees of 32 tokens on the same, 215-238 us, shared memory and
+// the chain of a tile (scores, read twice, maximum, exponentials, product): beside more than 40 rows of width 128 half an SM's holds two slots, one of keys and one of values, so that a copy waits for the
+// product with what was there before (trees of 8 tokens 181 us, 10: 185, 11: 200), and more warps with rows take longer (16: 208, 20: 222, 32: 231).  Of chunks of 2048
+// and 1021 tokens, window 4096, it is that chain: 320-331 us, 0.62-0.65 PFLOP/s (0.82-0.85 where all is seen).
 //
-// As in window attention S = Q K^T goes to tensor memory, a thread takes the weights of one row and writes them over S, from where they go into O += P V.
+// Heads that do not divide 128 evenly pay for the entries of 256 tokens that an item does not cross: 3 to a key head make items of 84, 84, 84 and 4 tokens, the last in the other kernel (chunks that see
+// all: 0.67 PFLOP/s with 3, 0.76 with 5, 0.83-0.85 with 4 and 8).  Widths are taken in blocks of 64 columns: 80 costs what 128 does (470 us, 489), and rows that do not start on whole lines
+// more than that (one token: 206 us with 80, 176 with 128).
+//
+// As in window attention S = Q K^T goes to tensor memory, a thread takes the weights of one row and writes them over S, from where they go into O += P V: rounded to 16 bits, as the product
+// takes them, which is as much as an output's own rounding; the row's sum is of those before.
 //
 // Keys that only a part of the item's rows sees (the window's edge, new tokens, a tree, missing pages) go by bits, a word for 32 of them.  A value that is not finite would
 // reach every row there, as zero times it: it is taken out of the tile, and added to the rows that see it when they have been written (poison_row).
 constexpr int PG_BLOCK = SEQ_TILE * 128, PG_RING = 4, PG_THERE = 8, PG_MAX_SLOTS = 8;
-// What an item takes beside its tiles of keys, in tiles: of one tile of rows 2 (trees of 32 tokens for 32 sequences 215 us, 235 with 1, 213-216 with 4; 96 single tokens on up to 3800
-// 141-143, 147-154, 147), of two tiles 1 (chunks 340-345 us, 348 with 2, 344-364 with 4).
+// What an item takes beside its tiles of keys, in tiles: of one tile of rows 2 (trees of 32 tokens for 32 sequences 237 us, 250 with 1, 236 with 4; 96 single tokens on up to 3800
+// 144, 142, 146), of two tiles 1 (chunks 331 us, 330 with 2, 328 with 4).
 template <int TILES> constexpr int PG_ITEM = TILES == 1 ? 2 : 1;
 constexpr float PG_NO_SUM = 0x1p60f;   // some exponent was not a number (exp2_poly)
 constexpr float PG_MET = 0x1p-126f;    // a row's sum is at least this if it has seen a key; of a tile that all see the polynomial's least, 2^-125, comes to more

@@ -52,8 +52,9 @@ __device__ __forceinline__ float advance(float h, float ld, float x) {
 //
 // Gradients are the same from the end, on what flows back between tokens, c_t = a_t G_t: G_t = dout_t + c_(t+1), dx_t = G_t, dlog_decay_t = c_t h_(t-1).
 //
-// What bounds it: a unit takes some 8000 clocks, three of them run on an SM (two of gradients); 1200 go to each walk, 2000 to 4000 to looking back, as the tiles before run at the same time.  65536 tokens,
-// 2048 channels, bf16: 218 us, 3.7 TB/s; 64 sequences of 128 tokens, 4096 channels, where nothing looks back: 43 us, 4.8 TB/s.
+// What bounds it: the steps of a unit, which wait for one another (copies, first walk, fold, looking back, second walk with its stores), and three units on an SM (two of gradients), which do not fill them.
+// 65536 tokens, 2048 channels, bf16: 217 us, 3.7 TB/s (fp32 354 us, 4.5; gradients 319 and 551 us, 4.2 and 4.9), 5.9 us a unit, or 11600 clocks at 1965 MHz; 1200 go to each walk, and more than
+// half to looking back, as the tiles before run at the same time.  64 sequences of 128 tokens, 4096 channels, where nothing looks back: 43 us, 4.8 TB/s.
 //
 // Blocks take units from a counter, tiles in order, so that what a tile waits for is always taken by a running block; a ninth warp takes the next one, starts its
 // copies, and looks back.
@@ -73,7 +74,7 @@ struct RecurrenceKernel {
     int *err;
 };
 
-// exp of two log decays, at most 0: above -1/4 as 1 + ld (..), a polynomial of least maximum relative error (2.5e-7) by Lawson's iteration, so that a decay next to 1 is
+// exp of two log decays, at most 0: above -1/4 as 1 + ld (..), a polynomial of least maximum relative error (6.7e-8, as computed here 1.1e-7) by Lawson's iteration, so that a decay next to 1 is
 // rounded to the nearest -- the special-function unit's is not, and a sum over thousands of tokens would show it.  Below, that unit's.
 __device__ __forceinline__ f32x2 decay_of(f32x2 ld) {
     f32x2 y = fma2(ld, pack2(0.037709992f, 0.037709992f), pack2(0.16605508f, 0.16605508f));
@@ -87,7 +88,7 @@ __device__ __forceinline__ f32x2 decay_of(f32x2 ld) {
     return pack2(l[0] > -0.25f ? near[0] : ex2_approx(far[0]), l[1] > -0.25f ? near[1] : ex2_approx(far[1]));   // what is not a number stays that
 }
 // Multipliers of maps, from sums of log decays below zero: exp or, above -1/4, exp - 1, which is below zero.  A map's multiplier next to 1 that is rounded to FP32 would leave a sum
-// over many tiles off where decays are all alike (3e-8 a tile); exp - 1 keeps its bits, by a polynomial as above (2.5e-9).
+// over many tiles off where decays are all alike (3e-8 a tile); exp - 1 keeps its bits, by a polynomial as above (7.8e-9, as computed here 9.4e-8).
 __device__ __forceinline__ f32x2 multiplier(f32x2 ld) {
     f32x2 y = fma2(ld, pack2(0.0075102216f, 0.0075102216f), pack2(0.041488953f, 0.041488953f));
     y = fma2(y, ld, pack2(0.16665082f, 0.16665082f));
@@ -354,7 +355,7 @@ __global__ void __launch_bounds__(GR_THREADS, BACK ? 2 : 3) recurrence_tiles(con
                     } else {
                         const f32x2 d = add2(h, x);
                         h = mul2(m[i], d);
-                        f32x2 past = Two<T>::open(raw_of(2, i));
+                        f32x2 past = Two<T>::open(raw_of(2, i));   // as rounded in `out`: half a step of the type in dlog_decay, and no second walk forward
                         if (i == 0 && e.z + r0 == 0) past = a.state_in && in ? *reinterpret_cast<const f32x2 *>(a.state_in + (int64_t)e.w * a.channels + c) : 0;
                         float ll, lh, dl, dh;
                         unpack2(Two<T>::open(raw_of(1, i)), ll, lh);

@@ -17,9 +17,13 @@ of the arrays stand in include/f3m.h.
 New tokens are packed, as in `sequence`: row t of q, k, v is token t of all sequences laid end to end.  Token i of a sequence is token lengths + i of its cache.  Without
 `parents` new tokens follow one another; `parents` (tokens) int32 makes them a tree: the number, among the sequence's new tokens, of the token before each one, -1 where
 that is the cache's last.  A new token sees the cache, itself and those above it; its position is the cache's length plus its depth.  The tokens of a cache that is one array
-(n, capacity, kv_heads, width) are pages too: `cache.view(n * capacity // 128, 128, kv_heads, width)`.
+(n, capacity, kv_heads, width) are pages too: `cache.view(n * capacity // 128, 128, kv_heads, width)`.  For one new token of each sequence over such an array `sequence.window_attention_step`
+needs no plan and no table; `paged_attention` shares long caches more evenly (32 sequences up to 16384, 32 heads on 8, width 128: 177 us, 235).
 
-No call waits for the GPU: lengths, tables, parents and paths are read there, and all that they say is held within the arrays.
+A plan holds the numbers of new tokens.  Making one copies a table from host memory and waits for that: a program whose numbers change from step to step keeps a plan for each that comes
+up -- one new token for n sequences, drafts of one size (a draft that came out shorter may be filled up: what is appended behind a sequence's kept tokens is written over by the next call).
+
+No call with a plan in hand waits for the GPU: lengths, tables, parents and paths are read there, and all that they say is held within the arrays.
 """
 from __future__ import annotations
 
@@ -38,7 +42,7 @@ _NO_ROWS = Rows(None, 0, 0)
 
 class Rotation:
     """Turns of the first `columns` columns, a multiple of 16, by position: pair i by base^(-2 i / columns) radians a position, or by frequencies[i] where these
-    are given.  Pair i is columns (i, i + columns / 2), or (2 i, 2 i + 1) if interleaved.  Kept for any number of calls on any stream of the device."""
+    are given.  Pair i is columns (i, i + columns / 2), or (2 i, 2 i + 1) if interleaved.  Kept for any number of calls on any stream of the device (as long as any graph that holds one of them)."""
 
     def __init__(self, columns: int, base: float = 10000.0, interleaved: bool = False, frequencies: Optional[Sequence[float]] = None, device="cuda:0"):
         if columns < 16 or columns > _lib.MAX_WIDTH or columns % 16:
