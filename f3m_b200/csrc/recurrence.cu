@@ -43,7 +43,7 @@ __device__ __forceinline__ float advance(float h, float ld, float x) {
 }
 
 // ---- whole sequences --------------------------------------------------------------------------------------------------------
-// A unit is a tile of 128 tokens by 128 bytes of channels, a lane two channels.  Its tokens are cut into runs, one for 32 or 16 lanes each; a run is the map h -> A h + B, with
+// A scan in one pass with look-back (D. Merrill and M. Garland, 2016).  A unit is a tile of 128 tokens by 128 bytes of channels, a lane two channels.  Its tokens are cut into runs, one for 32 or 16 lanes each; a run is the map h -> A h + B, with
 // A from the sum of its log decays, and so is the tile.  What enters a tile is found by looking back over the tiles before it, of which each tells its map as soon as it
 // has it, and what leaves it as soon as it knows what entered: the nearest such state goes through the maps in between, always one after the other, so that a call's bits
 // do not depend on how far that was.  Then every run is walked again, from what enters it.  Each array is read and written once.
